@@ -45,6 +45,7 @@ extern "C" {
 #define PKV_STATUS_BAD_SLOT 1   /* slot_mapping entry outside [0, num_slots) */
 #define PKV_STATUS_BAD_PAGE 2   /* kv_indices entry outside [0, num_blocks) */
 #define PKV_STATUS_BAD_BLOCK 4  /* copy/gather/scatter id outside [0, num_blocks) */
+#define PKV_STATUS_BAD_POSITION 8  /* position without a row of the rotation table */
 
 /* Version of this ABI; bumped on any signature change. */
 int pkv_abi_version(void);
@@ -65,6 +66,31 @@ int pkv_append_kv(void* k_pool, void* v_pool, int64_t num_slots,
                   const void* k, const void* v, const int32_t* slot_mapping,
                   int64_t n_tokens, int32_t n_kv_heads, int32_t head_dim,
                   int32_t dtype, int32_t* status_word, void* stream);
+
+/*
+ * KV append with the position rotation on the way — no counterpart in the
+ * reference, whose models rotate q and k before append_kv. Row t of q is
+ * rotated into row t of q_out, row t of k is rotated into row slot_mapping[t]
+ * of the K pool, row t of v copied into that row of the V pool. q, k and v
+ * have heads of head_dim consecutive elements, one head after another, and
+ * rows q_stride / k_stride / v_stride elements apart (slices of one
+ * projection's output); q_out is contiguous. Of each head the first rotary_dim
+ * elements (even, at most head_dim) form pairs, (i, i + rotary_dim / 2) or,
+ * with interleaved != 0, (2 i, 2 i + 1); pair i of a token at position p =
+ * positions[t] becomes (a c - b s, b c + a s) with c = table[p][0][i], s =
+ * table[p][1][i] of the float [max_positions][2][rotary_dim / 2] table, in 32
+ * bits with one rounding to the pool dtype. Slots outside [0, num_slots) are
+ * skipped and flagged; positions outside [0, max_positions) are flagged, write
+ * no row and get a zero row of q_out. No two tokens may share a slot, and
+ * q_out may not overlap the inputs.
+ */
+int pkv_append_rotated(void* k_pool, void* v_pool, int64_t num_slots, const void* q,
+                       int64_t q_stride, void* q_out, const void* k, int64_t k_stride,
+                       const void* v, int64_t v_stride, const int32_t* slot_mapping,
+                       const int64_t* positions, int64_t n_tokens, const float* table,
+                       int64_t max_positions, int32_t rotary_dim, int32_t interleaved,
+                       int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t dtype,
+                       int32_t* status_word, void* stream);
 
 /*
  * Decode plan (host function, synchronous, no device access) — the

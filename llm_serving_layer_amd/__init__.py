@@ -8,6 +8,7 @@ hand-written gfx950 kernels (include/pagedkv.h, csrc/):
 * ``paging``    — BlockAllocator, SequenceBlocks, build_csr;
 * ``assembly``  — ScheduledSeq, build_batch_meta, build_token_tensor;
 * ``backend``   — MI355XBackend (append_kv / attend / copy_block[s]);
+* ``rotary``    — RotaryTable (MI355XBackend.append_kv_rotated);
 * ``swap``      — KVSwapSpace / SwapHandle (preemption swap);
 * ``sizing``    — plan_kv_pool / KVPoolPlan (pool sizing for one MI355X).
 * ``sampling``  — greedy (argmax on the device), StepTimer, greedy_step (the
@@ -17,10 +18,11 @@ hand-written gfx950 kernels (include/pagedkv.h, csrc/):
 from .assembly import ScheduledSeq, build_batch_meta, build_token_tensor
 from .contract import AttentionBackend, BatchMeta
 from .paging import AllocationError, BlockAllocator, SequenceBlocks, build_csr
+from .rotary import RotaryTable
 
 __all__ = ["AttentionBackend", "BatchMeta", "AllocationError", "BlockAllocator",
            "SequenceBlocks", "build_csr", "ScheduledSeq", "build_batch_meta",
-           "build_token_tensor", "MI355XBackend", "KVSwapSpace", "SwapHandle",
+           "build_token_tensor", "RotaryTable", "MI355XBackend", "KVSwapSpace", "SwapHandle",
            "SwapSpaceFull", "is_available", "unavailable_reason"]
 
 

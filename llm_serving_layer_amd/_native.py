@@ -15,12 +15,12 @@ from pathlib import Path
 # PKV_LIBRARY selects another build of the same library (e.g. a tuning variant).
 LIB_PATH = Path(os.environ.get("PKV_LIBRARY") or
                 Path(__file__).resolve().parent / "_native" / "libpagedkv.so")
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
 DECODE_SCRATCH_BYTES = 64 * 1024 * 1024   # PKV_DECODE_SCRATCH_BYTES
 OK, ERR_INVALID, ERR_RANGE, ERR_HIP, ERR_CAPACITY = 0, 1, 2, 3, 4
-STATUS_BAD_SLOT, STATUS_BAD_PAGE, STATUS_BAD_BLOCK = 1, 2, 4
+STATUS_BAD_SLOT, STATUS_BAD_PAGE, STATUS_BAD_BLOCK, STATUS_BAD_POSITION = 1, 2, 4, 8
 
 _p, _i32, _i64, _f32 = C.c_void_p, C.c_int32, C.c_int64, C.c_float
 
@@ -29,6 +29,9 @@ SIGNATURES = {
     "pkv_abi_version": (C.c_int, []),
     "pkv_last_error": (C.c_char_p, []),
     "pkv_append_kv": (C.c_int, [_p, _p, _i64, _p, _p, _p, _i64, _i32, _i32, _i32, _p, _p]),
+    "pkv_append_rotated": (C.c_int, [_p, _p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _p, _p,
+                                     _i64, _p, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _p,
+                                     _p]),
     "pkv_plan_decode": (C.c_int, [_p, _p, _p, _p, _i32, _i32, _i64, _i32, _i32, _i32, _p, _i64,
                                   _p, _p, _p, _p]),
     "pkv_decode_workgroups": (C.c_int, [_i32, _i32, _i32, _i32, _i32]),

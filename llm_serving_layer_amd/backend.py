@@ -39,6 +39,7 @@ thread-safe and not re-entrant, like the reference backends.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from array import array
 from operator import eq
@@ -48,6 +49,7 @@ import torch
 
 from . import _native
 from .contract import BatchMeta
+from .rotary import RotaryTable
 from .upload import uploader
 from .sizing import DEFAULT_PART_PAGES  # split-K pieces: 17 pages = 272 tokens
 
@@ -145,6 +147,8 @@ def unavailable_reason() -> str | None:
     return _native.reason()
 
 
+_HERE = contextlib.nullcontext()
+
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
@@ -178,8 +182,16 @@ class _Pending:
     __slots__ = ("layer", "k", "v", "meta", "slots", "stream", "kver", "vver")
 
 
+class _Rows:
+    """Where one BatchMeta's new rows go, on the device (``append_kv_rotated``)."""
+
+    __slots__ = ("meta", "slots", "positions", "far")
+
+
 class MI355XBackend:
     """Paged KV storage plus attention on gfx950 kernels."""
+
+    _rows: _Rows | None = None
 
     def __init__(self, num_layers: int, num_blocks: int, block_size: int, n_kv_heads: int,
                  n_heads: int, head_dim: int, device: str | torch.device = "cuda:0",
@@ -363,6 +375,8 @@ class MI355XBackend:
                 what.append("kv_indices entry outside [0, num_blocks)")
             if bits & _native.STATUS_BAD_BLOCK:
                 what.append("block id outside [0, num_blocks)")
+            if bits & _native.STATUS_BAD_POSITION:
+                what.append("position outside the rotation table")
             raise IndexError("device kernels skipped invalid ids: " + "; ".join(what))
 
     # -- write path -----------------------------------------------------------------
@@ -440,6 +454,90 @@ class MI355XBackend:
                     _native.check(rc, "append_kv")
                 return
         self._launch_append(layer_idx, k, v, self._slots_for(meta), stream)
+
+    def append_kv_rotated(self, layer_idx: int, q: torch.Tensor, k: torch.Tensor,
+                          v: torch.Tensor, meta: BatchMeta, table: RotaryTable) -> torch.Tensor:
+        """
+        Rotate this step's queries and keys by ``meta.positions`` and scatter
+        the rotated K and V into the pool through ``meta.slot_mapping``, in one
+        launch; returns the rotated queries (a new ``(tokens, n_heads,
+        head_dim)`` tensor), ready for an ``attend``.
+
+        ``q``, ``k`` and ``v`` may be slices of one projection's output: any
+        stride between tokens, heads one after another. Rotation in 32 bits,
+        rounded once to the pool dtype; inputs of another dtype are brought to
+        it first, as ``append_kv`` does. A position past the table is refused
+        where the meta's host mirror tells it, and else flagged for
+        ``check_device_errors`` (its row is not written, its query is zero).
+        """
+        if layer_idx is None or not 0 <= layer_idx < self.num_layers:
+            self._check_layer(layer_idx)
+        if meta.slot_mapping is None:
+            raise ValueError("MI355XBackend.append_kv_rotated requires meta.slot_mapping")
+        tokens, d = q.shape[0], self.head_dim
+        for name, x, h in (("q", q, self.n_heads), ("k", k, self.n_kv_heads),
+                           ("v", v, self.n_kv_heads)):
+            if x.shape != (tokens, h, d):
+                raise ValueError(f"{name} has shape {tuple(x.shape)}, expected "
+                                 f"({tokens}, {h}, {d})")
+        if meta.slot_mapping.shape[0] != tokens or meta.n_tokens != tokens:
+            raise ValueError(f"meta describes {meta.n_tokens} tokens and "
+                             f"{meta.slot_mapping.shape[0]} slots but {tokens} tokens were "
+                             "supplied")
+        if not isinstance(table, RotaryTable):
+            raise TypeError(f"table must be a RotaryTable, got {type(table).__name__}")
+        if table.device != self.device:
+            raise ValueError(f"the rotation table is on {table.device}, the pool on "
+                             f"{self.device}")
+        if table.rotary_dim > d:
+            raise ValueError(f"rotary_dim={table.rotary_dim} exceeds head_dim={d}")
+        r = self._rows
+        if r is None or r.meta is not meta:
+            r = self._rows_for(meta)
+        if r.far >= table.max_positions:
+            raise ValueError(f"position {r.far} is outside the rotation table of "
+                             f"{table.max_positions} positions")
+        if self._pending is not None:
+            self._flush()
+        q, k, v = self._token_rows(q), self._token_rows(k), self._token_rows(v)
+        out = torch.empty((tokens, self.n_heads, d), dtype=self.dtype, device=self.device)
+        with self._on_device():
+            rc = self._lib.pkv_append_rotated(
+                self._k_ptr[layer_idx], self._v_ptr[layer_idx], self.num_blocks * self.block_size,
+                q.data_ptr(), q.stride(0), out.data_ptr(), k.data_ptr(), k.stride(0),
+                v.data_ptr(), v.stride(0), r.slots.data_ptr(), r.positions.data_ptr(), tokens,
+                table.table.data_ptr(), table.max_positions, table.rotary_dim, table.interleaved,
+                self.n_heads, self.n_kv_heads, d, self._code, self._status_ptr,
+                _current_stream(self.device))
+        if rc:
+            _native.check(rc, "append_kv_rotated")
+        return out
+
+    def _rows_for(self, meta: BatchMeta) -> _Rows:
+        """The meta's slots and positions on the device, once per meta, and its
+        last position as far as the host knows it (else -1)."""
+        r = _Rows()
+        r.slots = self._slots_for(meta)
+        r.positions = meta.positions.to(device=self.device, dtype=torch.int64).contiguous()
+        mirror = meta.host_arrays()
+        r.far = int(mirror["kv_lens"].max()) - 1 if mirror is not None else -1
+        r.meta = meta
+        self._rows = r
+        return r
+
+    def _token_rows(self, x: torch.Tensor) -> torch.Tensor:
+        """x in the pool dtype on this device, heads contiguous in each token's
+        row, rows any distance apart."""
+        if (x.dtype is self.dtype and x.get_device() == self.device.index
+                and (x.is_contiguous() or (x.stride(2) == 1 and x.stride(1) == x.shape[2]))):
+            return x
+        return x.to(device=self.device, dtype=self.dtype).contiguous()
+
+    def _on_device(self):
+        """Launches go to this backend's device, whichever is current."""
+        if torch.cuda.current_device() == self.device.index:
+            return _HERE
+        return torch.cuda.device(self.device)
 
     def _slots_for(self, meta: BatchMeta) -> torch.Tensor:
         p = self._planned
@@ -730,6 +828,7 @@ class MI355XBackend:
         self._flush()
         self._planned = None
         self._slot_cache = None
+        self._rows = None
 
     # -- misc -------------------------------------------------------------------------
 

@@ -324,6 +324,63 @@ int pkv_attend_batch(const void* batch, const void* q, void* out, void* k_pool, 
                      float scale, const void* k_new, const void* v_new, void* stream);
 
 /*
+ * Key bounds of pages — no counterpart in the reference. For each of the
+ * n_ids pages of ids (NULL: pages 0 .. n_ids - 1) and each of n_layers layers,
+ * row id of lo and hi ([num_blocks, n_kv_heads, head_dim], the pool dtype)
+ * receives the elementwise minimum and maximum of the page's page_size key
+ * rows; a NaN among them gives NaN. Layer l's K plane, lo and hi start
+ * l * pool_step and l * bounds_step bytes from the given ones. Ids outside
+ * [0, num_blocks) are skipped and flagged; equal ids are harmless.
+ */
+int pkv_page_bounds(const void* k_pool, int64_t pool_step, void* lo, void* hi,
+                    int64_t bounds_step, int32_t n_layers, int64_t num_blocks,
+                    const int32_t* ids, int64_t n_ids, int32_t n_kv_heads, int32_t head_dim,
+                    int32_t page_size, int32_t dtype, int32_t* status_word, void* stream);
+
+/*
+ * Choice of pages for a batch of one-token sequences — no counterpart in the
+ * reference. A sequence of np pages gets, per KV head, all of them if np <=
+ * pages; else its last page and the pages - 1 of the others with the largest
+ * score, the largest over the KV head's query heads of sum_d q_d * (q_d < 0 ?
+ * lo_d : hi_d) in 64 bits (equal scores: the lower index; a NaN beats every
+ * number). lo and hi are one layer's bounds (pkv_page_bounds). ids and
+ * ordinals, int32 [n_seqs, n_kv_heads, min(pages, max_pages)], receive the
+ * chosen pages' kv_indices entries and indices in the sequence's page list, in
+ * ascending order, -1 behind shorter lists. max_pages is at least every
+ * sequence's page count; scores holds n_seqs * n_kv_heads * max_pages doubles
+ * (NULL if max_pages <= pages). Out-of-range page ids are scored by page 0's
+ * bounds and flagged.
+ */
+int pkv_select_pages(const void* q, const void* lo, const void* hi, int64_t num_blocks,
+                     const int32_t* kv_indptr, const int32_t* kv_indices, const int32_t* kv_lens,
+                     int32_t n_seqs, int32_t max_pages, int32_t pages, int32_t n_heads,
+                     int32_t n_kv_heads, int32_t head_dim, int32_t page_size, int32_t dtype,
+                     double* scores, int32_t* ids, int32_t* ordinals, int32_t* status_word,
+                     void* stream);
+
+/*
+ * Decode attention over the pages pkv_select_pages chose (its ids, n_seqs,
+ * max_pages and pages): sequence i's single query attends the rows of its
+ * chosen pages, of the last one those below kv_lens[i]. Lists are cut into
+ * pieces of part_pages pages, as pkv_plan_decode cuts sequences, and cut ones
+ * merge through `workspace` (256-byte aligned, pkv_selected_workspace_bytes
+ * long; zero before the first launch that uses it, and left with zero
+ * counters by each; launches that share it must not overlap in time).
+ * Geometries without the fast decode path run a generic kernel, with no
+ * workspace.
+ */
+int64_t pkv_selected_workspace_bytes(int32_t n_seqs, int32_t max_pages, int32_t pages,
+                                     int32_t part_pages, int32_t n_heads, int32_t n_kv_heads,
+                                     int32_t head_dim, int32_t page_size, int64_t num_blocks,
+                                     int32_t dtype);
+int pkv_attend_selected(const void* q, void* out, void* k_pool, void* v_pool, int64_t num_blocks,
+                        const int32_t* ids, const int32_t* kv_lens, int32_t n_seqs,
+                        int32_t max_pages, int32_t pages, int32_t part_pages, int32_t n_heads,
+                        int32_t n_kv_heads, int32_t head_dim, int32_t page_size, float scale,
+                        int32_t dtype, void* workspace, int64_t workspace_bytes,
+                        int32_t* status_word, void* stream);
+
+/*
  * Batched block copy over every layer, K and V — replaces
  * PagedTorchBackend.copy_block (serving/backends/paged_torch.py:181-207),
  * called once per pair by RadixCache.ensure_writable

@@ -185,20 +185,30 @@ class _Pending:
 class _Rows:
     """Where one BatchMeta's new rows go, on the device (``append_kv_rotated``)."""
 
-    __slots__ = ("meta", "slots", "positions", "far")
+    __slots__ = ("meta", "slots", "positions", "far", "complete", "buffers", "stream")
+
+
+class _Selected:
+    """What ``attend_selected`` keeps for one BatchMeta and page budget."""
+
+    __slots__ = ("meta", "pages", "n", "max_pages", "indptr", "indices", "kv_lens", "scores",
+                 "ids", "ordinals", "part", "ws", "buffers", "stream")
 
 
 class MI355XBackend:
     """Paged KV storage plus attention on gfx950 kernels."""
 
     _rows: _Rows | None = None
+    _selected: _Selected | None = None
+    _bounds: torch.Tensor | None = None
 
     def __init__(self, num_layers: int, num_blocks: int, block_size: int, n_kv_heads: int,
                  n_heads: int, head_dim: int, device: str | torch.device = "cuda:0",
                  dtype: torch.dtype = torch.float16, *,
                  part_pages: int = DEFAULT_PART_PAGES, q_tile: int | None = None,
                  fuse_append: bool = True, decode_workgroups_per_cu: int = 2,
-                 decode_workgroups: int | None = None, decode_workspace_bytes: int = 0):
+                 decode_workgroups: int | None = None, decode_workspace_bytes: int = 0,
+                 page_bounds: bool = False):
         if n_heads % n_kv_heads != 0:
             raise ValueError(
                 f"n_heads={n_heads} must be divisible by n_kv_heads={n_kv_heads}; "
@@ -254,7 +264,8 @@ class MI355XBackend:
         self._code = _DTYPES[dtype]
         self._fast_decode = bool(self._lib.pkv_decode_fast_path(
             n_heads, n_kv_heads, head_dim, block_size, self._code, part_pages))
-        self._fuse_append = fuse_append and self._fast_decode
+        # (with page bounds the append runs first: the bounds follow from its rows)
+        self._fuse_append = fuse_append and self._fast_decode and not page_bounds
         # The decode grid: every bin of the plan a resident workgroup (per
         # group of KV heads), so none waits for a slot. ``decode_workgroups``
         # overrides the count (tests force many sequences into a bin with it).
@@ -290,6 +301,13 @@ class MI355XBackend:
         self._planned: _Plan | None = None
         self._set_workspace(torch.zeros(decode_workspace_bytes, dtype=torch.uint8,
                                         device=self.device))
+        # Per page and KV head the elementwise minimum and maximum of its keys
+        # (attend_selected's cheap score), laid out like a pool of one-row pages.
+        if page_bounds:
+            self._bounds = torch.zeros((num_layers, 2, num_blocks, n_kv_heads, head_dim),
+                                       dtype=dtype, device=self.device)
+        # what graphs were captured with: it stays as long as the backend
+        self._captured: list = []
         self._slot_cache: tuple[BatchMeta, torch.Tensor] | None = None
         self._pending: _Pending | None = None
         self.n_plans = 0
@@ -306,6 +324,24 @@ class MI355XBackend:
     def v_pool(self) -> list[torch.Tensor]:
         self._flush()
         return self._v_pool
+
+    @property
+    def key_bounds(self) -> list[torch.Tensor]:
+        """Per layer ``(2, num_blocks, n_kv_heads, head_dim)``: the elementwise
+        minimum and maximum of each page's keys, renewed when an append
+        completes the page, when blocks are copied and swapped in, and by
+        ``refresh_page_bounds``. Needs ``page_bounds=True``."""
+        self._need_bounds("key_bounds")
+        self._flush()
+        return list(self._bounds.unbind(0))
+
+    def _need_bounds(self, what: str) -> None:
+        if self._bounds is None:
+            raise ValueError(f"{what} needs a backend built with page_bounds=True")
+
+    def bounds_bytes(self) -> int:
+        """Device bytes of the page bounds (beside ``pool_bytes``)."""
+        return 0 if self._bounds is None else self._bounds.numel() * self._bounds.element_size()
 
     # -- pool construction / accounting ---------------------------------------
 
@@ -407,6 +443,46 @@ class MI355XBackend:
                                        ids.data_ptr(), ids.data_ptr() + 4 * n, n,
                                        self._status.data_ptr(), _current_stream(self.device))
         _native.check(rc, "copy_blocks")
+        if self._bounds is not None:
+            row = self._block_bytes // self.block_size
+            rc = self._lib.pkv_copy_blocks(self._bounds.data_ptr(), self.num_layers,
+                                           self.num_blocks * row, row, self.num_blocks,
+                                           ids.data_ptr(), ids.data_ptr() + 4 * n, n,
+                                           self._status.data_ptr(), _current_stream(self.device))
+            _native.check(rc, "copy_blocks (page bounds)")
+
+    def refresh_page_bounds(self, blocks=None) -> None:
+        """
+        Renew every layer's key bounds of ``blocks`` (all of the pool by
+        default) from the pool: for a caller that wrote ``k_pool`` itself.
+        Appends, block copies and swaps keep the bounds by themselves.
+        """
+        self._need_bounds("refresh_page_bounds")
+        self._flush()
+        if blocks is None:
+            return self._renew_bounds(None, self.num_blocks, _current_stream(self.device))
+        ids = block_ids(blocks)
+        if ids.shape[0] == 0:
+            return
+        if ids.min() < 0 or ids.max() >= self.num_blocks:
+            raise IndexError(f"block id outside [0, {self.num_blocks})")
+        ids = torch.from_numpy(ids.astype(np.int32)).pin_memory().to(self.device,
+                                                                     non_blocking=True)
+        self._renew_bounds(ids, ids.shape[0], _current_stream(self.device))
+
+    def _renew_bounds(self, ids, n: int, stream: int, layer: int | None = None) -> None:
+        """Bounds of the blocks ``ids`` (device int32; None: the pool's first
+        ``n``) in one layer or in all of them."""
+        l, b = layer or 0, self._bounds
+        half = b.stride(1) * b.element_size()
+        at = b.data_ptr() + 2 * l * half
+        with self._on_device():
+            rc = self._lib.pkv_page_bounds(
+                self._k_ptr[l], 2 * self._plane_bytes, at, at + half, 2 * half,
+                self.num_layers if layer is None else 1, self.num_blocks,
+                None if ids is None else ids.data_ptr(), n, self.n_kv_heads, self.head_dim,
+                self.block_size, self._code, self._status_ptr, stream)
+        _native.check(rc, "page bounds")
 
     def append_kv(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor,
                   meta: BatchMeta) -> None:
@@ -454,6 +530,8 @@ class MI355XBackend:
                     _native.check(rc, "append_kv")
                 return
         self._launch_append(layer_idx, k, v, self._slots_for(meta), stream)
+        if self._bounds is not None:
+            self._complete_bounds(layer_idx, meta)
 
     def append_kv_rotated(self, layer_idx: int, q: torch.Tensor, k: torch.Tensor,
                           v: torch.Tensor, meta: BatchMeta, table: RotaryTable) -> torch.Tensor:
@@ -492,14 +570,18 @@ class MI355XBackend:
         if table.rotary_dim > d:
             raise ValueError(f"rotary_dim={table.rotary_dim} exceeds head_dim={d}")
         r = self._rows
-        if r is None or r.meta is not meta:
-            r = self._rows_for(meta)
-        if r.far >= table.max_positions:
-            raise ValueError(f"position {r.far} is outside the rotation table of "
+        if r is not None and r.meta is not meta:
+            r = None
+        far = r.far if r is not None else self._last_position(meta)
+        if far >= table.max_positions:
+            raise ValueError(f"position {far} is outside the rotation table of "
                              f"{table.max_positions} positions")
+        if r is None:
+            r = self._rows_for(meta)
         if self._pending is not None:
             self._flush()
         q, k, v = self._token_rows(q), self._token_rows(k), self._token_rows(v)
+        stream = self._enter(r)
         out = torch.empty((tokens, self.n_heads, d), dtype=self.dtype, device=self.device)
         with self._on_device():
             rc = self._lib.pkv_append_rotated(
@@ -507,23 +589,59 @@ class MI355XBackend:
                 q.data_ptr(), q.stride(0), out.data_ptr(), k.data_ptr(), k.stride(0),
                 v.data_ptr(), v.stride(0), r.slots.data_ptr(), r.positions.data_ptr(), tokens,
                 table.table.data_ptr(), table.max_positions, table.rotary_dim, table.interleaved,
-                self.n_heads, self.n_kv_heads, d, self._code, self._status_ptr,
-                _current_stream(self.device))
+                self.n_heads, self.n_kv_heads, d, self._code, self._status_ptr, stream)
         if rc:
             _native.check(rc, "append_kv_rotated")
+        if self._bounds is not None:
+            self._complete_bounds(layer_idx, meta)
         return out
 
+    @staticmethod
+    def _last_position(meta: BatchMeta) -> int:
+        """The meta's furthest position as far as the host knows it (else -1)."""
+        mirror = meta.host_arrays()
+        return int(mirror["kv_lens"].max()) - 1 if mirror is not None else -1
+
     def _rows_for(self, meta: BatchMeta) -> _Rows:
-        """The meta's slots and positions on the device, once per meta, and its
-        last position as far as the host knows it (else -1)."""
+        """The meta's slots and positions on the device, once per meta."""
         r = _Rows()
         r.slots = self._slots_for(meta)
         r.positions = meta.positions.to(device=self.device, dtype=torch.int64).contiguous()
-        mirror = meta.host_arrays()
-        r.far = int(mirror["kv_lens"].max()) - 1 if mirror is not None else -1
+        r.far = self._last_position(meta)
+        r.complete = None
+        if self._bounds is not None:
+            pages = self._completed_pages(meta)
+            if pages.shape[0]:
+                r.complete = self._upload(pages)
+        r.buffers = [t for t in (r.slots, r.positions, r.complete) if t is not None]
+        r.stream = _current_stream(self.device)
         r.meta = meta
         self._rows = r
         return r
+
+    def _completed_pages(self, meta: BatchMeta) -> np.ndarray:
+        """Pages whose last row this meta's append writes: the bounds of a page
+        are those of all its rows, and only whole pages are ever chosen by them.
+        Rows that go elsewhere than the page table says renew their pages each
+        time."""
+        ql, cu, kvl, indptr, last, indices, slots = self._host_index(meta, True)
+        ps = self.block_size
+        seq = np.repeat(np.arange(ql.shape[0]), ql)
+        pos = np.arange(seq.shape[0]) + (kvl - ql - cu[:-1])[seq]
+        at = indptr[:-1][seq] + pos // ps
+        if at.shape[0] == slots.shape[0] and (at < indices.shape[0]).all() and (pos >= 0).all():
+            pages = indices[at]
+            if (pages * ps + pos % ps == slots).all():
+                return np.ascontiguousarray(pages[pos % ps == ps - 1], dtype=np.int32)
+        pages = np.unique(slots // ps)
+        return pages[(pages >= 0) & (pages < self.num_blocks)].astype(np.int32)
+
+    def _complete_bounds(self, layer: int, meta: BatchMeta) -> None:
+        r = self._rows
+        if r is None or r.meta is not meta:
+            r = self._rows_for(meta)
+        if r.complete is not None:
+            self._renew_bounds(r.complete, r.complete.shape[0], self._enter(r), layer)
 
     def _token_rows(self, x: torch.Tensor) -> torch.Tensor:
         """x in the pool dtype on this device, heads contiguous in each token's
@@ -626,6 +744,138 @@ class MI355XBackend:
             _native.check(rc, "attend (prefill)" if p.use_prefill else "attend (decode)")
         return out
 
+    def attend_selected(self, q: torch.Tensor, layer_idx: int, scale: float, meta: BatchMeta,
+                        pages: int, return_pages: bool = False):
+        """
+        Attention of a decode batch over at most ``pages`` pages a sequence
+        and KV head: the sequence's last page and, of the others, those whose
+        key bounds allow the largest score (the largest over the KV head's
+        query heads of ``sum_d max(q_d lo_d, q_d hi_d)``, summed in 64 bits;
+        equal scores: the earlier page; a NaN beats every number). Sequences of
+        at most ``pages`` pages are attended whole, as ``attend`` does.
+
+        Needs ``page_bounds=True``, one token per sequence and a positive
+        scale. With ``return_pages`` also returns the chosen pages' indices in
+        each sequence's page list, int32 ``(n_seqs, n_kv_heads, min(pages,
+        longest list))``, ascending, -1 behind a shorter list. Graphs captured
+        with one meta share its buffers, so their replays must not overlap.
+        """
+        if layer_idx is None or not 0 <= layer_idx < self.num_layers:
+            self._check_layer(layer_idx)
+        self._need_bounds("attend_selected")
+        tokens = q.shape[0]
+        if q.shape != (tokens, self.n_heads, self.head_dim):
+            raise ValueError(f"q has shape {tuple(q.shape)}, expected "
+                             f"({tokens}, {self.n_heads}, {self.head_dim})")
+        if meta.n_tokens != tokens:
+            raise ValueError(f"meta describes {meta.n_tokens} tokens but q has {tokens}")
+        if pages < 1:
+            raise ValueError(f"pages must be positive, got {pages}")
+        if not float(scale) > 0:
+            raise ValueError(f"attend_selected needs a positive scale, got {scale}: the bounds "
+                             "are of the largest score")
+        p = self._selected
+        if p is None or p.meta is not meta or p.pages != pages:
+            p = self._plan_selected(meta, int(pages))
+        self._flush()
+        stream = self._enter(p)
+        if not (q.dtype is self.dtype and q.get_device() == self.device.index
+                and q.is_contiguous()):
+            q = self._as_pool(q)
+        if q.data_ptr() % 16:
+            q = q.clone()
+        out = torch.empty_like(q)
+        width = min(p.pages, p.max_pages)
+        if return_pages:
+            ordinals = torch.empty((p.n, self.n_kv_heads, width), dtype=torch.int32,
+                                   device=self.device)
+        else:
+            ordinals = p.ordinals
+        b = self._bounds[layer_idx]
+        with self._on_device():
+            rc = self._lib.pkv_select_pages(
+                q.data_ptr(), b[0].data_ptr(), b[1].data_ptr(), self.num_blocks,
+                p.indptr.data_ptr(), p.indices.data_ptr(), p.kv_lens.data_ptr(), p.n,
+                p.max_pages, p.pages, self.n_heads, self.n_kv_heads, self.head_dim,
+                self.block_size, self._code, p.scores.data_ptr(), p.ids.data_ptr(),
+                ordinals.data_ptr(), self._status_ptr, stream)
+            _native.check(rc, "attend_selected (choice)")
+            rc = self._lib.pkv_attend_selected(
+                q.data_ptr(), out.data_ptr(), self._k_ptr[layer_idx], self._v_ptr[layer_idx],
+                self.num_blocks, p.ids.data_ptr(), p.kv_lens.data_ptr(), p.n, p.max_pages,
+                p.pages, p.part, self.n_heads, self.n_kv_heads, self.head_dim, self.block_size,
+                float(scale), self._code, p.ws.data_ptr(), p.ws.numel(), self._status_ptr, stream)
+            _native.check(rc, "attend_selected")
+        self.n_runs += 1
+        return (out, ordinals) if return_pages else out
+
+    def _plan_selected(self, meta: BatchMeta, pages: int) -> _Selected:
+        ql, cu, kvl, indptr, last, indices, _ = self._host_index(meta, False)
+        n = int(ql.shape[0])
+        if (ql != 1).any() or n != meta.n_tokens:
+            raise ValueError("attend_selected takes decode batches: one token per sequence "
+                             f"(query_lens up to {int(ql.max())} over {meta.n_tokens} tokens)")
+        self._check_pages(kvl, indptr, last, int(indices.shape[0]))
+        p = _Selected()
+        p.pages, p.n, p.max_pages = pages, n, int(np.diff(indptr).max())
+        width = min(pages, p.max_pages)
+        dev = {"device": self.device}
+        p.indptr = self._dev_i32(meta.kv_indptr)
+        p.indices = self._dev_i32(meta.kv_indices)
+        p.kv_lens = self._dev_i32(meta.kv_lens)
+        many = n * self.n_kv_heads
+        p.scores = torch.empty(many * p.max_pages if p.max_pages > pages else 0,
+                               dtype=torch.float64, **dev)
+        p.ids = torch.empty(many * width, dtype=torch.int32, **dev)
+        p.ordinals = torch.empty(many * width, dtype=torch.int32, **dev)
+        p.part = self.part_pages
+        while True:   # partials are addressed with 32 bits: longer pieces where they pass 2 GiB
+            need = self._lib.pkv_selected_workspace_bytes(
+                n, p.max_pages, pages, p.part, self.n_heads, self.n_kv_heads, self.head_dim,
+                self.block_size, self.num_blocks, self._code)
+            if need < 2**31 or p.part >= MAX_PART_PAGES:
+                break
+            p.part = min(2 * p.part, MAX_PART_PAGES)
+        p.ws = torch.zeros(need, dtype=torch.uint8, **dev)
+        p.buffers = [p.indptr, p.indices, p.kv_lens, p.scores, p.ids, p.ordinals, p.ws]
+        p.stream = _current_stream(self.device)
+        p.meta = meta
+        self._selected = p
+        self.n_plans += 1
+        return p
+
+    def _check_pages(self, kvl, indptr, last, n_pages: int) -> None:
+        """Every sequence's page list fits its length (ValueError naming the first
+        that does not)."""
+        ps = self.block_size
+        if int(indptr[0]) != 0 or int(indptr[-1]) != n_pages:
+            raise ValueError(f"kv_indptr spans [{int(indptr[0])}, {int(indptr[-1])}) but "
+                             f"kv_indices holds {n_pages} pages")
+        need = (kvl + ps - 1) // ps
+        bad = (kvl < 1) | (np.diff(indptr) != need) | (last != kvl - (need - 1) * ps)
+        if bad.any():
+            i = int(np.argmax(bad))
+            raise ValueError(f"seq {i}: kv_len={int(kvl[i])} with "
+                             f"{int(indptr[i + 1] - indptr[i])} pages of {ps} and "
+                             f"kv_last_page_len={int(last[i])} disagree")
+
+    def _enter(self, p) -> int:
+        """The current stream's handle, ordered behind the plan's last launch:
+        launches of one plan share its buffers. A plan that a graph captures
+        stays as long as the backend does."""
+        stream = _current_stream(self.device)
+        if torch.cuda.is_current_stream_capturing():
+            if not any(c is p for c in self._captured):
+                self._captured.append(p)
+        elif p.stream != stream:
+            cur, ev = torch.cuda.current_stream(self.device), torch.cuda.Event()
+            ev.record(torch.cuda.ExternalStream(p.stream, device=self.device))
+            cur.wait_event(ev)
+            for t in p.buffers:     # not reused before this stream is done with them
+                t.record_stream(cur)
+            p.stream = stream
+        return stream
+
     # -- planning ---------------------------------------------------------------
 
     def _ensure_planned(self, meta: BatchMeta) -> _Plan:
@@ -641,28 +891,8 @@ class MI355XBackend:
         n = meta.n_seqs
         with_slots = (meta.slot_mapping is not None and meta.slot_mapping.shape[0] == n
                       and meta.kv_indices.shape[0] > 0 and meta.kv_indptr.shape[0] == n + 1)
-        mirror = meta.host_arrays()
         n_pages = int(meta.kv_indices.shape[0])
-        if mirror is not None:
-            # the assembler's own host arrays: no device read-back
-            ql, cu = mirror["query_lens"], mirror["cu_query_lens"]
-            kvl, indptr = mirror["kv_lens"], mirror["kv_indptr"]
-            last, indices = mirror["kv_last_page_len"], mirror["kv_indices"]
-            if with_slots:
-                new_slot = mirror["slot_mapping"]
-        else:
-            parts = [meta.query_lens, meta.cu_query_lens, meta.kv_lens, meta.kv_indptr,
-                     meta.kv_last_page_len, meta.kv_indices]
-            if with_slots:
-                parts.append(meta.slot_mapping)
-            # ONE device->host transfer for everything the host plan reads.
-            host = torch.cat([t.reshape(-1).to(torch.int64) for t in parts]).cpu().numpy()
-            ql, cu = host[:n], host[n:2 * n + 1]
-            kvl, indptr = host[2 * n + 1:3 * n + 1], host[3 * n + 1:4 * n + 2]
-            last = host[4 * n + 2:5 * n + 2]
-            indices = host[5 * n + 2:5 * n + 2 + n_pages]
-            if with_slots:
-                new_slot = host[5 * n + 2 + n_pages:6 * n + 2 + n_pages]
+        ql, cu, kvl, indptr, last, indices, new_slot = self._host_index(meta, with_slots)
         if with_slots:  # for the fused append: each sequence's last page id
             last_page = indices[np.clip(indptr[1:] - 1, 0, n_pages - 1)]
         use_prefill = bool((ql > 1).any())
@@ -726,6 +956,24 @@ class MI355XBackend:
         self._planned = p
         self.n_plans += 1
         return p
+
+    @staticmethod
+    def _host_index(meta: BatchMeta, with_slots: bool) -> tuple:
+        """The meta's index fields on the host: query_lens, cu_query_lens,
+        kv_lens, kv_indptr, kv_last_page_len, kv_indices and, if asked for,
+        slot_mapping (else None)."""
+        names = ["query_lens", "cu_query_lens", "kv_lens", "kv_indptr", "kv_last_page_len",
+                 "kv_indices"] + ["slot_mapping"] * with_slots
+        mirror = meta.host_arrays()
+        if mirror is not None:
+            # the assembler's own host arrays: no device read-back
+            out = [mirror[k] for k in names]
+        else:
+            # ONE device->host transfer for everything the host plan reads.
+            parts = [getattr(meta, k).reshape(-1).to(torch.int64) for k in names]
+            host = torch.cat(parts).cpu().numpy()
+            out = np.split(host, np.cumsum([t.shape[0] for t in parts])[:-1])
+        return (*out, *[None] * (not with_slots))
 
     def _describe(self, p: _Plan) -> int:
         """Address of the plan's ``pkv_batch``: the arguments its launches share,
@@ -828,7 +1076,7 @@ class MI355XBackend:
         self._flush()
         self._planned = None
         self._slot_cache = None
-        self._rows = None
+        self._rows = self._selected = None
 
     # -- misc -------------------------------------------------------------------------
 
@@ -836,6 +1084,8 @@ class MI355XBackend:
         """Zero every pool and drop the plan. Tests only."""
         self._pending = None
         self._pool.zero_()
+        if self._bounds is not None:
+            self._bounds.zero_()
         self.invalidate_plan()
 
     def __repr__(self) -> str:

@@ -186,14 +186,31 @@ template <typename T, int D, int G> struct PieceLds {
   static_assert(4 * 64 * 16 * PartLayout<D, G>::NGR <= V, "the merge's weights fit");
 };
 
-template <typename T, int D, int G>
+// Pieces of the pages chosen for each sequence and KV head (selection.hip)
+// instead of a plan's: nothing of them is known on the host but their number,
+// so a piece's item follows from the sequence's length, by the plan's cut.
+struct Chosen {
+  const int32_t* ids;       // [n_seqs][n_kv_heads][width], a list's pages in order
+  const int32_t* kv_lens;
+  int32_t width, pages, part_pages, max_parts, n_seqs;
+};
+
+// Pieces of np pages, and the folded remainder.
+__host__ __device__ static inline int n_pieces(int np, int part, bool* fold) {
+  const int full = np / part, rem = np % part;
+  const int least = kMinTail < (part + 1) / 2 ? kMinTail : (part + 1) / 2;
+  *fold = full > 0 && rem > 0 && rem < least;
+  return full + (rem > 0 && !*fold ? 1 : 0);
+}
+
+template <typename T, int D, int G, bool CHOSEN = false>
 __device__ __forceinline__ void decode_piece(
     unsigned char* smem, int h, int bin,
     const T* __restrict__ q, T* __restrict__ out, T* __restrict__ kpool, T* __restrict__ vpool,
     int64_t num_blocks, const int32_t* __restrict__ plan, int32_t stride, int32_t n_kv_heads,
     float scale_log2, const T* __restrict__ k_new, const T* __restrict__ v_new,
     const int32_t* __restrict__ slot_mapping, float* part_o, float* part_ml, uint32_t o_bytes,
-    uint32_t ml_bytes, int32_t* counters, int32_t* status) {
+    uint32_t ml_bytes, int32_t* counters, int32_t* status, const Chosen& ch = Chosen{}) {
 #pragma clang fp contract(off)
   typedef typename Mma<T>::vec8 vec8;
   typedef typename Mma<T>::vec4 vec4;
@@ -231,18 +248,49 @@ __device__ __forceinline__ void decode_piece(
   // One item where the launch follows few_pieces; any plan is served. (The
   // count, the item and its words come in one round trip; the slot below a
   // bin's last item still lies inside its plan block.)
-  const int n_items = bp[0];
+  const int n_items = CHOSEN ? 1 : bp[0];
   int p0 = 0;
   for (int item = 0;; ++item) {
-    const int32_t* it = bp + stride - (int64_t)(item + 1) * kItemInts;
-    const int seq = it[0], np = it[1], tok0 = it[2], kv = it[3], slot = it[4], nparts = it[5],
-              slot0 = it[6];
-    const int row = it[7] >> kRowShift;
-    const bool fuse = k_new != nullptr && (it[7] & kItemLast);
-    // the first chunk's page words, word i in lane i (reads past the bin's
-    // words stay inside the plan: kPlanTail)
-    int wd = words[p0 + lane];
-    asm volatile("" ::"s"(seq), "s"(np), "s"(kv), "s"(it[7]), "s"(n_items));
+    int seq, np, tok0, kv, slot, nparts, slot0, row, flags = 0;
+    if constexpr (CHOSEN) {
+      if (item > 0) break;
+      seq = row = bin / ch.max_parts;
+      const int p = bin - seq * ch.max_parts;
+      const int len = max(ch.kv_lens[seq], 1), all = (len + PS - 1) / PS;
+      const int n = min(min(all, ch.pages), ch.width), part = ch.part_pages;
+      bool fold;
+      nparts = n_pieces(n, part, &fold);
+      if (p >= nparts) break;
+      const int full = n / part;
+      np = p < full ? part + (fold && p + 1 == full ? n % part : 0) : n % part;
+      tok0 = p * part * PS;
+      kv = len - (all - n) * PS;     // of the chosen pages, the last page last
+      slot0 = nparts > 1 ? seq * ch.max_parts : -1;
+      slot = nparts > 1 ? slot0 + p : -1;
+    } else {
+      const int32_t* it = bp + stride - (int64_t)(item + 1) * kItemInts;
+      seq = it[0], np = it[1], tok0 = it[2], kv = it[3], slot = it[4], nparts = it[5],
+      slot0 = it[6];
+      flags = it[7];
+      row = flags >> kRowShift;
+    }
+    const bool fuse = k_new != nullptr && (flags & kItemLast);
+    // a chunk's page words, word i in lane i (reads past the bin's words stay
+    // inside the plan: kPlanTail)
+    auto page_words = [&](int c0) __attribute__((always_inline)) {
+      if constexpr (CHOSEN) {
+        const int i = tok0 / PS + c0 + lane;   // of the chosen list
+        const int id = c0 + lane < np ? ch.ids[((int64_t)seq * n_kv_heads + h) * ch.width + i] : 0;
+        const bool out_of = id < 0 || (int64_t)id >= num_blocks;
+        const int live = min(PS, kv - i * PS);
+        return (int)((uint32_t)(out_of ? 0 : id) | ((uint32_t)(live - 1) & 15u) << kPageIdBits |
+                     (out_of ? 0x80000000u : 0u));
+      } else {
+        return words[p0 + c0 + lane];
+      }
+    };
+    int wd = page_words(0);
+    asm volatile("" ::"s"(seq), "s"(np), "s"(kv), "s"(flags), "s"(n_items));
     if (item >= n_items) break;
 
     // Q^T, the QK B operand (column n = query head h*G + n, zero beyond G)
@@ -281,7 +329,7 @@ __device__ __forceinline__ void decode_piece(
     bool bad = false;
     for (int c0 = 0; c0 < np; c0 += CH) {
       const int cn = min(CH, np - c0);
-      if (c0 > 0) wd = words[p0 + c0 + lane];
+      if (c0 > 0) wd = page_words(c0);
       bad |= lane < cn && wd < 0;   // an id outside the pool: the plan put page 0
       // This wave's pages c0 + 4 i + wave: K into registers, lane (row n, g)
       // its chunks 4 c + g, V into LDS. Only rows below kv_len are inside a

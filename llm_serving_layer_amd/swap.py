@@ -221,6 +221,8 @@ class KVSwapSpace:
                                            staging.data_ptr(), b._status.data_ptr(),
                                            side.cuda_stream)
             _native.check(rc, "swap_in scatter")
+            if getattr(b, "_bounds", None) is not None:
+                b._renew_bounds(ids, nb, side.cuda_stream)
             ids.record_stream(side)
             staging.record_stream(side)
         main.wait_stream(side)

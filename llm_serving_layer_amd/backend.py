@@ -59,6 +59,8 @@ _DTYPES = {torch.float16: _native.DTYPE_F16, torch.bfloat16: _native.DTYPE_BF16,
            torch.float32: _native.DTYPE_F32}
 
 MAX_PART_PAGES = 64      # a partition's page ids are read by one wavefront
+SHARED_MIN_PAGES = 4     # shorter runs of shared pages stay each sequence's own
+SHARED_TILES = 512       # workgroups that share the work on a batch's shared pages
 DEFAULT_Q_TILE = 64      # prefill tile when the geometry has no matrix-core kernel
 
 
@@ -188,6 +190,14 @@ class _Rows:
     __slots__ = ("meta", "slots", "positions", "far", "complete", "buffers", "stream")
 
 
+class _Shared:
+    """What ``attend_shared`` keeps for one BatchMeta: None where nothing is
+    worth sharing (``n_tiles`` 0: the batch takes ``attend``)."""
+
+    __slots__ = ("meta", "n", "n_tiles", "tiles", "plan", "indices", "slots", "n_work", "n_slots",
+                 "stride", "ws", "fusable", "buffers", "stream")
+
+
 class _Selected:
     """What ``attend_selected`` keeps for one BatchMeta and page budget."""
 
@@ -200,6 +210,7 @@ class MI355XBackend:
 
     _rows: _Rows | None = None
     _selected: _Selected | None = None
+    _shared: _Shared | None = None
     _bounds: torch.Tensor | None = None
 
     def __init__(self, num_layers: int, num_blocks: int, block_size: int, n_kv_heads: int,
@@ -744,6 +755,125 @@ class MI355XBackend:
             _native.check(rc, "attend (prefill)" if p.use_prefill else "attend (decode)")
         return out
 
+    def attend_shared(self, q: torch.Tensor, layer_idx: int, scale: float,
+                      meta: BatchMeta) -> torch.Tensor:
+        """
+        ``attend`` for a decode batch whose sequences begin with the same
+        pages (a system prompt, a document, the branches of a search): the
+        shared pages, found by their ids in the page lists, are read once for
+        all the sequences that begin with them, and so are the pages that some
+        of those share further on. The result is ``attend``'s up to rounding,
+        and depends, in its last bits, on what shares the batch.
+
+        Batches with prompt chunks, geometries without the fast decode path, a
+        scale that is not positive and batches that share too little to gain
+        by it run ``attend`` itself. Graphs captured with one meta share its
+        buffers, so their replays must not overlap.
+        """
+        if layer_idx is None or not 0 <= layer_idx < self.num_layers:
+            self._check_layer(layer_idx)
+        tokens = q.shape[0]
+        if q.shape != (tokens, self.n_heads, self.head_dim):
+            raise ValueError(f"q has shape {tuple(q.shape)}, expected "
+                             f"({tokens}, {self.n_heads}, {self.head_dim})")
+        if meta.n_tokens != tokens:
+            raise ValueError(f"meta describes {meta.n_tokens} tokens but q has {tokens}")
+        p = self._shared
+        if p is None or p.meta is not meta:
+            p = self._plan_shared(meta)
+        if not p.n_tiles or not float(scale) > 0:
+            return self.attend(q, layer_idx, scale, meta)
+        pend = self._pending
+        fused = (pend is not None and pend.layer == layer_idx and pend.meta is meta
+                 and pend.stream == _current_stream(self.device) and p.fusable)
+        if fused:
+            self._check_pending_intact(pend)
+            self._pending = None
+        elif pend is not None:
+            self._flush()
+        stream = self._enter(p)
+        q = self._as_pool(q)
+        if q.data_ptr() % 16:
+            q = q.clone()
+        out = torch.empty_like(q)
+        with self._on_device():
+            rc = self._lib.pkv_attend_shared(
+                q.data_ptr(), out.data_ptr(), self._k_ptr[layer_idx], self._v_ptr[layer_idx],
+                self.num_blocks, p.indices.data_ptr(), p.n, self.n_heads, self.n_kv_heads,
+                self.head_dim, self.block_size, float(scale), self._code, p.tiles.data_ptr(),
+                p.n_tiles, p.plan.data_ptr(), p.n_work, p.n_slots, p.stride,
+                pend.k.data_ptr() if fused else None, pend.v.data_ptr() if fused else None,
+                p.slots.data_ptr() if fused else None, p.ws.data_ptr(), p.ws.numel(),
+                self._status_ptr, stream)
+        if rc:
+            _native.check(rc, "attend_shared")
+        self.n_runs += 1
+        return out
+
+    def _plan_shared(self, meta: BatchMeta) -> _Shared:
+        n = meta.n_seqs
+        with_slots = (meta.slot_mapping is not None and meta.slot_mapping.shape[0] == n
+                      and meta.kv_indices.shape[0] > 0)
+        ql, cu, kvl, indptr, last, indices, slots = self._host_index(meta, with_slots)
+        p = _Shared()
+        p.n, p.n_tiles, p.buffers = n, 0, []
+        if self._split_mixed and n > 1 and not (ql != 1).any() and n == meta.n_tokens:
+            self._check_pages(kvl, indptr, last, int(indices.shape[0]))
+            self._fill_shared(p, meta, *(np.ascontiguousarray(a, dtype=np.int32)
+                                         for a in (indptr, indices, kvl, last)))
+            # (as for attend: each new row at the end of its own page list)
+            p.fusable = with_slots and bool(
+                (slots == indices[indptr[1:] - 1] * self.block_size + last - 1).all())
+        p.stream = _current_stream(self.device)
+        p.meta = meta
+        self._shared = p
+        return p
+
+    def _fill_shared(self, p: _Shared, meta: BatchMeta, indptr, indices, kvl, last) -> None:
+        """Plan the batch's shared runs and own pages (pkv_plan_shared)."""
+        ptr = lambda a: a.ctypes.data  # noqa: E731
+        n_work, n_slots, stride, n_tiles = (C.c_int32() for _ in range(4))
+        needed, tiles_needed = C.c_int64(), C.c_int64()
+        cap = 10 * self._decode_wgs + 2 * int(indptr[-1]) + 24 * p.n + 128
+        tiles_cap = 8 * SHARED_TILES + 16 * p.n
+        part = self.part_pages
+        while True:
+            for _ in range(3):
+                buf, tiles = np.empty(cap, np.int32), np.empty(tiles_cap, np.int32)
+                rc = self._lib.pkv_plan_shared(
+                    ptr(indptr), ptr(indices), ptr(kvl), ptr(last), p.n, self.block_size,
+                    self.num_blocks, self.n_heads, self.n_kv_heads, part, self._decode_wgs,
+                    SHARED_MIN_PAGES, SHARED_TILES, ptr(buf), cap, C.byref(needed),
+                    C.byref(n_work), C.byref(n_slots), C.byref(stride), ptr(tiles), tiles_cap,
+                    C.byref(tiles_needed), C.byref(n_tiles))
+                if rc != _native.ERR_CAPACITY or (needed.value <= cap
+                                                  and tiles_needed.value <= tiles_cap):
+                    break
+                cap, tiles_cap = max(cap, needed.value), max(tiles_cap, tiles_needed.value)
+            _native.check(rc, "plan (shared)")
+            need = self._lib.pkv_decode_workspace_bytes(p.n, n_slots.value, self.n_heads,
+                                                        self.n_kv_heads, self.head_dim)
+            if need < 2**31 or part >= MAX_PART_PAGES:
+                break
+            part = min(2 * part, MAX_PART_PAGES)
+        if not n_tiles.value or need >= 2**31:
+            return
+        p.n_tiles, p.n_work, p.n_slots = n_tiles.value, n_work.value, n_slots.value
+        p.stride = stride.value
+        p.plan = self._upload(buf[:needed.value])
+        p.tiles = self._upload(tiles[:tiles_needed.value])
+        p.indices = self._dev_i32(meta.kv_indices)
+        p.slots = self._dev_i32(meta.slot_mapping) if meta.slot_mapping is not None else None
+        p.ws = self._counted_workspace(need, p.n)
+        p.buffers = [t for t in (p.plan, p.tiles, p.indices, p.slots, p.ws) if t is not None]
+        self.n_plans += 1
+
+    def _counted_workspace(self, need: int, n: int) -> torch.Tensor:
+        """A workspace whose arrival counters (at its front) are zero."""
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        ws[:4 * n * self.n_kv_heads].zero_()
+        return ws
+
     def attend_selected(self, q: torch.Tensor, layer_idx: int, scale: float, meta: BatchMeta,
                         pages: int, return_pages: bool = False):
         """
@@ -836,7 +966,7 @@ class MI355XBackend:
             if need < 2**31 or p.part >= MAX_PART_PAGES:
                 break
             p.part = min(2 * p.part, MAX_PART_PAGES)
-        p.ws = torch.zeros(need, dtype=torch.uint8, **dev)
+        p.ws = self._counted_workspace(need, n)
         p.buffers = [p.indptr, p.indices, p.kv_lens, p.scores, p.ids, p.ordinals, p.ws]
         p.stream = _current_stream(self.device)
         p.meta = meta
@@ -1076,7 +1206,7 @@ class MI355XBackend:
         self._flush()
         self._planned = None
         self._slot_cache = None
-        self._rows = self._selected = None
+        self._rows = self._selected = self._shared = None
 
     # -- misc -------------------------------------------------------------------------
 

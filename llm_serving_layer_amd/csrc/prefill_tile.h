@@ -67,14 +67,26 @@ template <typename T, int D> struct PrefillLds {
   static constexpr int LPT = TILE / 2 / 1024;          // wave loads of a page of one tensor
 };
 
-template <typename T, int D, int G>
+// A tile over pages that several one-token sequences share (shared.hip): its
+// rows are those sequences' queries, all of which see every key, and its
+// result is a partial (o, m, l) per sequence, in the decode kernels' layout.
+struct SharedTile {
+  const int32_t* items;      // {first page in kv_indices, pages, first member, members, split}
+  const int32_t* members;    // {row of q, sequence, partial slot of split 0, 0}
+  float* part_o;
+  float* part_ml;
+  int32_t* counters;
+};
+constexpr int kSharedItem = 8, kSharedMember = 4;   // ints of each
+
+template <typename T, int D, int G, bool SHARED = false>
 __device__ __forceinline__ void prefill_tile(
     unsigned char* smem, int block,
     const T* __restrict__ q, T* __restrict__ out, const T* __restrict__ kpool,
     const T* __restrict__ vpool, int64_t num_blocks, const int32_t* __restrict__ cu_q,
     const int32_t* __restrict__ kv_indptr, const int32_t* __restrict__ kv_indices,
     const int32_t* __restrict__ kv_lens, const int32_t* __restrict__ plan,
-    int32_t n_kv_heads, float scale_log2, int32_t* status) {
+    int32_t n_kv_heads, float scale_log2, int32_t* status, const SharedTile& sh = SharedTile{}) {
   typedef typename Mma<T>::vec8 vec8;
   typedef typename Mma<T>::vec4 vec4;
   typedef PrefillLds<T, D> L;
@@ -98,15 +110,30 @@ __device__ __forceinline__ void prefill_tile(
   const int n = lane & 31, g = lane >> 5;
   const int item = block / n_kv_heads;
   const int h = block - item * n_kv_heads;
-  const int seq = plan[4 * item], qs = plan[4 * item + 1], qn = plan[4 * item + 2];
-  const int q0 = cu_q[seq];
-  const int q_len = cu_q[seq + 1] - q0;
-  const int kv_len = kv_lens[seq];
-  const int pbase = kv_indptr[seq];
+  int qs = 0, qn, q0 = 0, kv_len, pbase, base_pos;
+  const int32_t* members = nullptr;
+  int split = 0;
+  if constexpr (SHARED) {
+    const int32_t* it = sh.items + (int64_t)item * kSharedItem;
+    pbase = it[0];
+    kv_len = it[1] * PS;
+    members = sh.members + (int64_t)it[2] * kSharedMember;
+    qn = it[3];
+    split = it[4];
+    base_pos = kv_len - 1;      // every row sees every key
+  } else {
+    const int seq = plan[4 * item];
+    qs = plan[4 * item + 1];
+    qn = plan[4 * item + 2];
+    q0 = cu_q[seq];
+    const int q_len = cu_q[seq + 1] - q0;
+    kv_len = kv_lens[seq];
+    pbase = kv_indptr[seq];
+    base_pos = kv_len - q_len + qs;
+  }
   const int Hq = n_kv_heads * G;
   const int64_t row = (int64_t)n_kv_heads * D;
-  const int base_pos = kv_len - q_len + qs;
-  const int kv_end = base_pos + qn;
+  const int kv_end = SHARED ? kv_len : base_pos + qn;
   const int ntiles = (kv_end + TT - 1) / TT;
 
   // This lane's query row (column n of every 32x32 tile) and Q^T as the B
@@ -114,10 +141,12 @@ __device__ __forceinline__ void prefill_tile(
   const int r = wave * 32 + n;
   const int tok = r / G;
   const bool valid = tok < qn;
-  const int qpos = valid ? base_pos + tok : kv_len - 1;
+  const int qpos = valid && !SHARED ? base_pos + tok : kv_len - 1;
   vec8 qb[NC];
   {
-    const T* qr = q + ((int64_t)(q0 + qs + (valid ? tok : 0)) * Hq + h * G + r % G) * D + g * 8;
+    int token = q0 + qs + (valid ? tok : 0);
+    if constexpr (SHARED) token = members[(valid ? tok : 0) * kSharedMember];
+    const T* qr = q + ((int64_t)token * Hq + h * G + r % G) * D + g * 8;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const vec8 t = *reinterpret_cast<const vec8*>(qr + c * 16);
@@ -359,6 +388,29 @@ __device__ __forceinline__ void prefill_tile(
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
   l_run = sum_x32(l_run);
+  if constexpr (SHARED) {
+    // the partial of the row's sequence and head; its arrival is counted with
+    // a head's first row (the launch's end orders the stores before the merge)
+    if (valid) {
+      constexpr int NDB = D / 16, FLOATS = (G + 3) / 4 * NDB * 64;
+      const int hd = r % G;
+      const int32_t* mb = members + tok * kSharedMember;
+      const int64_t slot = mb[2] + split;
+      float* po = sh.part_o + (slot * n_kv_heads + h) * FLOATS + (hd / 4) * NDB * 64 + (hd & 3);
+#pragma unroll
+      for (int dh = 0; dh < NDH; ++dh) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) po[(32 * dh + 8 * (j >> 2) + 4 * g + (j & 3)) * 4] = o[dh][j];
+      }
+      if (g == 0) {
+        float* ml = sh.part_ml + (slot * Hq + h * G + hd) * 2;
+        ml[0] = m_run;
+        ml[1] = l_run;
+        if (hd == 0) atomicAdd(sh.counters + (int64_t)mb[1] * n_kv_heads + h, 1);
+      }
+    }
+    return;
+  }
   if (valid) {
     const float inv = 1.f / l_run;
     T* orow = out + ((int64_t)(q0 + qs + tok) * Hq + h * G + r % G) * D + 4 * g;

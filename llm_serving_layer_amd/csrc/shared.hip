@@ -1,0 +1,295 @@
+// Decode attention for sequences that begin with the same pages: each shared
+// run of pages is read once for all of them instead of once each.
+//
+// A softmax over a sequence's keys splits over any partition of them: part j
+// leaves m_j = max s, l_j = sum e^(s - m_j), o_j = sum e^(s - m_j) v, and the
+// whole is sum_j w_j o_j / sum_j w_j l_j, w_j = e^(m_j - max m). Page lists that
+// begin alike form a tree; each of its inner runs is one part of every sequence
+// below it, and its own pages are the sequence's last part (its last page
+// always is its own, so every sequence has one).
+//  * shared_kernel takes a run: the queries of the sequences that share it are
+//    the 128 rows of a prefill tile (prefill_tile.h), so a tile of K and V
+//    loaded once serves 128 / G sequences on the matrix cores. Long runs are
+//    split over workgroups. Its parts go to the decode kernels' partial slots,
+//    with their arrival counts.
+//  * the decode kernels take the own pages as pieces of cut sequences, with the
+//    shared parts counted among each sequence's pieces: whichever piece comes
+//    last merges all of them.
+#include <algorithm>
+#include <numeric>
+#include <vector>
+
+#include "decode_piece.h"
+#include "prefill_tile.h"
+
+namespace pkv {
+
+template <typename T, int D, int G>
+__global__ __launch_bounds__(kPrefillThreads) void shared_kernel(
+    const T* __restrict__ q, const T* __restrict__ kpool, const T* __restrict__ vpool,
+    int64_t num_blocks, const int32_t* __restrict__ kv_indices, int32_t n_kv_heads,
+    float scale_log2, SharedTile sh, int32_t* status) {
+  __shared__ __align__(16) unsigned char smem[PrefillLds<T, D>::BYTES];
+  prefill_tile<T, D, G, true>(smem, blockIdx.x, q, nullptr, kpool, vpool, num_blocks, nullptr,
+                              nullptr, kv_indices, nullptr, nullptr, n_kv_heads, scale_log2,
+                              status, sh);
+}
+
+struct SharedArgs {
+  const void* q; const void* kp; const void* vp; int64_t nb; const int32_t* indices;
+  int32_t Hkv; float sl2; SharedTile sh; int32_t n_tiles; int32_t* status;
+};
+
+template <typename T, int D, int G>
+static void launch_shared(const SharedArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((shared_kernel<T, D, G>), dim3((unsigned)(a.n_tiles * a.Hkv)),
+                     dim3(kPrefillThreads), 0, s, (const T*)a.q, (const T*)a.kp, (const T*)a.vp,
+                     a.nb, a.indices, a.Hkv, a.sl2, a.sh, a.status);
+}
+
+typedef void (*SharedFn)(const SharedArgs&, hipStream_t);
+
+template <typename T, int D>
+static SharedFn shared_g(int G) {
+  switch (G) {
+    case 1: return launch_shared<T, D, 1>;
+    case 2: return launch_shared<T, D, 2>;
+    case 4: return launch_shared<T, D, 4>;
+    case 8: return launch_shared<T, D, 8>;
+    case 16: return launch_shared<T, D, 16>;
+    default: return nullptr;
+  }
+}
+
+static SharedFn shared_fn(int32_t dtype, int32_t D, int32_t G) {
+  if (dtype == PKV_DTYPE_F16)
+    return D == 64 ? shared_g<_Float16, 64>(G) : D == 128 ? shared_g<_Float16, 128>(G) : nullptr;
+  if (dtype == PKV_DTYPE_BF16)
+    return D == 64 ? shared_g<__bf16, 64>(G) : D == 128 ? shared_g<__bf16, 128>(G) : nullptr;
+  return nullptr;
+}
+
+int check_geometry(int32_t Hq, int32_t Hkv, int32_t D, int32_t ps, int32_t dtype);
+int check_seq_pages(int32_t i, int32_t np, int32_t kv, int32_t last, int32_t ps);
+int split_workspace(void* workspace, int64_t workspace_bytes, int32_t n_seqs, int32_t n_slots,
+                    int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, DecodeWorkspace* w);
+
+namespace {
+
+// A run of pages [first, last) of the members' lists, which they share.
+struct Run {
+  int32_t first, last;
+  std::vector<int32_t> members;
+};
+
+// The runs of the tree of page lists, of at least min_pages pages and two
+// members; `own` marks per kv_indices entry the pages that stay a sequence's own.
+struct Tree {
+  const int32_t* indptr;
+  const int32_t* indices;
+  int32_t min_pages;
+  std::vector<Run> runs;
+  std::vector<char> own;
+
+  int32_t room(int32_t i) const { return indptr[i + 1] - indptr[i] - 1; }   // the last page is own
+  int32_t page(int32_t i, int32_t p) const { return indices[indptr[i] + p]; }
+
+  void grow(int32_t n_seqs) {
+    own.assign(indptr[n_seqs], 1);
+    std::vector<Run> open(1);   // runs whose members may share more pages behind them
+    open[0].first = open[0].last = 0;
+    open[0].members.resize(n_seqs);
+    std::iota(open[0].members.begin(), open[0].members.end(), 0);
+    while (!open.empty()) {
+      const Run run = std::move(open.back());
+      open.pop_back();
+      const int32_t at = run.last;
+      std::vector<int32_t> m;
+      for (int32_t i : run.members)
+        if (room(i) > at) m.push_back(i);
+      std::stable_sort(m.begin(), m.end(),
+                       [&](int32_t a, int32_t b) { return page(a, at) < page(b, at); });
+      for (size_t a = 0, b; a < m.size(); a = b) {
+        for (b = a + 1; b < m.size() && page(m[b], at) == page(m[a], at);) ++b;
+        if (b - a < 2) continue;
+        const int32_t* lead = indices + indptr[m[a]];
+        int32_t end = room(m[a]);
+        for (size_t j = a + 1; j < b; ++j) {
+          const int32_t* mine = indices + indptr[m[j]];
+          end = std::min(end, room(m[j]));
+          end = (int32_t)(std::mismatch(lead + at, lead + end, mine + at).first - lead);
+        }
+        Run child{at, end, std::vector<int32_t>(m.begin() + a, m.begin() + b)};
+        if (end - at >= min_pages) {
+          for (int32_t i : child.members)
+            std::fill(own.begin() + indptr[i] + at, own.begin() + indptr[i] + end, 0);
+          runs.push_back(child);
+        }
+        open.push_back(std::move(child));
+      }
+    }
+  }
+};
+
+}  // namespace
+}  // namespace pkv
+
+using namespace pkv;
+
+extern "C" int pkv_plan_shared(const int32_t* kv_indptr, const int32_t* kv_indices,
+                               const int32_t* kv_lens, const int32_t* kv_last_page_len,
+                               int32_t n_seqs, int32_t page_size, int64_t num_blocks,
+                               int32_t n_heads, int32_t n_kv_heads, int32_t part_pages,
+                               int32_t max_workgroups, int32_t min_pages, int32_t tile_target,
+                               int32_t* plan, int64_t plan_capacity, int64_t* plan_needed,
+                               int32_t* n_work_out, int32_t* n_slots_out,
+                               int32_t* plan_stride_out, int32_t* tiles, int64_t tiles_capacity,
+                               int64_t* tiles_needed, int32_t* n_tiles_out) {
+  if (n_seqs <= 0 || page_size <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads)
+    return fail(PKV_ERR_INVALID, "n_seqs, page_size and heads must be positive, n_heads a "
+                "multiple of n_kv_heads");
+  const int32_t G = n_heads / n_kv_heads;
+  if (G > kPrefillRows || kPrefillRows % G || min_pages < 1 || tile_target < 1)
+    return fail(PKV_ERR_INVALID, "%d query heads a KV head, min_pages=%d or tile_target=%d is "
+                "not supported", G, min_pages, tile_target);
+  if (kv_indptr[0] != 0) return fail(PKV_ERR_INVALID, "kv_indptr must start at 0");
+  for (int32_t i = 0; i < n_seqs; ++i) {
+    const int rc = check_seq_pages(i, kv_indptr[i + 1] - kv_indptr[i], kv_lens[i],
+                                   kv_last_page_len[i], page_size);
+    if (rc) return rc;
+  }
+  Tree tree{kv_indptr, kv_indices, min_pages, {}, {}};
+  tree.grow(n_seqs);
+
+  // The own pages as a batch of their own, planned by pkv_plan_decode. (Only
+  // the number of a sequence's keys matters to a one-token query, not where
+  // they stand, so its own pages count from 0.)
+  std::vector<int32_t> ptr(n_seqs + 1, 0), ids, lens(n_seqs);
+  ids.reserve(kv_indptr[n_seqs]);
+  for (int32_t i = 0; i < n_seqs; ++i) {
+    for (int32_t p = kv_indptr[i]; p < kv_indptr[i + 1]; ++p)
+      if (tree.own[p]) ids.push_back(kv_indices[p]);
+    ptr[i + 1] = (int32_t)ids.size();
+    lens[i] = (ptr[i + 1] - ptr[i] - 1) * page_size + kv_last_page_len[i];
+  }
+  int32_t n_work = 0, own_slots = 0, stride = 0;
+  int64_t need = 0;
+  int rc = pkv_plan_decode(ptr.data(), ids.data(), lens.data(), kv_last_page_len, n_seqs, page_size,
+                           num_blocks, n_kv_heads, part_pages, max_workgroups, plan, plan_capacity,
+                           &need, &n_work, &own_slots, &stride);
+  if (plan_needed) *plan_needed = need;
+  if (rc) return rc;
+
+  // Runs in splits of `split` pages (an even number: a tile's step is two
+  // pages), so that about tile_target workgroups share the work.
+  const int32_t per_tile = kPrefillRows / G;
+  int64_t steps = 0;   // pages times row tiles, over all runs
+  for (const Run& r : tree.runs)
+    steps += (int64_t)(r.last - r.first) * ((r.members.size() + per_tile - 1) / per_tile);
+  const int64_t target = std::max<int64_t>(1, tile_target / n_kv_heads);
+  const int32_t split = (int32_t)std::max<int64_t>(8, ((steps + target - 1) / target + 1) / 2 * 2);
+  std::vector<int32_t> shared(n_seqs, 0);   // shared parts of each sequence
+  int64_t n_tiles = 0, n_members = 0;
+  for (const Run& r : tree.runs) {
+    const int32_t splits = (r.last - r.first + split - 1) / split;
+    n_tiles += splits * (int64_t)((r.members.size() + per_tile - 1) / per_tile);
+    n_members += (int64_t)r.members.size();
+    for (int32_t i : r.members) shared[i] += splits;
+  }
+  const int64_t want = n_tiles * kSharedItem + n_members * kSharedMember;
+  if (tiles_needed) *tiles_needed = want;
+  if (want > tiles_capacity || n_tiles * n_kv_heads > 0x7fffffffLL)
+    return fail(PKV_ERR_CAPACITY, "shared tiles need %lld entries, capacity %lld",
+                (long long)want, (long long)tiles_capacity);
+
+  // Partial slots: a sequence's shared parts, then its own pieces.
+  std::vector<int32_t> pieces(n_seqs, 1), base(n_seqs + 1, 0);
+  const int64_t bins = n_work / (n_kv_heads / heads_per_wg(n_kv_heads));
+  auto each_item = [&](auto&& f) {
+    for (int64_t b = 0; b < bins; ++b)
+      for (int32_t j = 0; j < plan[b * stride]; ++j)
+        f(plan + (b + 1) * stride - (int64_t)(j + 1) * kItemInts);
+  };
+  each_item([&](int32_t* it) { pieces[it[0]] = it[4] < 0 ? 1 : it[5]; });
+  for (int32_t i = 0; i < n_seqs; ++i) {
+    const int32_t parts = shared[i] + pieces[i];
+    base[i + 1] = base[i] + (parts > 1 ? parts : 0);
+  }
+  each_item([&](int32_t* it) {
+    const int32_t i = it[0], parts = shared[i] + pieces[i];
+    if (parts < 2) return;
+    const int32_t ord = it[4] < 0 ? 0 : it[4] - it[6];
+    it[4] = base[i] + shared[i] + ord;
+    it[5] = parts;
+    it[6] = base[i];
+  });
+
+  // Tiles, longest first; a run's members in order, 128 / G of them a tile.
+  int32_t* item = tiles;
+  int32_t* member = tiles + n_tiles * kSharedItem;
+  int32_t at = 0;
+  std::vector<int32_t> next(base.begin(), base.end() - 1);   // each sequence's next shared slot
+  for (const Run& r : tree.runs) {
+    const int32_t splits = (r.last - r.first + split - 1) / split, n = (int32_t)r.members.size();
+    for (int32_t s = 0; s < splits; ++s) {
+      const int32_t first = r.first + s * split, pages = std::min(split, r.last - first);
+      for (int32_t m = 0; m < n; m += per_tile) {
+        const int32_t vals[kSharedItem] = {kv_indptr[r.members[0]] + first, pages, at + m,
+                                           std::min(per_tile, n - m), s, 0, 0, 0};
+        item = std::copy(vals, vals + kSharedItem, item);
+      }
+    }
+    for (int32_t i : r.members) {
+      const int32_t vals[kSharedMember] = {i, i, next[i], 0};
+      member = std::copy(vals, vals + kSharedMember, member);
+      next[i] += splits;
+    }
+    at += n;
+  }
+  *n_work_out = n_work;
+  *n_slots_out = base[n_seqs];
+  *plan_stride_out = stride;
+  *n_tiles_out = (int32_t)n_tiles;
+  return PKV_OK;
+}
+
+extern "C" int pkv_attend_shared(const void* q, void* out, void* k_pool, void* v_pool,
+                                 int64_t num_blocks, const int32_t* kv_indices, int32_t n_seqs,
+                                 int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                                 int32_t page_size, float scale, int32_t dtype,
+                                 const int32_t* tiles, int32_t n_tiles, const int32_t* plan,
+                                 int32_t n_work, int32_t n_slots, int32_t plan_stride,
+                                 const void* k_new, const void* v_new,
+                                 const int32_t* slot_mapping, void* workspace,
+                                 int64_t workspace_bytes, int32_t* status_word, void* stream) {
+  int rc = check_geometry(n_heads, n_kv_heads, head_dim, page_size, dtype);
+  if (rc) return rc;
+  if (n_seqs <= 0) return PKV_OK;
+  const int32_t G = n_heads / n_kv_heads;
+  SharedFn fn = page_size == 16 ? shared_fn(dtype, head_dim, G) : nullptr;
+  if (!fn || !pkv_decode_fast_path(n_heads, n_kv_heads, head_dim, page_size, dtype, 1))
+    return fail(PKV_ERR_INVALID, "shared pages need the fast decode path (see "
+                "pkv_decode_fast_path)");
+  if (!(scale > 0.f)) return fail(PKV_ERR_INVALID, "shared pages need a positive scale");
+  if (!q || !out || !k_pool || !v_pool) return fail(PKV_ERR_INVALID, "null pointer argument");
+  const uintptr_t al = (uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool |
+                       (uintptr_t)k_new | (uintptr_t)v_new;
+  if (al % 16) return fail(PKV_ERR_INVALID, "q, out, pools and new rows must be 16-byte aligned");
+  if (n_tiles > 0) {
+    if (!kv_indices || !tiles || n_slots <= 0)
+      return fail(PKV_ERR_INVALID, "shared tiles need kv_indices, tiles and partial slots");
+    DecodeWorkspace w;
+    rc = split_workspace(workspace, workspace_bytes, n_seqs, n_slots, n_heads, n_kv_heads,
+                         head_dim, &w);
+    if (rc) return rc;
+    SharedArgs a{q, k_pool, v_pool, num_blocks, kv_indices, n_kv_heads, scale * kLog2e,
+                 {tiles, tiles + (int64_t)n_tiles * kSharedItem, w.part_o, w.part_ml, w.counters},
+                 n_tiles, status_word};
+    fn(a, (hipStream_t)stream);
+    PKV_LAUNCH_CHECK();
+  }
+  return pkv_attend_decode(q, out, k_pool, v_pool, num_blocks, nullptr, nullptr, nullptr, n_seqs,
+                           n_heads, n_kv_heads, head_dim, page_size, scale, dtype, plan, n_work,
+                           n_slots, plan_stride, k_new, v_new, slot_mapping, workspace,
+                           workspace_bytes, status_word, stream);
+}

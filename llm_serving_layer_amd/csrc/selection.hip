@@ -22,7 +22,8 @@ int check_geometry(int32_t Hq, int32_t Hkv, int32_t D, int32_t ps, int32_t dtype
 // ------------------------------------------------------------- page bounds ---
 // One workgroup a page and layer, one vector of V elements of the page's rows a
 // thread at a time, all rows of the page in a row. A NaN stays: it bounds nothing.
-template <typename T, int V>
+// PS rows a page, all of them in flight (0: page_size, one after another).
+template <typename T, int V, int PS>
 __global__ __launch_bounds__(256) void page_bounds_kernel(
     const char* __restrict__ k_pool, int64_t pool_step, char* __restrict__ lo,
     char* __restrict__ hi, int64_t bounds_step, int64_t num_blocks,
@@ -37,10 +38,8 @@ __global__ __launch_bounds__(256) void page_bounds_kernel(
   const vec* src = reinterpret_cast<const vec*>(k_pool + layer * pool_step) +
                    id * page_size * row_vecs;
   for (int c = threadIdx.x; c < row_vecs; c += blockDim.x) {
-    vec mn = src[c], mx = mn;
-#pragma unroll 16
-    for (int r = 1; r < page_size; ++r) {
-      const vec x = src[(int64_t)r * row_vecs + c];
+    vec mn, mx;
+    auto take = [&](const vec& x) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const float e = Elem<T>::to_f(x[i]);
@@ -48,6 +47,17 @@ __global__ __launch_bounds__(256) void page_bounds_kernel(
         if (nan || e < Elem<T>::to_f(mn[i])) mn[i] = x[i];
         if (nan || e > Elem<T>::to_f(mx[i])) mx[i] = x[i];
       }
+    };
+    if constexpr (PS > 0) {
+      vec x[PS];
+#pragma unroll
+      for (int r = 0; r < PS; ++r) x[r] = src[(int64_t)r * row_vecs + c];
+      mn = mx = x[0];
+#pragma unroll
+      for (int r = 1; r < PS; ++r) take(x[r]);
+    } else {
+      mn = mx = src[c];
+      for (int r = 1; r < page_size; ++r) take(src[(int64_t)r * row_vecs + c]);
     }
     reinterpret_cast<vec*>(lo + layer * bounds_step)[id * row_vecs + c] = mn;
     reinterpret_cast<vec*>(hi + layer * bounds_step)[id * row_vecs + c] = mx;
@@ -99,6 +109,139 @@ __global__ __launch_bounds__(64) void score_kernel(
     best = g == 0 || s > best || s != s ? s : best;
   }
   scores[((int64_t)seq * n_kv_heads + h) * stride + p] = best;
+}
+
+// The same for head dims of 64 and 128 and 1, 2, 4, 8 or 16 query heads a KV
+// head. A row of bounds is spread over D / V lanes, 16 bytes each, so loads are
+// whole lines and a wave takes 64 V / D pages at a step; a lane keeps its V
+// elements of up to GQ = 4 query heads in 64 bits. The bound's choice of lo or
+// hi is made in 32 bits, where it is one instruction: with the conversion and
+// the product that follow, 3 a query element, and 2 to unpack each element of
+// lo and hi. The row's sum over its lanes halves the query heads held with the
+// lanes left (each lane keeps half of what it has and adds its partner's), so
+// 4 heads over 16 lanes take 5 additions, not 16. More than 4 query heads are
+// split over the waves of a workgroup.
+constexpr int kScoreSteps = 4;   // page groups a wave has in flight
+
+template <int Mask> __device__ __forceinline__ double lane_xor(double v) {
+  return __builtin_bit_cast(double, __shfl_xor((unsigned long long)__builtin_bit_cast(
+                                                   unsigned long long, v), Mask));
+}
+
+template <typename T, int D, int G>
+struct ScoreShape {
+  static constexpr int V = 16 / (int)sizeof(T);
+  static constexpr int L = D / V;                 // lanes a page
+  static constexpr int GQ = G < 4 ? G : 4;        // query heads a wave
+  static constexpr int QW = G / GQ;               // waves that share a page
+  static constexpr int PW = 64 / L;               // pages of a wave's step
+  static constexpr int PAGES = 4 / QW * PW * kScoreSteps;   // of a workgroup
+};
+
+// The maximum over the heads of the sums over a page's L lanes of s[0 .. N - 1],
+// in every one of the page's lanes; NaN if one of them is.
+template <int N, int L> __device__ __forceinline__ double head_max(const double* s) {
+  auto larger = [](double a, double b) { return a != a || a > b ? a : b; };
+  if constexpr (L == 1) {
+    double m = s[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = larger(s[i], m);
+    return m;
+  } else if constexpr (N > 1) {
+    const bool up = threadIdx.x & (L / 2);
+    double t[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const double mine = up ? s[N / 2 + i] : s[i], other = up ? s[i] : s[N / 2 + i];
+      t[i] = mine + lane_xor<L / 2>(other);
+    }
+    const double m = head_max<N / 2, L / 2>(t);
+    return larger(lane_xor<L / 2>(m), m);
+  } else {
+    const double t[1] = {s[0] + lane_xor<L / 2>(s[0])};
+    return head_max<1, L / 2>(t);
+  }
+}
+
+template <typename T, int D, int G>
+__global__ __launch_bounds__(256) void score_rows_kernel(
+    const T* __restrict__ q, const T* __restrict__ lo, const T* __restrict__ hi,
+    int64_t num_blocks, const int32_t* __restrict__ kv_indptr,
+    const int32_t* __restrict__ kv_indices, const int32_t* __restrict__ kv_lens,
+    int32_t n_kv_heads, int32_t page_size, int32_t pages, int64_t stride,
+    double* __restrict__ scores, int32_t* status) {
+  typedef ScoreShape<T, D, G> S;
+  constexpr int V = S::V, L = S::L, GQ = S::GQ, PW = S::PW;
+  typedef T vec __attribute__((ext_vector_type(V)));
+  __shared__ double part[S::QW > 1 ? 4 * PW * kScoreSteps : 1];
+  const int h = blockIdx.x, seq = blockIdx.z;
+  const int np = seq_pages(kv_indptr, kv_lens, seq, page_size, stride);
+  const int n = np - 1;    // candidates; the last page is in
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int quad = wave % S::QW, group = wave / S::QW;
+  const int first = blockIdx.y * S::PAGES + group * (PW * kScoreSteps);
+  if (np <= pages || (int)blockIdx.y * S::PAGES >= n) return;
+  const int32_t* table = kv_indices + kv_indptr[seq];
+  const int c = lane % L;
+  int64_t at[kScoreSteps];
+#pragma unroll
+  for (int i = 0; i < kScoreSteps; ++i) {
+    const int p = first + i * PW + lane / L;
+    int64_t id = table[min(p, n - 1)];
+    if (id < 0 || id >= num_blocks) {
+      flag(status, PKV_STATUS_BAD_PAGE);
+      id = 0;
+    }
+    at[i] = (id * n_kv_heads + h) * D + c * V;
+  }
+  vec a[kScoreSteps], b[kScoreSteps];
+#pragma unroll
+  for (int i = 0; i < kScoreSteps; ++i) {
+    a[i] = *reinterpret_cast<const vec*>(lo + at[i]);
+    b[i] = *reinterpret_cast<const vec*>(hi + at[i]);
+  }
+  double x[GQ][V];
+#pragma unroll
+  for (int g = 0; g < GQ; ++g) {
+    const vec t = *reinterpret_cast<const vec*>(
+        q + (((int64_t)seq * n_kv_heads + h) * G + quad * GQ + g) * D + c * V);
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[g][j] = (double)Elem<T>::to_f(t[j]);
+  }
+#pragma unroll
+  for (int i = 0; i < kScoreSteps; ++i) {
+    double s[GQ];
+#pragma unroll
+    for (int g = 0; g < GQ; ++g) s[g] = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float l = Elem<T>::to_f(a[i][j]), u = Elem<T>::to_f(b[i][j]);
+#pragma unroll
+      for (int g = 0; g < GQ; ++g)
+        s[g] = __builtin_fma(x[g][j], (double)(x[g][j] < 0 ? l : u), s[g]);
+    }
+    double m = head_max<GQ, L>(s);
+    const int p = first + i * PW + lane / L;
+    if constexpr (S::QW > 1) {
+      if (c == 0) part[(wave * kScoreSteps + i) * PW + lane / L] = m;
+    } else {
+      if (c == 0 && p < n) scores[((int64_t)seq * n_kv_heads + h) * stride + p] = m;
+    }
+  }
+  if constexpr (S::QW > 1) {
+    __syncthreads();
+    constexpr int N = PW * kScoreSteps;   // pages of a group of waves
+    for (int i = threadIdx.x; i < 4 / S::QW * N; i += 256) {
+      const int w = i / N * S::QW, k = i % N, p = blockIdx.y * S::PAGES + i;
+      double m = part[w * N + k];
+#pragma unroll
+      for (int j = 1; j < S::QW; ++j) {
+        const double o = part[(w + j) * N + k];
+        m = o != o || o > m ? o : m;
+      }
+      if (p < n) scores[((int64_t)seq * n_kv_heads + h) * stride + p] = m;
+    }
+  }
 }
 
 // ------------------------------------------------------------------- choice ---
@@ -184,6 +327,206 @@ __global__ __launch_bounds__(256) void select_kernel(
   }
 }
 
+// The same for up to B * K pages, a page's order value in a register: B threads
+// with K values each. The values of a head lie close together, so the digits
+// start at the highest bit in which the largest and the smallest differ, and
+// end as soon as a digit's bin holds exactly the pages still needed: two or
+// three rounds, not eight.
+template <int B, int K>
+__global__ __launch_bounds__(B) void select_rows_kernel(
+    const double* __restrict__ scores, int64_t stride, const int32_t* __restrict__ kv_indptr,
+    const int32_t* __restrict__ kv_indices, const int32_t* __restrict__ kv_lens,
+    int32_t n_kv_heads, int32_t page_size, int32_t pages, int32_t width,
+    int32_t* __restrict__ ids, int32_t* __restrict__ ordinals) {
+  constexpr int W = B / 64;          // waves
+  static_assert(B >= 256 && W * K <= 256, "a bin a thread, a count a lane of four");
+  __shared__ int32_t hist[256], counts[2][W * K];
+  __shared__ uint64_t range[2][W];
+  __shared__ int32_t digit, above, inside;
+  const int seq = blockIdx.y, h = blockIdx.x, tid = threadIdx.x;
+  const int wave = tid >> 6, lane = tid & 63;
+  const int np = seq_pages(kv_indptr, kv_lens, seq, page_size, stride);
+  const int32_t* table = kv_indices + kv_indptr[seq];
+  const int64_t row = ((int64_t)seq * n_kv_heads + h) * width;
+  auto put = [&](int j, int p) {
+    ids[row + j] = table[p];
+    ordinals[row + j] = p;
+  };
+  if (np <= pages) {
+    for (int j = tid; j < width; j += B) {
+      if (j < np) put(j, j);
+      else { ids[row + j] = -1; ordinals[row + j] = -1; }
+    }
+    return;
+  }
+  const int n = np - 1, k = pages - 1;
+  if (tid == 0) put(k, n);
+  if (k == 0) return;
+  const double* sc = scores + ((int64_t)seq * n_kv_heads + h) * stride;
+  uint64_t u[K], lo = ~0ull, hi = 0;
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const int p = i * B + tid;
+    u[i] = p < n ? order_of(sc[p]) : 0;   // (0 is no number's order value)
+    if (p < n) {
+      lo = u[i] < lo ? u[i] : lo;
+      hi = u[i] > hi ? u[i] : hi;
+    }
+  }
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const uint64_t a = __shfl_xor((unsigned long long)lo, m);
+    const uint64_t b = __shfl_xor((unsigned long long)hi, m);
+    lo = a < lo ? a : lo;
+    hi = b > hi ? b : hi;
+  }
+  if (lane == 0) { range[0][wave] = lo; range[1][wave] = hi; }
+  if (tid < 256) hist[tid] = 0;
+  __syncthreads();
+  for (int w = 0; w < W; ++w) {
+    lo = range[0][w] < lo ? range[0][w] : lo;
+    hi = range[1][w] > hi ? range[1][w] : hi;
+  }
+  // values from `least` on are taken, and of those in [least, least + 2^shift)
+  // the first `need` if `ties`
+  uint64_t least = lo;
+  int need = k, shift = lo == hi ? 0 : 64 - __builtin_clzll(lo ^ hi);
+  bool ties = lo == hi;
+  if (shift < 64) least = lo >> shift << shift;
+  else least = 0;
+  while (shift > 0) {
+    const int next = shift > 8 ? shift - 8 : 0;
+    // values that agree above `shift`, by their next bits
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      const bool in = i * B + tid < n && (shift == 64 || (u[i] ^ least) >> shift == 0);
+      // The largest first: digit b counts in hist[255 ^ b], so that wave 0's
+      // addresses below grow with the lane. Read as hist[255 - 4 l - j] they
+      // became a negative base plus an offset, and those reads returned other
+      // data in every workgroup whose LDS does not start at 0.
+      if (in) atomicAdd(&hist[255 ^ (int)((u[i] - least) >> next)], 1);
+    }
+    __syncthreads();
+    if (wave == 0) {
+      // lane l has the bins 255 - (4 l + 0..3)
+      int c[4], sum = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        c[j] = hist[4 * lane + j];
+        sum += c[j];
+      }
+      int run = sum;
+#pragma unroll
+      for (int m = 1; m < 64; m <<= 1) {
+        const int o = __shfl_up(run, m);
+        run += lane >= m ? o : 0;
+      }
+      int before = run - sum;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (before < need && before + c[j] >= need) {
+          digit = 255 ^ (4 * lane + j);
+          above = before;
+          inside = c[j];
+        }
+        before += c[j];
+      }
+    }
+    __syncthreads();
+    least += (uint64_t)digit << next;
+    need -= above;
+    shift = next;
+    ties = inside > need;
+    if (!ties) break;
+    if (tid < 256) hist[tid] = 0;
+    __syncthreads();
+  }
+  // Now `ties` only if the values in question are all equal to `least`. Page
+  // order is (i, thread): a count a wave and i, and their sums before each.
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const bool in = i * B + tid < n && u[i] >= least;
+    const bool eq = in && ties && u[i] == least;
+    const uint64_t bi = __builtin_amdgcn_ballot_w64(in), be = __builtin_amdgcn_ballot_w64(eq);
+    if (lane == 0) {
+      counts[0][i * W + wave] = __builtin_popcountll(bi & ~be);
+      counts[1][i * W + wave] = __builtin_popcountll(be);
+    }
+  }
+  __syncthreads();
+  if (wave == 0) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      constexpr int C = (W * K + 63) / 64;
+      int c[C], sum = 0;
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        c[j] = lane * C + j < W * K ? counts[t][lane * C + j] : 0;
+        sum += c[j];
+      }
+      int run = sum;
+#pragma unroll
+      for (int m = 1; m < 64; m <<= 1) {
+        const int o = __shfl_up(run, m);
+        run += lane >= m ? o : 0;
+      }
+      run -= sum;
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        if (lane * C + j < W * K) counts[t][lane * C + j] = run;
+        run += c[j];
+      }
+    }
+  }
+  __syncthreads();
+  const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const int p = i * B + tid;
+    const bool in = p < n && u[i] >= least;
+    const bool eq = in && ties && u[i] == least;
+    const uint64_t bi = __builtin_amdgcn_ballot_w64(in), be = __builtin_amdgcn_ballot_w64(eq);
+    const int a = counts[0][i * W + wave] + __builtin_popcountll(bi & ~be & below);
+    const int e = counts[1][i * W + wave] + __builtin_popcountll(be & below);
+    if (in && (!eq || e < need)) put(a + (ties ? min(e, need) : 0), p);
+  }
+}
+
+struct ScoreArgs {
+  const void* q; const void* lo; const void* hi; int64_t nb;
+  const int32_t* indptr; const int32_t* indices; const int32_t* kv_lens;
+  int32_t n_seqs, Hkv, page_size, pages, max_pages; double* scores; int32_t* status;
+};
+typedef void (*ScoreFn)(const ScoreArgs&, hipStream_t);
+
+template <typename T, int D, int G>
+static void launch_scores(const ScoreArgs& a, hipStream_t s) {
+  constexpr int PAGES = ScoreShape<T, D, G>::PAGES;
+  hipLaunchKernelGGL((score_rows_kernel<T, D, G>),
+                     dim3((unsigned)a.Hkv, (unsigned)((a.max_pages - 1 + PAGES - 1) / PAGES),
+                          (unsigned)a.n_seqs),
+                     dim3(256), 0, s, (const T*)a.q, (const T*)a.lo, (const T*)a.hi, a.nb, a.indptr,
+                     a.indices, a.kv_lens, a.Hkv, a.page_size, a.pages, (int64_t)a.max_pages,
+                     a.scores, a.status);
+}
+
+template <typename T, int D>
+static ScoreFn score_g(int G) {
+  switch (G) {
+    case 1: return launch_scores<T, D, 1>;
+    case 2: return launch_scores<T, D, 2>;
+    case 4: return launch_scores<T, D, 4>;
+    case 8: return launch_scores<T, D, 8>;
+    case 16: return launch_scores<T, D, 16>;
+    default: return nullptr;
+  }
+}
+
+template <typename T>
+static ScoreFn score_fn(int32_t D, int32_t G) {
+  return D == 64 ? score_g<T, 64>(G) : D == 128 ? score_g<T, 128>(G) : nullptr;
+}
+
 }  // namespace pkv
 
 using namespace pkv;
@@ -215,12 +558,16 @@ extern "C" int pkv_page_bounds(const void* k_pool, int64_t pool_step, void* lo, 
                        pool_step, (char*)lo, (char*)hi, bounds_step, num_blocks, ids, page_size,
                        vecs, status_word);
   };
-  if (dtype == PKV_DTYPE_F16)
-    V == 8 ? go(page_bounds_kernel<_Float16, 8>) : go(page_bounds_kernel<_Float16, 1>);
-  else if (dtype == PKV_DTYPE_BF16)
-    V == 8 ? go(page_bounds_kernel<__bf16, 8>) : go(page_bounds_kernel<__bf16, 1>);
-  else
-    V == 4 ? go(page_bounds_kernel<float, 4>) : go(page_bounds_kernel<float, 1>);
+  auto pick = [&](auto type) {
+    typedef decltype(type) T;
+    constexpr int W = 16 / (int)sizeof(T);
+    if (V == 1) go(page_bounds_kernel<T, 1, 0>);
+    else if (page_size == 16) go(page_bounds_kernel<T, W, 16>);
+    else go(page_bounds_kernel<T, W, 0>);
+  };
+  if (dtype == PKV_DTYPE_F16) pick(_Float16{});
+  else if (dtype == PKV_DTYPE_BF16) pick(__bf16{});
+  else pick(float{});
   PKV_LAUNCH_CHECK();
   return PKV_OK;
 }
@@ -244,28 +591,43 @@ extern "C" int pkv_select_pages(const void* q, const void* lo, const void* hi, i
   const int32_t width = std::min(pages, max_pages);
   hipStream_t s = (hipStream_t)stream;
   if (max_pages > pages && pages > 1) {
-    const uintptr_t at = (uintptr_t)lo | (uintptr_t)hi |
+    const uintptr_t at = (uintptr_t)q | (uintptr_t)lo | (uintptr_t)hi |
                          (uintptr_t)((int64_t)head_dim * elem_bytes(dtype));
-    const bool wide = at % 16 == 0;
-    auto go = [&](auto kernel, auto type) {
+    auto score = [&](auto type) {
       typedef decltype(type) T;
-      hipLaunchKernelGGL(kernel, dim3((unsigned)((max_pages + 62) / 64), (unsigned)n_kv_heads,
-                                      (unsigned)n_seqs),
-                         dim3(64), 0, s, (const T*)q, (const T*)lo, (const T*)hi, num_blocks,
-                         kv_indptr, kv_indices, kv_lens, n_heads, n_kv_heads, head_dim, page_size,
-                         pages, (int64_t)max_pages, scores, status_word);
+      const bool wide = at % 16 == 0;
+      // (a grid of up to 65535 workgroups of at least 8 pages)
+      const ScoreFn fn = wide && max_pages <= 8 * 65535
+                             ? score_fn<T>(head_dim, n_heads / n_kv_heads) : nullptr;
+      if (fn) {
+        fn({q, lo, hi, num_blocks, kv_indptr, kv_indices, kv_lens, n_seqs, n_kv_heads, page_size,
+            pages, max_pages, scores, status_word}, s);
+        return;
+      }
+      auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((max_pages + 62) / 64), (unsigned)n_kv_heads,
+                                        (unsigned)n_seqs),
+                           dim3(64), 0, s, (const T*)q, (const T*)lo, (const T*)hi, num_blocks,
+                           kv_indptr, kv_indices, kv_lens, n_heads, n_kv_heads, head_dim,
+                           page_size, pages, (int64_t)max_pages, scores, status_word);
+      };
+      if (wide) go(score_kernel<T, 16 / (int)sizeof(T)>);
+      else go(score_kernel<T, 1>);
     };
-    if (dtype == PKV_DTYPE_F16)
-      wide ? go(score_kernel<_Float16, 8>, _Float16{}) : go(score_kernel<_Float16, 1>, _Float16{});
-    else if (dtype == PKV_DTYPE_BF16)
-      wide ? go(score_kernel<__bf16, 8>, __bf16{}) : go(score_kernel<__bf16, 1>, __bf16{});
-    else
-      wide ? go(score_kernel<float, 4>, float{}) : go(score_kernel<float, 1>, float{});
+    if (dtype == PKV_DTYPE_F16) score(_Float16{});
+    else if (dtype == PKV_DTYPE_BF16) score(__bf16{});
+    else score(float{});
     PKV_LAUNCH_CHECK();
   }
-  hipLaunchKernelGGL(select_kernel, dim3((unsigned)n_kv_heads, (unsigned)n_seqs), dim3(256), 0, s,
-                     scores, (int64_t)max_pages, kv_indptr, kv_indices, kv_lens, n_kv_heads,
-                     page_size, pages, width, ids, ordinals);
+  auto choose = [&](auto kernel, int threads) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)n_kv_heads, (unsigned)n_seqs), dim3(threads), 0, s,
+                       scores, (int64_t)max_pages, kv_indptr, kv_indices, kv_lens, n_kv_heads,
+                       page_size, pages, width, ids, ordinals);
+  };
+  if (max_pages <= 256 * 4) choose(select_rows_kernel<256, 4>, 256);
+  else if (max_pages <= 1024 * 4) choose(select_rows_kernel<1024, 4>, 1024);
+  else if (max_pages <= 1024 * 16) choose(select_rows_kernel<1024, 16>, 1024);
+  else choose(select_kernel, 256);
   PKV_LAUNCH_CHECK();
   return PKV_OK;
 }

@@ -402,8 +402,8 @@ int pkv_select_pages(const void* q, const void* lo, const void* hi, int64_t num_
  * Decode attention over the pages pkv_select_pages chose (its ids, n_seqs,
  * max_pages and pages): sequence i's single query attends the rows of its
  * chosen pages, of the last one those below kv_lens[i]. Lists are cut into
- * pieces of part_pages pages, as pkv_plan_decode cuts sequences, and cut ones
- * merge through `workspace` (256-byte aligned, pkv_selected_workspace_bytes
+ * pieces of part_pages pages (8 is what the kernel stages at a time), the
+ * remainder last, and cut ones merge through `workspace` (256-byte aligned, pkv_selected_workspace_bytes
  * long; zero before the first launch that uses it, and left with zero
  * counters by each; launches that share it must not overlap in time).
  * Geometries without the fast decode path run a generic kernel, with no

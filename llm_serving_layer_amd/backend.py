@@ -59,6 +59,7 @@ _DTYPES = {torch.float16: _native.DTYPE_F16, torch.bfloat16: _native.DTYPE_BF16,
            torch.float32: _native.DTYPE_F32}
 
 MAX_PART_PAGES = 64      # a partition's page ids are read by one wavefront
+SELECTED_PART_PAGES = 8  # of chosen pages; what their kernel stages at a time
 SHARED_MIN_PAGES = 4     # shorter runs of shared pages stay each sequence's own
 SHARED_TILES = 512       # workgroups that share the work on a batch's shared pages
 DEFAULT_Q_TILE = 64      # prefill tile when the geometry has no matrix-core kernel
@@ -958,7 +959,7 @@ class MI355XBackend:
                                dtype=torch.float64, **dev)
         p.ids = torch.empty(many * width, dtype=torch.int32, **dev)
         p.ordinals = torch.empty(many * width, dtype=torch.int32, **dev)
-        p.part = self.part_pages
+        p.part = min(self.part_pages, SELECTED_PART_PAGES)
         while True:   # partials are addressed with 32 bits: longer pieces where they pass 2 GiB
             need = self._lib.pkv_selected_workspace_bytes(
                 n, p.max_pages, pages, p.part, self.n_heads, self.n_kv_heads, self.head_dim,

@@ -175,9 +175,9 @@ __device__ __forceinline__ void merge_head(T* __restrict__ out, float* wts, int 
 //    for its own dims (V in LDS), and merges those dims of a cut sequence.
 // One 1371-token sequence (5 pieces, 8 KV heads, 32 query heads, d 64): 16.4
 // us a launch in decode_kernel; 9.4 here; 16 layers of such steps 271 -> 157 us.
-template <typename T, int D, int G> struct PieceLds {
-  static constexpr int CH = 20;                   // pages staged at a time: any piece of
-                                                  // the default cut (17 + a folded tail)
+template <typename T, int D, int G, int CHUNK = 20> struct PieceLds {
+  static constexpr int CH = CHUNK;                // pages staged at a time: 20 hold any piece
+                                                  // of the default cut (17 + a folded tail)
   static constexpr int VPAGE = 16 * D * (int)sizeof(T);
   static constexpr int V = CH * VPAGE;            // V rows, chunks swizzled
   static constexpr int P = CH * 512;              // probabilities, lane order
@@ -188,20 +188,15 @@ template <typename T, int D, int G> struct PieceLds {
 
 // Pieces of the pages chosen for each sequence and KV head (selection.hip)
 // instead of a plan's: nothing of them is known on the host but their number,
-// so a piece's item follows from the sequence's length, by the plan's cut.
+// so a piece's item follows from the sequence's length: part_pages pages, the
+// remainder last.
 struct Chosen {
   const int32_t* ids;       // [n_seqs][n_kv_heads][width], a list's pages in order
   const int32_t* kv_lens;
   int32_t width, pages, part_pages, max_parts, n_seqs;
 };
 
-// Pieces of np pages, and the folded remainder.
-__host__ __device__ static inline int n_pieces(int np, int part, bool* fold) {
-  const int full = np / part, rem = np % part;
-  const int least = kMinTail < (part + 1) / 2 ? kMinTail : (part + 1) / 2;
-  *fold = full > 0 && rem > 0 && rem < least;
-  return full + (rem > 0 && !*fold ? 1 : 0);
-}
+constexpr int kChosenChunk = 8;   // pages of them staged at a time
 
 template <typename T, int D, int G, bool CHOSEN = false>
 __device__ __forceinline__ void decode_piece(
@@ -215,7 +210,7 @@ __device__ __forceinline__ void decode_piece(
   typedef typename Mma<T>::vec8 vec8;
   typedef typename Mma<T>::vec4 vec4;
   typedef PartLayout<D, G> PL;
-  typedef PieceLds<T, D, G> L;
+  typedef PieceLds<T, D, G, CHOSEN ? kChosenChunk : 20> L;
   constexpr int PS = 16;
   constexpr int NCH = D / 32;          // QK MFMA k-chunks per head row
   constexpr int NDB = D / 16;          // PV dim blocks
@@ -258,11 +253,9 @@ __device__ __forceinline__ void decode_piece(
       const int p = bin - seq * ch.max_parts;
       const int len = max(ch.kv_lens[seq], 1), all = (len + PS - 1) / PS;
       const int n = min(min(all, ch.pages), ch.width), part = ch.part_pages;
-      bool fold;
-      nparts = n_pieces(n, part, &fold);
+      nparts = (n + part - 1) / part;
       if (p >= nparts) break;
-      const int full = n / part;
-      np = p < full ? part + (fold && p + 1 == full ? n % part : 0) : n % part;
+      np = min(part, n - p * part);
       tok0 = p * part * PS;
       kv = len - (all - n) * PS;     // of the chosen pages, the last page last
       slot0 = nparts > 1 ? seq * ch.max_parts : -1;

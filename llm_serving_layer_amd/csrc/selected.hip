@@ -11,14 +11,17 @@ int check_geometry(int32_t Hq, int32_t Hkv, int32_t D, int32_t ps, int32_t dtype
 int split_workspace(void* workspace, int64_t workspace_bytes, int32_t n_seqs, int32_t n_slots,
                     int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, DecodeWorkspace* w);
 
+// Waves a SIMD the kernel is compiled for: the merge's registers grow with G.
+template <int G> constexpr int kSelectedWaves = G <= 4 ? 4 : G == 8 ? 3 : 2;
+
 // The piece kernel (decode_piece.h) over chosen pages: a workgroup a piece and
 // KV head, heads first, so that a head's workgroups meet one L2.
 template <typename T, int D, int G>
-__global__ __launch_bounds__(256, kPieceWaves<D>) void selected_kernel(
+__global__ __launch_bounds__(256, kSelectedWaves<G>) void selected_kernel(
     const T* __restrict__ q, T* __restrict__ out, T* __restrict__ kpool, T* __restrict__ vpool,
     int64_t num_blocks, int32_t n_kv_heads, float scale_log2, Chosen ch, DecodeWorkspace w,
     int32_t* status) {
-  __shared__ __align__(16) unsigned char smem[PieceLds<T, D, G>::BYTES];
+  __shared__ __align__(16) unsigned char smem[PieceLds<T, D, G, kChosenChunk>::BYTES];
   const int bin = blockIdx.x / n_kv_heads;
   decode_piece<T, D, G, true>(smem, blockIdx.x - bin * n_kv_heads, bin, q, out, kpool, vpool,
                               num_blocks, nullptr, 0, n_kv_heads, scale_log2, nullptr, nullptr,
@@ -126,9 +129,7 @@ static SelectedFn selected_fn(int32_t dtype, int32_t D, int32_t G, int32_t page_
 }
 
 static int max_parts(int32_t max_pages, int32_t pages, int32_t part_pages) {
-  // a shorter list never has more pieces than a longer one
-  bool fold;
-  return n_pieces(std::min(max_pages, pages), part_pages, &fold);
+  return (std::min(max_pages, pages) + part_pages - 1) / part_pages;
 }
 
 }  // namespace pkv

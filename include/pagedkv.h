@@ -334,8 +334,9 @@ int pkv_attend_batch(const void* batch, const void* q, void* out, void* k_pool, 
  * (arguments and outputs as there), with each sequence's shared parts counted
  * among its pieces and given its first partial slots. `tiles` receives
  * *n_tiles_out items {index of the first page in kv_indices, pages, first
- * member, members, split, 0, 0, 0}, then the members {row of q, sequence,
- * partial slot of split 0, 0}; *tiles_needed ints in all. A buffer too small
+ * member, members, split, 0, 0, 0}, *n_merges_out merges {sequence, parts,
+ * first partial slot, 0} of the sequences with shared parts, then the members
+ * {row of q, partial slot of split 0}; *tiles_needed ints in all. A buffer too small
  * gives PKV_ERR_CAPACITY with the needed sizes set (tiles_needed once plan
  * suffices).
  */
@@ -345,23 +346,25 @@ int pkv_plan_shared(const int32_t* kv_indptr, const int32_t* kv_indices, const i
                     int32_t max_workgroups, int32_t min_pages, int32_t tile_target, int32_t* plan,
                     int64_t plan_capacity, int64_t* plan_needed, int32_t* n_work_out,
                     int32_t* n_slots_out, int32_t* plan_stride_out, int32_t* tiles,
-                    int64_t tiles_capacity, int64_t* tiles_needed, int32_t* n_tiles_out);
+                    int64_t tiles_capacity, int64_t* tiles_needed, int32_t* n_tiles_out,
+                    int32_t* n_merges_out);
 
 /*
  * pkv_attend_decode with pkv_plan_shared's tiles and plan (device copies): the
  * same result up to rounding, with each shared run of pages read once per tile
  * of sequences. kv_indices is the device copy of the planned one; workspace
  * and fused append as for pkv_attend_decode (no shared page may be a slot's of
- * slot_mapping). Needs the fast decode path and a positive scale
- * (PKV_ERR_INVALID otherwise, nothing launched).
+ * slot_mapping). Needs at least one tile, the fast decode path and a positive
+ * scale (PKV_ERR_INVALID otherwise, nothing launched).
  */
 int pkv_attend_shared(const void* q, void* out, void* k_pool, void* v_pool, int64_t num_blocks,
                       const int32_t* kv_indices, int32_t n_seqs, int32_t n_heads,
                       int32_t n_kv_heads, int32_t head_dim, int32_t page_size, float scale,
-                      int32_t dtype, const int32_t* tiles, int32_t n_tiles, const int32_t* plan,
-                      int32_t n_work, int32_t n_slots, int32_t plan_stride, const void* k_new,
-                      const void* v_new, const int32_t* slot_mapping, void* workspace,
-                      int64_t workspace_bytes, int32_t* status_word, void* stream);
+                      int32_t dtype, const int32_t* tiles, int32_t n_tiles, int32_t n_merges,
+                      const int32_t* plan, int32_t n_work, int32_t n_slots, int32_t plan_stride,
+                      const void* k_new, const void* v_new, const int32_t* slot_mapping,
+                      void* workspace, int64_t workspace_bytes, int32_t* status_word,
+                      void* stream);
 
 /*
  * Key bounds of pages — no counterpart in the reference. For each of the

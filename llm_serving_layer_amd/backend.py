@@ -61,7 +61,7 @@ _DTYPES = {torch.float16: _native.DTYPE_F16, torch.bfloat16: _native.DTYPE_BF16,
 MAX_PART_PAGES = 64      # a partition's page ids are read by one wavefront
 SELECTED_PART_PAGES = 8  # of chosen pages; what their kernel stages at a time
 SHARED_MIN_PAGES = 4     # shorter runs of shared pages stay each sequence's own
-SHARED_TILES = 512       # workgroups that share the work on a batch's shared pages
+SHARED_TILES = 256       # workgroups that share the work on a batch's shared pages
 DEFAULT_Q_TILE = 64      # prefill tile when the geometry has no matrix-core kernel
 
 
@@ -195,7 +195,7 @@ class _Shared:
     """What ``attend_shared`` keeps for one BatchMeta: None where nothing is
     worth sharing (``n_tiles`` 0: the batch takes ``attend``)."""
 
-    __slots__ = ("meta", "n", "n_tiles", "tiles", "plan", "indices", "slots", "n_work", "n_slots",
+    __slots__ = ("meta", "n", "n_tiles", "n_merges", "tiles", "plan", "indices", "slots", "n_work", "n_slots",
                  "stride", "ws", "fusable", "buffers", "stream")
 
 
@@ -802,7 +802,7 @@ class MI355XBackend:
                 q.data_ptr(), out.data_ptr(), self._k_ptr[layer_idx], self._v_ptr[layer_idx],
                 self.num_blocks, p.indices.data_ptr(), p.n, self.n_heads, self.n_kv_heads,
                 self.head_dim, self.block_size, float(scale), self._code, p.tiles.data_ptr(),
-                p.n_tiles, p.plan.data_ptr(), p.n_work, p.n_slots, p.stride,
+                p.n_tiles, p.n_merges, p.plan.data_ptr(), p.n_work, p.n_slots, p.stride,
                 pend.k.data_ptr() if fused else None, pend.v.data_ptr() if fused else None,
                 p.slots.data_ptr() if fused else None, p.ws.data_ptr(), p.ws.numel(),
                 self._status_ptr, stream)
@@ -833,7 +833,7 @@ class MI355XBackend:
     def _fill_shared(self, p: _Shared, meta: BatchMeta, indptr, indices, kvl, last) -> None:
         """Plan the batch's shared runs and own pages (pkv_plan_shared)."""
         ptr = lambda a: a.ctypes.data  # noqa: E731
-        n_work, n_slots, stride, n_tiles = (C.c_int32() for _ in range(4))
+        n_work, n_slots, stride, n_tiles, n_merges = (C.c_int32() for _ in range(5))
         needed, tiles_needed = C.c_int64(), C.c_int64()
         cap = 10 * self._decode_wgs + 2 * int(indptr[-1]) + 24 * p.n + 128
         tiles_cap = 8 * SHARED_TILES + 16 * p.n
@@ -846,7 +846,7 @@ class MI355XBackend:
                     self.num_blocks, self.n_heads, self.n_kv_heads, part, self._decode_wgs,
                     SHARED_MIN_PAGES, SHARED_TILES, ptr(buf), cap, C.byref(needed),
                     C.byref(n_work), C.byref(n_slots), C.byref(stride), ptr(tiles), tiles_cap,
-                    C.byref(tiles_needed), C.byref(n_tiles))
+                    C.byref(tiles_needed), C.byref(n_tiles), C.byref(n_merges))
                 if rc != _native.ERR_CAPACITY or (needed.value <= cap
                                                   and tiles_needed.value <= tiles_cap):
                     break
@@ -860,7 +860,7 @@ class MI355XBackend:
         if not n_tiles.value or need >= 2**31:
             return
         p.n_tiles, p.n_work, p.n_slots = n_tiles.value, n_work.value, n_slots.value
-        p.stride = stride.value
+        p.stride, p.n_merges = stride.value, n_merges.value
         p.plan = self._upload(buf[:needed.value])
         p.tiles = self._upload(tiles[:tiles_needed.value])
         p.indices = self._dev_i32(meta.kv_indices)

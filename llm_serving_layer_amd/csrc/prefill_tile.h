@@ -67,17 +67,47 @@ template <typename T, int D> struct PrefillLds {
   static constexpr int LPT = TILE / 2 / 1024;          // wave loads of a page of one tensor
 };
 
+// Lane 4 k + i of v[e] becomes lane 4 k + e of v[i]: a 4 x 4 transpose in every
+// quad of lanes (a swap of pairs a lane apart, then of pairs two apart).
+__device__ __forceinline__ f32x4 quad_transpose(f32x4 v) {
+  const int lane = threadIdx.x;
+  const bool a = lane & 1, b = lane & 2;
+  f32x4 t;
+#pragma unroll
+  for (int e = 0; e < 4; e += 2) {   // quad_perm [1,0,3,2]
+    const float x = dpp<0xB1>(a ? v[e] : v[e + 1]);
+    t[e] = a ? x : v[e];
+    t[e + 1] = a ? v[e + 1] : x;
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {      // quad_perm [2,3,0,1]
+    const float x = dpp<0x4E>(b ? t[e] : t[e + 2]);
+    v[e] = b ? x : t[e];
+    v[e + 2] = b ? t[e + 2] : x;
+  }
+  return v;
+}
+
 // A tile over pages that several one-token sequences share (shared.hip): its
 // rows are those sequences' queries, all of which see every key, and its
 // result is a partial (o, m, l) per sequence, in the decode kernels' layout.
 struct SharedTile {
   const int32_t* items;      // {first page in kv_indices, pages, first member, members, split}
-  const int32_t* members;    // {row of q, sequence, partial slot of split 0, 0}
+  const int32_t* members;    // {row of q, partial slot of split 0}
   float* part_o;
   float* part_ml;
-  int32_t* counters;
 };
-constexpr int kSharedItem = 8, kSharedMember = 4;   // ints of each
+constexpr int kSharedItem = 8, kSharedMember = 2;   // ints of each
+
+// A shared tile's ring: as many buffers as fit 80 KiB (two workgroups a compute
+// unit; at head_dim 64 eight are enough), tiles loaded RING - 2 ahead. Such a
+// tile has at most one more workgroup beside it, so its own loads have to cover
+// the memory's latency, where a prefill tile's neighbours do.
+template <typename T, int D> struct SharedRing {
+  static constexpr int N = 81920 / (2 * PrefillLds<T, D>::TILE) < 8
+                               ? 81920 / (2 * PrefillLds<T, D>::TILE) : 8;
+  static constexpr int BYTES = N * 2 * PrefillLds<T, D>::TILE;
+};
 
 template <typename T, int D, int G, bool SHARED = false>
 __device__ __forceinline__ void prefill_tile(
@@ -333,55 +363,92 @@ __device__ __forceinline__ void prefill_tile(
     l_run += ls;
   };
 
-  // The ring: tile t in buffer t % 4. Each step waits for its tile's loads
-  // (this wave's, then every wave's at the barrier, which also ends every
-  // wave's reads of the buffer the step then refills: the one of tile t - 2,
-  // whose PV ran in the previous step), loads the pages of tile t + 2,
-  // computes tile t beside the PV of tile t - 1, and loads the page ids of
-  // tile t + 3.
-  // The first step's PV meets zero probabilities in buf3, which no tile has
-  // filled yet: zeros there (visible to every wave at the step's barrier).
-  for (int i = tid; i < L::TILE / 16; i += kPrefillThreads)
-    reinterpret_cast<u32x4*>(buf3 + L::TILE)[i] = u32x4{0u, 0u, 0u, 0u};
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  int id0 = load_id(0), id1 = load_id(1), id2 = load_id(2), id3;   // of tile j in id(j % 4)
-  load_tile(0, id0, buf0);
-  load_tile(1, id1, buf1);
-  // Q arrives here: waited for inside the loop, where the compiler cannot see
-  // the tile loads, it would drain them in every step
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    u32x4 w = __builtin_bit_cast(u32x4, qb[c]);
-    asm volatile("" : "+v"(w));
-    qb[c] = __builtin_bit_cast(vec8, w);
-  }
-  auto step = [&](int t, unsigned char* cur, unsigned char* prev, unsigned char* nxt2,
-                  int& id_t2, int& id_t3) {
-    // Every tile load but the latest step's has landed; after the barrier,
-    // every wave's have. (A fenced barrier would wait for all of them.)
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LPT) : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    load_tile(t + 2, id_t2, nxt2);
-    compute(t, cur, prev + L::TILE);
-    // (after the tile's LDS reads: a scalar load in flight would make every
-    // wait for them a wait for it too)
-    id_t3 = load_id(t + 3);
-  };
   unsigned char* last = buf0;   // the buffer of the last tile computed
-  for (int t = 0;; t += 4) {
-    step(t, buf0, buf3, buf2, id2, id3);
-    last = buf0;
-    if (t + 1 >= ntiles) break;
-    step(t + 1, buf1, buf0, buf3, id3, id0);
-    last = buf1;
-    if (t + 2 >= ntiles) break;
-    step(t + 2, buf2, buf1, buf0, id0, id1);
-    last = buf2;
-    if (t + 3 >= ntiles) break;
-    step(t + 3, buf3, buf2, buf1, id1, id2);
-    last = buf3;
-    if (t + 4 >= ntiles) break;
+  if constexpr (SHARED) {
+    // The ring of a shared tile: tile t in buffer t % N, tile t + AHEAD loaded
+    // in step t, into the buffer that step t - 2 was the last to read.
+    constexpr int N = SharedRing<T, D>::N, AHEAD = N - 2;
+    unsigned char* prev = smem + (N - 1) * 2 * L::TILE;
+    for (int i = tid; i < L::TILE / 16; i += kPrefillThreads)
+      reinterpret_cast<u32x4*>(prev + L::TILE)[i] = u32x4{0u, 0u, 0u, 0u};
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    int ids[AHEAD + 1];
+#pragma unroll
+    for (int t = 0; t <= AHEAD; ++t) ids[t] = load_id(t);
+#pragma unroll
+    for (int t = 0; t < AHEAD; ++t) load_tile(t, ids[t], smem + t * 2 * L::TILE);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {   // Q arrives here (see below)
+      u32x4 w = __builtin_bit_cast(u32x4, qb[c]);
+      asm volatile("" : "+v"(w));
+      qb[c] = __builtin_bit_cast(vec8, w);
+    }
+    int id = ids[AHEAD];
+    unsigned char* next = smem + AHEAD * 2 * L::TILE;
+    unsigned char* const end = smem + N * 2 * L::TILE;
+    last = smem;
+    for (int t = 0;; ++t) {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((AHEAD - 1) * LPT) : "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      load_tile(t + AHEAD, id, next);
+      compute(t, last, prev + L::TILE);
+      id = load_id(t + AHEAD + 1);
+      if (t + 1 >= ntiles) break;
+      prev = last;
+      last = last + 2 * L::TILE == end ? smem : last + 2 * L::TILE;
+      next = next + 2 * L::TILE == end ? smem : next + 2 * L::TILE;
+    }
+  } else {
+    // The ring: tile t in buffer t % 4. Each step waits for its tile's loads
+    // (this wave's, then every wave's at the barrier, which also ends every
+    // wave's reads of the buffer the step then refills: the one of tile t - 2,
+    // whose PV ran in the previous step), loads the pages of tile t + 2,
+    // computes tile t beside the PV of tile t - 1, and loads the page ids of
+    // tile t + 3.
+    // The first step's PV meets zero probabilities in buf3, which no tile has
+    // filled yet: zeros there (visible to every wave at the step's barrier).
+    for (int i = tid; i < L::TILE / 16; i += kPrefillThreads)
+      reinterpret_cast<u32x4*>(buf3 + L::TILE)[i] = u32x4{0u, 0u, 0u, 0u};
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    int id0 = load_id(0), id1 = load_id(1), id2 = load_id(2), id3;   // of tile j in id(j % 4)
+    load_tile(0, id0, buf0);
+    load_tile(1, id1, buf1);
+    // Q arrives here: waited for inside the loop, where the compiler cannot see
+    // the tile loads, it would drain them in every step
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      u32x4 w = __builtin_bit_cast(u32x4, qb[c]);
+      asm volatile("" : "+v"(w));
+      qb[c] = __builtin_bit_cast(vec8, w);
+    }
+    auto step = [&](int t, unsigned char* cur, unsigned char* prev, unsigned char* nxt2,
+                    int& id_t2, int& id_t3) {
+      // Every tile load but the latest step's has landed; after the barrier,
+      // every wave's have. (A fenced barrier would wait for all of them.)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LPT) : "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      load_tile(t + 2, id_t2, nxt2);
+      compute(t, cur, prev + L::TILE);
+      // (after the tile's LDS reads: a scalar load in flight would make every
+      // wait for them a wait for it too)
+      id_t3 = load_id(t + 3);
+    };
+    for (int t = 0;; t += 4) {
+      step(t, buf0, buf3, buf2, id2, id3);
+      last = buf0;
+      if (t + 1 >= ntiles) break;
+      step(t + 1, buf1, buf0, buf3, id3, id0);
+      last = buf1;
+      if (t + 2 >= ntiles) break;
+      step(t + 2, buf2, buf1, buf0, id0, id1);
+      last = buf2;
+      if (t + 3 >= ntiles) break;
+      step(t + 3, buf3, buf2, buf1, id1, id2);
+      last = buf3;
+      if (t + 4 >= ntiles) break;
+    }
   }
   pv(last + L::TILE);   // the last tile's PV
   // the loads of the tiles past the end land in LDS before the workgroup ends
@@ -389,26 +456,33 @@ __device__ __forceinline__ void prefill_tile(
 
   l_run = sum_x32(l_run);
   if constexpr (SHARED) {
-    // the partial of the row's sequence and head; its arrival is counted with
-    // a head's first row (the launch's end orders the stores before the merge)
-    if (valid) {
-      constexpr int NDB = D / 16, FLOATS = (G + 3) / 4 * NDB * 64;
-      const int hd = r % G;
-      const int32_t* mb = members + tok * kSharedMember;
-      const int64_t slot = mb[2] + split;
-      float* po = sh.part_o + (slot * n_kv_heads + h) * FLOATS + (hd / 4) * NDB * 64 + (hd & 3);
+    // The partial of the row's sequence and head: groups of four heads, a
+    // float4 over them per dim. Four heads are four lanes here, so a quad of
+    // lanes transposes its four dims (j & 3) into one 16-byte store each: a
+    // quad then writes 64 bytes in a row. (Below four heads the groups are
+    // padded, and each lane stores its own.)
+    constexpr int NDB = D / 16, FLOATS = (G + 3) / 4 * NDB * 64;
+    const int hd = r % G;
+    const int32_t* mb = members + (valid ? tok : 0) * kSharedMember;
+    const int64_t slot = mb[1] + split;
+    float* po = sh.part_o + (slot * n_kv_heads + h) * FLOATS + (hd / 4) * NDB * 64;
 #pragma unroll
-      for (int dh = 0; dh < NDH; ++dh) {
+    for (int dh = 0; dh < NDH; ++dh) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) po[(32 * dh + 8 * (j >> 2) + 4 * g + (j & 3)) * 4] = o[dh][j];
-      }
-      if (g == 0) {
-        float* ml = sh.part_ml + (slot * Hq + h * G + hd) * 2;
-        ml[0] = m_run;
-        ml[1] = l_run;
-        if (hd == 0) atomicAdd(sh.counters + (int64_t)mb[1] * n_kv_heads + h, 1);
+      for (int j = 0; j < 4; ++j) {
+        f32x4 v{o[dh][4 * j], o[dh][4 * j + 1], o[dh][4 * j + 2], o[dh][4 * j + 3]};
+        const int d0 = 32 * dh + 8 * j + 4 * g;
+        if constexpr (G >= 4) {
+          v = quad_transpose(v);   // lane hd & 3: dim d0 + (hd & 3) of the group's heads
+          if (valid) *reinterpret_cast<f32x4*>(po + (d0 + (hd & 3)) * 4) = v;
+        } else if (valid) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) po[(d0 + e) * 4 + hd] = v[e];
+        }
       }
     }
+    if (valid && g == 0)
+      *reinterpret_cast<f32x2*>(sh.part_ml + (slot * Hq + h * G + hd) * 2) = f32x2{m_run, l_run};
     return;
   }
   if (valid) {

@@ -7,47 +7,141 @@
 // begin alike form a tree; each of its inner runs is one part of every sequence
 // below it, and its own pages are the sequence's last part (its last page
 // always is its own, so every sequence has one).
-//  * shared_kernel takes a run: the queries of the sequences that share it are
-//    the 128 rows of a prefill tile (prefill_tile.h), so a tile of K and V
-//    loaded once serves 128 / G sequences on the matrix cores. Long runs are
-//    split over workgroups. Its parts go to the decode kernels' partial slots,
-//    with their arrival counts.
-//  * the decode kernels take the own pages as pieces of cut sequences, with the
-//    shared parts counted among each sequence's pieces: whichever piece comes
-//    last merges all of them.
+//  * A run is a prefill tile's work (prefill_tile.h): the queries of the
+//    sequences that share it are its 128 rows, so a tile of K and V loaded once
+//    serves 128 / G sequences on the matrix cores. Long runs are split over
+//    workgroups. Each leaves its parts in the decode kernels' partial slots.
+//  * The own pages are pieces of a decode plan, as pieces of cut sequences
+//    whose other parts are the shared ones.
+//  * Both run in one launch, side by side: the tiles are bound by the matrix
+//    cores, the own pages by memory, and a compute unit holds a workgroup of
+//    each. Neither knows when a sequence's parts are complete; a last small
+//    launch merges them.
 #include <algorithm>
 #include <numeric>
 #include <vector>
 
-#include "decode_piece.h"
+#include "decode_stream.h"
 #include "prefill_tile.h"
 
 namespace pkv {
 
-template <typename T, int D, int G>
-__global__ __launch_bounds__(kPrefillThreads) void shared_kernel(
-    const T* __restrict__ q, const T* __restrict__ kpool, const T* __restrict__ vpool,
-    int64_t num_blocks, const int32_t* __restrict__ kv_indices, int32_t n_kv_heads,
-    float scale_log2, SharedTile sh, int32_t* status) {
-  __shared__ __align__(16) unsigned char smem[PrefillLds<T, D>::BYTES];
-  prefill_tile<T, D, G, true>(smem, blockIdx.x, q, nullptr, kpool, vpool, num_blocks, nullptr,
-                              nullptr, kv_indices, nullptr, nullptr, n_kv_heads, scale_log2,
-                              status, sh);
-}
-
-struct SharedArgs {
-  const void* q; const void* kp; const void* vp; int64_t nb; const int32_t* indices;
-  int32_t Hkv; float sl2; SharedTile sh; int32_t n_tiles; int32_t* status;
+template <typename T> struct SharedArgs {
+  const T* q; T* out; T* kp; T* vp;
+  int64_t nb; const int32_t* indices; int32_t Hkv; float sl2; SharedTile sh; int32_t n_tiles;
+  const int32_t* plan; int32_t stride; const T* kn; const T* vn; const int32_t* slots;
+  DecodeWorkspace w; int32_t* status;
+  int32_t tiles, pieces, turn;   // workgroups of each kind, and in a row of one kind
 };
 
-template <typename T, int D, int G>
-static void launch_shared(const SharedArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((shared_kernel<T, D, G>), dim3((unsigned)(a.n_tiles * a.Hkv)),
-                     dim3(kPrefillThreads), 0, s, (const T*)a.q, (const T*)a.kp, (const T*)a.vp,
-                     a.nb, a.indices, a.Hkv, a.sl2, a.sh, a.status);
+// The launch's workgroup `block` as one of the tiles (>= 0) or of the pieces
+// (~ of its number): the kinds take turns, `turn` at a time, as long as both
+// have that many, then the rest of the tiles and of the pieces follow.
+__device__ __forceinline__ int shared_role(int block, int tiles, int pieces, int turn) {
+  const int rounds = min(tiles, pieces) / turn, both = rounds * 2 * turn;
+  if (block < both) {
+    const int round = block / (2 * turn), at = block - round * 2 * turn;
+    return at < turn ? round * turn + at : ~(round * turn + at - turn);
+  }
+  const int at = block - both + rounds * turn;
+  return at < tiles ? at : ~(at - tiles + rounds * turn);
 }
 
-typedef void (*SharedFn)(const SharedArgs&, hipStream_t);
+// Tiles beside the bins of the streaming decode kernel (four KV heads a bin's
+// workgroup).
+template <typename T, int D, int G>
+__global__ __launch_bounds__(256, 2) void shared_stream_kernel(SharedArgs<T> a) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int role = shared_role(blockIdx.x, a.tiles, a.pieces, a.turn);
+  if (role >= 0) {
+    prefill_tile<T, D, G, true>(smem, role, a.q, nullptr, a.kp, a.vp, a.nb, nullptr, nullptr,
+                                a.indices, nullptr, nullptr, a.Hkv, a.sl2, a.status, a.sh);
+  } else {
+    const int groups = a.Hkv / heads_per_wg(a.Hkv), bin = ~role / groups;
+    if ((int)(threadIdx.x >> 6) >= heads_per_wg(a.Hkv)) return;
+    decode_stream<T, D, G>(smem, bin, ~role - bin * groups, a.q, a.out, a.kp, a.vp, a.nb, a.plan,
+                           a.stride, a.Hkv, a.sl2, a.kn, a.vn, a.slots, a.w.part_o, a.w.part_ml,
+                           a.w.o_bytes, a.w.ml_bytes, a.w.counters, a.status);
+  }
+}
+
+// Tiles beside the small-batch decode kernel's workgroups, one a piece and KV head.
+template <typename T, int D, int G>
+__global__ __launch_bounds__(256, kPieceWaves<D>) void shared_piece_kernel(SharedArgs<T> a) {
+  constexpr int A = PieceLds<T, D, G>::BYTES, B = SharedRing<T, D>::BYTES;
+  __shared__ __align__(16) unsigned char smem[A > B ? A : B];
+  const int role = shared_role(blockIdx.x, a.tiles, a.pieces, a.turn);
+  if (role >= 0) {
+    prefill_tile<T, D, G, true>(smem, role, a.q, nullptr, a.kp, a.vp, a.nb, nullptr, nullptr,
+                                a.indices, nullptr, nullptr, a.Hkv, a.sl2, a.status, a.sh);
+  } else {
+    const int bin = ~role / a.Hkv;
+    decode_piece<T, D, G>(smem, ~role - bin * a.Hkv, bin, a.q, a.out, a.kp, a.vp, a.nb, a.plan,
+                          a.stride, a.Hkv, a.sl2, a.kn, a.vn, a.slots, a.w.part_o, a.w.part_ml,
+                          a.w.o_bytes, a.w.ml_bytes, a.w.counters, a.status);
+  }
+}
+
+// The merge of every sequence with shared parts: a wave a KV head; it clears the
+// arrivals that the sequence's own pieces counted.
+template <typename T, int D, int G>
+__global__ __launch_bounds__(64) void shared_merge_kernel(T* out, const int32_t* list,
+                                                          int32_t n_kv_heads, DecodeWorkspace w) {
+  constexpr int NGR = PartLayout<D, G>::NGR;
+  __shared__ __align__(16) float wts[64 * 4 * NGR];
+  const int i = blockIdx.x / n_kv_heads, h = blockIdx.x - i * n_kv_heads;
+  const int32_t* it = list + (int64_t)i * 4;   // {sequence, parts, first slot, 0}
+  const int seq = it[0], parts = it[1], slot0 = it[2];
+  f32x4 none[D / 16];
+#pragma unroll
+  for (int b = 0; b < D / 16; ++b) none[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  merge_head<T, D, G>(out, wts, seq, h, n_kv_heads, parts, slot0, ws_rsrc(w.part_o, w.o_bytes),
+                      ws_rsrc(w.part_ml, w.ml_bytes), false, none, 0.f, 0.f);
+  if (threadIdx.x == 0) w.counters[(int64_t)seq * n_kv_heads + h] = 0;
+}
+
+struct SharedLaunch {
+  const void* q; void* out; void* kp; void* vp; int64_t nb; const int32_t* indices; int32_t Hkv;
+  float sl2; SharedTile sh; int32_t n_tiles; const int32_t* list; int32_t n_list;
+  const int32_t* plan; int32_t n_work, stride; const void* kn; const void* vn;
+  const int32_t* slots; DecodeWorkspace w; int32_t* status; int32_t dtype;
+};
+
+// The decode launch of a plan (decode.hip).
+void run_decode(int32_t dtype, int32_t D, int32_t G, const void* q, void* out, void* kp, void* vp,
+                int64_t nb, const int32_t* plan, int32_t n_work, int32_t stride, int32_t Hkv,
+                float sl2, const void* kn, const void* vn, const int32_t* slots,
+                const DecodeWorkspace& w, int32_t* status, hipStream_t s);
+
+template <typename T, int D, int G>
+static void launch_shared(const SharedLaunch& l, hipStream_t s) {
+  const int groups = l.Hkv / heads_per_wg(l.Hkv);
+  const bool few = few_pieces(l.n_work, l.stride, l.Hkv, D);
+  SharedArgs<T> a{(const T*)l.q, (T*)l.out, (T*)l.kp, (T*)l.vp, l.nb, l.indices, l.Hkv, l.sl2, l.sh,
+                  l.n_tiles, l.plan, l.stride, (const T*)l.kn, (const T*)l.vn, l.slots, l.w,
+                  l.status, l.n_tiles * l.Hkv, few ? l.n_work / groups * l.Hkv : l.n_work,
+                  std::max(1, compute_units())};
+  // A bin's workgroup has a wave a KV head, four at most. With fewer than four
+  // it would leave the launch's other waves idle beside it, so it gets a launch
+  // of its own behind the tiles'.
+  const bool apart = !few && heads_per_wg(l.Hkv) < kMaxWaves;
+  if (apart) a.pieces = 0;
+  const dim3 grid((unsigned)(a.tiles + a.pieces));
+  if (few) {
+    hipLaunchKernelGGL((shared_piece_kernel<T, D, G>), grid, dim3(256), 0, s, a);
+  } else {
+    const size_t lds = std::max<size_t>(decode_lds_bytes<T, D, G>(heads_per_wg(l.Hkv)),
+                                        SharedRing<T, D>::BYTES);
+    hipLaunchKernelGGL((shared_stream_kernel<T, D, G>), grid, dim3(256), lds, s, a);
+  }
+  if (apart)
+    run_decode(l.dtype, D, G, l.q, l.out, l.kp, l.vp, l.nb, l.plan, l.n_work, l.stride, l.Hkv,
+               l.sl2, l.kn, l.vn, l.slots, l.w, l.status, s);
+  hipLaunchKernelGGL((shared_merge_kernel<T, D, G>), dim3((unsigned)(l.n_list * l.Hkv)), dim3(64),
+                     0, s, a.out, l.list, l.Hkv, l.w);
+}
+
+typedef void (*SharedFn)(const SharedLaunch&, hipStream_t);
 
 template <typename T, int D>
 static SharedFn shared_g(int G) {
@@ -144,7 +238,8 @@ extern "C" int pkv_plan_shared(const int32_t* kv_indptr, const int32_t* kv_indic
                                int32_t* plan, int64_t plan_capacity, int64_t* plan_needed,
                                int32_t* n_work_out, int32_t* n_slots_out,
                                int32_t* plan_stride_out, int32_t* tiles, int64_t tiles_capacity,
-                               int64_t* tiles_needed, int32_t* n_tiles_out) {
+                               int64_t* tiles_needed, int32_t* n_tiles_out,
+                               int32_t* n_merges_out) {
   if (n_seqs <= 0 || page_size <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads)
     return fail(PKV_ERR_INVALID, "n_seqs, page_size and heads must be positive, n_heads a "
                 "multiple of n_kv_heads");
@@ -196,7 +291,10 @@ extern "C" int pkv_plan_shared(const int32_t* kv_indptr, const int32_t* kv_indic
     n_members += (int64_t)r.members.size();
     for (int32_t i : r.members) shared[i] += splits;
   }
-  const int64_t want = n_tiles * kSharedItem + n_members * kSharedMember;
+  const int32_t n_merges = (int32_t)std::count_if(shared.begin(), shared.end(),
+                                                  [](int32_t x) { return x > 0; });
+  // items and merges of 8 and 4 ints, members of 2
+  const int64_t want = n_tiles * kSharedItem + (int64_t)n_merges * 4 + n_members * kSharedMember;
   if (tiles_needed) *tiles_needed = want;
   if (want > tiles_capacity || n_tiles * n_kv_heads > 0x7fffffffLL)
     return fail(PKV_ERR_CAPACITY, "shared tiles need %lld entries, capacity %lld",
@@ -224,9 +322,15 @@ extern "C" int pkv_plan_shared(const int32_t* kv_indptr, const int32_t* kv_indic
     it[6] = base[i];
   });
 
-  // Tiles, longest first; a run's members in order, 128 / G of them a tile.
+  // Merges; tiles and members, a run's members in order, 128 / G of them a tile.
   int32_t* item = tiles;
-  int32_t* member = tiles + n_tiles * kSharedItem;
+  int32_t* merge = tiles + n_tiles * kSharedItem;
+  int32_t* member = merge + (int64_t)n_merges * 4;
+  for (int32_t i = 0; i < n_seqs; ++i) {
+    if (!shared[i]) continue;
+    const int32_t vals[4] = {i, shared[i] + pieces[i], base[i], 0};
+    merge = std::copy(vals, vals + 4, merge);
+  }
   int32_t at = 0;
   std::vector<int32_t> next(base.begin(), base.end() - 1);   // each sequence's next shared slot
   for (const Run& r : tree.runs) {
@@ -240,7 +344,7 @@ extern "C" int pkv_plan_shared(const int32_t* kv_indptr, const int32_t* kv_indic
       }
     }
     for (int32_t i : r.members) {
-      const int32_t vals[kSharedMember] = {i, i, next[i], 0};
+      const int32_t vals[kSharedMember] = {i, next[i]};
       member = std::copy(vals, vals + kSharedMember, member);
       next[i] += splits;
     }
@@ -250,6 +354,7 @@ extern "C" int pkv_plan_shared(const int32_t* kv_indptr, const int32_t* kv_indic
   *n_slots_out = base[n_seqs];
   *plan_stride_out = stride;
   *n_tiles_out = (int32_t)n_tiles;
+  *n_merges_out = n_merges;
   return PKV_OK;
 }
 
@@ -257,8 +362,8 @@ extern "C" int pkv_attend_shared(const void* q, void* out, void* k_pool, void* v
                                  int64_t num_blocks, const int32_t* kv_indices, int32_t n_seqs,
                                  int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
                                  int32_t page_size, float scale, int32_t dtype,
-                                 const int32_t* tiles, int32_t n_tiles, const int32_t* plan,
-                                 int32_t n_work, int32_t n_slots, int32_t plan_stride,
+                                 const int32_t* tiles, int32_t n_tiles, int32_t n_merges,
+                                 const int32_t* plan, int32_t n_work, int32_t n_slots, int32_t plan_stride,
                                  const void* k_new, const void* v_new,
                                  const int32_t* slot_mapping, void* workspace,
                                  int64_t workspace_bytes, int32_t* status_word, void* stream) {
@@ -275,21 +380,23 @@ extern "C" int pkv_attend_shared(const void* q, void* out, void* k_pool, void* v
   const uintptr_t al = (uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool |
                        (uintptr_t)k_new | (uintptr_t)v_new;
   if (al % 16) return fail(PKV_ERR_INVALID, "q, out, pools and new rows must be 16-byte aligned");
-  if (n_tiles > 0) {
-    if (!kv_indices || !tiles || n_slots <= 0)
-      return fail(PKV_ERR_INVALID, "shared tiles need kv_indices, tiles and partial slots");
-    DecodeWorkspace w;
-    rc = split_workspace(workspace, workspace_bytes, n_seqs, n_slots, n_heads, n_kv_heads,
-                         head_dim, &w);
-    if (rc) return rc;
-    SharedArgs a{q, k_pool, v_pool, num_blocks, kv_indices, n_kv_heads, scale * kLog2e,
-                 {tiles, tiles + (int64_t)n_tiles * kSharedItem, w.part_o, w.part_ml, w.counters},
-                 n_tiles, status_word};
-    fn(a, (hipStream_t)stream);
-    PKV_LAUNCH_CHECK();
-  }
-  return pkv_attend_decode(q, out, k_pool, v_pool, num_blocks, nullptr, nullptr, nullptr, n_seqs,
-                           n_heads, n_kv_heads, head_dim, page_size, scale, dtype, plan, n_work,
-                           n_slots, plan_stride, k_new, v_new, slot_mapping, workspace,
-                           workspace_bytes, status_word, stream);
+  const int32_t groups = n_kv_heads / heads_per_wg(n_kv_heads);
+  if (!plan || n_work <= 0 || n_work % groups || plan_stride < kHdrInts + kStageMax * kItemInts)
+    return fail(PKV_ERR_INVALID, "shared pages need a plan (pkv_plan_shared)");
+  if (!kv_indices || !tiles || n_tiles <= 0 || n_merges <= 0 || n_merges > n_seqs || n_slots <= 0)
+    return fail(PKV_ERR_INVALID, "shared pages need kv_indices, tiles, merges and partial slots");
+  if ((k_new == nullptr) != (v_new == nullptr) || (k_new && !slot_mapping))
+    return fail(PKV_ERR_INVALID, "a fused append needs k_new, v_new and slot_mapping");
+  if ((int64_t)n_tiles * n_kv_heads + (int64_t)n_work * n_kv_heads > 0x7fffffffLL)
+    return fail(PKV_ERR_INVALID, "too many tiles and pieces in one launch");
+  DecodeWorkspace w;
+  rc = split_workspace(workspace, workspace_bytes, n_seqs, n_slots, n_heads, n_kv_heads, head_dim,
+                       &w);
+  if (rc) return rc;
+  const int32_t* list = tiles + (int64_t)n_tiles * kSharedItem;
+  fn({q, out, k_pool, v_pool, num_blocks, kv_indices, n_kv_heads, scale * kLog2e,
+      {tiles, list + (int64_t)n_merges * 4, w.part_o, w.part_ml}, n_tiles, list, n_merges, plan,
+      n_work, plan_stride, k_new, v_new, slot_mapping, w, status_word, dtype}, (hipStream_t)stream);
+  PKV_LAUNCH_CHECK();
+  return PKV_OK;
 }

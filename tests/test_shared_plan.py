@@ -17,14 +17,14 @@ from llm_serving_layer_amd import _native
 
 def plan_shared(tables, tails, *, n_kv=8, G=4, part=17, wgs=512, min_pages=4, target=512, ps=16,
                 blocks=1 << 20):
-    """Plan and parse: (n_slots, tiles, members, items)."""
+    """Plan and parse: (ids, n_slots, tiles, merges, members, items)."""
     lib = _native.load()
     indptr = np.concatenate([[0], np.cumsum([len(t) for t in tables])]).astype(np.int32)
     ids = np.array([b for t in tables for b in t], np.int32)
     kvl = np.array([(len(t) - 1) * ps + x for t, x in zip(tables, tails)], np.int32)
     last = np.array(tails, np.int32)
     p = lambda a: a.ctypes.data_as(C.c_void_p)  # noqa: E731
-    nw, ns, st, nt = (C.c_int32() for _ in range(4))
+    nw, ns, st, nt, nm = (C.c_int32() for _ in range(5))
     need, tneed = C.c_int64(), C.c_int64()
     cap = tcap = 1
     for _ in range(4):
@@ -32,7 +32,7 @@ def plan_shared(tables, tails, *, n_kv=8, G=4, part=17, wgs=512, min_pages=4, ta
         rc = lib.pkv_plan_shared(p(indptr), p(ids), p(kvl), p(last), len(tables), ps, blocks,
                                  n_kv * G, n_kv, part, wgs, min_pages, target, p(buf), cap,
                                  C.byref(need), C.byref(nw), C.byref(ns), C.byref(st), p(tiles),
-                                 tcap, C.byref(tneed), C.byref(nt))
+                                 tcap, C.byref(tneed), C.byref(nt), C.byref(nm))
         if rc != _native.ERR_CAPACITY:
             break
         cap, tcap = max(cap, need.value), max(tcap, tneed.value)
@@ -47,8 +47,9 @@ def plan_shared(tables, tails, *, n_kv=8, G=4, part=17, wgs=512, min_pages=4, ta
                           [(int(w) >> 27 & 15) + 1 for w in blk[at:at + f[1]]]))
             at += f[1]
     t = tiles[:8 * nt.value].reshape(-1, 8)
-    m = tiles[8 * nt.value:tneed.value].reshape(-1, 4)
-    return ids, ns.value, t, m, items
+    at = 8 * nt.value + 4 * nm.value
+    merges = tiles[8 * nt.value:at].reshape(-1, 4)
+    return ids, ns.value, t, merges, tiles[at:tneed.value].reshape(-1, 2), items
 
 
 def tree(rng, n, depth, ps_pages):
@@ -71,15 +72,14 @@ def tree(rng, n, depth, ps_pages):
 
 
 def check(tables, tails, **kw):
-    ids, n_slots, tiles, members, items = plan_shared(tables, tails, **kw)
+    ids, n_slots, tiles, merges, members, items = plan_shared(tables, tails, **kw)
     G, min_pages = kw.get("G", 4), kw.get("min_pages", 4)
     read = {i: [] for i in range(len(tables))}
     slots = {i: [] for i in range(len(tables))}
     for first, pages, at, count, split, *rest in tiles.tolist():
         assert 1 <= count <= 128 // G and pages >= 1 and not any(rest)
         run = ids[first:first + pages].tolist()
-        for row, seq, slot, _ in members[at:at + count].tolist():
-            assert row == seq
+        for seq, slot in members[at:at + count].tolist():
             read[seq] += run
             slots[seq].append(slot + split)
     shared = {i: len(s) for i, s in slots.items()}
@@ -104,6 +104,7 @@ def check(tables, tails, **kw):
             assert sorted(slots[i]) == list(range(min(slots[i]), min(slots[i]) + len(slots[i])))
             assert set(parts) == {len(slots[i])}
             assert {f[6] for f, _, _ in items if f[0] == i} == {min(slots[i])}
+    assert merges.tolist() == [[i, len(slots[i]), min(slots[i]), 0] for i in shared if shared[i]]
     used = sorted(s for v in slots.values() for s in v)
     assert used == list(range(n_slots)), "no two parts share a slot"
     return tiles, members, min_pages
@@ -161,7 +162,8 @@ def test_refusals():
         one = (C.c_int32 * 2)(0, 2)
         ids, kv, last = (C.c_int32 * 2)(1, 2), (C.c_int32 * 1)(20), (C.c_int32 * 1)(5)
         _native.check(lib.pkv_plan_shared(one, ids, kv, last, 1, 16, 8, 8, 2, 17, 4, 4, 8, None,
-                                          0, None, None, None, None, None, 0, None, None), "plan")
+                                          0, None, None, None, None, None, 0, None, None, None),
+                      "plan")
     for kw, match in (({"G": 3}, "not supported"), ({"min_pages": 0}, "not supported"),
                       ({"target": 0}, "not supported"), ({"part": 0}, "part_pages")):
         with pytest.raises(ValueError, match=match):
@@ -173,7 +175,7 @@ def test_launch_refusals():
 
     def call(n_heads=8, d=64, page=16, dtype=0, scale=0.1, q=16, tiles=16, n_slots=4, ws=0):
         return lib.pkv_attend_shared(q, 16, 16, 16, 8, 16, 2, n_heads, 2, d, page, scale, dtype,
-                                     tiles, 1, 16, 1, n_slots, 72, None, None, None, None, ws,
+                                     tiles, 1, 1, 16, 1, n_slots, 72, None, None, None, None, ws,
                                      None, None)
     for kw, match in (({"d": 80}, "fast decode path"), ({"dtype": 2}, "fast decode path"),
                       ({"page": 8}, "fast decode path"), ({"n_heads": 6}, "fast decode path"),

@@ -99,6 +99,17 @@ struct SharedTile {
 };
 constexpr int kSharedItem = 8, kSharedMember = 2;   // ints of each
 
+// The swizzle of a shared tile's rows (16-byte chunk c of row r at chunk
+// position c ^ wide_xr(r)): LDS hands 256 bytes a cycle to 16 lanes of a 16-byte
+// read, or 32 of an 8-byte one. 16 rows read at one chunk (K) and four rows,
+// from a multiple of four on, at four chunks, from a multiple of four on (V),
+// then meet 16 different positions of the 256 bytes; a row of 128 bytes is half
+// of them. (By the eight-row swizzle of the other kernels half of the LDS
+// cycles were bank conflicts.)
+template <int RB> __device__ __forceinline__ int wide_xr(int row) {
+  return RB == 128 ? ((row >> 1) & 1) << 2 | ((row >> 2) & 3) : (row & 3) << 2 | ((row >> 2) & 3);
+}
+
 // A shared tile's ring: as many buffers as fit 80 KiB (two workgroups a compute
 // unit; at head_dim 64 eight are enough), tiles loaded RING - 2 ahead. Such a
 // tile has at most one more workgroup beside it, so its own loads have to cover
@@ -207,7 +218,8 @@ __device__ __forceinline__ void prefill_tile(
 #pragma unroll
   for (int k = 0; k < LPT; ++k) {
     const int rr = k * RPI + lane / CPR;
-    const int lc = ((lane % CPR) ^ xr(rr)) & 7 | ((lane % CPR) & ~7);
+    const int lc = SHARED ? (lane % CPR) ^ wide_xr<RB>(rr)
+                          : ((lane % CPR) ^ xr(rr)) & 7 | ((lane % CPR) & ~7);
     voff[k] = (uint32_t)rr * rowbytes + (uint32_t)(h * RB + lc * 16);
   }
   auto load_id = [&](int t) {   // this wave's page id for tile t
@@ -237,6 +249,10 @@ __device__ __forceinline__ void prefill_tile(
   const int vrow = lane & 15;
   const int vcol = (lane & 16) + 4 * (vrow & 3);
 
+  // element e of row `row` of a tile
+  auto in_tile = [&](int row, int e) __attribute__((always_inline)) {
+    return SHARED ? row * RB + ((e >> 3) ^ wide_xr<RB>(row)) * 16 + (e & 7) * 2 : swz<RB>(row, e);
+  };
   // P^T of the previous tile (the B operand of its PV), kept for the next step.
   vec8 pb[NH * 2];
 #pragma unroll
@@ -250,9 +266,9 @@ __device__ __forceinline__ void prefill_tile(
 #pragma unroll
       for (int dh = 0; dh < NDH; ++dh) {
         const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_i16x4*)(vl + swz<RB>(key, vcol + 32 * dh)));
+            (lds_i16x4*)(vl + in_tile(key, vcol + 32 * dh)));
         const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_i16x4*)(vl + swz<RB>(key + 8, vcol + 32 * dh)));
+            (lds_i16x4*)(vl + in_tile(key + 8, vcol + 32 * dh)));
         va[kb * NDH + dh] = __builtin_bit_cast(
             vec8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
       }
@@ -278,17 +294,38 @@ __device__ __forceinline__ void prefill_tile(
     const bool full = t0 + TT - 1 <= base_pos;
     // the previous tile's V operands, read while QK runs
     vec8 va[NH * 2 * NDH];
-    read_v(vprev, va);
     // S^T = K Q^T: s[hf][rr] = score of key t0 + 32 hf + 8 (rr / 4) + 4 g + rr % 4.
     f32x16 s[NH];
+    if constexpr (SHARED) {
+      // One wave a SIMD runs such tiles, in step with the workgroup's others:
+      // K is read first, so that QK starts while V is still being read.
+      vec8 ka[NH * NC];
 #pragma unroll
-    for (int hf = 0; hf < NH; ++hf) {
-      s[hf] = f32x16{};
-      const int kr = hf * 32 + n;
+      for (int hf = 0; hf < NH; ++hf)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          ka[hf * NC + c] =
+              *reinterpret_cast<const vec8*>(kl + in_tile(hf * 32 + n, 16 * c + 8 * g));
+      asm volatile("" ::: "memory");
+      read_v(vprev, va);
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int hf = 0; hf < NH; ++hf) s[hf] = f32x16{};
 #pragma unroll
       for (int c = 0; c < NC; ++c)
-        s[hf] = Mma32<T>::mma(*reinterpret_cast<const vec8*>(kl + swz<RB>(kr, 16 * c + 8 * g)),
-                              qb[c], s[hf]);
+#pragma unroll
+        for (int hf = 0; hf < NH; ++hf) s[hf] = Mma32<T>::mma(ka[hf * NC + c], qb[c], s[hf]);
+    } else {
+      read_v(vprev, va);
+#pragma unroll
+      for (int hf = 0; hf < NH; ++hf) {
+        s[hf] = f32x16{};
+        const int kr = hf * 32 + n;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          s[hf] = Mma32<T>::mma(*reinterpret_cast<const vec8*>(kl + in_tile(kr, 16 * c + 8 * g)),
+                                qb[c], s[hf]);
+      }
     }
     // Keys past the row's position are masked only on tiles that reach them.
     if (!full) {

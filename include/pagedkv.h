@@ -93,6 +93,25 @@ int pkv_append_rotated(void* k_pool, void* v_pool, int64_t num_slots, const void
                        int32_t* status_word, void* stream);
 
 /*
+ * pkv_append_rotated with the arguments that do not change from layer to layer
+ * set once, and, where n_complete is not 0, pkv_page_bounds of the pages
+ * `complete` that these rows complete, in the layer whose bounds lo and hi are.
+ */
+typedef struct pkv_rotated {
+  int64_t num_blocks, n_tokens, max_positions, n_complete;
+  const int32_t* slot_mapping;
+  const int64_t* positions;
+  const float* table;
+  const int32_t* complete;
+  int32_t* status_word;
+  int32_t n_heads, n_kv_heads, head_dim, page_size, dtype, rotary_dim, interleaved, reserved;
+} pkv_rotated;
+
+int pkv_append_rotated_batch(const void* batch, void* k_pool, void* v_pool, const void* q,
+                             int64_t q_stride, void* q_out, const void* k, int64_t k_stride,
+                             const void* v, int64_t v_stride, void* lo, void* hi, void* stream);
+
+/*
  * Decode plan (host function, synchronous, no device access) — the
  * counterpart of the reference fast path's plan step
  * (serving/backends/flashinfer_backend.py:566-676), computed once per batch
@@ -367,6 +386,26 @@ int pkv_attend_shared(const void* q, void* out, void* k_pool, void* v_pool, int6
                       void* stream);
 
 /*
+ * pkv_attend_shared with the arguments that do not change from layer to layer
+ * set once.
+ */
+typedef struct pkv_shared {
+  int64_t num_blocks, workspace_bytes;
+  const int32_t* kv_indices;
+  const int32_t* tiles;
+  const int32_t* plan;
+  const int32_t* slot_mapping;
+  void* workspace;
+  int32_t* status_word;
+  int32_t n_seqs, n_heads, n_kv_heads, head_dim, page_size, dtype;
+  int32_t n_tiles, n_merges, n_work, n_slots, plan_stride, reserved;
+} pkv_shared;
+
+int pkv_attend_shared_batch(const void* batch, const void* q, void* out, void* k_pool,
+                            void* v_pool, float scale, const void* k_new, const void* v_new,
+                            void* stream);
+
+/*
  * Key bounds of pages — no counterpart in the reference. For each of the
  * n_ids pages of ids (NULL: pages 0 .. n_ids - 1) and each of n_layers layers,
  * row id of lo and hi ([num_blocks, n_kv_heads, head_dim], the pool dtype)
@@ -422,6 +461,28 @@ int pkv_attend_selected(const void* q, void* out, void* k_pool, void* v_pool, in
                         int32_t n_kv_heads, int32_t head_dim, int32_t page_size, float scale,
                         int32_t dtype, void* workspace, int64_t workspace_bytes,
                         int32_t* status_word, void* stream);
+
+/*
+ * pkv_select_pages and pkv_attend_selected of one layer, with the arguments
+ * that do not change from layer to layer set once. lo and hi are the layer's
+ * bounds.
+ */
+typedef struct pkv_selected {
+  int64_t num_blocks, workspace_bytes;
+  const int32_t* kv_indptr;
+  const int32_t* kv_indices;
+  const int32_t* kv_lens;
+  double* scores;
+  int32_t* ids;
+  void* workspace;
+  int32_t* status_word;
+  int32_t n_seqs, max_pages, pages, part_pages;
+  int32_t n_heads, n_kv_heads, head_dim, page_size, dtype, reserved;
+} pkv_selected;
+
+int pkv_attend_selected_batch(const void* batch, const void* q, void* out, void* k_pool,
+                              void* v_pool, const void* lo, const void* hi, int32_t* ordinals,
+                              float scale, void* stream);
 
 /*
  * Batched block copy over every layer, K and V — replaces

@@ -66,6 +66,10 @@ SIGNATURES = {
                                                  _i64, _i32]),
     "pkv_attend_selected": (C.c_int, [_p, _p, _p, _p, _i64, _p, _p, _i32, _i32, _i32, _i32, _i32,
                                       _i32, _i32, _i32, _f32, _i32, _p, _i64, _p, _p]),
+    "pkv_append_rotated_batch": (C.c_int, [_p, _p, _p, _p, _i64, _p, _p, _i64, _p, _i64, _p, _p,
+                                           _p]),
+    "pkv_attend_shared_batch": (C.c_int, [_p, _p, _p, _p, _p, _f32, _p, _p, _p]),
+    "pkv_attend_selected_batch": (C.c_int, [_p, _p, _p, _p, _p, _p, _p, _p, _f32, _p]),
     "pkv_copy_blocks": (C.c_int, [_p, _i32, _i64, _i64, _i64, _p, _p, _i32, _p, _p]),
     "pkv_gather_blocks": (C.c_int, [_p, _i32, _i64, _i64, _i64, _p, _i32, _p, _p, _p]),
     "pkv_scatter_blocks": (C.c_int, [_p, _i32, _i64, _i64, _i64, _p, _i32, _p, _p, _p]),
@@ -84,6 +88,38 @@ class Batch(C.Structure):
             "n_seqs", "n_tokens", "n_heads", "n_kv_heads", "head_dim", "page_size", "dtype",
             "is_prefill", "n_tiles", "q_tile", "n_decodes", "n_work", "n_slots",
             "plan_stride")]]
+
+
+class Rotated(C.Structure):
+    """``pkv_rotated``: an ``append_kv_rotated``'s arguments, set once per plan."""
+
+    _fields_ = [*[(n, _i64) for n in ("num_blocks", "n_tokens", "max_positions", "n_complete")],
+                *[(n, _p) for n in ("slot_mapping", "positions", "table", "complete",
+                                    "status_word")],
+                *[(n, _i32) for n in ("n_heads", "n_kv_heads", "head_dim", "page_size", "dtype",
+                                      "rotary_dim", "interleaved", "reserved")]]
+
+
+class Shared(C.Structure):
+    """``pkv_shared``: an ``attend_shared``'s arguments, set once per plan."""
+
+    _fields_ = [("num_blocks", _i64), ("workspace_bytes", _i64),
+                *[(n, _p) for n in ("kv_indices", "tiles", "plan", "slot_mapping", "workspace",
+                                    "status_word")],
+                *[(n, _i32) for n in ("n_seqs", "n_heads", "n_kv_heads", "head_dim", "page_size",
+                                      "dtype", "n_tiles", "n_merges", "n_work", "n_slots",
+                                      "plan_stride", "reserved")]]
+
+
+class Selected(C.Structure):
+    """``pkv_selected``: an ``attend_selected``'s arguments, set once per plan."""
+
+    _fields_ = [("num_blocks", _i64), ("workspace_bytes", _i64),
+                *[(n, _p) for n in ("kv_indptr", "kv_indices", "kv_lens", "scores", "ids",
+                                    "workspace", "status_word")],
+                *[(n, _i32) for n in ("n_seqs", "max_pages", "pages", "part_pages", "n_heads",
+                                      "n_kv_heads", "head_dim", "page_size", "dtype",
+                                      "reserved")]]
 
 
 _LIB = None

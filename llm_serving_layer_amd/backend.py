@@ -151,6 +151,10 @@ def unavailable_reason() -> str | None:
 
 
 _HERE = contextlib.nullcontext()
+# (the plain queries: torch.cuda's own check first whether it is initialised)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing",
+                     torch.cuda.is_current_stream_capturing)
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
@@ -188,7 +192,8 @@ class _Pending:
 class _Rows:
     """Where one BatchMeta's new rows go, on the device (``append_kv_rotated``)."""
 
-    __slots__ = ("meta", "slots", "positions", "far", "complete", "buffers", "stream")
+    __slots__ = ("meta", "slots", "positions", "complete", "table", "args", "ptr", "buffers",
+                 "stream")
 
 
 class _Shared:
@@ -196,14 +201,14 @@ class _Shared:
     worth sharing (``n_tiles`` 0: the batch takes ``attend``)."""
 
     __slots__ = ("meta", "n", "n_tiles", "n_merges", "tiles", "plan", "indices", "slots", "n_work", "n_slots",
-                 "stride", "ws", "fusable", "buffers", "stream")
+                 "stride", "ws", "fusable", "args", "ptr", "buffers", "stream")
 
 
 class _Selected:
     """What ``attend_selected`` keeps for one BatchMeta and page budget."""
 
     __slots__ = ("meta", "pages", "n", "max_pages", "indptr", "indices", "kv_lens", "scores",
-                 "ids", "ordinals", "part", "ws", "buffers", "stream")
+                 "ids", "ordinals", "part", "ws", "width", "args", "ptr", "buffers", "stream")
 
 
 class MI355XBackend:
@@ -318,6 +323,10 @@ class MI355XBackend:
         if page_bounds:
             self._bounds = torch.zeros((num_layers, 2, num_blocks, n_kv_heads, head_dim),
                                        dtype=dtype, device=self.device)
+            half = self._bounds.stride(1) * self._bounds.element_size()
+            at = self._bounds.data_ptr()
+            self._bounds_ptr = [(at + 2 * l * half, at + (2 * l + 1) * half)
+                                for l in range(num_layers)]
         # what graphs were captured with: it stays as long as the backend
         self._captured: list = []
         self._slot_cache: tuple[BatchMeta, torch.Tensor] | None = None
@@ -485,12 +494,11 @@ class MI355XBackend:
     def _renew_bounds(self, ids, n: int, stream: int, layer: int | None = None) -> None:
         """Bounds of the blocks ``ids`` (device int32; None: the pool's first
         ``n``) in one layer or in all of them."""
-        l, b = layer or 0, self._bounds
-        half = b.stride(1) * b.element_size()
-        at = b.data_ptr() + 2 * l * half
+        l = layer or 0
+        lo, hi = self._bounds_ptr[l]
         with self._on_device():
             rc = self._lib.pkv_page_bounds(
-                self._k_ptr[l], 2 * self._plane_bytes, at, at + half, 2 * half,
+                self._k_ptr[l], 2 * self._plane_bytes, lo, hi, 2 * (hi - lo),
                 self.num_layers if layer is None else 1, self.num_blocks,
                 None if ids is None else ids.data_ptr(), n, self.n_kv_heads, self.head_dim,
                 self.block_size, self._code, self._status_ptr, stream)
@@ -564,72 +572,103 @@ class MI355XBackend:
             self._check_layer(layer_idx)
         if meta.slot_mapping is None:
             raise ValueError("MI355XBackend.append_kv_rotated requires meta.slot_mapping")
-        tokens, d = q.shape[0], self.head_dim
-        for name, x, h in (("q", q, self.n_heads), ("k", k, self.n_kv_heads),
-                           ("v", v, self.n_kv_heads)):
-            if x.shape != (tokens, h, d):
-                raise ValueError(f"{name} has shape {tuple(x.shape)}, expected "
-                                 f"({tokens}, {h}, {d})")
+        tokens, d, hkv = q.shape[0], self.head_dim, self.n_kv_heads
+        if q.shape != (tokens, self.n_heads, d):
+            raise ValueError(f"q has shape {tuple(q.shape)}, expected "
+                             f"({tokens}, {self.n_heads}, {d})")
+        if k.shape != (tokens, hkv, d):
+            raise ValueError(f"k has shape {tuple(k.shape)}, expected ({tokens}, {hkv}, {d})")
+        if v.shape != k.shape:
+            raise ValueError(f"v has shape {tuple(v.shape)}, expected ({tokens}, {hkv}, {d})")
         if meta.slot_mapping.shape[0] != tokens or meta.n_tokens != tokens:
             raise ValueError(f"meta describes {meta.n_tokens} tokens and "
                              f"{meta.slot_mapping.shape[0]} slots but {tokens} tokens were "
                              "supplied")
-        if not isinstance(table, RotaryTable):
-            raise TypeError(f"table must be a RotaryTable, got {type(table).__name__}")
-        if table.device != self.device:
-            raise ValueError(f"the rotation table is on {table.device}, the pool on "
-                             f"{self.device}")
-        if table.rotary_dim > d:
-            raise ValueError(f"rotary_dim={table.rotary_dim} exceeds head_dim={d}")
         r = self._rows
-        if r is not None and r.meta is not meta:
-            r = None
-        far = r.far if r is not None else self._last_position(meta)
-        if far >= table.max_positions:
-            raise ValueError(f"position {far} is outside the rotation table of "
-                             f"{table.max_positions} positions")
-        if r is None:
-            r = self._rows_for(meta)
+        if r is None or r.meta is not meta or r.table is not table:
+            r = self._rows_for(meta, table)
         if self._pending is not None:
             self._flush()
         q, k, v = self._token_rows(q), self._token_rows(k), self._token_rows(v)
         stream = self._enter(r)
         out = torch.empty((tokens, self.n_heads, d), dtype=self.dtype, device=self.device)
+        lo, hi = self._bounds_ptr[layer_idx] if r.complete is not None else (None, None)
         with self._on_device():
-            rc = self._lib.pkv_append_rotated(
-                self._k_ptr[layer_idx], self._v_ptr[layer_idx], self.num_blocks * self.block_size,
-                q.data_ptr(), q.stride(0), out.data_ptr(), k.data_ptr(), k.stride(0),
-                v.data_ptr(), v.stride(0), r.slots.data_ptr(), r.positions.data_ptr(), tokens,
-                table.table.data_ptr(), table.max_positions, table.rotary_dim, table.interleaved,
-                self.n_heads, self.n_kv_heads, d, self._code, self._status_ptr, stream)
+            rc = self._lib.pkv_append_rotated_batch(
+                r.ptr, self._k_ptr[layer_idx], self._v_ptr[layer_idx], q.data_ptr(), q.stride(0),
+                out.data_ptr(), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), lo, hi,
+                stream)
         if rc:
             _native.check(rc, "append_kv_rotated")
-        if self._bounds is not None:
-            self._complete_bounds(layer_idx, meta)
         return out
 
-    @staticmethod
-    def _last_position(meta: BatchMeta) -> int:
-        """The meta's furthest position as far as the host knows it (else -1)."""
-        mirror = meta.host_arrays()
-        return int(mirror["kv_lens"].max()) - 1 if mirror is not None else -1
+    def _check_table(self, meta: BatchMeta, table) -> None:
+        if not isinstance(table, RotaryTable):
+            raise TypeError(f"table must be a RotaryTable, got {type(table).__name__}")
+        if table.device != self.device:
+            raise ValueError(f"the rotation table is on {table.device}, the pool on "
+                             f"{self.device}")
+        if table.rotary_dim > self.head_dim:
+            raise ValueError(f"rotary_dim={table.rotary_dim} exceeds head_dim={self.head_dim}")
+        mirror = meta.host_arrays()   # (without one the kernel flags it)
+        far = int(mirror["kv_lens"].max()) - 1 if mirror is not None else -1
+        if far >= table.max_positions:
+            raise ValueError(f"position {far} is outside the rotation table of "
+                             f"{table.max_positions} positions")
 
-    def _rows_for(self, meta: BatchMeta) -> _Rows:
-        """The meta's slots and positions on the device, once per meta."""
-        r = _Rows()
-        r.slots = self._slots_for(meta)
-        r.positions = meta.positions.to(device=self.device, dtype=torch.int64).contiguous()
-        r.far = self._last_position(meta)
-        r.complete = None
-        if self._bounds is not None:
-            pages = self._completed_pages(meta)
-            if pages.shape[0]:
-                r.complete = self._upload(pages)
-        r.buffers = [t for t in (r.slots, r.positions, r.complete) if t is not None]
-        r.stream = _current_stream(self.device)
-        r.meta = meta
+    def _rows_for(self, meta: BatchMeta, table: RotaryTable | None = None) -> _Rows:
+        """The meta's slots, positions and completed pages on the device, once
+        per meta, described for appends that rotate by ``table``."""
+        if table is not None:
+            self._check_table(meta, table)
+        r = self._rows
+        if r is None or r.meta is not meta:
+            r = _Rows()
+            r.slots = self._slots_for(meta)
+            r.positions = meta.positions.to(device=self.device, dtype=torch.int64).contiguous()
+            r.complete = None
+            if self._bounds is not None:
+                pages = self._completed_pages(meta)
+                if pages.shape[0]:
+                    r.complete = self._upload(pages)
+            r.buffers = [t for t in (r.slots, r.positions, r.complete) if t is not None]
+            r.stream = _current_stream(self.device)
+            r.meta = meta
+        else:   # another table: what a captured launch read stays described as it was
+            old, r = r, _Rows()
+            for name in ("meta", "slots", "positions", "complete", "buffers", "stream"):
+                setattr(r, name, getattr(old, name))
+        r.table = table
+        r.args = r.ptr = None
+        if table is not None:
+            r.args = _native.Rotated(
+                num_blocks=self.num_blocks, n_tokens=r.positions.shape[0],
+                max_positions=table.max_positions,
+                n_complete=0 if r.complete is None else r.complete.shape[0],
+                slot_mapping=r.slots.data_ptr(), positions=r.positions.data_ptr(),
+                table=table.table.data_ptr(),
+                complete=None if r.complete is None else r.complete.data_ptr(),
+                status_word=self._status_ptr, n_heads=self.n_heads, n_kv_heads=self.n_kv_heads,
+                head_dim=self.head_dim, page_size=self.block_size, dtype=self._code,
+                rotary_dim=table.rotary_dim, interleaved=table.interleaved)
+            r.ptr = C.addressof(r.args)
         self._rows = r
         return r
+
+    def _token_rows(self, x: torch.Tensor) -> torch.Tensor:
+        """x in the pool dtype on this device, heads contiguous in each token's
+        row, rows any distance apart."""
+        if x.dtype is self.dtype and x.get_device() == self.device.index:
+            _, head, one = x.stride()
+            if one == 1 and head == self.head_dim:
+                return x
+        return x.to(device=self.device, dtype=self.dtype).contiguous()
+
+    def _on_device(self):
+        """Launches go to this backend's device, whichever is current."""
+        if _current_device() == self.device.index:
+            return _HERE
+        return torch.cuda.device(self.device)
 
     def _completed_pages(self, meta: BatchMeta) -> np.ndarray:
         """Pages whose last row this meta's append writes: the bounds of a page
@@ -654,20 +693,6 @@ class MI355XBackend:
             r = self._rows_for(meta)
         if r.complete is not None:
             self._renew_bounds(r.complete, r.complete.shape[0], self._enter(r), layer)
-
-    def _token_rows(self, x: torch.Tensor) -> torch.Tensor:
-        """x in the pool dtype on this device, heads contiguous in each token's
-        row, rows any distance apart."""
-        if (x.dtype is self.dtype and x.get_device() == self.device.index
-                and (x.is_contiguous() or (x.stride(2) == 1 and x.stride(1) == x.shape[2]))):
-            return x
-        return x.to(device=self.device, dtype=self.dtype).contiguous()
-
-    def _on_device(self):
-        """Launches go to this backend's device, whichever is current."""
-        if torch.cuda.current_device() == self.device.index:
-            return _HERE
-        return torch.cuda.device(self.device)
 
     def _slots_for(self, meta: BatchMeta) -> torch.Tensor:
         p = self._planned
@@ -793,19 +818,19 @@ class MI355XBackend:
         elif pend is not None:
             self._flush()
         stream = self._enter(p)
-        q = self._as_pool(q)
-        if q.data_ptr() % 16:
+        if not (q.dtype is self.dtype and q.get_device() == self.device.index
+                and q.is_contiguous()):
+            q = self._as_pool(q)
+        q_ptr = q.data_ptr()
+        if q_ptr % 16:
             q = q.clone()
+            q_ptr = q.data_ptr()
         out = torch.empty_like(q)
         with self._on_device():
-            rc = self._lib.pkv_attend_shared(
-                q.data_ptr(), out.data_ptr(), self._k_ptr[layer_idx], self._v_ptr[layer_idx],
-                self.num_blocks, p.indices.data_ptr(), p.n, self.n_heads, self.n_kv_heads,
-                self.head_dim, self.block_size, float(scale), self._code, p.tiles.data_ptr(),
-                p.n_tiles, p.n_merges, p.plan.data_ptr(), p.n_work, p.n_slots, p.stride,
-                pend.k.data_ptr() if fused else None, pend.v.data_ptr() if fused else None,
-                p.slots.data_ptr() if fused else None, p.ws.data_ptr(), p.ws.numel(),
-                self._status_ptr, stream)
+            rc = self._lib.pkv_attend_shared_batch(
+                p.ptr, q_ptr, out.data_ptr(), self._k_ptr[layer_idx], self._v_ptr[layer_idx],
+                float(scale), pend.k.data_ptr() if fused else None,
+                pend.v.data_ptr() if fused else None, stream)
         if rc:
             _native.check(rc, "attend_shared")
         self.n_runs += 1
@@ -867,6 +892,15 @@ class MI355XBackend:
         p.slots = self._dev_i32(meta.slot_mapping) if meta.slot_mapping is not None else None
         p.ws = self._counted_workspace(need, p.n)
         p.buffers = [t for t in (p.plan, p.tiles, p.indices, p.slots, p.ws) if t is not None]
+        p.args = _native.Shared(
+            num_blocks=self.num_blocks, workspace_bytes=need, kv_indices=p.indices.data_ptr(),
+            tiles=p.tiles.data_ptr(), plan=p.plan.data_ptr(),
+            slot_mapping=None if p.slots is None else p.slots.data_ptr(),
+            workspace=p.ws.data_ptr(), status_word=self._status_ptr, n_seqs=p.n,
+            n_heads=self.n_heads, n_kv_heads=self.n_kv_heads, head_dim=self.head_dim,
+            page_size=self.block_size, dtype=self._code, n_tiles=p.n_tiles, n_merges=p.n_merges,
+            n_work=p.n_work, n_slots=p.n_slots, plan_stride=p.stride)
+        p.ptr = C.addressof(p.args)
         self.n_plans += 1
 
     def _counted_workspace(self, need: int, n: int) -> torch.Tensor:
@@ -913,29 +947,21 @@ class MI355XBackend:
         if not (q.dtype is self.dtype and q.get_device() == self.device.index
                 and q.is_contiguous()):
             q = self._as_pool(q)
-        if q.data_ptr() % 16:
+        q_ptr = q.data_ptr()
+        if q_ptr % 16:
             q = q.clone()
+            q_ptr = q.data_ptr()
         out = torch.empty_like(q)
-        width = min(p.pages, p.max_pages)
+        ordinals = p.ordinals
         if return_pages:
-            ordinals = torch.empty((p.n, self.n_kv_heads, width), dtype=torch.int32,
+            ordinals = torch.empty((p.n, self.n_kv_heads, p.width), dtype=torch.int32,
                                    device=self.device)
-        else:
-            ordinals = p.ordinals
-        b = self._bounds[layer_idx]
+        lo, hi = self._bounds_ptr[layer_idx]
         with self._on_device():
-            rc = self._lib.pkv_select_pages(
-                q.data_ptr(), b[0].data_ptr(), b[1].data_ptr(), self.num_blocks,
-                p.indptr.data_ptr(), p.indices.data_ptr(), p.kv_lens.data_ptr(), p.n,
-                p.max_pages, p.pages, self.n_heads, self.n_kv_heads, self.head_dim,
-                self.block_size, self._code, p.scores.data_ptr(), p.ids.data_ptr(),
-                ordinals.data_ptr(), self._status_ptr, stream)
-            _native.check(rc, "attend_selected (choice)")
-            rc = self._lib.pkv_attend_selected(
-                q.data_ptr(), out.data_ptr(), self._k_ptr[layer_idx], self._v_ptr[layer_idx],
-                self.num_blocks, p.ids.data_ptr(), p.kv_lens.data_ptr(), p.n, p.max_pages,
-                p.pages, p.part, self.n_heads, self.n_kv_heads, self.head_dim, self.block_size,
-                float(scale), self._code, p.ws.data_ptr(), p.ws.numel(), self._status_ptr, stream)
+            rc = self._lib.pkv_attend_selected_batch(
+                p.ptr, q_ptr, out.data_ptr(), self._k_ptr[layer_idx], self._v_ptr[layer_idx],
+                lo, hi, ordinals.data_ptr(), float(scale), stream)
+        if rc:
             _native.check(rc, "attend_selected")
         self.n_runs += 1
         return (out, ordinals) if return_pages else out
@@ -949,7 +975,7 @@ class MI355XBackend:
         self._check_pages(kvl, indptr, last, int(indices.shape[0]))
         p = _Selected()
         p.pages, p.n, p.max_pages = pages, n, int(np.diff(indptr).max())
-        width = min(pages, p.max_pages)
+        width = p.width = min(pages, p.max_pages)
         dev = {"device": self.device}
         p.indptr = self._dev_i32(meta.kv_indptr)
         p.indices = self._dev_i32(meta.kv_indices)
@@ -969,6 +995,14 @@ class MI355XBackend:
             p.part = min(2 * p.part, MAX_PART_PAGES)
         p.ws = self._counted_workspace(need, n)
         p.buffers = [p.indptr, p.indices, p.kv_lens, p.scores, p.ids, p.ordinals, p.ws]
+        at = lambda t: t.data_ptr() if t.numel() else None  # noqa: E731
+        p.args = _native.Selected(
+            num_blocks=self.num_blocks, workspace_bytes=need, kv_indptr=at(p.indptr),
+            kv_indices=at(p.indices), kv_lens=at(p.kv_lens), scores=at(p.scores), ids=at(p.ids),
+            workspace=at(p.ws), status_word=self._status_ptr, n_seqs=n, max_pages=p.max_pages,
+            pages=pages, part_pages=p.part, n_heads=self.n_heads, n_kv_heads=self.n_kv_heads,
+            head_dim=self.head_dim, page_size=self.block_size, dtype=self._code)
+        p.ptr = C.addressof(p.args)
         p.stream = _current_stream(self.device)
         p.meta = meta
         self._selected = p
@@ -995,7 +1029,7 @@ class MI355XBackend:
         launches of one plan share its buffers. A plan that a graph captures
         stays as long as the backend does."""
         stream = _current_stream(self.device)
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing():
             if not any(c is p for c in self._captured):
                 self._captured.append(p)
         elif p.stream != stream:

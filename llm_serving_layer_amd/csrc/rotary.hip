@@ -164,3 +164,21 @@ extern "C" int pkv_append_rotated(void* k_pool, void* v_pool, int64_t num_slots,
   if (dtype == PKV_DTYPE_BF16) return launch_rotated<__bf16>(a, wide, s);
   return launch_rotated<float>(a, wide, s);
 }
+
+static_assert(sizeof(pkv_rotated) == 104, "the layout the Python binding fills");
+
+extern "C" int pkv_append_rotated_batch(const void* batch, void* k_pool, void* v_pool,
+                                        const void* q, int64_t q_stride, void* q_out,
+                                        const void* k, int64_t k_stride, const void* v,
+                                        int64_t v_stride, void* lo, void* hi, void* stream) {
+  if (!batch) return fail(PKV_ERR_INVALID, "null batch");
+  const pkv_rotated& b = *static_cast<const pkv_rotated*>(batch);
+  const int rc = pkv_append_rotated(k_pool, v_pool, b.num_blocks * b.page_size, q, q_stride, q_out,
+                                    k, k_stride, v, v_stride, b.slot_mapping, b.positions,
+                                    b.n_tokens, b.table, b.max_positions, b.rotary_dim,
+                                    b.interleaved, b.n_heads, b.n_kv_heads, b.head_dim, b.dtype,
+                                    b.status_word, stream);
+  if (rc || b.n_complete <= 0) return rc;
+  return pkv_page_bounds(k_pool, 0, lo, hi, 0, 1, b.num_blocks, b.complete, b.n_complete,
+                         b.n_kv_heads, b.head_dim, b.page_size, b.dtype, b.status_word, stream);
+}

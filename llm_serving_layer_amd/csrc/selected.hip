@@ -199,3 +199,22 @@ extern "C" int pkv_attend_selected(const void* q, void* out, void* k_pool, void*
   PKV_LAUNCH_CHECK();
   return PKV_OK;
 }
+
+static_assert(sizeof(pkv_selected) == 112, "the layout the Python binding fills");
+
+extern "C" int pkv_attend_selected_batch(const void* batch, const void* q, void* out,
+                                         void* k_pool, void* v_pool, const void* lo,
+                                         const void* hi, int32_t* ordinals, float scale,
+                                         void* stream) {
+  if (!batch) return fail(PKV_ERR_INVALID, "null batch");
+  const pkv_selected& b = *static_cast<const pkv_selected*>(batch);
+  const int rc = pkv_select_pages(q, lo, hi, b.num_blocks, b.kv_indptr, b.kv_indices, b.kv_lens,
+                                  b.n_seqs, b.max_pages, b.pages, b.n_heads, b.n_kv_heads,
+                                  b.head_dim, b.page_size, b.dtype, b.scores, b.ids, ordinals,
+                                  b.status_word, stream);
+  if (rc) return rc;
+  return pkv_attend_selected(q, out, k_pool, v_pool, b.num_blocks, b.ids, b.kv_lens, b.n_seqs,
+                             b.max_pages, b.pages, b.part_pages, b.n_heads, b.n_kv_heads,
+                             b.head_dim, b.page_size, scale, b.dtype, b.workspace,
+                             b.workspace_bytes, b.status_word, stream);
+}

@@ -400,3 +400,17 @@ extern "C" int pkv_attend_shared(const void* q, void* out, void* k_pool, void* v
   PKV_LAUNCH_CHECK();
   return PKV_OK;
 }
+
+static_assert(sizeof(pkv_shared) == 112, "the layout the Python binding fills");
+
+extern "C" int pkv_attend_shared_batch(const void* batch, const void* q, void* out, void* k_pool,
+                                       void* v_pool, float scale, const void* k_new,
+                                       const void* v_new, void* stream) {
+  if (!batch) return fail(PKV_ERR_INVALID, "null batch");
+  const pkv_shared& b = *static_cast<const pkv_shared*>(batch);
+  return pkv_attend_shared(q, out, k_pool, v_pool, b.num_blocks, b.kv_indices, b.n_seqs, b.n_heads,
+                           b.n_kv_heads, b.head_dim, b.page_size, scale, b.dtype, b.tiles,
+                           b.n_tiles, b.n_merges, b.plan, b.n_work, b.n_slots, b.plan_stride,
+                           k_new, v_new, k_new ? b.slot_mapping : nullptr, b.workspace,
+                           b.workspace_bytes, b.status_word, stream);
+}

@@ -46,3 +46,15 @@ def test_a_mixed_batch_needs_the_decode_kernel_that_reads_its_plan(n_heads, n_kv
     with pytest.raises(ValueError, match="fast decode path"):
         _native.check(lib.pkv_attend_batch(C.addressof(b), 16, 16, 16, 16, 0.125, None, None,
                                            None), "attend")
+
+
+def test_the_operators_structs_and_refusals():
+    assert [C.sizeof(x) for x in (_native.Rotated, _native.Shared, _native.Selected)] == [
+        104, 112, 112]
+    lib = _native.load()
+    for call in (lambda: lib.pkv_append_rotated_batch(None, *[None] * 3, 0, *[None] * 2, 0, None, 0,
+                                                      None, None, None),
+                 lambda: lib.pkv_attend_shared_batch(*[None] * 5, 1.0, None, None, None),
+                 lambda: lib.pkv_attend_selected_batch(*[None] * 8, 1.0, None)):
+        with pytest.raises(ValueError, match="null batch"):
+            _native.check(call(), "call")

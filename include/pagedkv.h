@@ -431,14 +431,31 @@ int pkv_page_bounds(const void* k_pool, int64_t pool_step, void* lo, void* hi,
  * ascending order, -1 behind shorter lists. max_pages is at least every
  * sequence's page count; scores holds n_seqs * n_kv_heads * max_pages doubles
  * (NULL if max_pages <= pages). Out-of-range page ids are scored by page 0's
- * bounds and flagged.
+ * bounds and flagged. With `words` the chosen pages go there instead of ids, as
+ * page words of pkv_plan_selected's plan (its places, part_pages, and head_words
+ * its size), KV head h's at words + h * head_words.
  */
 int pkv_select_pages(const void* q, const void* lo, const void* hi, int64_t num_blocks,
                      const int32_t* kv_indptr, const int32_t* kv_indices, const int32_t* kv_lens,
                      int32_t n_seqs, int32_t max_pages, int32_t pages, int32_t n_heads,
                      int32_t n_kv_heads, int32_t head_dim, int32_t page_size, int32_t dtype,
-                     double* scores, int32_t* ids, int32_t* ordinals, int32_t* status_word,
-                     void* stream);
+                     double* scores, int32_t* ids, int32_t* ordinals, int32_t* words,
+                     const int32_t* places, int64_t head_words, int32_t part_pages,
+                     int32_t* status_word, void* stream);
+
+/*
+ * Plan over chosen pages (host function), for batches whose pieces fill the
+ * device: pkv_plan_decode's over lists of min(pages, pages of the sequence)
+ * pages, whose page words pkv_select_pages fills in on the device, and
+ * `places`, where each list's words go: {first piece, pieces} a sequence, then
+ * the position of each piece's first word. Needs the fast decode path.
+ */
+int pkv_plan_selected(const int32_t* kv_lens, int32_t n_seqs, int32_t pages, int32_t n_heads,
+                      int32_t n_kv_heads, int32_t head_dim, int32_t dtype, int32_t part_pages,
+                      int32_t max_workgroups, int32_t* plan, int64_t plan_capacity,
+                      int64_t* plan_needed, int32_t* n_work_out, int32_t* n_slots_out,
+                      int32_t* plan_stride_out, int32_t* places, int64_t places_capacity,
+                      int64_t* places_needed);
 
 /*
  * Decode attention over the pages pkv_select_pages chose (its ids, n_seqs,
@@ -449,7 +466,9 @@ int pkv_select_pages(const void* q, const void* lo, const void* hi, int64_t num_
  * long; zero before the first launch that uses it, and left with zero
  * counters by each; launches that share it must not overlap in time).
  * Geometries without the fast decode path run a generic kernel, with no
- * workspace.
+ * workspace. With a plan (pkv_plan_selected's, its words filled by
+ * pkv_select_pages) the streaming decode kernel runs it, with the workspace of
+ * pkv_decode_workspace_bytes for its n_slots; ids and part_pages are not read.
  */
 int64_t pkv_selected_workspace_bytes(int32_t n_seqs, int32_t max_pages, int32_t pages,
                                      int32_t part_pages, int32_t n_heads, int32_t n_kv_heads,
@@ -459,8 +478,10 @@ int pkv_attend_selected(const void* q, void* out, void* k_pool, void* v_pool, in
                         const int32_t* ids, const int32_t* kv_lens, int32_t n_seqs,
                         int32_t max_pages, int32_t pages, int32_t part_pages, int32_t n_heads,
                         int32_t n_kv_heads, int32_t head_dim, int32_t page_size, float scale,
-                        int32_t dtype, void* workspace, int64_t workspace_bytes,
-                        int32_t* status_word, void* stream);
+                        int32_t dtype, const int32_t* plan, int32_t n_work, int32_t n_slots,
+                        int32_t plan_stride, const int32_t* words, int64_t head_words,
+                        void* workspace, int64_t workspace_bytes, int32_t* status_word,
+                        void* stream);
 
 /*
  * pkv_select_pages and pkv_attend_selected of one layer, with the arguments
@@ -468,16 +489,20 @@ int pkv_attend_selected(const void* q, void* out, void* k_pool, void* v_pool, in
  * bounds.
  */
 typedef struct pkv_selected {
-  int64_t num_blocks, workspace_bytes;
+  int64_t num_blocks, workspace_bytes, head_words;
   const int32_t* kv_indptr;
   const int32_t* kv_indices;
   const int32_t* kv_lens;
   double* scores;
   int32_t* ids;
+  int32_t* words;
+  const int32_t* places;
+  const int32_t* plan;
   void* workspace;
   int32_t* status_word;
   int32_t n_seqs, max_pages, pages, part_pages;
-  int32_t n_heads, n_kv_heads, head_dim, page_size, dtype, reserved;
+  int32_t n_heads, n_kv_heads, head_dim, page_size, dtype;
+  int32_t n_work, n_slots, plan_stride;
 } pkv_selected;
 
 int pkv_attend_selected_batch(const void* batch, const void* q, void* out, void* k_pool,

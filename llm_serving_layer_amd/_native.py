@@ -61,11 +61,14 @@ SIGNATURES = {
     "pkv_page_bounds": (C.c_int, [_p, _i64, _p, _p, _i64, _i32, _i64, _p, _i64, _i32, _i32, _i32,
                                   _i32, _p, _p]),
     "pkv_select_pages": (C.c_int, [_p, _p, _p, _i64, _p, _p, _p, _i32, _i32, _i32, _i32, _i32,
-                                   _i32, _i32, _i32, _p, _p, _p, _p, _p]),
+                                   _i32, _i32, _i32, _p, _p, _p, _p, _p, _i64, _i32, _p, _p]),
+    "pkv_plan_selected": (C.c_int, [_p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p, _i64,
+                                    _p, _p, _p, _p, _p, _i64, _p]),
     "pkv_selected_workspace_bytes": (C.c_int64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
                                                  _i64, _i32]),
     "pkv_attend_selected": (C.c_int, [_p, _p, _p, _p, _i64, _p, _p, _i32, _i32, _i32, _i32, _i32,
-                                      _i32, _i32, _i32, _f32, _i32, _p, _i64, _p, _p]),
+                                      _i32, _i32, _i32, _f32, _i32, _p, _i32, _i32, _i32, _p,
+                                      _i64, _p, _i64, _p, _p]),
     "pkv_append_rotated_batch": (C.c_int, [_p, _p, _p, _p, _i64, _p, _p, _i64, _p, _i64, _p, _p,
                                            _p]),
     "pkv_attend_shared_batch": (C.c_int, [_p, _p, _p, _p, _p, _f32, _p, _p, _p]),
@@ -114,12 +117,12 @@ class Shared(C.Structure):
 class Selected(C.Structure):
     """``pkv_selected``: an ``attend_selected``'s arguments, set once per plan."""
 
-    _fields_ = [("num_blocks", _i64), ("workspace_bytes", _i64),
+    _fields_ = [*[(n, _i64) for n in ("num_blocks", "workspace_bytes", "head_words")],
                 *[(n, _p) for n in ("kv_indptr", "kv_indices", "kv_lens", "scores", "ids",
-                                    "workspace", "status_word")],
+                                    "words", "places", "plan", "workspace", "status_word")],
                 *[(n, _i32) for n in ("n_seqs", "max_pages", "pages", "part_pages", "n_heads",
-                                      "n_kv_heads", "head_dim", "page_size", "dtype",
-                                      "reserved")]]
+                                      "n_kv_heads", "head_dim", "page_size", "dtype", "n_work",
+                                      "n_slots", "plan_stride")]]
 
 
 _LIB = None

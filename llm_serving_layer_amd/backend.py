@@ -60,6 +60,11 @@ _DTYPES = {torch.float16: _native.DTYPE_F16, torch.bfloat16: _native.DTYPE_BF16,
 
 MAX_PART_PAGES = 64      # a partition's page ids are read by one wavefront
 SELECTED_PART_PAGES = 8  # of chosen pages; what their kernel stages at a time
+# Pieces (of 8 pages) up to which each of them gets a workgroup of its own; the
+# streaming kernel takes more. us a call, workgroups against streaming: 64 pieces
+# 20.4 and 29.7, 512 20.0 and 26.8, 1024 26.9 and 29.3 (head_dim 64) or 36.2 and
+# 36.7 (128), 2048 40.7 and 34.5, 3072 81.7 and 72.5.
+SELECTED_PIECES = 1024
 SHARED_MIN_PAGES = 4     # shorter runs of shared pages stay each sequence's own
 SHARED_TILES = 256       # workgroups that share the work on a batch's shared pages
 DEFAULT_Q_TILE = 64      # prefill tile when the geometry has no matrix-core kernel
@@ -208,7 +213,7 @@ class _Selected:
     """What ``attend_selected`` keeps for one BatchMeta and page budget."""
 
     __slots__ = ("meta", "pages", "n", "max_pages", "indptr", "indices", "kv_lens", "scores",
-                 "ids", "ordinals", "part", "ws", "width", "args", "ptr", "buffers", "stream")
+                 "ids", "ordinals", "words", "places", "plan", "part", "ws", "width", "args", "ptr", "buffers", "stream")
 
 
 class MI355XBackend:
@@ -906,7 +911,8 @@ class MI355XBackend:
     def _counted_workspace(self, need: int, n: int) -> torch.Tensor:
         """A workspace whose arrival counters (at its front) are zero."""
         ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-        ws[:4 * n * self.n_kv_heads].zero_()
+        if need:
+            ws[:4 * n * self.n_kv_heads].zero_()
         return ws
 
     def attend_selected(self, q: torch.Tensor, layer_idx: int, scale: float, meta: BatchMeta,
@@ -985,29 +991,73 @@ class MI355XBackend:
                                dtype=torch.float64, **dev)
         p.ids = torch.empty(many * width, dtype=torch.int32, **dev)
         p.ordinals = torch.empty(many * width, dtype=torch.int32, **dev)
-        p.part = min(self.part_pages, SELECTED_PART_PAGES)
-        while True:   # partials are addressed with 32 bits: longer pieces where they pass 2 GiB
-            need = self._lib.pkv_selected_workspace_bytes(
-                n, p.max_pages, pages, p.part, self.n_heads, self.n_kv_heads, self.head_dim,
-                self.block_size, self.num_blocks, self._code)
-            if need < 2**31 or p.part >= MAX_PART_PAGES:
-                break
-            p.part = min(2 * p.part, MAX_PART_PAGES)
+        p.plan = p.places = p.words = None
+        n_work = n_slots = stride = 0
+        pieces = many * -(-width // SELECTED_PART_PAGES)
+        if self._fast_decode and pieces > SELECTED_PIECES:
+            p.part = self.part_pages
+            plan, places, n_work, n_slots, stride, need = self._plan_chosen(kvl, pages, p)
+            p.plan, p.places = self._upload(plan), self._upload(places)
+            p.words = torch.empty(self.n_kv_heads * plan.shape[0], dtype=torch.int32, **dev)
+        else:
+            p.part = min(self.part_pages, SELECTED_PART_PAGES)
+            while True:   # partials take 32-bit offsets: longer pieces where they pass 2 GiB
+                need = self._lib.pkv_selected_workspace_bytes(
+                    n, p.max_pages, pages, p.part, self.n_heads, self.n_kv_heads, self.head_dim,
+                    self.block_size, self.num_blocks, self._code)
+                if need < 2**31 or p.part >= MAX_PART_PAGES:
+                    break
+                p.part = min(2 * p.part, MAX_PART_PAGES)
         p.ws = self._counted_workspace(need, n)
-        p.buffers = [p.indptr, p.indices, p.kv_lens, p.scores, p.ids, p.ordinals, p.ws]
-        at = lambda t: t.data_ptr() if t.numel() else None  # noqa: E731
+        p.buffers = [t for t in (p.indptr, p.indices, p.kv_lens, p.scores, p.ids, p.ordinals,
+                                 p.words, p.places, p.plan, p.ws) if t is not None]
+        at = lambda t: t.data_ptr() if t is not None and t.numel() else None  # noqa: E731
         p.args = _native.Selected(
-            num_blocks=self.num_blocks, workspace_bytes=need, kv_indptr=at(p.indptr),
+            num_blocks=self.num_blocks, workspace_bytes=need,
+            head_words=0 if p.plan is None else p.plan.shape[0], kv_indptr=at(p.indptr),
             kv_indices=at(p.indices), kv_lens=at(p.kv_lens), scores=at(p.scores), ids=at(p.ids),
-            workspace=at(p.ws), status_word=self._status_ptr, n_seqs=n, max_pages=p.max_pages,
-            pages=pages, part_pages=p.part, n_heads=self.n_heads, n_kv_heads=self.n_kv_heads,
-            head_dim=self.head_dim, page_size=self.block_size, dtype=self._code)
+            words=at(p.words), places=at(p.places), plan=at(p.plan), workspace=at(p.ws),
+            status_word=self._status_ptr, n_seqs=n, max_pages=p.max_pages, pages=pages,
+            part_pages=p.part, n_heads=self.n_heads, n_kv_heads=self.n_kv_heads,
+            head_dim=self.head_dim, page_size=self.block_size, dtype=self._code, n_work=n_work,
+            n_slots=n_slots, plan_stride=stride)
         p.ptr = C.addressof(p.args)
         p.stream = _current_stream(self.device)
         p.meta = meta
         self._selected = p
         self.n_plans += 1
         return p
+
+    def _plan_chosen(self, kvl, pages: int, p: _Selected) -> tuple:
+        """Plan the chosen lists for the streaming kernel (pkv_plan_selected):
+        (plan, places, n_work, n_slots, stride, workspace bytes)."""
+        lens = np.ascontiguousarray(kvl, dtype=np.int32)
+        n_work, n_slots, stride = (C.c_int32() for _ in range(3))
+        needed, places_needed = C.c_int64(), C.c_int64()
+        listed = p.n * p.width
+        cap = 10 * self._decode_wgs + 2 * listed + 24 * p.n + 128
+        places_cap = 4 * p.n + listed
+        ptr = lambda a: a.ctypes.data  # noqa: E731
+        while True:
+            for _ in range(3):
+                plan, places = np.empty(cap, np.int32), np.empty(places_cap, np.int32)
+                rc = self._lib.pkv_plan_selected(
+                    ptr(lens), p.n, pages, self.n_heads, self.n_kv_heads, self.head_dim,
+                    self._code, p.part, self._decode_wgs, ptr(plan), cap, C.byref(needed),
+                    C.byref(n_work), C.byref(n_slots), C.byref(stride), ptr(places), places_cap,
+                    C.byref(places_needed))
+                if rc != _native.ERR_CAPACITY or (needed.value <= cap
+                                                  and places_needed.value <= places_cap):
+                    break
+                cap, places_cap = max(cap, needed.value), max(places_cap, places_needed.value)
+            _native.check(rc, "plan (selected)")
+            need = self._lib.pkv_decode_workspace_bytes(p.n, n_slots.value, self.n_heads,
+                                                        self.n_kv_heads, self.head_dim)
+            if need < 2**31 or p.part >= MAX_PART_PAGES:
+                break
+            p.part = min(2 * p.part, MAX_PART_PAGES)
+        return (plan[:needed.value], places[:places_needed.value], n_work.value, n_slots.value,
+                stride.value, need)
 
     def _check_pages(self, kvl, indptr, last, n_pages: int) -> None:
         """Every sequence's page list fits its length (ValueError naming the first

@@ -89,14 +89,19 @@ template <typename T, int D, int G> struct Rings {
 // summation, so both paths produce the same output) and never stored;
 // otherwise it publishes and counts its own arrival, and whichever piece
 // arrives last merges.
-template <typename T, int D, int G>
+//
+// CHOSEN: the page words are not the plan's but each KV head's own, chosen on
+// the device (selection.hip): head h's at `chosen` + h * head_words, where the
+// plan has them.
+template <typename T, int D, int G, bool CHOSEN = false>
 __device__ __forceinline__ void decode_stream(
     unsigned char* smem, int bin, int group,
     const T* __restrict__ q, T* __restrict__ out, T* __restrict__ kpool, T* __restrict__ vpool,
     int64_t num_blocks, const int32_t* __restrict__ plan, int32_t stride, int32_t n_kv_heads,
     float scale_log2, const T* __restrict__ k_new, const T* __restrict__ v_new,
     const int32_t* __restrict__ slot_mapping, float* part_o, float* part_ml, uint32_t o_bytes,
-    uint32_t ml_bytes, int32_t* counters, int32_t* status) {
+    uint32_t ml_bytes, int32_t* counters, int32_t* status,
+    const int32_t* __restrict__ chosen = nullptr, int64_t head_words = 0) {
   typedef typename Mma<T>::vec8 vec8;
   typedef typename Mma<T>::vec4 vec4;
   typedef PartLayout<D, G> PL;
@@ -129,6 +134,9 @@ __device__ __forceinline__ void decode_stream(
 
   const int32_t* bp = plan + (int64_t)bin * stride;
   const int32_t* words = bp + kHdrInts;
+  if constexpr (CHOSEN)
+    words = chosen + __builtin_amdgcn_readfirstlane(h) * head_words + (int64_t)bin * stride +
+            kHdrInts;
   const int32_t* items_end = bp + stride;   // item i: items_end - (i + 1) * kItemInts
   typedef Stage<T, D, G> SG;
   static_assert(SG::C <= kStageMax, "the first batch's items lie inside the block");

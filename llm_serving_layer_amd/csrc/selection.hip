@@ -252,6 +252,59 @@ __device__ __forceinline__ uint64_t order_of(double s) {
   return u >> 63 ? ~u : u | 1ull << 63;
 }
 
+// Where the choice of a sequence and KV head goes: the page ids in order, or the
+// page words of a decode plan whose sequences are the chosen lists, each head's
+// in a copy of the plan of its own. places: {first, pieces} a sequence, then for
+// piece first + i the position of its first word.
+struct Choice {
+  int32_t* ids;
+  int32_t* ordinals;
+  int32_t* words;
+  const int32_t* places;
+  int64_t head_words, num_blocks;
+  int32_t n_seqs, part_pages;
+};
+
+struct ChoiceRow {
+  const Choice& c;
+  const int32_t* table;
+  int64_t row;
+  int32_t* words;
+  const int32_t* offsets;
+  int pieces, last, tail;   // the list's last index, and its page's rows
+
+  __device__ ChoiceRow(const Choice& ch, const int32_t* pages, int seq, int h, int n_kv_heads,
+                       int width, int chosen, int rows)
+      : c(ch), table(pages), row(((int64_t)seq * n_kv_heads + h) * width), words(nullptr),
+        offsets(nullptr), pieces(1), last(chosen - 1), tail(rows) {
+    if (c.words) {
+      words = c.words + h * c.head_words;
+      offsets = c.places + 2 * c.n_seqs + c.places[2 * seq];
+      pieces = c.places[2 * seq + 1];
+    }
+  }
+  // the j-th chosen page is page p of the sequence
+  __device__ void put(int j, int p) const {
+    const int id = table[p];
+    c.ordinals[row + j] = p;
+    if (!words) {
+      c.ids[row + j] = id;
+      return;
+    }
+    const int piece = min(j / c.part_pages, pieces - 1);
+    const bool bad = id < 0 || (int64_t)id >= c.num_blocks;
+    const int live = j == last ? tail : 16;
+    const int64_t at = (int64_t)offsets[piece] + j - piece * c.part_pages;
+    if (at < c.head_words)
+      words[at] = (int)((uint32_t)(bad ? 0 : id) | ((uint32_t)(live - 1) & 15u) << 27 |
+                        (bad ? 0x80000000u : 0u));
+  }
+  __device__ void none(int j) const {
+    c.ordinals[row + j] = -1;
+    if (!words) c.ids[row + j] = -1;
+  }
+};
+
 // One workgroup of 256 threads a sequence and KV head. The k-th largest order
 // value is found 8 bits at a time from a histogram of the values that agree
 // with the bits found so far; then pages above it, and the first of those equal
@@ -259,23 +312,19 @@ __device__ __forceinline__ uint64_t order_of(double s) {
 __global__ __launch_bounds__(256) void select_kernel(
     const double* __restrict__ scores, int64_t stride, const int32_t* __restrict__ kv_indptr,
     const int32_t* __restrict__ kv_indices, const int32_t* __restrict__ kv_lens,
-    int32_t n_kv_heads, int32_t page_size, int32_t pages, int32_t width,
-    int32_t* __restrict__ ids, int32_t* __restrict__ ordinals) {
+    int32_t n_kv_heads, int32_t page_size, int32_t pages, int32_t width, Choice choice) {
   __shared__ int32_t hist[256], tails[256];
   __shared__ uint64_t found;
   __shared__ int32_t need;
   const int seq = blockIdx.y, h = blockIdx.x, tid = threadIdx.x;
   const int np = seq_pages(kv_indptr, kv_lens, seq, page_size, stride);
-  const int32_t* table = kv_indices + kv_indptr[seq];
-  const int64_t row = ((int64_t)seq * n_kv_heads + h) * width;
-  auto put = [&](int j, int p) {
-    ids[row + j] = table[p];
-    ordinals[row + j] = p;
-  };
+  const ChoiceRow to(choice, kv_indices + kv_indptr[seq], seq, h, n_kv_heads, width,
+                     min(np, pages), kv_lens[seq] - (np - 1) * page_size);
+  auto put = [&](int j, int p) { to.put(j, p); };
   if (np <= pages) {
     for (int j = tid; j < width; j += 256) {
       if (j < np) put(j, j);
-      else { ids[row + j] = -1; ordinals[row + j] = -1; }
+      else to.none(j);
     }
     return;
   }
@@ -336,8 +385,7 @@ template <int B, int K>
 __global__ __launch_bounds__(B) void select_rows_kernel(
     const double* __restrict__ scores, int64_t stride, const int32_t* __restrict__ kv_indptr,
     const int32_t* __restrict__ kv_indices, const int32_t* __restrict__ kv_lens,
-    int32_t n_kv_heads, int32_t page_size, int32_t pages, int32_t width,
-    int32_t* __restrict__ ids, int32_t* __restrict__ ordinals) {
+    int32_t n_kv_heads, int32_t page_size, int32_t pages, int32_t width, Choice choice) {
   constexpr int W = B / 64;          // waves
   static_assert(B >= 256 && W * K <= 256, "a bin a thread, a count a lane of four");
   __shared__ int32_t hist[256], counts[2][W * K];
@@ -346,16 +394,13 @@ __global__ __launch_bounds__(B) void select_rows_kernel(
   const int seq = blockIdx.y, h = blockIdx.x, tid = threadIdx.x;
   const int wave = tid >> 6, lane = tid & 63;
   const int np = seq_pages(kv_indptr, kv_lens, seq, page_size, stride);
-  const int32_t* table = kv_indices + kv_indptr[seq];
-  const int64_t row = ((int64_t)seq * n_kv_heads + h) * width;
-  auto put = [&](int j, int p) {
-    ids[row + j] = table[p];
-    ordinals[row + j] = p;
-  };
+  const ChoiceRow to(choice, kv_indices + kv_indptr[seq], seq, h, n_kv_heads, width,
+                     min(np, pages), kv_lens[seq] - (np - 1) * page_size);
+  auto put = [&](int j, int p) { to.put(j, p); };
   if (np <= pages) {
     for (int j = tid; j < width; j += B) {
       if (j < np) put(j, j);
-      else { ids[row + j] = -1; ordinals[row + j] = -1; }
+      else to.none(j);
     }
     return;
   }
@@ -578,16 +623,20 @@ extern "C" int pkv_select_pages(const void* q, const void* lo, const void* hi, i
                                 int32_t pages, int32_t n_heads, int32_t n_kv_heads,
                                 int32_t head_dim, int32_t page_size, int32_t dtype,
                                 double* scores, int32_t* ids, int32_t* ordinals,
-                                int32_t* status_word, void* stream) {
+                                int32_t* words, const int32_t* places, int64_t head_words,
+                                int32_t part_pages, int32_t* status_word, void* stream) {
   int rc = check_geometry(n_heads, n_kv_heads, head_dim, page_size, dtype);
   if (rc) return rc;
   if (n_seqs < 0 || n_seqs > 65535 || n_kv_heads > 65535 || max_pages <= 0 || pages <= 0)
     return fail(PKV_ERR_INVALID, "max_pages and pages must be positive, and one call takes up to "
                 "65535 sequences and KV heads");
   if (n_seqs == 0) return PKV_OK;
-  if (!q || !lo || !hi || !kv_indptr || !kv_indices || !kv_lens || !ids || !ordinals ||
-      (max_pages > pages && !scores))
+  if (!q || !lo || !hi || !kv_indptr || !kv_indices || !kv_lens || !ordinals ||
+      (max_pages > pages && !scores) || (words ? !places : !ids))
     return fail(PKV_ERR_INVALID, "null pointer argument");
+  if (words && (part_pages < 1 || head_words < 1 || page_size != 16 ||
+                num_blocks > (1LL << 27)))
+    return fail(PKV_ERR_INVALID, "page words need a plan (pkv_plan_selected)");
   const int32_t width = std::min(pages, max_pages);
   hipStream_t s = (hipStream_t)stream;
   if (max_pages > pages && pages > 1) {
@@ -622,7 +671,9 @@ extern "C" int pkv_select_pages(const void* q, const void* lo, const void* hi, i
   auto choose = [&](auto kernel, int threads) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)n_kv_heads, (unsigned)n_seqs), dim3(threads), 0, s,
                        scores, (int64_t)max_pages, kv_indptr, kv_indices, kv_lens, n_kv_heads,
-                       page_size, pages, width, ids, ordinals);
+                       page_size, pages, width,
+                       Choice{ids, ordinals, words, places, head_words, num_blocks, n_seqs,
+                              part_pages});
   };
   if (max_pages <= 256 * 4) choose(select_rows_kernel<256, 4>, 256);
   else if (max_pages <= 1024 * 4) choose(select_rows_kernel<1024, 4>, 1024);

@@ -50,7 +50,7 @@ def test_a_mixed_batch_needs_the_decode_kernel_that_reads_its_plan(n_heads, n_kv
 
 def test_the_operators_structs_and_refusals():
     assert [C.sizeof(x) for x in (_native.Rotated, _native.Shared, _native.Selected)] == [
-        104, 112, 112]
+        104, 112, 152]
     lib = _native.load()
     for call in (lambda: lib.pkv_append_rotated_batch(None, *[None] * 3, 0, *[None] * 2, 0, None, 0,
                                                       None, None, None),

@@ -13,7 +13,8 @@ import dataclasses
 import pytest
 import torch
 
-from llm_serving_layer_amd import (BlockAllocator, KVSwapSpace, RotaryTable, SequenceBlocks)
+from llm_serving_layer_amd import (BlockAllocator, KVSwapSpace, RotaryTable, SequenceBlocks,
+                                   backend)
 from llm_serving_layer_amd.backend import MI355XBackend
 
 from ._ops64 import assert_within, attend64, chosen64
@@ -106,6 +107,29 @@ def test_pieces_of_any_size(part_pages):
     q = c.q()
     out, chosen = c.bk.attend_selected(q, 0, 0.125, c.meta, 90, return_pages=True)
     c.check(q, 90, out, chosen)
+
+
+@pytest.mark.parametrize("n_heads, n_kv, d", [
+    (32, 8, 64), (8, 2, 128), (8, 8, 64), (16, 1, 64), (12, 3, 128), (16, 2, 128)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("pages, part_pages", [(1, 17), (7, 3), (30, 17), (100, 1), (1000, 64)])
+def test_the_streaming_kernel(n_heads, n_kv, d, dtype, pages, part_pages, monkeypatch):
+    """The kernel for many pieces, whatever their number: page words placed by
+    the plan, pieces with a folded remainder, whole lists and cut ones."""
+    print(f"selected stream {n_heads}/{n_kv}/{d} {dtype} {pages} {part_pages}", flush=True)
+    monkeypatch.setattr(backend, "SELECTED_PIECES", 0)
+    c = Cache(LENS, n_heads, n_kv, d, dtype, part_pages=part_pages)
+    q = c.q()
+    out, chosen = c.bk.attend_selected(q, 0, 0.125, c.meta, pages, return_pages=True)
+    c.bk.check_device_errors()
+    assert c.bk._selected.plan is not None
+    c.check(q, pages, out, chosen)
+    assert torch.equal(c.bk.attend_selected(q, 0, 0.125, c.meta, pages), out)
+
+
+def test_bad_pages_in_a_streamed_choice(monkeypatch):
+    monkeypatch.setattr(backend, "SELECTED_PIECES", 0)
+    test_bad_pages_are_flagged_and_read_nothing()
 
 
 def test_a_long_history_and_many_sequences():

@@ -174,7 +174,8 @@ __device__ __forceinline__ void decode_stream(
   // Page p of the stream (p wave-uniform, word w = words[p]); past the
   // bin's last page every load is outside its range: no access, zeros.
   auto load_page = [&](int p, int w, vec8* kr, vec8* vr) __attribute__((always_inline)) {
-    const bool in = p < n_pages;
+    // (a plan's ids are checked on the host; chosen words are written on the device)
+    const bool in = p < n_pages && (!CHOSEN || (w & ((1 << kPageIdBits) - 1)) < num_blocks);
     const int64_t page = in ? (w & ((1 << kPageIdBits) - 1)) : 0;
     const uint32_t live = in ? (((uint32_t)w >> kPageIdBits) & 15u) + 1u : 0u;
     const __amdgpu_buffer_rsrc_t rk = ws_rsrc(kpool + page * PS * row_elems, live * frow);

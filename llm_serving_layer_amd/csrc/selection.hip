@@ -6,12 +6,14 @@
 //  * score_kernel bounds a page's scores from them: for query head g of KV
 //    head h, q_g . k <= sum_d q_gd * (q_gd < 0 ? lo_d : hi_d) for every key k of
 //    the page; the page's score is the largest over the KV head's query heads.
-//    Sums run in 64 bits: which page is in and which is out must not hang on
-//    the order of a sum.
+//    A score is a sum in 64 bits: which page is in and which is out must not
+//    hang on the order of a sum. 16-bit pools sum in 32 bits first, and only
+//    pages whose sums lie too close to the cut for that are summed in 64.
 //  * select_kernel takes a sequence's last page and the best of the others
 //    (equal scores: the lower page; a NaN beats every number), in page order.
 //  * the attention then runs over the chosen pages (attend_selected).
 #include <algorithm>
+#include <type_traits>
 
 #include "mfma.h"
 
@@ -244,6 +246,164 @@ __global__ __launch_bounds__(256) void score_rows_kernel(
   }
 }
 
+// 16-bit pools: the same sums in 32 bits, a product or two an instruction, lo or
+// hi taken for two elements at once by q's sign bits: 1 or 1.5 instructions a
+// query element instead of 3 and no unpacking, which leaves the kernel bound by
+// its loads (16 sequences of 20 000 to 60 000 tokens, 8 KV heads, head_dim 128,
+// bf16: 43.5 -> 30.6 us, 5.2 TB/s). near() says how far such a sum may be off; for it each workgroup also
+// leaves the largest magnitude among its pages' bounds.
+constexpr int kNearSteps = 4;
+
+template <typename T, int D, int G>
+struct NearShape {
+  static constexpr int L = D / 8;                 // lanes a page, 8 elements each
+  static constexpr int GQ = G < 4 ? G : 4;        // query heads a wave
+  static constexpr int QW = G / GQ;               // waves that share a page
+  static constexpr int PW = 64 / L;               // pages of a wave's step
+  static constexpr int PAGES = 4 / QW * PW * kNearSteps;   // of a workgroup
+};
+
+// How far a score in 32 bits may be off: a lane's 8 products and the sums over up
+// to 16 lanes are at most 12 steps (the bf16 dot2, measured over 2^20 random
+// operands of sizes down to 2^-20, is off by 1.7 2^-24 of its terms' magnitudes,
+// less than two roundings), together less than 16 2^-23 of sum |q| times the
+// largest bound. Not a number or infinite if anything is: then nothing is settled by the
+// 32-bit sums.
+__device__ __forceinline__ float near(float q_sum, float b_max) {
+  return q_sum * b_max * (16.f * 1.1920929e-7f) + 1e-36f;
+}
+
+// (fp16: dot2 loses low bits of products below 2^-24 or so, a mixed fma does not)
+__device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c, _Float16) {
+  const f16x2 x = __builtin_bit_cast(f16x2, a), y = __builtin_bit_cast(f16x2, b);
+  return __builtin_fmaf((float)x[1], (float)y[1], __builtin_fmaf((float)x[0], (float)y[0], c));
+}
+__device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c, __bf16) {
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, a), __builtin_bit_cast(b2, b), c,
+                                         false);
+}
+
+template <typename T, int D, int G>
+__global__ __launch_bounds__(256) void near_scores_kernel(
+    const T* __restrict__ q, const T* __restrict__ lo, const T* __restrict__ hi,
+    int64_t num_blocks, const int32_t* __restrict__ kv_indptr,
+    const int32_t* __restrict__ kv_indices, const int32_t* __restrict__ kv_lens,
+    int32_t n_kv_heads, int32_t page_size, int32_t pages, int64_t stride,
+    float* __restrict__ scores, int32_t* status) {
+  typedef NearShape<T, D, G> S;
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  typedef short i16x2 __attribute__((ext_vector_type(2)));
+  constexpr int L = S::L, GQ = S::GQ, PW = S::PW, N = PW * kNearSteps;
+  __shared__ float part[S::QW > 1 ? 4 * N : 1], largest[4];
+  const int h = blockIdx.x, seq = blockIdx.z;
+  const int np = seq_pages(kv_indptr, kv_lens, seq, page_size, stride);
+  const int n = np - 1;    // candidates; the last page is in
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int quad = wave % S::QW, group = wave / S::QW;
+  const int first = blockIdx.y * S::PAGES + group * N;
+  if (np <= pages || (int)blockIdx.y * S::PAGES >= n) return;
+  const int32_t* table = kv_indices + kv_indptr[seq];
+  const int c = lane % L;
+  int64_t at[kNearSteps];
+#pragma unroll
+  for (int i = 0; i < kNearSteps; ++i) {
+    int64_t id = table[min(first + i * PW + lane / L, n - 1)];
+    if (id < 0 || id >= num_blocks) {
+      flag(status, PKV_STATUS_BAD_PAGE);
+      id = 0;
+    }
+    at[i] = (id * n_kv_heads + h) * D + c * 8;
+  }
+  u32x4 a[kNearSteps], b[kNearSteps];
+#pragma unroll
+  for (int i = 0; i < kNearSteps; ++i) {
+    a[i] = *reinterpret_cast<const u32x4*>(lo + at[i]);
+    b[i] = *reinterpret_cast<const u32x4*>(hi + at[i]);
+  }
+  u32x4 x[GQ], neg[GQ];   // q, and ones where it is below zero
+#pragma unroll
+  for (int g = 0; g < GQ; ++g) {
+    x[g] = *reinterpret_cast<const u32x4*>(
+        q + (((int64_t)seq * n_kv_heads + h) * G + quad * GQ + g) * D + c * 8);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t w = x[g][j];
+      neg[g][j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, w) >> 15);
+    }
+  }
+  // The largest magnitude: of lo as whole numbers (a negative one, of the largest
+  // magnitude, before any positive), of hi as signed ones.
+  u16x2 ml{0, 0};
+  i16x2 mh{-32768, -32768};
+  float out[kNearSteps];
+#pragma unroll
+  for (int i = 0; i < kNearSteps; ++i) {
+    float s[GQ];
+#pragma unroll
+    for (int g = 0; g < GQ; ++g) s[g] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // (as scalars: a bit cast of a vector's element takes the vector's first)
+      const uint32_t wl = a[i][j], wh = b[i][j];
+      ml = __builtin_elementwise_max(ml, __builtin_bit_cast(u16x2, wl));
+      mh = __builtin_elementwise_max(mh, __builtin_bit_cast(i16x2, wh));
+#pragma unroll
+      for (int g = 0; g < GQ; ++g)
+        s[g] = dot2(x[g][j], (neg[g][j] & wl) | (~neg[g][j] & wh), s[g], T{});
+    }
+#pragma unroll
+    for (int g = 0; g < GQ; ++g) {   // over the page's L lanes
+      s[g] += dpp<0xB1>(s[g]);
+      s[g] += dpp<0x4E>(s[g]);
+      s[g] += dpp<0x141>(s[g]);
+      if (L == 16) s[g] += dpp<0x140>(s[g]);
+    }
+    out[i] = s[0];
+#pragma unroll
+    for (int g = 1; g < GQ; ++g) out[i] = fmaxf(out[i], s[g]);
+  }
+  // the pages' scores, then the workgroups' maxima
+  float* row = scores + ((int64_t)seq * n_kv_heads + h) * 2 * stride;
+  auto magnitude = [](uint32_t bits) {
+    return Elem<T>::to_f(__builtin_bit_cast(T, (unsigned short)(bits & 0x7fff)));
+  };
+  float m = fmaxf(fmaxf(magnitude(ml[0]), magnitude(ml[1])),
+                  fmaxf(magnitude((unsigned short)mh[0]), magnitude((unsigned short)mh[1])));
+  // (a NaN shows: fmaxf would drop it)
+  auto special = [](uint32_t bits) {
+    return (bits & 0x7fff) >= (__is_same(T, _Float16) ? 0x7c00 : 0x7f80);
+  };
+  if (special(ml[0]) || special(ml[1]) || special((unsigned short)mh[0]) ||
+      special((unsigned short)mh[1]))
+    m = INFINITY;
+  m = wave_max(m);
+  if (lane == 0) largest[wave] = m;
+  if constexpr (S::QW > 1) {
+#pragma unroll
+    for (int i = 0; i < kNearSteps; ++i)
+      if (c == 0) part[wave * N + i * PW + lane / L] = out[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < kNearSteps; ++i) {
+      const int p = first + i * PW + lane / L;
+      if (c == 0 && p < n) row[p] = out[i];
+    }
+  }
+  __syncthreads();
+  if constexpr (S::QW > 1) {
+    for (int i = threadIdx.x; i < 4 / S::QW * N; i += 256) {
+      const int w = i / N * S::QW, k = i % N, p = blockIdx.y * S::PAGES + i;
+      float best = part[w * N + k];
+#pragma unroll
+      for (int j = 1; j < S::QW; ++j) best = fmaxf(best, part[(w + j) * N + k]);
+      if (p < n) row[p] = best;
+    }
+  }
+  if (threadIdx.x == 0)
+    row[stride + blockIdx.y] = fmaxf(fmaxf(largest[0], largest[1]), fmaxf(largest[2], largest[3]));
+}
+
 // ------------------------------------------------------------------- choice ---
 // A score as an unsigned number of the same order, a NaN above every number.
 __device__ __forceinline__ uint64_t order_of(double s) {
@@ -271,12 +431,12 @@ struct ChoiceRow {
   int64_t row;
   int32_t* words;
   const int32_t* offsets;
-  int pieces, last, tail;   // the list's last index, and its page's rows
+  int pieces, width, last, tail;   // the list's last index, and its page's rows
 
   __device__ ChoiceRow(const Choice& ch, const int32_t* pages, int seq, int h, int n_kv_heads,
-                       int width, int chosen, int rows)
-      : c(ch), table(pages), row(((int64_t)seq * n_kv_heads + h) * width), words(nullptr),
-        offsets(nullptr), pieces(1), last(chosen - 1), tail(rows) {
+                       int columns, int chosen, int rows)
+      : c(ch), table(pages), row(((int64_t)seq * n_kv_heads + h) * columns), words(nullptr),
+        offsets(nullptr), pieces(1), width(columns), last(chosen - 1), tail(rows) {
     if (c.words) {
       words = c.words + h * c.head_words;
       offsets = c.places + 2 * c.n_seqs + c.places[2 * seq];
@@ -285,6 +445,7 @@ struct ChoiceRow {
   }
   // the j-th chosen page is page p of the sequence
   __device__ void put(int j, int p) const {
+    if ((unsigned)j >= (unsigned)width) return;   // (never: a list has `width` at most)
     const int id = table[p];
     c.ordinals[row + j] = p;
     if (!words) {
@@ -381,75 +542,74 @@ __global__ __launch_bounds__(256) void select_kernel(
 // start at the highest bit in which the largest and the smallest differ, and
 // end as soon as a digit's bin holds exactly the pages still needed: two or
 // three rounds, not eight.
-template <int B, int K>
-__global__ __launch_bounds__(B) void select_rows_kernel(
-    const double* __restrict__ scores, int64_t stride, const int32_t* __restrict__ kv_indptr,
-    const int32_t* __restrict__ kv_indices, const int32_t* __restrict__ kv_lens,
-    int32_t n_kv_heads, int32_t page_size, int32_t pages, int32_t width, Choice choice) {
-  constexpr int W = B / 64;          // waves
+//
+// NEAR: the scores are the 32-bit sums. The cut t of those settles a page whose
+// sum is more than two errors above it (in: fewer than k pages can beat it) or
+// below it (out: k pages beat it). Of the pages between, the rest of the k are
+// in: all of them, mostly; else their 64-bit scores decide.
+constexpr int kOpenRanks = 64;   // open pages up to which each counts the others
+
+__device__ __forceinline__ double shift_xor(double v, int m) {
+  return __builtin_bit_cast(double, __shfl_xor(__builtin_bit_cast(unsigned long long, v), m));
+}
+
+template <int B, int K> struct SelectLds {
+  static constexpr int W = B / 64;
+  int32_t hist[256], counts[2][W * K], page[kOpenRanks], sums[2][W];
+  uint64_t range[2][W], value[kOpenRanks];
+  int32_t digit, above, inside;
+  float q_sum[W], b_max[W];
+};
+
+template <typename U> struct Cut {
+  U least;      // values from here on are taken,
+  int need;     // of those equal to it (only if `ties`) the first `need`
+  bool ties;
+};
+
+// The k largest of the values u[i] with bit i of `valid` (k at most their number;
+// called by every thread of the workgroup).
+template <typename U, int B, int K>
+__device__ __forceinline__ Cut<U> find_cut(SelectLds<B, K>& l, const U* u, uint32_t valid, int k) {
+  constexpr int W = B / 64, BITS = 8 * (int)sizeof(U);
   static_assert(B >= 256 && W * K <= 256, "a bin a thread, a count a lane of four");
-  __shared__ int32_t hist[256], counts[2][W * K];
-  __shared__ uint64_t range[2][W];
-  __shared__ int32_t digit, above, inside;
-  const int seq = blockIdx.y, h = blockIdx.x, tid = threadIdx.x;
-  const int wave = tid >> 6, lane = tid & 63;
-  const int np = seq_pages(kv_indptr, kv_lens, seq, page_size, stride);
-  const ChoiceRow to(choice, kv_indices + kv_indptr[seq], seq, h, n_kv_heads, width,
-                     min(np, pages), kv_lens[seq] - (np - 1) * page_size);
-  auto put = [&](int j, int p) { to.put(j, p); };
-  if (np <= pages) {
-    for (int j = tid; j < width; j += B) {
-      if (j < np) put(j, j);
-      else to.none(j);
-    }
-    return;
-  }
-  const int n = np - 1, k = pages - 1;
-  if (tid == 0) put(k, n);
-  if (k == 0) return;
-  const double* sc = scores + ((int64_t)seq * n_kv_heads + h) * stride;
-  uint64_t u[K], lo = ~0ull, hi = 0;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  U lo = ~(U)0, hi = 0;
 #pragma unroll
   for (int i = 0; i < K; ++i) {
-    const int p = i * B + tid;
-    u[i] = p < n ? order_of(sc[p]) : 0;   // (0 is no number's order value)
-    if (p < n) {
+    if (valid >> i & 1) {
       lo = u[i] < lo ? u[i] : lo;
       hi = u[i] > hi ? u[i] : hi;
     }
   }
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) {
-    const uint64_t a = __shfl_xor((unsigned long long)lo, m);
-    const uint64_t b = __shfl_xor((unsigned long long)hi, m);
+    const U a = (U)__shfl_xor((unsigned long long)lo, m);
+    const U b = (U)__shfl_xor((unsigned long long)hi, m);
     lo = a < lo ? a : lo;
     hi = b > hi ? b : hi;
   }
-  if (lane == 0) { range[0][wave] = lo; range[1][wave] = hi; }
-  if (tid < 256) hist[tid] = 0;
+  if (lane == 0) { l.range[0][wave] = lo; l.range[1][wave] = hi; }
+  if (tid < 256) l.hist[tid] = 0;
   __syncthreads();
   for (int w = 0; w < W; ++w) {
-    lo = range[0][w] < lo ? range[0][w] : lo;
-    hi = range[1][w] > hi ? range[1][w] : hi;
+    lo = (U)l.range[0][w] < lo ? (U)l.range[0][w] : lo;
+    hi = (U)l.range[1][w] > hi ? (U)l.range[1][w] : hi;
   }
-  // values from `least` on are taken, and of those in [least, least + 2^shift)
-  // the first `need` if `ties`
-  uint64_t least = lo;
-  int need = k, shift = lo == hi ? 0 : 64 - __builtin_clzll(lo ^ hi);
-  bool ties = lo == hi;
-  if (shift < 64) least = lo >> shift << shift;
-  else least = 0;
+  // of the values in [least, least + 2^shift) the largest `need` are in
+  int shift = lo == hi ? 0 : 64 - __builtin_clzll((uint64_t)(lo ^ hi));
+  Cut<U> cut{shift < BITS ? (U)(lo >> shift << shift) : (U)0, k, lo == hi};
   while (shift > 0) {
     const int next = shift > 8 ? shift - 8 : 0;
-    // values that agree above `shift`, by their next bits
+    // values that agree above `shift`, by their next bits. The largest first:
+    // digit b counts in hist[255 ^ b], so that wave 0's addresses below grow with
+    // the lane. Read as hist[255 - 4 l - j] they became a negative base plus an
+    // offset, and those reads returned other data in every workgroup whose LDS
+    // does not start at 0.
 #pragma unroll
     for (int i = 0; i < K; ++i) {
-      const bool in = i * B + tid < n && (shift == 64 || (u[i] ^ least) >> shift == 0);
-      // The largest first: digit b counts in hist[255 ^ b], so that wave 0's
-      // addresses below grow with the lane. Read as hist[255 - 4 l - j] they
-      // became a negative base plus an offset, and those reads returned other
-      // data in every workgroup whose LDS does not start at 0.
-      if (in) atomicAdd(&hist[255 ^ (int)((u[i] - least) >> next)], 1);
+      const bool in = (valid >> i & 1) && (shift == BITS || (u[i] ^ cut.least) >> shift == 0);
+      if (in) atomicAdd(&l.hist[255 ^ (int)((u[i] - cut.least) >> next)], 1);
     }
     __syncthreads();
     if (wave == 0) {
@@ -457,7 +617,7 @@ __global__ __launch_bounds__(B) void select_rows_kernel(
       int c[4], sum = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        c[j] = hist[4 * lane + j];
+        c[j] = l.hist[4 * lane + j];
         sum += c[j];
       }
       int run = sum;
@@ -469,33 +629,209 @@ __global__ __launch_bounds__(B) void select_rows_kernel(
       int before = run - sum;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (before < need && before + c[j] >= need) {
-          digit = 255 ^ (4 * lane + j);
-          above = before;
-          inside = c[j];
+        if (before < cut.need && before + c[j] >= cut.need) {
+          l.digit = 255 ^ (4 * lane + j);
+          l.above = before;
+          l.inside = c[j];
         }
         before += c[j];
       }
     }
     __syncthreads();
-    least += (uint64_t)digit << next;
-    need -= above;
+    cut.least += (U)l.digit << next;
+    cut.need -= l.above;
     shift = next;
-    ties = inside > need;
-    if (!ties) break;
-    if (tid < 256) hist[tid] = 0;
+    cut.ties = l.inside > cut.need;
+    if (!cut.ties) break;
+    if (tid < 256) l.hist[tid] = 0;
     __syncthreads();
   }
-  // Now `ties` only if the values in question are all equal to `least`. Page
-  // order is (i, thread): a count a wave and i, and their sums before each.
+  __syncthreads();   // l may be used again
+  return cut;
+}
+
+// The sums over the workgroup of a and b.
+template <int B, int K>
+__device__ __forceinline__ void block_sum(SelectLds<B, K>& l, int& a, int& b) {
+  const int wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    a += __shfl_xor(a, m);
+    b += __shfl_xor(b, m);
+  }
+  if ((threadIdx.x & 63) == 0) { l.sums[0][wave] = a; l.sums[1][wave] = b; }
+  __syncthreads();
+  a = b = 0;
+  for (int w = 0; w < B / 64; ++w) { a += l.sums[0][w]; b += l.sums[1][w]; }
+}
+
+struct NearArgs {
+  const void* q; const void* lo; const void* hi;
+  int64_t num_blocks;
+  int32_t D, G, block_pages;     // pages of a workgroup of near_scores_kernel
+};
+
+template <typename T, bool NEAR, int B, int K>
+__global__ __launch_bounds__(B) void select_rows_kernel(
+    const double* __restrict__ scores, int64_t stride, const int32_t* __restrict__ kv_indptr,
+    const int32_t* __restrict__ kv_indices, const int32_t* __restrict__ kv_lens,
+    int32_t n_kv_heads, int32_t page_size, int32_t pages, int32_t width, Choice choice,
+    NearArgs na) {
+  constexpr int W = B / 64;          // waves
+  __shared__ SelectLds<B, K> l;
+  const int seq = blockIdx.y, h = blockIdx.x, tid = threadIdx.x;
+  const int wave = tid >> 6, lane = tid & 63;
+  const int np = seq_pages(kv_indptr, kv_lens, seq, page_size, stride);
+  const int32_t* table = kv_indices + kv_indptr[seq];
+  const ChoiceRow to(choice, table, seq, h, n_kv_heads, width, min(np, pages),
+                     kv_lens[seq] - (np - 1) * page_size);
+  if (np <= pages) {
+    for (int j = tid; j < width; j += B) {
+      if (j < np) to.put(j, j);
+      else to.none(j);
+    }
+    return;
+  }
+  const int n = np - 1, k = pages - 1;
+  if (tid == 0) to.put(k, n);
+  if (k == 0) return;
+  const double* sc = scores + ((int64_t)seq * n_kv_heads + h) * stride;
+  uint32_t valid = 0, sure = 0;      // bit i: page i B + tid; settled as in
+#pragma unroll
+  for (int i = 0; i < K; ++i) valid |= (uint32_t)(i * B + tid < n) << i;
+  uint64_t u[K];
+  Cut<uint64_t> cut;
+  if constexpr (!NEAR) {
+#pragma unroll
+    for (int i = 0; i < K; ++i) u[i] = valid >> i & 1 ? order_of(sc[i * B + tid]) : 0;
+    cut = find_cut<uint64_t, B, K>(l, u, valid, k);
+  } else {
+    const float* near_row = reinterpret_cast<const float*>(sc);   // scores, then maxima
+    const T* q = (const T*)na.q + ((int64_t)seq * n_kv_heads + h) * na.G * na.D;
+    // sum |q| of each query head, a head a wave; the largest bound
+    float q_sum = 0.f, b_max = 0.f;
+    for (int g = wave; g < na.G; g += W) {
+      float t = 0.f;
+      for (int d = lane; d < na.D; d += 64) t += __builtin_fabsf(Elem<T>::to_f(q[g * na.D + d]));
+      t = wave_sum(t);
+      q_sum = t > q_sum || t != t ? t : q_sum;
+    }
+    for (int i = tid; i < (n + na.block_pages - 1) / na.block_pages; i += B)
+      b_max = fmaxf(b_max, near_row[stride + i]);
+    b_max = wave_max(b_max);
+    if (lane == 0) { l.q_sum[wave] = q_sum; l.b_max[wave] = b_max; }
+    float a[K];
+    uint32_t v[K];
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      a[i] = valid >> i & 1 ? near_row[i * B + tid] : 0.f;
+      const uint32_t bits = __builtin_bit_cast(uint32_t, a[i] + 0.f);
+      v[i] = bits >> 31 ? ~bits : bits | 1u << 31;
+    }
+    const Cut<uint32_t> c32 = find_cut<uint32_t, B, K>(l, v, valid, k);   // (a barrier inside)
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      q_sum = l.q_sum[w] > q_sum || l.q_sum[w] != l.q_sum[w] ? l.q_sum[w] : q_sum;
+      b_max = fmaxf(b_max, l.b_max[w]);
+    }
+    const float t = __builtin_bit_cast(
+        float, c32.least >> 31 ? c32.least ^ 1u << 31 : ~c32.least);
+    const float e = 2.01f * near(q_sum, b_max) + 4.8e-7f * __builtin_fabsf(t);
+    uint32_t open = 0;
+    int n_sure = 0, n_open = 0;
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      if (!(valid >> i & 1)) continue;
+      // (a comparison with something that is no number settles nothing)
+      const float d = a[i] - t;
+      if (e < INFINITY && d > e) { sure |= 1u << i; ++n_sure; }
+      else if (!(e < INFINITY && d < -e)) { open |= 1u << i; ++n_open; }
+    }
+    block_sum(l, n_sure, n_open);
+    // (all k may be settled with pages open below them: t can lie between the
+    // k-th sum and the next)
+    if (n_sure == k || n_open == k - n_sure) {
+      if (n_sure < k) sure |= open;
+      valid = 0;
+      cut = Cut<uint64_t>{0, 0, false};
+    } else {
+      // 64-bit scores of the open pages, one of a wave at a time: D / 8 lanes a
+      // query head, 64 / (D / 8) heads side by side
+      typedef T vec __attribute__((ext_vector_type(8)));
+      const int L = na.D / 8, side = 64 / L, c = lane % L;
+#pragma unroll
+      for (int i = 0; i < K; ++i) {
+        u[i] = 0;
+        for (uint64_t who = __builtin_amdgcn_ballot_w64(open >> i & 1); who; who &= who - 1) {
+          const int owner = __builtin_ctzll(who);
+          int64_t id = table[i * B + wave * 64 + owner];
+          if (id < 0 || id >= na.num_blocks) id = 0;      // (flagged by the first pass)
+          const int64_t off = (id * n_kv_heads + h) * na.D + c * 8;
+          const vec x = *reinterpret_cast<const vec*>((const T*)na.lo + off);
+          const vec y = *reinterpret_cast<const vec*>((const T*)na.hi + off);
+          double best = -INFINITY;
+          for (int g0 = 0; g0 < na.G; g0 += side) {
+            const vec z = *reinterpret_cast<const vec*>(
+                q + min(g0 + lane / L, na.G - 1) * na.D + c * 8);
+            double s = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float f = Elem<T>::to_f(z[j]);
+              s = __builtin_fma((double)f, (double)Elem<T>::to_f(f < 0.f ? x[j] : y[j]), s);
+            }
+            for (int m = 1; m < L; m <<= 1) s += shift_xor(s, m);
+            for (int m = L; m < 64; m <<= 1) {
+              const double o = shift_xor(s, m);
+              s = o != o || o > s ? o : s;
+            }
+            best = s != s || s > best ? s : best;
+          }
+          if (lane == owner) u[i] = order_of(best);
+        }
+      }
+      valid = open;
+      if (n_open <= kOpenRanks) {
+        // few: each counts those that beat it
+        if (tid == 0) l.digit = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+          if (open >> i & 1) {
+            const int at = atomicAdd(&l.digit, 1);
+            l.value[at] = u[i];
+            l.page[at] = i * B + tid;
+          }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+          if (open >> i & 1) {
+            int beaten = 0;
+            for (int e = 0; e < n_open; ++e)
+              beaten += l.value[e] > u[i] || (l.value[e] == u[i] && l.page[e] < i * B + tid);
+            if (beaten < k - n_sure) sure |= 1u << i;
+          }
+        }
+        valid = 0;
+        cut = Cut<uint64_t>{0, 0, false};
+      } else {
+        cut = find_cut<uint64_t, B, K>(l, u, valid, k - n_sure);
+      }
+    }
+  }
+  // Page order is (i, thread): a count a wave and i, and their sums before each.
+  uint32_t in = sure, eq = 0;
 #pragma unroll
   for (int i = 0; i < K; ++i) {
-    const bool in = i * B + tid < n && u[i] >= least;
-    const bool eq = in && ties && u[i] == least;
-    const uint64_t bi = __builtin_amdgcn_ballot_w64(in), be = __builtin_amdgcn_ballot_w64(eq);
+    if (valid >> i & 1) {
+      in |= (uint32_t)(u[i] >= cut.least) << i;
+      eq |= (uint32_t)(cut.ties && u[i] == cut.least) << i;
+    }
+    const uint64_t bi = __builtin_amdgcn_ballot_w64(in >> i & 1);
+    const uint64_t be = __builtin_amdgcn_ballot_w64(eq >> i & 1);
     if (lane == 0) {
-      counts[0][i * W + wave] = __builtin_popcountll(bi & ~be);
-      counts[1][i * W + wave] = __builtin_popcountll(be);
+      l.counts[0][i * W + wave] = __builtin_popcountll(bi & ~be);
+      l.counts[1][i * W + wave] = __builtin_popcountll(be);
     }
   }
   __syncthreads();
@@ -506,7 +842,7 @@ __global__ __launch_bounds__(B) void select_rows_kernel(
       int c[C], sum = 0;
 #pragma unroll
       for (int j = 0; j < C; ++j) {
-        c[j] = lane * C + j < W * K ? counts[t][lane * C + j] : 0;
+        c[j] = lane * C + j < W * K ? l.counts[t][lane * C + j] : 0;
         sum += c[j];
       }
       int run = sum;
@@ -518,7 +854,7 @@ __global__ __launch_bounds__(B) void select_rows_kernel(
       run -= sum;
 #pragma unroll
       for (int j = 0; j < C; ++j) {
-        if (lane * C + j < W * K) counts[t][lane * C + j] = run;
+        if (lane * C + j < W * K) l.counts[t][lane * C + j] = run;
         run += c[j];
       }
     }
@@ -527,13 +863,12 @@ __global__ __launch_bounds__(B) void select_rows_kernel(
   const uint64_t below = (1ull << lane) - 1;
 #pragma unroll
   for (int i = 0; i < K; ++i) {
-    const int p = i * B + tid;
-    const bool in = p < n && u[i] >= least;
-    const bool eq = in && ties && u[i] == least;
-    const uint64_t bi = __builtin_amdgcn_ballot_w64(in), be = __builtin_amdgcn_ballot_w64(eq);
-    const int a = counts[0][i * W + wave] + __builtin_popcountll(bi & ~be & below);
-    const int e = counts[1][i * W + wave] + __builtin_popcountll(be & below);
-    if (in && (!eq || e < need)) put(a + (ties ? min(e, need) : 0), p);
+    const uint64_t bi = __builtin_amdgcn_ballot_w64(in >> i & 1);
+    const uint64_t be = __builtin_amdgcn_ballot_w64(eq >> i & 1);
+    const int before = l.counts[0][i * W + wave] + __builtin_popcountll(bi & ~be & below);
+    const int e = l.counts[1][i * W + wave] + __builtin_popcountll(be & below);
+    if ((in >> i & 1) && (!(eq >> i & 1) || e < cut.need))
+      to.put(before + (cut.ties ? min(e, cut.need) : 0), i * B + tid);
   }
 }
 
@@ -542,6 +877,12 @@ struct ScoreArgs {
   const int32_t* indptr; const int32_t* indices; const int32_t* kv_lens;
   int32_t n_seqs, Hkv, page_size, pages, max_pages; double* scores; int32_t* status;
 };
+constexpr int kSelectMax = 1024 * 16;   // pages select_rows_kernel holds
+// Elements of lo (of all candidates, KV heads and sequences) from which the scores
+// run in 32 bits first: the choice then takes 4 to 5 us more, for the pages left
+// open. us of scores and choice, 32 bits against 64: 1M elements 16.6 and 14.6,
+// 3M 17.5 and 15.9, 25M 27.7 and 29.0, 61M 45.4 and 54.2.
+constexpr int64_t kNearLeast = 16 << 20;
 typedef void (*ScoreFn)(const ScoreArgs&, hipStream_t);
 
 template <typename T, int D, int G>
@@ -553,6 +894,32 @@ static void launch_scores(const ScoreArgs& a, hipStream_t s) {
                      dim3(256), 0, s, (const T*)a.q, (const T*)a.lo, (const T*)a.hi, a.nb, a.indptr,
                      a.indices, a.kv_lens, a.Hkv, a.page_size, a.pages, (int64_t)a.max_pages,
                      a.scores, a.status);
+}
+
+template <typename T, int D, int G>
+static void launch_near(const ScoreArgs& a, hipStream_t s) {
+  constexpr int PAGES = NearShape<T, D, G>::PAGES;
+  hipLaunchKernelGGL((near_scores_kernel<T, D, G>),
+                     dim3((unsigned)a.Hkv, (unsigned)((a.max_pages - 1 + PAGES - 1) / PAGES),
+                          (unsigned)a.n_seqs),
+                     dim3(256), 0, s, (const T*)a.q, (const T*)a.lo, (const T*)a.hi, a.nb, a.indptr,
+                     a.indices, a.kv_lens, a.Hkv, a.page_size, a.pages, (int64_t)a.max_pages,
+                     (float*)a.scores, a.status);
+}
+
+// The 32-bit scores of a 16-bit pool, and the pages of its workgroups.
+struct NearFn { ScoreFn launch; int block_pages; };
+
+template <typename T, int D>
+static NearFn near_g(int G) {
+  switch (G) {
+    case 1: return {launch_near<T, D, 1>, NearShape<T, D, 1>::PAGES};
+    case 2: return {launch_near<T, D, 2>, NearShape<T, D, 2>::PAGES};
+    case 4: return {launch_near<T, D, 4>, NearShape<T, D, 4>::PAGES};
+    case 8: return {launch_near<T, D, 8>, NearShape<T, D, 8>::PAGES};
+    case 16: return {launch_near<T, D, 16>, NearShape<T, D, 16>::PAGES};
+    default: return {nullptr, 0};
+  }
 }
 
 template <typename T, int D>
@@ -639,20 +1006,26 @@ extern "C" int pkv_select_pages(const void* q, const void* lo, const void* hi, i
     return fail(PKV_ERR_INVALID, "page words need a plan (pkv_plan_selected)");
   const int32_t width = std::min(pages, max_pages);
   hipStream_t s = (hipStream_t)stream;
+  NearFn near{nullptr, 0};
   if (max_pages > pages && pages > 1) {
     const uintptr_t at = (uintptr_t)q | (uintptr_t)lo | (uintptr_t)hi |
                          (uintptr_t)((int64_t)head_dim * elem_bytes(dtype));
+    const ScoreArgs args{q, lo, hi, num_blocks, kv_indptr, kv_indices, kv_lens, n_seqs, n_kv_heads,
+                         page_size, pages, max_pages, scores, status_word};
+    const bool wide = at % 16 == 0;
+    const int32_t G = n_heads / n_kv_heads;
     auto score = [&](auto type) {
       typedef decltype(type) T;
-      const bool wide = at % 16 == 0;
-      // (a grid of up to 65535 workgroups of at least 8 pages)
-      const ScoreFn fn = wide && max_pages <= 8 * 65535
-                             ? score_fn<T>(head_dim, n_heads / n_kv_heads) : nullptr;
-      if (fn) {
-        fn({q, lo, hi, num_blocks, kv_indptr, kv_indices, kv_lens, n_seqs, n_kv_heads, page_size,
-            pages, max_pages, scores, status_word}, s);
-        return;
+      if constexpr (sizeof(T) == 2) {
+        // (a list that fits the registers of select_rows_kernel)
+        if (wide && max_pages <= kSelectMax &&
+            (int64_t)n_seqs * n_kv_heads * max_pages * head_dim >= kNearLeast)
+          near = head_dim == 64 ? near_g<T, 64>(G) : head_dim == 128 ? near_g<T, 128>(G) : near;
+        if (near.launch) return near.launch(args, s);
       }
+      // (a grid of up to 65535 workgroups of at least 8 pages)
+      const ScoreFn fn = wide && max_pages <= 8 * 65535 ? score_fn<T>(head_dim, G) : nullptr;
+      if (fn) return fn(args, s);
       auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)((max_pages + 62) / 64), (unsigned)n_kv_heads,
                                         (unsigned)n_seqs),
@@ -668,17 +1041,24 @@ extern "C" int pkv_select_pages(const void* q, const void* lo, const void* hi, i
     else score(float{});
     PKV_LAUNCH_CHECK();
   }
-  auto choose = [&](auto kernel, int threads) {
+  const Choice choice{ids, ordinals, words, places, head_words, num_blocks, n_seqs, part_pages};
+  const NearArgs na{q, lo, hi, num_blocks, head_dim, n_heads / n_kv_heads, near.block_pages};
+  auto choose = [&](auto kernel, int threads, auto... more) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)n_kv_heads, (unsigned)n_seqs), dim3(threads), 0, s,
                        scores, (int64_t)max_pages, kv_indptr, kv_indices, kv_lens, n_kv_heads,
-                       page_size, pages, width,
-                       Choice{ids, ordinals, words, places, head_words, num_blocks, n_seqs,
-                              part_pages});
+                       page_size, pages, width, choice, more...);
   };
-  if (max_pages <= 256 * 4) choose(select_rows_kernel<256, 4>, 256);
-  else if (max_pages <= 1024 * 4) choose(select_rows_kernel<1024, 4>, 1024);
-  else if (max_pages <= 1024 * 16) choose(select_rows_kernel<1024, 16>, 1024);
-  else choose(select_kernel, 256);
+  auto rows = [&](auto type, auto is_near) {
+    typedef decltype(type) T;
+    constexpr bool N = decltype(is_near)::value;
+    if (max_pages <= 256 * 4) choose(select_rows_kernel<T, N, 256, 4>, 256, na);
+    else if (max_pages <= 1024 * 4) choose(select_rows_kernel<T, N, 1024, 4>, 1024, na);
+    else choose(select_rows_kernel<T, N, 1024, 16>, 1024, na);
+  };
+  if (max_pages > kSelectMax) choose(select_kernel, 256);
+  else if (!near.launch) rows(float{}, std::false_type{});
+  else if (dtype == PKV_DTYPE_F16) rows(_Float16{}, std::true_type{});
+  else rows(__bf16{}, std::true_type{});
   PKV_LAUNCH_CHECK();
   return PKV_OK;
 }

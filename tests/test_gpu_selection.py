@@ -155,6 +155,85 @@ def test_equal_scores_take_the_earlier_pages():
     assert chosen[1].tolist() == [list(range(11)) + [39]] * 2
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n_heads, n_kv, d", [(32, 8, 64), (8, 1, 128), (16, 1, 64)])
+def test_scores_that_only_64_bits_tell_apart(n_heads, n_kv, d, dtype):
+    """Every page the same but for the last place of one small element: scores
+    that differ by far less than 32-bit sums do."""
+    c = Cache([1500, 900, 40], n_heads, n_kv, d, dtype)
+    for s in c.seqs[:2]:
+        ids = torch.tensor(s.block_ids, device=DEV)
+        page = c.rand((16, n_kv, d)).abs() + 1
+        page[..., 5] = 2.0 ** -9
+        kp = page.repeat(len(ids), 1, 1, 1)
+        step = torch.randperm(len(ids), generator=c.g, device=DEV) % 7
+        kp[..., 5] *= (1 + step * torch.finfo(dtype).eps)[:, None, None].to(dtype)
+        c.bk.k_pool[0][ids] = kp
+    c.bk.refresh_page_bounds()
+    q = c.q().abs()
+    for pages in (2, 9, 30):
+        out, chosen = c.bk.attend_selected(q, 0, 0.125, c.meta, pages, return_pages=True)
+        c.check(q, pages, out, chosen)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_lists_longer_than_a_workgroup_holds(dtype):
+    """16 500 candidates: the choice that re-reads its scores."""
+    c = Cache([16500 * 16 + 5, 4], 8, 1, 64, dtype)
+    q = c.q()
+    out, chosen = c.bk.attend_selected(q, 0, 0.125, c.meta, 40, return_pages=True)
+    c.bk.check_device_errors()
+    c.check(q, 40, out, chosen)
+
+
+@pytest.mark.parametrize("n_heads, n_kv, d", [
+    (32, 8, 64), (8, 8, 128), (16, 8, 64), (64, 8, 128), (64, 4, 64)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["random", "close", "whole numbers", "nan"])
+def test_many_candidates(n_heads, n_kv, d, dtype, kind):
+    """Enough of them that their scores run in 32 bits first: random pages,
+    pages that only 64 bits tell apart, ties, and a NaN key."""
+    pages = (17 << 20) // (n_kv * d)
+    lens = [pages * 16 // 4 + 16, pages * 16 // 4 + 3, 40 * 16, 5]
+    print(f"many candidates {n_heads}/{n_kv}/{d} {dtype} {kind} {lens}", flush=True)
+    c = Cache(lens, n_heads, n_kv, d, dtype)
+    q, kp = c.q(), c.bk.k_pool[0]
+    if kind == "close":
+        page = c.rand((16, n_kv, d)).abs() + 1
+        page[..., 5] = 2.0 ** -9
+        step = torch.randperm(kp.shape[0], generator=c.g, device=DEV) % 50
+        kp.copy_(page)
+        kp[..., 5] *= (1 + step * torch.finfo(dtype).eps)[:, None, None].to(dtype)
+        q = q.abs()
+    elif kind == "whole numbers":
+        kp.copy_(torch.randint(-1, 2, kp.shape, generator=c.g, device=DEV))
+        q = torch.randint(-2, 3, q.shape, generator=c.g, device=DEV).to(dtype)
+    c.bk.refresh_page_bounds()
+    if kind == "nan":                                  # in one KV head of one sequence
+        ids = c.seqs[0].block_ids
+        c.bk.key_bounds[0][:, ids[77], n_kv - 1, 3] = float("nan")
+        out, chosen = c.bk.attend_selected(q, 0, 0.125, c.meta, 30, return_pages=True)
+        assert (chosen[0, n_kv - 1] == 77).any()
+        lo, hi = (b[ids] for b in c.bk.key_bounds[0])
+        want = chosen64(q[0], lo, hi, len(ids), 30)
+        assert chosen[0].tolist() == want
+        return
+    for pages in (2, 30):
+        out, chosen = c.bk.attend_selected(q, 0, 0.125, c.meta, pages, return_pages=True)
+        c.bk.check_device_errors()
+        c.check(q, pages, out, chosen)
+
+
+def test_lists_of_every_kernel_size():
+    """Around 1024, 4096 and 16384 pages, where the choice's kernels change."""
+    for n in (1023, 1024, 1025, 4096, 4097, 16384, 16385):
+        print("pages", n, flush=True)
+        c = Cache([n * 16 - 3], 4, 2, 64, torch.bfloat16)
+        q = c.q()
+        out, chosen = c.bk.attend_selected(q, 0, 0.125, c.meta, 21, return_pages=True)
+        c.check(q, 21, out, chosen)
+
+
 def test_signs_and_sizes_of_scores():
     """All scores negative, all zero, of one exponent, and far apart."""
     c = Cache([900] * 4, 4, 4, 64, torch.bfloat16)

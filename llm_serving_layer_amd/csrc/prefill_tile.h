@@ -114,10 +114,14 @@ template <int RB> __device__ __forceinline__ int wide_xr(int row) {
 // unit; at head_dim 64 eight are enough), tiles loaded RING - 2 ahead. Such a
 // tile has at most one more workgroup beside it, so its own loads have to cover
 // the memory's latency, where a prefill tile's neighbours do.
+// At head_dim 64 a tile has 64 keys: a step's fixed cost (about 50 scalar
+// instructions, a barrier, the wait for the first LDS reads) is paid half as
+// often, and two score products run side by side.
 template <typename T, int D> struct SharedRing {
-  static constexpr int N = 81920 / (2 * PrefillLds<T, D>::TILE) < 8
-                               ? 81920 / (2 * PrefillLds<T, D>::TILE) : 8;
-  static constexpr int BYTES = N * 2 * PrefillLds<T, D>::TILE;
+  static constexpr int TT = D == 64 ? 64 : 32;              // keys of a tile
+  static constexpr int TILE = TT * D * (int)sizeof(T);      // one K (or V) tile
+  static constexpr int N = 81920 / (2 * TILE) < 8 ? 81920 / (2 * TILE) : 8;
+  static constexpr int BYTES = N * 2 * TILE;
 };
 
 template <typename T, int D, int G, bool SHARED = false>
@@ -131,7 +135,8 @@ __device__ __forceinline__ void prefill_tile(
   typedef typename Mma<T>::vec8 vec8;
   typedef typename Mma<T>::vec4 vec4;
   typedef PrefillLds<T, D> L;
-  constexpr int TT = L::TT;
+  constexpr int TT = SHARED ? SharedRing<T, D>::TT : L::TT;
+  constexpr int TILE = SHARED ? SharedRing<T, D>::TILE : L::TILE;
   constexpr int PS = 16;
   constexpr int NH = TT / 32;            // 32-key halves per tile
   constexpr int NC = D / 16;             // QK k-chunks of 16 dims
@@ -140,10 +145,10 @@ __device__ __forceinline__ void prefill_tile(
   constexpr int CPR = RB / 16;           // 16-byte chunks per row
   constexpr int LPT = L::LPT;
   static_assert(64 % CPR == 0 && PS % (64 / CPR) == 0, "a wave load stays in one page");
-  unsigned char* const buf0 = smem + 0 * 2 * L::TILE;
-  unsigned char* const buf1 = smem + 1 * 2 * L::TILE;
-  unsigned char* const buf2 = smem + 2 * 2 * L::TILE;
-  unsigned char* const buf3 = smem + 3 * 2 * L::TILE;
+  unsigned char* const buf0 = smem + 0 * 2 * TILE;
+  unsigned char* const buf1 = smem + 1 * 2 * TILE;
+  unsigned char* const buf2 = smem + 2 * 2 * TILE;
+  unsigned char* const buf3 = smem + 3 * 2 * TILE;
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -209,10 +214,12 @@ __device__ __forceinline__ void prefill_tile(
   const uint32_t pagebytes = PS * rowbytes;
   // ids at or past this are out of range (kv_indices entries are int32)
   const uint32_t nb32 = num_blocks > 0x7fffffffLL ? 0x80000000u : (uint32_t)num_blocks;
-  static_assert(TT == 2 * PS, "a tile is two pages");
-  const int wpage = wave & 1;
-  const T* const wpool = wave < 2 ? kpool : vpool;
-  const uint32_t wdst = (wave < 2 ? 0 : L::TILE) + wpage * PS * RB;
+  // (a tile of four pages: a wave loads one page of both tensors)
+  constexpr bool BOTH = TT == 4 * PS;
+  static_assert(BOTH || TT == 2 * PS, "a tile is two pages or four");
+  const int wpage = BOTH ? wave : wave & 1;
+  const T* const wpool = BOTH || wave < 2 ? kpool : vpool;
+  const uint32_t wdst = (BOTH || wave < 2 ? 0 : TILE) + wpage * PS * RB;
   constexpr int RPI = 64 / CPR;                  // rows of a wave load
   uint32_t voff[LPT];
 #pragma unroll
@@ -223,12 +230,12 @@ __device__ __forceinline__ void prefill_tile(
     voff[k] = (uint32_t)rr * rowbytes + (uint32_t)(h * RB + lc * 16);
   }
   auto load_id = [&](int t) {   // this wave's page id for tile t
-    return __builtin_amdgcn_readfirstlane(kv_indices[pbase + min(2 * t + wpage, npages - 1)]);
+    return __builtin_amdgcn_readfirstlane(kv_indices[pbase + min(TT / PS * t + wpage, npages - 1)]);
   };
   // Rows past kv_len, pages past the last and out-of-range pages are outside
   // the buffer range: zeros land in LDS without a memory access.
   auto load_tile = [&](int t, int raw, const unsigned char* dst) {
-    const int pg = 2 * t + wpage;
+    const int pg = TT / PS * t + wpage;
     const bool bad = (uint32_t)raw >= nb32;   // (negative ids too)
     if (bad && pg < npages && lane == 0) flag(status, PKV_STATUS_BAD_PAGE);
     const int live_rows = bad ? 0 : min(PS, kv_len - pg * PS);   // <= 0 past the end
@@ -237,6 +244,11 @@ __device__ __forceinline__ void prefill_tile(
         raw_rsrc(reinterpret_cast<const char*>(wpool) + (uint64_t)pid * pagebytes,
                  live_rows > 0 ? (uint32_t)live_rows * rowbytes : 0u),
         voff, lds_address(dst) + wdst);
+    if constexpr (BOTH)
+      load_to_lds<LPT>(
+          raw_rsrc(reinterpret_cast<const char*>(vpool) + (uint64_t)pid * pagebytes,
+                   live_rows > 0 ? (uint32_t)live_rows * rowbytes : 0u),
+          voff, lds_address(dst) + wdst + TILE);
   };
 
   // O^T accumulators: o[dh][rr] = O[row][32 dh + 8 (rr / 4) + 4 g + rr % 4].
@@ -405,15 +417,15 @@ __device__ __forceinline__ void prefill_tile(
     // The ring of a shared tile: tile t in buffer t % N, tile t + AHEAD loaded
     // in step t, into the buffer that step t - 2 was the last to read.
     constexpr int N = SharedRing<T, D>::N, AHEAD = N - 2;
-    unsigned char* prev = smem + (N - 1) * 2 * L::TILE;
-    for (int i = tid; i < L::TILE / 16; i += kPrefillThreads)
-      reinterpret_cast<u32x4*>(prev + L::TILE)[i] = u32x4{0u, 0u, 0u, 0u};
+    unsigned char* prev = smem + (N - 1) * 2 * TILE;
+    for (int i = tid; i < TILE / 16; i += kPrefillThreads)
+      reinterpret_cast<u32x4*>(prev + TILE)[i] = u32x4{0u, 0u, 0u, 0u};
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     int ids[AHEAD + 1];
 #pragma unroll
     for (int t = 0; t <= AHEAD; ++t) ids[t] = load_id(t);
 #pragma unroll
-    for (int t = 0; t < AHEAD; ++t) load_tile(t, ids[t], smem + t * 2 * L::TILE);
+    for (int t = 0; t < AHEAD; ++t) load_tile(t, ids[t], smem + t * 2 * TILE);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {   // Q arrives here (see below)
       u32x4 w = __builtin_bit_cast(u32x4, qb[c]);
@@ -421,20 +433,20 @@ __device__ __forceinline__ void prefill_tile(
       qb[c] = __builtin_bit_cast(vec8, w);
     }
     int id = ids[AHEAD];
-    unsigned char* next = smem + AHEAD * 2 * L::TILE;
-    unsigned char* const end = smem + N * 2 * L::TILE;
+    unsigned char* next = smem + AHEAD * 2 * TILE;
+    unsigned char* const end = smem + N * 2 * TILE;
     last = smem;
     for (int t = 0;; ++t) {
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((AHEAD - 1) * LPT) : "memory");
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((AHEAD - 1) * LPT * (BOTH ? 2 : 1)) : "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       load_tile(t + AHEAD, id, next);
-      compute(t, last, prev + L::TILE);
+      compute(t, last, prev + TILE);
       id = load_id(t + AHEAD + 1);
       if (t + 1 >= ntiles) break;
       prev = last;
-      last = last + 2 * L::TILE == end ? smem : last + 2 * L::TILE;
-      next = next + 2 * L::TILE == end ? smem : next + 2 * L::TILE;
+      last = last + 2 * TILE == end ? smem : last + 2 * TILE;
+      next = next + 2 * TILE == end ? smem : next + 2 * TILE;
     }
   } else {
     // The ring: tile t in buffer t % 4. Each step waits for its tile's loads
@@ -445,8 +457,8 @@ __device__ __forceinline__ void prefill_tile(
     // tile t + 3.
     // The first step's PV meets zero probabilities in buf3, which no tile has
     // filled yet: zeros there (visible to every wave at the step's barrier).
-    for (int i = tid; i < L::TILE / 16; i += kPrefillThreads)
-      reinterpret_cast<u32x4*>(buf3 + L::TILE)[i] = u32x4{0u, 0u, 0u, 0u};
+    for (int i = tid; i < TILE / 16; i += kPrefillThreads)
+      reinterpret_cast<u32x4*>(buf3 + TILE)[i] = u32x4{0u, 0u, 0u, 0u};
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     int id0 = load_id(0), id1 = load_id(1), id2 = load_id(2), id3;   // of tile j in id(j % 4)
     load_tile(0, id0, buf0);
@@ -467,7 +479,7 @@ __device__ __forceinline__ void prefill_tile(
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       load_tile(t + 2, id_t2, nxt2);
-      compute(t, cur, prev + L::TILE);
+      compute(t, cur, prev + TILE);
       // (after the tile's LDS reads: a scalar load in flight would make every
       // wait for them a wait for it too)
       id_t3 = load_id(t + 3);
@@ -487,7 +499,7 @@ __device__ __forceinline__ void prefill_tile(
       if (t + 4 >= ntiles) break;
     }
   }
-  pv(last + L::TILE);   // the last tile's PV
+  pv(last + TILE);   // the last tile's PV
   // the loads of the tiles past the end land in LDS before the workgroup ends
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 

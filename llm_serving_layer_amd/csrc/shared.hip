@@ -67,7 +67,7 @@ __global__ __launch_bounds__(256, 2) void shared_stream_kernel(SharedArgs<T> a) 
 
 // Tiles beside the small-batch decode kernel's workgroups, one a piece and KV head.
 template <typename T, int D, int G>
-__global__ __launch_bounds__(256, kPieceWaves<D>) void shared_piece_kernel(SharedArgs<T> a) {
+__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void shared_piece_kernel(SharedArgs<T> a) {
   constexpr int A = PieceLds<T, D, G>::BYTES, B = SharedRing<T, D>::BYTES;
   __shared__ __align__(16) unsigned char smem[A > B ? A : B];
   const int role = shared_role(blockIdx.x, a.tiles, a.pieces, a.turn);

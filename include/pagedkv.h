@@ -346,7 +346,9 @@ int pkv_attend_batch(const void* batch, const void* q, void* out, void* k_pool, 
  * Shared-prefix plan (host function) — no counterpart in the reference, whose
  * radix cache shares pages but whose attention reads them once a sequence.
  * Page lists that begin with the same ids form a tree; each of its runs of at
- * least min_pages pages with two or more sequences below it becomes tiles of
+ * least min_pages pages with n >= 2 sequences below it that saves more bytes a
+ * KV head ((n - 1) * pages * page_bytes, page_bytes a page's of a KV head) than
+ * it costs (n * part_bytes, a part more for each sequence) becomes tiles of
  * pkv_attend_shared, 128 / (n_heads / n_kv_heads) sequences and a split of the
  * run each, splits sized for about tile_target workgroups. A sequence's last
  * page is never shared. `plan` is pkv_plan_decode's over the remaining pages
@@ -357,12 +359,14 @@ int pkv_attend_batch(const void* batch, const void* q, void* out, void* k_pool, 
  * first partial slot, 0} of the sequences with shared parts, then the members
  * {row of q, partial slot of split 0}; *tiles_needed ints in all. A buffer too small
  * gives PKV_ERR_CAPACITY with the needed sizes set (tiles_needed once plan
- * suffices).
+ * suffices). Where all runs together save less than least_bytes over the KV
+ * heads nothing is shared: *n_tiles_out is 0 and no plan is written.
  */
 int pkv_plan_shared(const int32_t* kv_indptr, const int32_t* kv_indices, const int32_t* kv_lens,
                     const int32_t* kv_last_page_len, int32_t n_seqs, int32_t page_size,
                     int64_t num_blocks, int32_t n_heads, int32_t n_kv_heads, int32_t part_pages,
-                    int32_t max_workgroups, int32_t min_pages, int32_t tile_target, int32_t* plan,
+                    int32_t max_workgroups, int32_t min_pages, int64_t page_bytes,
+                    int64_t part_bytes, int64_t least_bytes, int32_t tile_target, int32_t* plan,
                     int64_t plan_capacity, int64_t* plan_needed, int32_t* n_work_out,
                     int32_t* n_slots_out, int32_t* plan_stride_out, int32_t* tiles,
                     int64_t tiles_capacity, int64_t* tiles_needed, int32_t* n_tiles_out,

@@ -54,7 +54,7 @@ SIGNATURES = {
     "pkv_append_batch": (C.c_int, [_p, _p, _p, _p, _p, _p]),
     "pkv_attend_batch": (C.c_int, [_p, _p, _p, _p, _p, _f32, _p, _p, _p]),
     "pkv_plan_shared": (C.c_int, [_p, _p, _p, _p, _i32, _i32, _i64, _i32, _i32, _i32, _i32, _i32,
-                                  _i32, _p, _i64, _p, _p, _p, _p, _p, _i64, _p, _p, _p]),
+                                  _i64, _i64, _i64, _i32, _p, _i64, _p, _p, _p, _p, _p, _i64, _p, _p, _p]),
     "pkv_attend_shared": (C.c_int, [_p, _p, _p, _p, _i64, _p, _i32, _i32, _i32, _i32, _i32, _f32,
                                     _i32, _p, _i32, _i32, _p, _i32, _i32, _i32, _p, _p, _p, _p, _i64,
                                     _p, _p]),

@@ -65,7 +65,12 @@ SELECTED_PART_PAGES = 8  # of chosen pages; what their kernel stages at a time
 # 20.4 and 29.7, 512 20.0 and 26.8, 1024 26.9 and 29.3 (head_dim 64) or 36.2 and
 # 36.7 (128), 2048 40.7 and 34.5, 3072 81.7 and 72.5.
 SELECTED_PIECES = 1024
-SHARED_MIN_PAGES = 4     # shorter runs of shared pages stay each sequence's own
+# What attend_shared must save to be worth its tiles and its merge: a run of
+# shared pages at least 4 pages long, in bytes a KV head more than 25 KiB a
+# sequence (the part it adds), all runs together 16 MiB. us a call, attend against
+# shared: 6 sequences over 96 pages 9.8 and 10.7, 200 over 8 28.6 and 30.9, 2
+# over 512 15.8 and 13.8, 32 over 32 16.6 and 14.1, 256 over 128 134 and 46.
+SHARED_MIN_PAGES, SHARED_PART_BYTES, SHARED_LEAST_BYTES = 4, 25 << 10, 16 << 20
 SHARED_TILES = 256       # workgroups that share the work on a batch's shared pages
 DEFAULT_Q_TILE = 64      # prefill tile when the geometry has no matrix-core kernel
 
@@ -874,7 +879,8 @@ class MI355XBackend:
                 rc = self._lib.pkv_plan_shared(
                     ptr(indptr), ptr(indices), ptr(kvl), ptr(last), p.n, self.block_size,
                     self.num_blocks, self.n_heads, self.n_kv_heads, part, self._decode_wgs,
-                    SHARED_MIN_PAGES, SHARED_TILES, ptr(buf), cap, C.byref(needed),
+                    SHARED_MIN_PAGES, self._block_bytes * 2 // self.n_kv_heads, SHARED_PART_BYTES,
+                    SHARED_LEAST_BYTES, SHARED_TILES, ptr(buf), cap, C.byref(needed),
                     C.byref(n_work), C.byref(n_slots), C.byref(stride), ptr(tiles), tiles_cap,
                     C.byref(tiles_needed), C.byref(n_tiles), C.byref(n_merges))
                 if rc != _native.ERR_CAPACITY or (needed.value <= cap

@@ -177,13 +177,19 @@ struct Run {
 };
 
 // The runs of the tree of page lists, of at least min_pages pages and two
-// members; `own` marks per kv_indices entry the pages that stay a sequence's own.
+// members, that save more than they cost: all but one member's reads of the run
+// against a part more of each member; `own` marks per kv_indices entry the pages that stay a sequence's own.
 struct Tree {
   const int32_t* indptr;
   const int32_t* indices;
   int32_t min_pages;
+  int64_t page_bytes, part_bytes;   // of a KV head
   std::vector<Run> runs;
   std::vector<char> own;
+
+  int64_t saved(int64_t members, int64_t pages) const {
+    return (members - 1) * pages * page_bytes - members * part_bytes;
+  }
 
   int32_t room(int32_t i) const { return indptr[i + 1] - indptr[i] - 1; }   // the last page is own
   int32_t page(int32_t i, int32_t p) const { return indices[indptr[i] + p]; }
@@ -214,7 +220,7 @@ struct Tree {
           end = (int32_t)(std::mismatch(lead + at, lead + end, mine + at).first - lead);
         }
         Run child{at, end, std::vector<int32_t>(m.begin() + a, m.begin() + b)};
-        if (end - at >= min_pages) {
+        if (end - at >= min_pages && saved((int64_t)(b - a), end - at) >= 0) {
           for (int32_t i : child.members)
             std::fill(own.begin() + indptr[i] + at, own.begin() + indptr[i] + end, 0);
           runs.push_back(child);
@@ -234,7 +240,8 @@ extern "C" int pkv_plan_shared(const int32_t* kv_indptr, const int32_t* kv_indic
                                const int32_t* kv_lens, const int32_t* kv_last_page_len,
                                int32_t n_seqs, int32_t page_size, int64_t num_blocks,
                                int32_t n_heads, int32_t n_kv_heads, int32_t part_pages,
-                               int32_t max_workgroups, int32_t min_pages, int32_t tile_target,
+                               int32_t max_workgroups, int32_t min_pages, int64_t page_bytes,
+                               int64_t part_bytes, int64_t least_bytes, int32_t tile_target,
                                int32_t* plan, int64_t plan_capacity, int64_t* plan_needed,
                                int32_t* n_work_out, int32_t* n_slots_out,
                                int32_t* plan_stride_out, int32_t* tiles, int64_t tiles_capacity,
@@ -253,8 +260,17 @@ extern "C" int pkv_plan_shared(const int32_t* kv_indptr, const int32_t* kv_indic
                                    kv_last_page_len[i], page_size);
     if (rc) return rc;
   }
-  Tree tree{kv_indptr, kv_indices, min_pages, {}, {}};
+  Tree tree{kv_indptr, kv_indices, min_pages, page_bytes, part_bytes, {}, {}};
   tree.grow(n_seqs);
+  int64_t saved = 0;
+  for (const Run& r : tree.runs)
+    saved += n_kv_heads * tree.saved((int64_t)r.members.size(), r.last - r.first);
+  if (plan_needed) *plan_needed = 0;
+  if (tiles_needed) *tiles_needed = 0;
+  if (tree.runs.empty() || saved < least_bytes) {
+    *n_work_out = *n_slots_out = *plan_stride_out = *n_tiles_out = *n_merges_out = 0;
+    return PKV_OK;
+  }
 
   // The own pages as a batch of their own, planned by pkv_plan_decode. (Only
   // the number of a sequence's keys matters to a one-token query, not where

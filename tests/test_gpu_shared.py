@@ -13,7 +13,7 @@ import dataclasses
 import pytest
 import torch
 
-from llm_serving_layer_amd import BlockAllocator, RotaryTable, SequenceBlocks
+from llm_serving_layer_amd import BlockAllocator, RotaryTable, SequenceBlocks, backend
 from llm_serving_layer_amd.backend import MI355XBackend
 
 from ._ops64 import assert_within, attend64
@@ -21,6 +21,14 @@ from ._util import grow_and_assemble, make_meta, meta_to_device
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
+
+
+@pytest.fixture(autouse=True)
+def share_all(request, monkeypatch):
+    """Small batches too, which by the rule run ``attend``."""
+    if request.function is not test_batches_that_save_too_little_run_attend:
+        monkeypatch.setattr(backend, "SHARED_PART_BYTES", 0)
+        monkeypatch.setattr(backend, "SHARED_LEAST_BYTES", 0)
 
 
 class Batch:
@@ -219,6 +227,19 @@ def test_what_runs_attend_itself():
     assert torch.equal(d.bk.attend_shared(q, 0, 0.125, bare), want)
     odd = torch.empty(q.numel() + 1, dtype=q.dtype, device=DEV)[1:].view_as(q).copy_(q)
     assert torch.equal(d.bk.attend_shared(odd, 0, 0.125, d.meta), want)
+
+
+def test_batches_that_save_too_little_run_attend():
+    few = Batch(96, [(0, [3, 20, 40])])
+    q = few.q()
+    assert torch.equal(few.bk.attend_shared(q, 0, 0.125, few.meta),
+                       few.bk.attend(q, 0, 0.125, few.meta))
+    assert not few.bk._shared.n_tiles
+    many = Batch(256, [(0, [5] * 40), (3, [9, 9])])
+    q = many.q()
+    out = many.bk.attend_shared(q, 0, 0.125, many.meta)
+    assert many.bk._shared.n_tiles and many.bk._shared.n_merges == 42
+    many.check(q, out)
 
 
 def test_two_graphs_and_another_stream():

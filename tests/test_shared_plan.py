@@ -16,7 +16,7 @@ from llm_serving_layer_amd import _native
 
 
 def plan_shared(tables, tails, *, n_kv=8, G=4, part=17, wgs=512, min_pages=4, target=512, ps=16,
-                blocks=1 << 20):
+                blocks=1 << 20, page_bytes=4096, part_bytes=0, least=0):
     """Plan and parse: (ids, n_slots, tiles, merges, members, items)."""
     lib = _native.load()
     indptr = np.concatenate([[0], np.cumsum([len(t) for t in tables])]).astype(np.int32)
@@ -30,13 +30,17 @@ def plan_shared(tables, tails, *, n_kv=8, G=4, part=17, wgs=512, min_pages=4, ta
     for _ in range(4):
         buf, tiles = np.zeros(cap, np.int32), np.zeros(tcap, np.int32)
         rc = lib.pkv_plan_shared(p(indptr), p(ids), p(kvl), p(last), len(tables), ps, blocks,
-                                 n_kv * G, n_kv, part, wgs, min_pages, target, p(buf), cap,
-                                 C.byref(need), C.byref(nw), C.byref(ns), C.byref(st), p(tiles),
+                                 n_kv * G, n_kv, part, wgs, min_pages, page_bytes, part_bytes,
+                                 least, target, p(buf), cap, C.byref(need), C.byref(nw), C.byref(ns), C.byref(st), p(tiles),
                                  tcap, C.byref(tneed), C.byref(nt), C.byref(nm))
         if rc != _native.ERR_CAPACITY:
             break
         cap, tcap = max(cap, need.value), max(tcap, tneed.value)
     _native.check(rc, "plan")
+    if not nt.value:     # nothing is shared: no plan either
+        assert not any((nw.value, ns.value, st.value, nm.value, need.value, tneed.value))
+        none = np.zeros((0, 8), np.int32)
+        return ids, 0, none, none[:, :4], none[:, :2], []
     per_wg = 4 if n_kv % 4 == 0 else 2 if n_kv % 2 == 0 else 1
     bins, S, items = nw.value // (n_kv // per_wg), st.value, []
     for b in range(bins):
@@ -74,6 +78,8 @@ def tree(rng, n, depth, ps_pages):
 def check(tables, tails, **kw):
     ids, n_slots, tiles, merges, members, items = plan_shared(tables, tails, **kw)
     G, min_pages = kw.get("G", 4), kw.get("min_pages", 4)
+    if not len(tiles):
+        return tiles, members, min_pages
     read = {i: [] for i in range(len(tables))}
     slots = {i: [] for i in range(len(tables))}
     for first, pages, at, count, split, *rest in tiles.tolist():
@@ -146,6 +152,23 @@ def test_equal_lists_and_lists_that_are_heads_of_others():
     assert len(tiles) == 0
 
 
+def test_what_saves_too_little_is_not_shared():
+    """A run must save more than its members' parts cost, all runs together the
+    least; else the batch stays whole (no tiles, no plan)."""
+    head, more = list(range(100, 110)), list(range(200, 260))
+    tables = [head + more + [1], head + more + [2], head + [3]]
+    # two members save 60 pages of the further run, three 20 of the head
+    def runs(**kw):
+        return sorted(set(plan_shared(tables, [1, 1, 1], target=1, **kw)[2][:, 1].tolist()))
+    assert runs() == [10, 60]
+    assert runs(part_bytes=20 * 4096 // 3) == [10, 60]
+    assert runs(part_bytes=20 * 4096 // 3 + 1) == [60]
+    assert runs(part_bytes=30 * 4096) == [60] and runs(part_bytes=30 * 4096 + 1) == []
+    assert runs(least=8 * 80 * 4096) == [10, 60] and runs(least=8 * 80 * 4096 + 1) == []
+    assert plan_shared(tables, [1, 1, 1], least=1 << 40)[1] == 0
+    check(tables, [1, 5, 16], part_bytes=20 * 4096 // 3 + 1)
+
+
 def test_splits_are_even_and_bounded():
     a = list(range(1000))
     tables = [a + [2000 + i] for i in range(40)]
@@ -161,13 +184,13 @@ def test_refusals():
         lib = _native.load()
         one = (C.c_int32 * 2)(0, 2)
         ids, kv, last = (C.c_int32 * 2)(1, 2), (C.c_int32 * 1)(20), (C.c_int32 * 1)(5)
-        _native.check(lib.pkv_plan_shared(one, ids, kv, last, 1, 16, 8, 8, 2, 17, 4, 4, 8, None,
-                                          0, None, None, None, None, None, 0, None, None, None),
-                      "plan")
+        _native.check(lib.pkv_plan_shared(one, ids, kv, last, 1, 16, 8, 8, 2, 17, 4, 4, 0, 0, 0,
+                                          8, None, 0, None, None, None, None, None, 0, None, None,
+                                          None), "plan")
     for kw, match in (({"G": 3}, "not supported"), ({"min_pages": 0}, "not supported"),
                       ({"target": 0}, "not supported"), ({"part": 0}, "part_pages")):
         with pytest.raises(ValueError, match=match):
-            plan_shared([[1, 2], [1, 3]], [1, 1], **kw)
+            plan_shared([[*range(8), 20], [*range(8), 30]], [1, 1], **kw)
 
 
 def test_launch_refusals():

@@ -42,7 +42,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 from array import array
-from operator import eq
+from operator import eq, index
 
 import numpy as np
 import torch
@@ -217,7 +217,7 @@ class _Shared:
 class _Selected:
     """What ``attend_selected`` keeps for one BatchMeta and page budget."""
 
-    __slots__ = ("meta", "pages", "n", "max_pages", "indptr", "indices", "kv_lens", "scores",
+    __slots__ = ("meta", "asked", "n", "max_pages", "indptr", "indices", "kv_lens", "scores",
                  "ids", "ordinals", "words", "places", "plan", "part", "ws", "width", "args", "ptr", "buffers", "stream")
 
 
@@ -946,14 +946,15 @@ class MI355XBackend:
                              f"({tokens}, {self.n_heads}, {self.head_dim})")
         if meta.n_tokens != tokens:
             raise ValueError(f"meta describes {meta.n_tokens} tokens but q has {tokens}")
+        pages = index(pages)
         if pages < 1:
             raise ValueError(f"pages must be positive, got {pages}")
         if not float(scale) > 0:
             raise ValueError(f"attend_selected needs a positive scale, got {scale}: the bounds "
                              "are of the largest score")
         p = self._selected
-        if p is None or p.meta is not meta or p.pages != pages:
-            p = self._plan_selected(meta, int(pages))
+        if p is None or p.meta is not meta or p.asked != pages:
+            p = self._plan_selected(meta, pages)
         self._flush()
         stream = self._enter(p)
         if not (q.dtype is self.dtype and q.get_device() == self.device.index
@@ -986,8 +987,8 @@ class MI355XBackend:
                              f"(query_lens up to {int(ql.max())} over {meta.n_tokens} tokens)")
         self._check_pages(kvl, indptr, last, int(indices.shape[0]))
         p = _Selected()
-        p.pages, p.n, p.max_pages = pages, n, int(np.diff(indptr).max())
-        width = p.width = min(pages, p.max_pages)
+        p.asked, p.n, p.max_pages = pages, n, int(np.diff(indptr).max())
+        pages = width = p.width = min(pages, p.max_pages)   # (the longest list: all of it)
         dev = {"device": self.device}
         p.indptr = self._dev_i32(meta.kv_indptr)
         p.indices = self._dev_i32(meta.kv_indices)

@@ -2,6 +2,7 @@
 // (selection.hip): a list of page ids each, in order, the sequence's last page
 // last. Only the last page may be partly filled.
 #include <algorithm>
+#include <exception>
 #include <vector>
 
 #include "decode_stream.h"
@@ -184,7 +185,7 @@ extern "C" int pkv_plan_selected(const int32_t* kv_lens, int32_t n_seqs, int32_t
                                  int32_t* plan, int64_t plan_capacity, int64_t* plan_needed,
                                  int32_t* n_work_out, int32_t* n_slots_out,
                                  int32_t* plan_stride_out, int32_t* places,
-                                 int64_t places_capacity, int64_t* places_needed) {
+                                 int64_t places_capacity, int64_t* places_needed) try {
   if (n_seqs <= 0 || pages <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads)
     return fail(PKV_ERR_INVALID, "n_seqs, pages and heads must be positive, n_heads a multiple of "
                 "n_kv_heads");
@@ -237,6 +238,8 @@ extern "C" int pkv_plan_selected(const int32_t* kv_lens, int32_t n_seqs, int32_t
   *n_slots_out = n_slots;
   *plan_stride_out = stride;
   return PKV_OK;
+} catch (const std::exception& e) {   // (no memory for the plan: nothing leaves a C entry)
+  return fail(PKV_ERR_CAPACITY, "pkv_plan_selected: %s", e.what());
 }
 
 extern "C" int pkv_attend_selected(const void* q, void* out, void* k_pool, void* v_pool,

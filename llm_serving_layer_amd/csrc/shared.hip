@@ -18,6 +18,7 @@
 //    each. Neither knows when a sequence's parts are complete; a last small
 //    launch merges them.
 #include <algorithm>
+#include <exception>
 #include <numeric>
 #include <vector>
 
@@ -246,7 +247,7 @@ extern "C" int pkv_plan_shared(const int32_t* kv_indptr, const int32_t* kv_indic
                                int32_t* n_work_out, int32_t* n_slots_out,
                                int32_t* plan_stride_out, int32_t* tiles, int64_t tiles_capacity,
                                int64_t* tiles_needed, int32_t* n_tiles_out,
-                               int32_t* n_merges_out) {
+                               int32_t* n_merges_out) try {
   if (n_seqs <= 0 || page_size <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads)
     return fail(PKV_ERR_INVALID, "n_seqs, page_size and heads must be positive, n_heads a "
                 "multiple of n_kv_heads");
@@ -396,6 +397,8 @@ extern "C" int pkv_plan_shared(const int32_t* kv_indptr, const int32_t* kv_indic
   *n_tiles_out = (int32_t)n_tiles;
   *n_merges_out = n_merges;
   return PKV_OK;
+} catch (const std::exception& e) {   // (no memory for the plan: nothing leaves a C entry)
+  return fail(PKV_ERR_CAPACITY, "pkv_plan_shared: %s", e.what());
 }
 
 extern "C" int pkv_attend_shared(const void* q, void* out, void* k_pool, void* v_pool,

@@ -189,10 +189,10 @@ def test_lists_longer_than_a_workgroup_holds(dtype):
 @pytest.mark.parametrize("n_heads, n_kv, d", [
     (32, 8, 64), (8, 8, 128), (16, 8, 64), (64, 8, 128), (64, 4, 64)])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("kind", ["random", "close", "whole numbers", "nan"])
+@pytest.mark.parametrize("kind", ["random", "close", "whole numbers", "tiny", "nan"])
 def test_many_candidates(n_heads, n_kv, d, dtype, kind):
     """Enough of them that their scores run in 32 bits first: random pages,
-    pages that only 64 bits tell apart, ties, and a NaN key."""
+    pages that only 64 bits tell apart, ties, subnormal keys, and a NaN key."""
     pages = (17 << 20) // (n_kv * d)
     lens = [pages * 16 // 4 + 16, pages * 16 // 4 + 3, 40 * 16, 5]
     print(f"many candidates {n_heads}/{n_kv}/{d} {dtype} {kind} {lens}", flush=True)
@@ -208,6 +208,9 @@ def test_many_candidates(n_heads, n_kv, d, dtype, kind):
     elif kind == "whole numbers":
         kp.copy_(torch.randint(-1, 2, kp.shape, generator=c.g, device=DEV))
         q = torch.randint(-2, 3, q.shape, generator=c.g, device=DEV).to(dtype)
+    elif kind == "tiny":
+        kp *= 2.0 ** -20 if dtype == torch.float16 else 2.0 ** -128
+        q *= 2.0 ** 9 if dtype == torch.float16 else 2.0 ** 120
     c.bk.refresh_page_bounds()
     if kind == "nan":                                  # in one KV head of one sequence
         ids = c.seqs[0].block_ids
@@ -466,11 +469,16 @@ def test_refusals():
                         ((q[:, :4], 0, 0.1, c.meta, 4), "q has shape"),
                         ((q[:1], 0, 0.1, c.meta, 4), "tokens"),
                         ((q, 0, 0.1, c.meta, 0), "pages"),
+                        ((q, 0, 0.1, c.meta, -1), "pages"),
                         ((q, 0, 0.0, c.meta, 4), "scale"),
                         ((q, 0, -1.0, c.meta, 4), "scale"),
                         ((q, 0, float("nan"), c.meta, 4), "scale")):
         with pytest.raises(ValueError, match=match):
             c.bk.attend_selected(*args)
+    with pytest.raises(TypeError):
+        c.bk.attend_selected(q, 0, 0.1, c.meta, 2.5)
+    every = c.bk.attend_selected(q, 0, 0.1, c.meta, 10 ** 12)
+    assert torch.equal(every, c.bk.attend_selected(q, 0, 0.1, c.meta, 19))
     chunk = meta_to_device(grow_and_assemble(c.seqs, [2, 1], 16), DEV)
     with pytest.raises(ValueError, match="one token per sequence"):
         c.bk.attend_selected(c.rand((3, 8, 64)), 0, 0.1, chunk, 4)

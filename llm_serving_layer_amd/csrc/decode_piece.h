@@ -246,14 +246,18 @@ __device__ __forceinline__ void decode_piece(
   const int n_items = CHOSEN ? 1 : bp[0];
   int p0 = 0;
   for (int item = 0;; ++item) {
-    int seq, np, tok0, kv, slot, nparts, slot0, row, flags = 0;
+    int seq, np, tok0, kv, slot, nparts, slot0, row, flags = 0, first_id = 0;
     if constexpr (CHOSEN) {
       if (item > 0) break;
       seq = row = bin / ch.max_parts;
       const int p = bin - seq * ch.max_parts;
+      // the first chunk's ids go out with the length, whose list they may end past
+      const int at = p * ch.part_pages + lane;
+      first_id = at < ch.width ? ch.ids[((int64_t)seq * n_kv_heads + h) * ch.width + at] : 0;
       const int len = max(ch.kv_lens[seq], 1), all = (len + PS - 1) / PS;
       const int n = min(min(all, ch.pages), ch.width), part = ch.part_pages;
       nparts = (n + part - 1) / part;
+      asm volatile("" ::"v"(first_id));   // (here at the latest)
       if (p >= nparts) break;
       np = min(part, n - p * part);
       tok0 = p * part * PS;
@@ -273,7 +277,9 @@ __device__ __forceinline__ void decode_piece(
     auto page_words = [&](int c0) __attribute__((always_inline)) {
       if constexpr (CHOSEN) {
         const int i = tok0 / PS + c0 + lane;   // of the chosen list
-        const int id = c0 + lane < np ? ch.ids[((int64_t)seq * n_kv_heads + h) * ch.width + i] : 0;
+        int id = c0 > 0 && c0 + lane < np
+                     ? ch.ids[((int64_t)seq * n_kv_heads + h) * ch.width + i] : 0;
+        if (c0 == 0 && lane < np) id = first_id;
         const bool out_of = id < 0 || (int64_t)id >= num_blocks;
         const int live = min(PS, kv - i * PS);
         return (int)((uint32_t)(out_of ? 0 : id) | ((uint32_t)(live - 1) & 15u) << kPageIdBits |

@@ -444,9 +444,9 @@ struct ChoiceRow {
     }
   }
   // the j-th chosen page is page p of the sequence
-  __device__ void put(int j, int p) const {
+  __device__ void put(int j, int p) const { put(j, p, table[p]); }
+  __device__ void put(int j, int p, int id) const {
     if ((unsigned)j >= (unsigned)width) return;   // (never: a list has `width` at most)
-    const int id = table[p];
     c.ordinals[row + j] = p;
     if (!words) {
       c.ids[row + j] = id;
@@ -681,8 +681,27 @@ __global__ __launch_bounds__(B) void select_rows_kernel(
   __shared__ SelectLds<B, K> l;
   const int seq = blockIdx.y, h = blockIdx.x, tid = threadIdx.x;
   const int wave = tid >> 6, lane = tid & 63;
+  // The scores go out with the lengths (a row has room for `stride` of them, and
+  // what lies past the sequence's is not used).
+  const double* sc = scores + ((int64_t)seq * n_kv_heads + h) * stride;
+  const float* near_row = reinterpret_cast<const float*>(sc);   // scores, then maxima
+  double wide_score[NEAR ? 1 : K];
+  float near_score[NEAR ? K : 1];
+  if (stride > pages && pages > 1) {
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      const int p = min((int64_t)i * B + tid, stride - 1);
+      if constexpr (NEAR) near_score[i] = near_row[p];
+      else wide_score[i] = sc[p];
+    }
+  }
   const int np = seq_pages(kv_indptr, kv_lens, seq, page_size, stride);
   const int32_t* table = kv_indices + kv_indptr[seq];
+#pragma unroll
+  for (int i = 0; i < K; ++i) {   // (here at the latest: not sunk to their first use)
+    if constexpr (NEAR) asm volatile("" ::"v"(near_score[i]));
+    else asm volatile("" ::"v"(wide_score[i]));
+  }
   const ChoiceRow to(choice, table, seq, h, n_kv_heads, width, min(np, pages),
                      kv_lens[seq] - (np - 1) * page_size);
   if (np <= pages) {
@@ -695,18 +714,20 @@ __global__ __launch_bounds__(B) void select_rows_kernel(
   const int n = np - 1, k = pages - 1;
   if (tid == 0) to.put(k, n);
   if (k == 0) return;
-  const double* sc = scores + ((int64_t)seq * n_kv_heads + h) * stride;
   uint32_t valid = 0, sure = 0;      // bit i: page i B + tid; settled as in
+  int32_t id[K];                     // (read beside the search, not after it)
 #pragma unroll
-  for (int i = 0; i < K; ++i) valid |= (uint32_t)(i * B + tid < n) << i;
+  for (int i = 0; i < K; ++i) {
+    valid |= (uint32_t)(i * B + tid < n) << i;
+    id[i] = table[min(i * B + tid, n - 1)];
+  }
   uint64_t u[K];
   Cut<uint64_t> cut;
   if constexpr (!NEAR) {
 #pragma unroll
-    for (int i = 0; i < K; ++i) u[i] = valid >> i & 1 ? order_of(sc[i * B + tid]) : 0;
+    for (int i = 0; i < K; ++i) u[i] = valid >> i & 1 ? order_of(wide_score[i]) : 0;
     cut = find_cut<uint64_t, B, K>(l, u, valid, k);
   } else {
-    const float* near_row = reinterpret_cast<const float*>(sc);   // scores, then maxima
     const T* q = (const T*)na.q + ((int64_t)seq * n_kv_heads + h) * na.G * na.D;
     // sum |q| of each query head, a head a wave; the largest bound
     float q_sum = 0.f, b_max = 0.f;
@@ -724,7 +745,7 @@ __global__ __launch_bounds__(B) void select_rows_kernel(
     uint32_t v[K];
 #pragma unroll
     for (int i = 0; i < K; ++i) {
-      a[i] = valid >> i & 1 ? near_row[i * B + tid] : 0.f;
+      a[i] = valid >> i & 1 ? near_score[i] : 0.f;
       const uint32_t bits = __builtin_bit_cast(uint32_t, a[i] + 0.f);
       v[i] = bits >> 31 ? ~bits : bits | 1u << 31;
     }
@@ -868,7 +889,7 @@ __global__ __launch_bounds__(B) void select_rows_kernel(
     const int before = l.counts[0][i * W + wave] + __builtin_popcountll(bi & ~be & below);
     const int e = l.counts[1][i * W + wave] + __builtin_popcountll(be & below);
     if ((in >> i & 1) && (!(eq >> i & 1) || e < cut.need))
-      to.put(before + (cut.ties ? min(e, cut.need) : 0), i * B + tid);
+      to.put(before + (cut.ties ? min(e, cut.need) : 0), i * B + tid, id[i]);
   }
 }
 

@@ -559,9 +559,14 @@ class MI355XBackend:
                 if rc:
                     _native.check(rc, "append_kv")
                 return
-        self._launch_append(layer_idx, k, v, self._slots_for(meta), stream)
+        r = None
         if self._bounds is not None:
-            self._complete_bounds(layer_idx, meta)
+            r = self._rows
+            if r is None or r.meta is not meta:
+                r = self._rows_for(meta)
+        self._launch_append(layer_idx, k, v, self._slots_for(meta), stream)
+        if r is not None and r.complete is not None:
+            self._renew_bounds(r.complete, r.complete.shape[0], self._enter(r), layer_idx)
 
     def append_kv_rotated(self, layer_idx: int, q: torch.Tensor, k: torch.Tensor,
                           v: torch.Tensor, meta: BatchMeta, table: RotaryTable) -> torch.Tensor:
@@ -577,6 +582,7 @@ class MI355XBackend:
         it first, as ``append_kv`` does. A position past the table is refused
         where the meta's host mirror tells it, and else flagged for
         ``check_device_errors`` (its row is not written, its query is zero).
+        To capture a graph, call it once with the meta before.
         """
         if layer_idx is None or not 0 <= layer_idx < self.num_layers:
             self._check_layer(layer_idx)
@@ -621,7 +627,7 @@ class MI355XBackend:
         if table.rotary_dim > self.head_dim:
             raise ValueError(f"rotary_dim={table.rotary_dim} exceeds head_dim={self.head_dim}")
         mirror = meta.host_arrays()   # (without one the kernel flags it)
-        far = int(mirror["kv_lens"].max()) - 1 if mirror is not None else -1
+        far = int(mirror["kv_lens"].max(initial=0)) - 1 if mirror is not None else -1
         if far >= table.max_positions:
             raise ValueError(f"position {far} is outside the rotation table of "
                              f"{table.max_positions} positions")
@@ -633,6 +639,7 @@ class MI355XBackend:
             self._check_table(meta, table)
         r = self._rows
         if r is None or r.meta is not meta:
+            self._refuse_capture("append_kv_rotated (or append_kv, with page bounds)")
             r = _Rows()
             r.slots = self._slots_for(meta)
             r.positions = meta.positions.to(device=self.device, dtype=torch.int64).contiguous()
@@ -696,13 +703,6 @@ class MI355XBackend:
                 return np.ascontiguousarray(pages[pos % ps == ps - 1], dtype=np.int32)
         pages = np.unique(slots // ps)
         return pages[(pages >= 0) & (pages < self.num_blocks)].astype(np.int32)
-
-    def _complete_bounds(self, layer: int, meta: BatchMeta) -> None:
-        r = self._rows
-        if r is None or r.meta is not meta:
-            r = self._rows_for(meta)
-        if r.complete is not None:
-            self._renew_bounds(r.complete, r.complete.shape[0], self._enter(r), layer)
 
     def _slots_for(self, meta: BatchMeta) -> torch.Tensor:
         p = self._planned
@@ -803,8 +803,9 @@ class MI355XBackend:
 
         Batches with prompt chunks, geometries without the fast decode path, a
         scale that is not positive and batches that share too little to gain
-        by it run ``attend`` itself. Graphs captured with one meta share its
-        buffers, so their replays must not overlap.
+        by it run ``attend`` itself. To capture a graph, call it once with the
+        meta before. Graphs captured with one meta share its buffers: neither
+        their replays nor eager calls with it may overlap.
         """
         if layer_idx is None or not 0 <= layer_idx < self.num_layers:
             self._check_layer(layer_idx)
@@ -847,6 +848,7 @@ class MI355XBackend:
         return out
 
     def _plan_shared(self, meta: BatchMeta) -> _Shared:
+        self._refuse_capture("attend_shared")
         n = meta.n_seqs
         with_slots = (meta.slot_mapping is not None and meta.slot_mapping.shape[0] == n
                       and meta.kv_indices.shape[0] > 0)
@@ -934,8 +936,10 @@ class MI355XBackend:
         Needs ``page_bounds=True``, one token per sequence and a positive
         scale. With ``return_pages`` also returns the chosen pages' indices in
         each sequence's page list, int32 ``(n_seqs, n_kv_heads, min(pages,
-        longest list))``, ascending, -1 behind a shorter list. Graphs captured
-        with one meta share its buffers, so their replays must not overlap.
+        longest list))``, ascending, -1 behind a shorter list. To capture a
+        graph, call it once with the meta and ``pages`` before. Graphs captured
+        with one meta share its buffers: neither their replays nor eager calls
+        with it may overlap.
         """
         if layer_idx is None or not 0 <= layer_idx < self.num_layers:
             self._check_layer(layer_idx)
@@ -980,8 +984,11 @@ class MI355XBackend:
         return (out, ordinals) if return_pages else out
 
     def _plan_selected(self, meta: BatchMeta, pages: int) -> _Selected:
+        self._refuse_capture("attend_selected")
         ql, cu, kvl, indptr, last, indices, _ = self._host_index(meta, False)
         n = int(ql.shape[0])
+        if n == 0:
+            raise ValueError("attend_selected needs at least one sequence")
         if (ql != 1).any() or n != meta.n_tokens:
             raise ValueError("attend_selected takes decode batches: one token per sequence "
                              f"(query_lens up to {int(ql.max())} over {meta.n_tokens} tokens)")
@@ -1080,6 +1087,13 @@ class MI355XBackend:
             raise ValueError(f"seq {i}: kv_len={int(kvl[i])} with "
                              f"{int(indptr[i + 1] - indptr[i])} pages of {ps} and "
                              f"kv_last_page_len={int(last[i])} disagree")
+
+    def _refuse_capture(self, what: str) -> None:
+        """What a plan uploads while a graph is captured is there only once the
+        graph has run, but the plan stays for eager calls too."""
+        if _capturing():
+            raise RuntimeError(f"{what} has to plan this meta before a graph is captured: call "
+                               "it once with the meta (and the same arguments), then capture")
 
     def _enter(self, p) -> int:
         """The current stream's handle, ordered behind the plan's last launch:

@@ -9,8 +9,10 @@
 //   a' = a c - b s,   b' = b c + a s
 // in 32 bits, rounded once to the pool dtype. Elements from R on are copied.
 //
-// Pure data movement otherwise: bound by the rows' bytes for prompts, by its
-// chain of two round trips (position, then table) for a few tokens.
+// Pure data movement otherwise: bound by the rows' bytes for prompts (5437
+// tokens of 32 + 2 x 8 heads of 128, bf16: 23.2 us, 5.8 TB/s of the rows read and
+// written), by its chain of two round trips (position, then table) for a few
+// tokens (1 of head_dim 64: 2.3 us, 256 of head_dim 128: 3.7, 777 of 64: 4.4).
 #include <algorithm>
 
 #include "pkv_common.h"

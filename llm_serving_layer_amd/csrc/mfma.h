@@ -1,6 +1,8 @@
 // gfx950 matrix-core and LDS helpers shared by the attention kernels.
 #pragma once
 
+#include <type_traits>
+
 #include "pkv_common.h"
 
 namespace pkv {
@@ -105,6 +107,38 @@ __device__ __forceinline__ void load_to_lds(u32x4 rs, const uint32_t* v, uint32_
                    "s"(lds + 1024), "s"(lds + 2048), "s"(lds + 3072)
                  : "memory");
 }
+// The same with load k's 1024 k bytes as its offset, which is added to both
+// addresses (v[k] is less by as much): m0 is written once.
+template <int NL>
+__device__ __forceinline__ void load_page_to_lds(u32x4 rs, const uint32_t* v, uint32_t lds) {
+  static_assert(NL == 2 || NL == 4, "a page of 2 or 4 KiB");
+  uint32_t m0;
+  if constexpr (NL == 2)
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\ts_nop 4\n\t"
+                 "buffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
+                 "buffer_load_dwordx4 %2, %3, 0 offen offset:1024 lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0)
+                 : "v"(v[0]), "v"(v[1]), "s"(rs), "s"(lds)
+                 : "memory");
+  else
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %6\n\ts_nop 4\n\t"
+                 "buffer_load_dwordx4 %1, %5, 0 offen lds\n\t"
+                 "buffer_load_dwordx4 %2, %5, 0 offen offset:1024 lds\n\t"
+                 "buffer_load_dwordx4 %3, %5, 0 offen offset:2048 lds\n\t"
+                 "buffer_load_dwordx4 %4, %5, 0 offen offset:3072 lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0)
+                 : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "s"(rs), "s"(lds)
+                 : "memory");
+}
+
+// f(0), ..., f(N - 1) as integral constants.
+template <int I, int N, typename F> __device__ __forceinline__ void template_for(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    template_for<I + 1, N>(f);
+  }
+}
+
 // The buffer resource of ws_rsrc as the four words load_to_lds takes.
 __device__ __forceinline__ u32x4 raw_rsrc(const void* base, uint32_t bytes) {
   const uint64_t a = (uint64_t)(uintptr_t)base;

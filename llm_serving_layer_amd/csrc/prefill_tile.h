@@ -110,17 +110,17 @@ template <int RB> __device__ __forceinline__ int wide_xr(int row) {
   return RB == 128 ? ((row >> 1) & 1) << 2 | ((row >> 2) & 3) : (row & 3) << 2 | ((row >> 2) & 3);
 }
 
-// A shared tile's ring: as many buffers as fit 80 KiB (two workgroups a compute
-// unit; at head_dim 64 eight are enough), tiles loaded RING - 2 ahead. Such a
+// A shared tile's ring: four slots of a K and a V tile, 64 KiB (two workgroups a
+// compute unit), K loaded three tiles ahead and V as far ahead of its use. Such a
 // tile has at most one more workgroup beside it, so its own loads have to cover
 // the memory's latency, where a prefill tile's neighbours do.
-// At head_dim 64 a tile has 64 keys: a step's fixed cost (about 50 scalar
-// instructions, a barrier, the wait for the first LDS reads) is paid half as
-// often, and two score products run side by side.
+// At head_dim 64 a tile has 64 keys: a step's fixed cost (scalar instructions, a
+// barrier, the wait for the first LDS reads) is paid half as often, and two score
+// products run side by side.
 template <typename T, int D> struct SharedRing {
   static constexpr int TT = D == 64 ? 64 : 32;              // keys of a tile
   static constexpr int TILE = TT * D * (int)sizeof(T);      // one K (or V) tile
-  static constexpr int N = 81920 / (2 * TILE) < 8 ? 81920 / (2 * TILE) : 8;
+  static constexpr int N = 4;
   static constexpr int BYTES = N * 2 * TILE;
 };
 
@@ -308,36 +308,15 @@ __device__ __forceinline__ void prefill_tile(
     vec8 va[NH * 2 * NDH];
     // S^T = K Q^T: s[hf][rr] = score of key t0 + 32 hf + 8 (rr / 4) + 4 g + rr % 4.
     f32x16 s[NH];
-    if constexpr (SHARED) {
-      // One wave a SIMD runs such tiles, in step with the workgroup's others:
-      // K is read first, so that QK starts while V is still being read.
-      vec8 ka[NH * NC];
+    read_v(vprev, va);
 #pragma unroll
-      for (int hf = 0; hf < NH; ++hf)
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-          ka[hf * NC + c] =
-              *reinterpret_cast<const vec8*>(kl + in_tile(hf * 32 + n, 16 * c + 8 * g));
-      asm volatile("" ::: "memory");
-      read_v(vprev, va);
-      asm volatile("" ::: "memory");
-#pragma unroll
-      for (int hf = 0; hf < NH; ++hf) s[hf] = f32x16{};
+    for (int hf = 0; hf < NH; ++hf) {
+      s[hf] = f32x16{};
+      const int kr = hf * 32 + n;
 #pragma unroll
       for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int hf = 0; hf < NH; ++hf) s[hf] = Mma32<T>::mma(ka[hf * NC + c], qb[c], s[hf]);
-    } else {
-      read_v(vprev, va);
-#pragma unroll
-      for (int hf = 0; hf < NH; ++hf) {
-        s[hf] = f32x16{};
-        const int kr = hf * 32 + n;
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-          s[hf] = Mma32<T>::mma(*reinterpret_cast<const vec8*>(kl + in_tile(kr, 16 * c + 8 * g)),
-                                qb[c], s[hf]);
-      }
+        s[hf] = Mma32<T>::mma(*reinterpret_cast<const vec8*>(kl + in_tile(kr, 16 * c + 8 * g)),
+                              qb[c], s[hf]);
     }
     // Keys past the row's position are masked only on tiles that reach them.
     if (!full) {
@@ -414,40 +393,217 @@ __device__ __forceinline__ void prefill_tile(
 
   unsigned char* last = buf0;   // the buffer of the last tile computed
   if constexpr (SHARED) {
-    // The ring of a shared tile: tile t in buffer t % N, tile t + AHEAD loaded
-    // in step t, into the buffer that step t - 2 was the last to read.
-    constexpr int N = SharedRing<T, D>::N, AHEAD = N - 2;
-    unsigned char* prev = smem + (N - 1) * 2 * TILE;
-    for (int i = tid; i < TILE / 16; i += kPrefillThreads)
-      reinterpret_cast<u32x4*>(prev + TILE)[i] = u32x4{0u, 0u, 0u, 0u};
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    int ids[AHEAD + 1];
+    // Three tiles are at work in a step, none waiting for another: tile t's
+    // scores and tile t - 2's PV on the matrix cores, tile t - 1's softmax on
+    // the vector unit. K of tile t is in slot t % N of the ring, V in the V half
+    // of the same slot; a step loads K of tile t + AHEAD and V of tile t - 2 +
+    // AHEAD, into the slots that step t - 1 was the last to read.
+    // One wave a SIMD is bound by its instructions, scalar ones too, so the
+    // steps are unrolled over the slots (constant LDS offsets) and a step's
+    // loads need few: page ids from a vector register, 64 tiles' at a time. At
+    // head_dim 128 a step has 141 instructions; with 267 and the softmax behind
+    // the step's own scores it took 1600 cycles, this way 1050, the matrix
+    // cores' part of it 512 (128 sequences over 1024 pages, 8 KV heads of 128:
+    // the tiles alone 55 -> 45 us, beside the own pages 83 -> 70 with the merge).
+    constexpr int N = SharedRing<T, D>::N, AHEAD = N - 1, TP = TT / PS;
+    static_assert(N == 4, "the steps below are unrolled over four slots");
+    auto k_slot = [&](int i) { return smem + (i & (N - 1)) * 2 * TILE; };
+    auto v_slot = [&](int i) { return smem + (i & (N - 1)) * 2 * TILE + TILE; };
+    const uint32_t lds0 = lds_address(smem) + wdst;   // (wdst: this wave's page; V's half)
+    uint32_t vnext[LPT];                              // voff without load k's offset
 #pragma unroll
-    for (int t = 0; t <= AHEAD; ++t) ids[t] = load_id(t);
-#pragma unroll
-    for (int t = 0; t < AHEAD; ++t) load_tile(t, ids[t], smem + t * 2 * TILE);
+    for (int k = 0; k < LPT; ++k) vnext[k] = voff[k] - 1024 * k;
+    uint32_t worst = 0;                               // of the page ids, unsigned
+    auto load_page = [&](const T* pool, uint32_t id, int left, uint32_t at) {
+      worst = max(worst, id);
+      load_page_to_lds<LPT>(raw_rsrc(reinterpret_cast<const char*>(pool) + (uint64_t)id * pagebytes,
+                                     id < nb32 && left > 0 ? pagebytes : 0u),
+                            vnext, at);
+    };
+    // A wave that loads V alone is two tiles behind. Lane l: this wave's page of
+    // tile 64 c + l - behind.
+    const int behind = !BOTH && wave >= 2 ? 2 : 0;
+    const int first_page = wpage - behind * TP;
+    int page_ids;
+    auto read_ids = [&](int j) {
+      page_ids = kv_indices[pbase + max(0, min(TP * (j + lane) + first_page, npages - 1))];
+    };
+    uint32_t id1 = 0, id2 = 0;                        // (BOTH) of tiles j - 1, j - 2
+    // K of tile j into slot j % N, V of tile j - 2 into its slot; none before tile 0
+    auto load_step = [&](int j, auto to, bool v_too) {
+      constexpr int S = decltype(to)::value;
+      const uint32_t id = __builtin_amdgcn_readlane(page_ids, j & 63);
+      const int left = npages - first_page - TP * j;  // pages from this wave's on
+      constexpr uint32_t k_at = S * 2 * TILE, v_at = ((S + N - 2) % N) * 2 * TILE;
+      if constexpr (BOTH) {
+        load_page(kpool, id, left, lds0 + k_at);
+        load_page(vpool, id2, v_too ? left + 2 * TP : 0, lds0 + v_at + TILE);
+        id2 = id1;
+        id1 = id;
+      } else {
+        load_page(wpool, id, behind && !v_too ? 0 : left, lds0 + (behind ? v_at : k_at));
+      }
+    };
+    template_for<0, AHEAD>([&](auto j) {
+      if constexpr (decltype(j)::value == 0) read_ids(0);
+      load_step(j, j, decltype(j)::value >= 2);
+    });
 #pragma unroll
     for (int c = 0; c < NC; ++c) {   // Q arrives here (see below)
       u32x4 w = __builtin_bit_cast(u32x4, qb[c]);
       asm volatile("" : "+v"(w));
       qb[c] = __builtin_bit_cast(vec8, w);
     }
-    int id = ids[AHEAD];
-    unsigned char* next = smem + AHEAD * 2 * TILE;
-    unsigned char* const end = smem + N * 2 * TILE;
-    last = smem;
-    for (int t = 0;; ++t) {
+    auto arrive = [&]() {            // tiles t (K) and t - 2 (V) are in their slots
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"((AHEAD - 1) * LPT * (BOTH ? 2 : 1)) : "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      load_tile(t + AHEAD, id, next);
-      compute(t, last, prev + TILE);
-      id = load_id(t + AHEAD + 1);
-      if (t + 1 >= ntiles) break;
-      prev = last;
-      last = last + 2 * TILE == end ? smem : last + 2 * TILE;
-      next = next + 2 * TILE == end ? smem : next + 2 * TILE;
+    };
+    typedef vec8 Keys[NH * NC];
+    typedef f32x16 Scores[NH];
+    typedef vec8 Probs[NH * 2];
+    auto read_k = [&](const unsigned char* kl, Keys& ka) {
+#pragma unroll
+      for (int hf = 0; hf < NH; ++hf)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          ka[hf * NC + c] =
+              *reinterpret_cast<const vec8*>(kl + in_tile(hf * 32 + n, 16 * c + 8 * g));
+      asm volatile("" ::: "memory");
+    };
+    auto qk = [&](const Keys& ka, Scores& s) {
+#pragma unroll
+      for (int hf = 0; hf < NH; ++hf) s[hf] = f32x16{};
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int hf = 0; hf < NH; ++hf) s[hf] = Mma32<T>::mma(ka[hf * NC + c], qb[c], s[hf]);
+    };
+    auto pv_of = [&](const vec8* va, const Probs& p) {
+#pragma unroll
+      for (int kb = 0; kb < NH * 2; ++kb)
+#pragma unroll
+        for (int dh = 0; dh < NDH; ++dh) o[dh] = Mma32<T>::mma(va[kb * NDH + dh], p[kb], o[dh]);
+    };
+    auto softmax = [&](const Scores& s, Probs& p, float& ls) {
+      ls = 0.f;
+#pragma unroll
+      for (int hf = 0; hf < NH; ++hf)
+#pragma unroll
+        for (int rr = 0; rr < 16; ++rr) {
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[hf][rr], scale_log2, -m_run));
+          ls += e;
+          p[2 * hf + (rr >> 3)][rr & 7] = (T)e;
+        }
+    };
+    // the lazy rescale of compute() above, with tile t - 2's PV in o
+    auto settle = [&](const Scores& s, Probs& p, float ls) {
+      if (__builtin_amdgcn_ballot_w64(!(ls <= 4096.f))) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int hf = 0; hf < NH; ++hf)
+#pragma unroll
+          for (int rr = 0; rr < 16; ++rr) mx = fmaxf(mx, s[hf][rr]);
+        mx = max_x32(mx) * scale_log2;
+        const float m_new = fmaxf(m_run, mx);
+        const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+        l_run *= alpha;
+        m_run = m_new;
+#pragma unroll
+        for (int dh = 0; dh < NDH; ++dh) o[dh] *= alpha;
+        softmax(s, p, ls);
+      }
+      l_run += ls;
+    };
+    auto pin = [&](Probs& p, float& ls) {   // (not behind the test)
+#pragma unroll
+      for (int i = 0; i < NH * 2; ++i) {
+        u32x4 w = __builtin_bit_cast(u32x4, p[i]);
+        asm volatile("" : "+v"(w));
+        p[i] = __builtin_bit_cast(vec8, w);
+      }
+      asm volatile("" : "+v"(ls));
+    };
+    constexpr int FIRST = 20, EACH = 3;
+    // Step t, t % N == S: scores of tile t into s1, the softmax of tile t - 1's
+    // (s0) into p1, PV of tile t - 2 (p0).
+    auto step = [&](int t, auto slot, const Scores& s0, Scores& s1, const Probs& p0, Probs& p1) {
+      constexpr int S = decltype(slot)::value;
+      arrive();
+      Keys ka;
+      vec8 va[NH * 2 * NDH];
+      read_k(k_slot(S), ka);
+      read_v(v_slot(S + N - 2), va);
+      asm volatile("" ::: "memory");
+      load_step(t + AHEAD, std::integral_constant<int, (S + AHEAD) % N>{}, true);
+      qk(ka, s1);
+      pv_of(va, p0);
+      float ls;
+      softmax(s0, p1, ls);
+      pin(p1, ls);
+      // vector work while the LDS reads are on their way, then beside each MFMA
+      __builtin_amdgcn_sched_group_barrier(0x002, FIRST * NH, 0);
+#pragma unroll
+      for (int i = 0; i < NH * NC + NH * 2 * NDH; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, EACH * NH, 0);
+      }
+      settle(s0, p1, ls);
+    };
+    // The last tile's softmax, with its missing keys, and the last two PVs.
+    auto drain = [&](Scores& s0, const Probs& p0, Probs& p1) {
+      arrive();
+      vec8 va[NH * 2 * NDH];
+      read_v(v_slot(ntiles - 2 + N), va);
+      if (ntiles * TT > kv_len) {
+#pragma unroll
+        for (int hf = 0; hf < NH; ++hf)
+#pragma unroll
+          for (int rr = 0; rr < 16; ++rr)
+            if ((ntiles - 1) * TT + 32 * hf + 8 * (rr >> 2) + 4 * g + (rr & 3) >= kv_len)
+              s0[hf][rr] = -INFINITY;
+      }
+      pv_of(va, p0);
+      float ls;
+      softmax(s0, p1, ls);
+      settle(s0, p1, ls);
+      // (all loads, those of the tiles past the end too, before the workgroup ends)
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      read_v(v_slot(ntiles - 1), va);
+      pv_of(va, p1);
+    };
+    Scores sa, sb;
+    Probs pa, pz;
+#pragma unroll
+    for (int i = 0; i < NH * 2; ++i) pa[i] = vec8{};
+    {
+      arrive();
+      load_step(AHEAD, std::integral_constant<int, AHEAD>{}, true);
+      Keys ka;
+      read_k(k_slot(0), ka);
+      qk(ka, sa);
     }
+    auto swap = [&]() {   // an odd number of steps: back to sa and pa
+#pragma unroll
+      for (int hf = 0; hf < NH; ++hf) sa[hf] = sb[hf];
+#pragma unroll
+      for (int i = 0; i < NH * 2; ++i) pa[i] = pz[i];
+    };
+    for (int t = 1;; t += 4) {
+      if (t >= ntiles) break;
+      if (((t + AHEAD) & 63) == 0) read_ids(t + AHEAD);
+      step(t, std::integral_constant<int, 1>{}, sa, sb, pa, pz);
+      if (t + 1 >= ntiles) { swap(); break; }
+      step(t + 1, std::integral_constant<int, 2>{}, sb, sa, pz, pa);
+      if (t + 2 >= ntiles) break;
+      step(t + 2, std::integral_constant<int, 3>{}, sa, sb, pa, pz);
+      if (t + 3 >= ntiles) { swap(); break; }
+      step(t + 3, std::integral_constant<int, 0>{}, sb, sa, pz, pa);
+    }
+    drain(sa, pa, pz);
+    if (worst >= nb32 && lane == 0) flag(status, PKV_STATUS_BAD_PAGE);
   } else {
     // The ring: tile t in buffer t % 4. Each step waits for its tile's loads
     // (this wave's, then every wave's at the barrier, which also ends every
@@ -499,9 +655,11 @@ __device__ __forceinline__ void prefill_tile(
       if (t + 4 >= ntiles) break;
     }
   }
-  pv(last + TILE);   // the last tile's PV
-  // the loads of the tiles past the end land in LDS before the workgroup ends
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  if constexpr (!SHARED) {
+    pv(last + TILE);   // the last tile's PV
+    // the loads of the tiles past the end land in LDS before the workgroup ends
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
 
   l_run = sum_x32(l_run);
   if constexpr (SHARED) {

@@ -284,18 +284,12 @@ extern "C" int pkv_plan_shared(const int32_t* kv_indptr, const int32_t* kv_indic
     ptr[i + 1] = (int32_t)ids.size();
     lens[i] = (ptr[i + 1] - ptr[i] - 1) * page_size + kv_last_page_len[i];
   }
-  int32_t n_work = 0, own_slots = 0, stride = 0;
-  int64_t need = 0;
-  int rc = pkv_plan_decode(ptr.data(), ids.data(), lens.data(), kv_last_page_len, n_seqs, page_size,
-                           num_blocks, n_kv_heads, part_pages, max_workgroups, plan, plan_capacity,
-                           &need, &n_work, &own_slots, &stride);
-  if (plan_needed) *plan_needed = need;
-  if (rc) return rc;
-
   // Runs in splits of about `split` pages: from 8 on, so that no more than
   // tile_target workgroups share the work (or one each, where that is more), and
-  // so that a tile takes about as long as the own pages beside it: 250 of those
-  // (times KV heads) stream in the time a tile takes for one page. Shorter tiles
+  // so that a tile takes about as long as the own pages beside it: 180 of those
+  // (times KV heads) stream in the time a tile takes for one page (at 250 and 130:
+  // 96 sequences, 256 shared pages, 4 KV heads of 128: 39.5 and 33.6 us; 128
+  // sequences, 1024 shared pages, 8 KV heads of 128: 70.5 and 84.4). Shorter tiles
   // only leave more parts to merge (96 sequences, 7 runs of 32 and 49 pages,
   // head_dim 128: 36.0 us with 30 tiles, 31.5 with 9).
   const int32_t per_tile = kPrefillRows / G;
@@ -307,7 +301,7 @@ extern "C" int pkv_plan_shared(const int32_t* kv_indptr, const int32_t* kv_indic
   }
   const int64_t target = std::max<int64_t>(1, tile_target / n_kv_heads);
   int64_t split = std::max<int64_t>({8, (steps + target - 1) / target,
-                                     (int64_t)ids.size() * n_kv_heads / 250});
+                                     (int64_t)ids.size() * n_kv_heads / 180});
   auto splits_of = [&](const Run& r) {   // (rounded, and at least one)
     const int32_t n = r.last - r.first;
     return (int32_t)std::max<int64_t>(1, (n + split / 2) / split);
@@ -333,6 +327,20 @@ extern "C" int pkv_plan_shared(const int32_t* kv_indptr, const int32_t* kv_indic
   }
   const int32_t n_merges = (int32_t)std::count_if(shared.begin(), shared.end(),
                                                   [](int32_t x) { return x > 0; });
+  // Two workgroups a compute unit (2 tile_target) are resident, tiles among them:
+  // with bins for all of those the last bins began when the first workgroups had
+  // ended (256 sequences, 64 tiles, head_dim 64: 47.3 us with 512, 39.1 with 448).
+  const bool beside = heads_per_wg(n_kv_heads) == kMaxWaves;   // (else a launch of their own)
+  const int32_t bins_wgs = beside ? (int32_t)std::min<int64_t>(max_workgroups, std::max<int64_t>(
+      tile_target, 2 * (int64_t)tile_target - n_tiles * n_kv_heads)) : max_workgroups;
+  int32_t n_work = 0, own_slots = 0, stride = 0;
+  int64_t need = 0;
+  int rc = pkv_plan_decode(ptr.data(), ids.data(), lens.data(), kv_last_page_len, n_seqs, page_size,
+                           num_blocks, n_kv_heads, part_pages, bins_wgs, plan, plan_capacity,
+                           &need, &n_work, &own_slots, &stride);
+  if (plan_needed) *plan_needed = need;
+  if (rc) return rc;
+
   // items and merges of 8 and 4 ints, members of 2
   const int64_t want = n_tiles * kSharedItem + (int64_t)n_merges * 4 + n_members * kSharedMember;
   if (tiles_needed) *tiles_needed = want;

@@ -113,6 +113,23 @@ def test_long_prefixes_and_any_pieces(root, part_pages):
     b.check(q, out)
 
 
+@pytest.mark.parametrize("root", [4, 5, 6, 7, 9, 10, 13, 16, 19, 131, 258, 531])
+@pytest.mark.parametrize("n_heads, n_kv, d", [(32, 8, 64), (8, 2, 128), (4, 4, 128)])
+def test_runs_in_one_tile(root, n_heads, n_kv, d, monkeypatch):
+    """Every number of a tile's steps around its pipeline's length, whole and
+    partial last steps, and runs past the page ids it holds at a time."""
+    print(f"one tile root={root} {n_heads}/{n_kv}/{d}", flush=True)
+    monkeypatch.setattr(backend, "SHARED_TILES", 1)
+    b = Batch(root, [(0, [1, 30, 200])], n_heads, n_kv, d)
+    q = b.q()
+    q[1] *= 30                      # (a peaked row, whose reference moves)
+    out = b.bk.attend_shared(q, 0, 0.125, b.meta)
+    b.bk.check_device_errors()
+    assert b.bk._shared.n_tiles == 1
+    b.check(q, out)
+    assert torch.equal(b.bk.attend_shared(q, 0, 0.125, b.meta), out)
+
+
 def test_large_scores_move_the_reference():
     """Scores that grow along the prefix: the running maximum moves in the
     middle of a split, and the parts' maxima lie far apart."""
@@ -289,6 +306,22 @@ def test_bad_pages_are_flagged():
         b.bk.attend_shared(b.q(), 0, 0.125, meta)
         with pytest.raises(IndexError, match="kv_indices"):
             b.bk.check_device_errors()
+
+
+@pytest.mark.parametrize("at, bad", [(0, -1), (299, 10 ** 6), (150, -2 ** 31)])
+def test_a_bad_page_anywhere_in_a_long_tile(at, bad, monkeypatch):
+    monkeypatch.setattr(backend, "SHARED_TILES", 1)
+    b = Batch(300, [(0, [5, 40])], 8, 2, 128)
+    q = b.q()
+    idx, ptr = b.meta.kv_indices.clone(), b.meta.kv_indptr.tolist()
+    idx[ptr[0] + at] = idx[ptr[1] + at] = bad
+    meta = dataclasses.replace(b.meta, kv_indices=idx, host=None)
+    b.bk.attend_shared(q, 0, 0.125, meta)
+    assert b.bk._shared.n_tiles == 1
+    with pytest.raises(IndexError, match="kv_indices"):
+        b.bk.check_device_errors()
+    b.check(q, b.bk.attend_shared(q, 0, 0.125, b.meta))
+    b.bk.check_device_errors()
 
 
 def test_refusals():

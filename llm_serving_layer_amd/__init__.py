@@ -7,7 +7,8 @@ hand-written gfx950 kernels (include/pagedkv.h, csrc/):
 * ``contract``  — BatchMeta and the AttentionBackend protocol;
 * ``paging``    — BlockAllocator, SequenceBlocks, build_csr;
 * ``assembly``  — ScheduledSeq, build_batch_meta, build_token_tensor;
-* ``backend``   — MI355XBackend (append_kv / attend / copy_block[s]);
+* ``backend``   — MI355XBackend (append_kv[_rotated] / attend[_shared, _selected] /
+  copy_block[s]);
 * ``rotary``    — RotaryTable (MI355XBackend.append_kv_rotated);
 * ``swap``      — KVSwapSpace / SwapHandle (preemption swap);
 * ``sizing``    — plan_kv_pool / KVPoolPlan (pool sizing for one MI355X).

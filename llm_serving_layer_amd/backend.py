@@ -23,6 +23,12 @@ Drop-in surface (same as both reference backends):
 * plan once per ``BatchMeta`` identity, run once per layer
   (flashinfer_backend.py:566-676), including the ``is_prefill`` cross-check.
 
+Beyond the reference's surface: ``append_kv_rotated`` (the position rotation
+with the append), ``attend_shared`` (decode attention that reads shared pages
+once) and, with ``page_bounds=True``, ``attend_selected`` (decode attention over
+the pages whose key bounds allow the largest scores), ``key_bounds``,
+``refresh_page_bounds`` and ``bounds_bytes``.
+
 One launch per layer on decode steps: for a decode-shaped batch on the fast
 geometry, ``append_kv`` records its rows and the following ``attend`` of the
 same layer performs the append inside the attention kernel (the result is

@@ -401,10 +401,10 @@ __device__ __forceinline__ void prefill_tile(
     // One wave a SIMD is bound by its instructions, scalar ones too, so the
     // steps are unrolled over the slots (constant LDS offsets) and a step's
     // loads need few: page ids from a vector register, 64 tiles' at a time. At
-    // head_dim 128 a step has 141 instructions; with 267 and the softmax behind
-    // the step's own scores it took 1600 cycles, this way 1050, the matrix
-    // cores' part of it 512 (128 sequences over 1024 pages, 8 KV heads of 128:
-    // the tiles alone 55 -> 45 us, beside the own pages 83 -> 70 with the merge).
+    // head_dim 128 a step has 141 instructions and takes 1250 cycles, 512 of them
+    // the matrix cores' part; with 267 instructions it took 1600 (128 sequences
+    // over 1024 pages, 8 KV heads of 128: the tiles alone 55 -> 45 us, beside the
+    // own pages and with the merge 83 -> 71).
     constexpr int N = SharedRing<T, D>::N, AHEAD = N - 1, TP = TT / PS;
     static_assert(N == 4, "the steps below are unrolled over four slots");
     auto k_slot = [&](int i) { return smem + (i & (N - 1)) * 2 * TILE; };

@@ -69,7 +69,7 @@ SELECTED_PART_PAGES = 8  # of chosen pages; what their kernel stages at a time
 # Pieces (of 8 pages) up to which each of them gets a workgroup of its own; the
 # streaming kernel takes more. us a call, workgroups against streaming: 64 pieces
 # 20.4 and 29.7, 512 20.0 and 26.8, 1024 26.9 and 29.3 (head_dim 64) or 36.2 and
-# 36.7 (128), 2048 40.7 and 34.5, 3072 81.7 and 72.5.
+# 36.7 (128), 2048 40.7 and 34.5.
 SELECTED_PIECES = 1024
 # What attend_shared must save to be worth its tiles and its merge: a run of
 # shared pages at least 4 pages long, in bytes a KV head more than 25 KiB a
@@ -828,7 +828,8 @@ class MI355XBackend:
             return self.attend(q, layer_idx, scale, meta)
         pend = self._pending
         fused = (pend is not None and pend.layer == layer_idx and pend.meta is meta
-                 and pend.stream == _current_stream(self.device) and p.fusable)
+                 and pend.stream == _current_stream(self.device) and p.fusable
+                 and not (pend.k.data_ptr() | pend.v.data_ptr()) % 16)
         if fused:
             self._check_pending_intact(pend)
             self._pending = None

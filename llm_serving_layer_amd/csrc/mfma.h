@@ -116,18 +116,19 @@ __device__ __forceinline__ void load_page_to_lds(u32x4 rs, const uint32_t* v, ui
   if constexpr (NL == 2)
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\ts_nop 4\n\t"
                  "buffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
-                 "buffer_load_dwordx4 %2, %3, 0 offen offset:1024 lds\n\ts_mov_b32 m0, %0"
+                 "buffer_load_dwordx4 %2, %3, 0 offen offset:%5 lds\n\ts_mov_b32 m0, %0"
                  : "=&s"(m0)
-                 : "v"(v[0]), "v"(v[1]), "s"(rs), "s"(lds)
+                 : "v"(v[0]), "v"(v[1]), "s"(rs), "s"(lds), "n"(1024)
                  : "memory");
   else
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %6\n\ts_nop 4\n\t"
                  "buffer_load_dwordx4 %1, %5, 0 offen lds\n\t"
-                 "buffer_load_dwordx4 %2, %5, 0 offen offset:1024 lds\n\t"
-                 "buffer_load_dwordx4 %3, %5, 0 offen offset:2048 lds\n\t"
-                 "buffer_load_dwordx4 %4, %5, 0 offen offset:3072 lds\n\ts_mov_b32 m0, %0"
+                 "buffer_load_dwordx4 %2, %5, 0 offen offset:%7 lds\n\t"
+                 "buffer_load_dwordx4 %3, %5, 0 offen offset:%8 lds\n\t"
+                 "buffer_load_dwordx4 %4, %5, 0 offen offset:%9 lds\n\ts_mov_b32 m0, %0"
                  : "=&s"(m0)
-                 : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "s"(rs), "s"(lds)
+                 : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "s"(rs), "s"(lds), "n"(1024),
+                   "n"(2 * 1024), "n"(3 * 1024)
                  : "memory");
 }
 

@@ -182,6 +182,18 @@ def test_a_deferred_append_of_another_layer_or_meta_lands_first():
     assert torch.equal(rows, k)
 
 
+def test_new_rows_at_an_odd_address():
+    b = Batch(20, [(0, [1, 30, 200])], 8, 2, 64)
+    q, n = b.q(), 3 * 2 * 64
+    k, v = (b.rand((n + 1,))[1:].view(3, 2, 64) for _ in range(2))
+    assert k.data_ptr() % 16
+    b.bk.append_kv(0, k, v, b.meta)
+    out = b.bk.attend_shared(q, 0, 0.125, b.meta)
+    slots = b.meta.slot_mapping.long()
+    assert torch.equal(b.bk.k_pool[0].view(-1, 2, 64)[slots], k)
+    b.check(q, out)
+
+
 def test_rows_behind_the_ends_and_other_pages_do_not_matter():
     b = Batch(9, [(0, [1, 5, 40])])
     q = b.q()

@@ -74,8 +74,8 @@ SELECTED_PIECES = 1024
 # What attend_shared must save to be worth its tiles and its merge: a run of
 # shared pages at least 4 pages long, in bytes a KV head more than 25 KiB a
 # sequence (the part it adds), all runs together 16 MiB. us a call, attend against
-# shared: 6 sequences over 96 pages 9.8 and 10.7, 200 over 8 28.6 and 30.9, 2
-# over 512 15.8 and 13.8, 32 over 32 16.6 and 14.1, 256 over 128 134 and 46.
+# shared: 6 sequences over 96 pages 10.0 and 10.7, 200 over 8 28.5 and 30.4, 2
+# over 512 15.9 and 14.3, 32 over 32 16.8 and 13.8, 256 over 128 130 and 39.
 SHARED_MIN_PAGES, SHARED_PART_BYTES, SHARED_LEAST_BYTES = 4, 25 << 10, 16 << 20
 SHARED_TILES = 256       # workgroups that share the work on a batch's shared pages
 DEFAULT_Q_TILE = 64      # prefill tile when the geometry has no matrix-core kernel

@@ -46,6 +46,7 @@ thread-safe and not re-entrant, like the reference backends.
 from __future__ import annotations
 
 import contextlib
+import copy
 import ctypes as C
 from array import array
 from operator import eq, index
@@ -213,11 +214,11 @@ class _Rows:
 
 
 class _Shared:
-    """What ``attend_shared`` keeps for one BatchMeta: None where nothing is
-    worth sharing (``n_tiles`` 0: the batch takes ``attend``)."""
+    """What ``attend_shared`` keeps for one BatchMeta. Where nothing is worth
+    sharing ``n_tiles`` is 0; ``whole`` is how such a batch runs, once it has."""
 
     __slots__ = ("meta", "n", "n_tiles", "n_merges", "tiles", "plan", "indices", "slots", "n_work", "n_slots",
-                 "stride", "ws", "fusable", "args", "ptr", "buffers", "stream")
+                 "stride", "ws", "fusable", "args", "ptr", "buffers", "stream", "whole")
 
 
 class _Selected:
@@ -547,10 +548,13 @@ class MI355XBackend:
             v = self._as_pool(v)
         stream = _raw_stream(di) if _raw_stream is not None else _current_stream(self.device)
         if self._fuse_append:
-            try:
-                p = self._ensure_planned(meta)
-            except ValueError:
-                p = None  # inconsistent paging metadata: append now, attend will raise
+            p = self._planned
+            if p is None or p.meta is not meta:
+                try:
+                    # (not within a capture: the rows are appended on their own)
+                    p = None if _capturing() else self._ensure_planned(meta)
+                except ValueError:
+                    p = None  # inconsistent paging metadata: append now, attend will raise
             if p is not None and p.fusable:
                 pend = _Pending()
                 pend.layer, pend.k, pend.v, pend.meta = layer_idx, k, v, meta
@@ -564,6 +568,8 @@ class MI355XBackend:
                     self._v_ptr[layer_idx], k.data_ptr(), v.data_ptr(), stream)
                 if rc:
                     _native.check(rc, "append_kv")
+                if _capturing():
+                    self._keep(p)
                 return
         r = None
         if self._bounds is not None:
@@ -718,7 +724,8 @@ class MI355XBackend:
         if sc is not None and sc[0] is meta:
             return sc[1]
         slots = self._dev_i32(meta.slot_mapping)
-        self._slot_cache = (meta, slots)
+        if not _capturing():   # (what a graph converts is there only once it has run)
+            self._slot_cache = (meta, slots)
         return slots
 
     def _launch_append(self, layer, k, v, slots, stream) -> None:
@@ -728,6 +735,8 @@ class MI355XBackend:
             k.shape[0], self.n_kv_heads, self.head_dim, self._code, self._status_ptr,
             stream)
         _native.check(rc, "append_kv")
+        if _capturing():
+            self._keep(slots)
 
     def _check_pending_intact(self, pend: _Pending) -> None:
         if pend.k._version != pend.kver or pend.v._version != pend.vver:
@@ -768,6 +777,11 @@ class MI355XBackend:
         p = self._planned
         if p is None or p.meta is not meta:
             p = self._ensure_planned(meta)
+        return self._attend_by(p, q, layer_idx, scale, meta)
+
+    def _attend_by(self, p: _Plan, q: torch.Tensor, layer_idx: int, scale: float,
+                   meta: BatchMeta) -> torch.Tensor:
+        """``attend`` by the meta's plan ``p``."""
         di = self.device.index
         stream = _raw_stream(di) if _raw_stream is not None else _current_stream(self.device)
         pend = self._pending
@@ -809,9 +823,10 @@ class MI355XBackend:
 
         Batches with prompt chunks, geometries without the fast decode path, a
         scale that is not positive and batches that share too little to gain
-        by it run ``attend`` itself. To capture a graph, call it once with the
-        meta before. Graphs captured with one meta share its buffers: neither
-        their replays nor eager calls with it may overlap.
+        by it run as ``attend`` runs them. To capture a graph, call it once with
+        the meta (and a scale of the same sign) before. Graphs captured with one
+        meta share its buffers: neither their replays nor eager calls with it may
+        overlap.
         """
         if layer_idx is None or not 0 <= layer_idx < self.num_layers:
             self._check_layer(layer_idx)
@@ -825,7 +840,10 @@ class MI355XBackend:
         if p is None or p.meta is not meta:
             p = self._plan_shared(meta)
         if not p.n_tiles or not float(scale) > 0:
-            return self.attend(q, layer_idx, scale, meta)
+            if p.whole is None:
+                self._plan_whole(p, meta)
+            self._enter(p)
+            return self._attend_by(p.whole, q, layer_idx, scale, meta)
         pend = self._pending
         fused = (pend is not None and pend.layer == layer_idx and pend.meta is meta
                  and pend.stream == _current_stream(self.device) and p.fusable
@@ -861,7 +879,7 @@ class MI355XBackend:
                       and meta.kv_indices.shape[0] > 0)
         ql, cu, kvl, indptr, last, indices, slots = self._host_index(meta, with_slots)
         p = _Shared()
-        p.n, p.n_tiles, p.buffers = n, 0, []
+        p.n, p.n_tiles, p.buffers, p.whole = n, 0, [], None
         if self._split_mixed and n > 1 and not (ql != 1).any() and n == meta.n_tokens:
             self._check_pages(kvl, indptr, last, int(indices.shape[0]))
             self._fill_shared(p, meta, *(np.ascontiguousarray(a, dtype=np.int32)
@@ -873,6 +891,23 @@ class MI355XBackend:
         p.meta = meta
         self._shared = p
         return p
+
+    def _plan_whole(self, p: _Shared, meta: BatchMeta) -> None:
+        """The batch as ``attend`` runs it: its plan, kept with ``p``, and a
+        workspace of its own, since other plans' partials in the backend's would
+        meet this one's arrival counters when a graph replays it."""
+        self._refuse_capture("attend_shared")
+        w = copy.copy(self._ensure_planned(meta))
+        self._enter(p)
+        d = w.dec or w
+        n = w.n_seqs if w.dec is None else w.dec.n
+        need = self._lib.pkv_decode_workspace_bytes(n, d.n_slots, self.n_heads, self.n_kv_heads,
+                                                    self.head_dim)
+        ws = self._counted_workspace(need, n)
+        self._describe(w, ws)
+        p.buffers += [t for t in (w.plan, w.indptr, w.indices, w.kv_lens, w.cu_q, w.bidx, w.slots,
+                                  d.plan, ws) if t is not None]
+        p.whole = w
 
     def _fill_shared(self, p: _Shared, meta: BatchMeta, indptr, indices, kvl, last) -> None:
         """Plan the batch's shared runs and own pages (pkv_plan_shared)."""
@@ -1108,8 +1143,7 @@ class MI355XBackend:
         stays as long as the backend does."""
         stream = _current_stream(self.device)
         if _capturing():
-            if not any(c is p for c in self._captured):
-                self._captured.append(p)
+            self._keep(p)
         elif p.stream != stream:
             cur, ev = torch.cuda.current_stream(self.device), torch.cuda.Event()
             ev.record(torch.cuda.ExternalStream(p.stream, device=self.device))
@@ -1118,6 +1152,11 @@ class MI355XBackend:
                 t.record_stream(cur)
             p.stream = stream
         return stream
+
+    def _keep(self, read) -> None:
+        """What a graph being captured reads stays as long as the backend does."""
+        if not any(c is read for c in self._captured):
+            self._captured.append(read)
 
     # -- planning ---------------------------------------------------------------
 
@@ -1218,16 +1257,19 @@ class MI355XBackend:
             out = np.split(host, np.cumsum([t.shape[0] for t in parts])[:-1])
         return (*out, *[None] * (not with_slots))
 
-    def _describe(self, p: _Plan) -> int:
+    def _describe(self, p: _Plan, ws: torch.Tensor | None = None) -> int:
         """Address of the plan's ``pkv_batch``: the arguments its launches share,
-        converted once instead of per layer."""
+        converted once instead of per layer; with ``ws`` in place of the backend's
+        workspace."""
+        own = ws is not None
         at = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
         d = p.dec or p
         p.batch = _native.Batch(
             num_blocks=self.num_blocks, cu_query_lens=at(p.cu_q), kv_indptr=at(p.indptr),
             kv_indices=at(p.indices), kv_lens=at(p.kv_lens), batch_indices=at(p.bidx),
             slot_mapping=at(p.slots), prefill_plan=at(p.plan), decode_plan=at(d.plan),
-            workspace=self._ws_ptr, workspace_bytes=self._ws_bytes,
+            workspace=ws.data_ptr() if own else self._ws_ptr,
+            workspace_bytes=ws.numel() if own else self._ws_bytes,
             status_word=self._status_ptr, n_seqs=p.n_seqs, n_tokens=p.n_tokens, n_heads=self.n_heads,
             n_kv_heads=self.n_kv_heads, head_dim=self.head_dim, page_size=self.block_size,
             dtype=self._code, is_prefill=p.use_prefill, n_tiles=p.n_work, q_tile=self.q_tile,

@@ -839,7 +839,7 @@ class MI355XBackend:
         p = self._shared
         if p is None or p.meta is not meta:
             p = self._plan_shared(meta)
-        if not p.n_tiles or not float(scale) > 0:
+        if not p.n_tiles or not C.c_float(float(scale)).value > 0:   # (as the kernels take it)
             if p.whole is None:
                 self._plan_whole(p, meta)
             self._enter(p)

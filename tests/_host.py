@@ -9,8 +9,10 @@ from __future__ import annotations
 import numpy as np
 import torch
 
-from llm_serving_layer_amd import _native, backend
+from llm_serving_layer_amd import BlockAllocator, SequenceBlocks, _native, backend
 from llm_serving_layer_amd.backend import MI355XBackend
+
+from ._util import grow_and_assemble
 
 LAUNCHES = ("pkv_append_kv", "pkv_append_batch", "pkv_append_rotated_batch", "pkv_attend_batch",
             "pkv_attend_shared_batch", "pkv_attend_selected_batch", "pkv_page_bounds",
@@ -77,3 +79,16 @@ def host_backend(monkeypatch, n_heads=32, n_kv=8, d=64, dtype=torch.float16, blo
         bk._bounds_ptr = [(b[0].data_ptr(), b[1].data_ptr()) for b in bk._bounds]
     bk._upload = lambda a: torch.from_numpy(np.array(a))
     return bk
+
+
+def sharing_batch(bk, pages=20, n=3):
+    """A decode step of n sequences that begin with the same pages."""
+    alloc = BlockAllocator(bk.num_blocks, bk.block_size)
+    head = alloc.allocate(pages)
+    seqs = []
+    for i in range(n):
+        s = SequenceBlocks(alloc, seq_id=i)
+        alloc.incref(head)
+        s.block_ids, s.num_tokens = list(head), pages * bk.block_size
+        seqs.append(s)
+    return grow_and_assemble(seqs, [1] * n, bk.block_size)

@@ -571,14 +571,15 @@ class MI355XBackend:
                 if _capturing():
                     self._keep(p)
                 return
-        r = None
-        if self._bounds is not None:
-            r = self._rows
-            if r is None or r.meta is not meta:
-                r = self._rows_for(meta)
-        self._launch_append(layer_idx, k, v, self._slots_for(meta), stream)
-        if r is not None and r.complete is not None:
-            self._renew_bounds(r.complete, r.complete.shape[0], self._enter(r), layer_idx)
+        if self._bounds is None:
+            return self._launch_append(layer_idx, k, v, self._slots_for(meta), stream)
+        r = self._rows
+        if r is None or r.meta is not meta:
+            r = self._rows_for(meta)
+        stream = self._enter(r)   # (before the rows: behind the upload of their slots)
+        self._launch_append(layer_idx, k, v, r.slots, stream)
+        if r.complete is not None:
+            self._renew_bounds(r.complete, r.complete.shape[0], stream, layer_idx)
 
     def append_kv_rotated(self, layer_idx: int, q: torch.Tensor, k: torch.Tensor,
                           v: torch.Tensor, meta: BatchMeta, table: RotaryTable) -> torch.Tensor:

@@ -666,11 +666,15 @@ class MI355XBackend:
             r.meta = meta
         else:   # another table: what a captured launch read stays described as it was
             old, r = r, _Rows()
-            for name in ("meta", "slots", "positions", "complete", "buffers", "stream"):
+            for name in ("meta", "slots", "positions", "complete", "stream"):
                 setattr(r, name, getattr(old, name))
+            r.buffers = [t for t in (r.slots, r.positions, r.complete) if t is not None]
         r.table = table
         r.args = r.ptr = None
         if table is not None:
+            r.buffers.append(table.table)
+            if table.stream != _current_stream(self.device) and not _capturing():
+                table.table.record_stream(torch.cuda.current_stream(self.device))
             r.args = _native.Rotated(
                 num_blocks=self.num_blocks, n_tokens=r.positions.shape[0],
                 max_positions=table.max_positions,

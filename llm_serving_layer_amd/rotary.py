@@ -51,6 +51,9 @@ class RotaryTable:
         self.device = torch.device(device)
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
+        # the stream whose memory the table is; launches on others record it there
+        self.stream = (torch.cuda.current_stream(self.device).cuda_stream
+                       if self.device.type == "cuda" else None)
         angle = (torch.arange(self.max_positions, dtype=torch.float64, device=self.device)[:, None]
                  * f.to(self.device))
         # [position][cosines, sines][pair]

@@ -142,7 +142,8 @@ def build_batch_meta(seqs: list[ScheduledSeq], device, page_size: int,
     fields = _upload(parts, positions, device, dtype_index)
     # the host arrays travel with the meta, so planning needs no read-back
     mirror = HostMirror(arrays={k: parts[k] for k in MIRRORED},
-                        of=tuple(fields[k] for k in MIRRORED))
+                        of=tuple(fields[k] for k in MIRRORED),
+                        positions=(fields["positions"], positions))
     return BatchMeta(**fields, page_size=page_size, is_prefill=bool((qlens > 1).any()),
                      host=mirror)
 

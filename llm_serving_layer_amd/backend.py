@@ -593,7 +593,7 @@ class MI355XBackend:
         stride between tokens, heads one after another. Rotation in 32 bits,
         rounded once to the pool dtype; inputs of another dtype are brought to
         it first, as ``append_kv`` does. A position past the table is refused
-        where the meta's host mirror tells it, and else flagged for
+        where the meta's host mirror holds it, and else flagged for
         ``check_device_errors`` (its row is not written, its query is zero).
         To capture a graph, call it once with the meta before.
         """
@@ -639,11 +639,12 @@ class MI355XBackend:
                              f"{self.device}")
         if table.rotary_dim > self.head_dim:
             raise ValueError(f"rotary_dim={table.rotary_dim} exceeds head_dim={self.head_dim}")
-        mirror = meta.host_arrays()   # (without one the kernel flags it)
-        far = int(mirror["kv_lens"].max(initial=0)) - 1 if mirror is not None else -1
-        if far >= table.max_positions:
-            raise ValueError(f"position {far} is outside the rotation table of "
-                             f"{table.max_positions} positions")
+        pos = meta.host_positions()   # (without them the kernel flags it)
+        if pos is not None and pos.shape[0]:
+            for p in (int(pos.max()), int(pos.min())):
+                if not 0 <= p < table.max_positions:
+                    raise ValueError(f"position {p} is outside the rotation table of "
+                                     f"{table.max_positions} positions")
 
     def _rows_for(self, meta: BatchMeta, table: RotaryTable | None = None) -> _Rows:
         """The meta's slots, positions and completed pages on the device, once

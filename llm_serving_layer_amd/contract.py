@@ -41,11 +41,14 @@ class HostMirror:
     the device tensors back. ``of`` holds the device tensors the arrays
     describe; the mirror speaks for a BatchMeta only while its fields are
     those very tensors (``BatchMeta.host_arrays``), so a meta rebuilt with
-    ``dataclasses.replace`` never plans from stale arrays.
+    ``dataclasses.replace`` never plans from stale arrays. ``positions``: the
+    positions' device tensor and its host copy, a mirror of their own
+    (``BatchMeta.host_positions``), since no launch plan reads them.
     """
 
     arrays: dict
     of: tuple
+    positions: Optional[tuple] = None
 
 
 @dataclass(frozen=True)
@@ -94,6 +97,14 @@ class BatchMeta:
             if getattr(self, name) is not t:
                 return None
         return h.arrays
+
+    def host_positions(self) -> Optional[np.ndarray]:
+        """The positions on the host, if the mirror holds those of this meta's
+        own ``positions`` tensor."""
+        h = self.host
+        if h is None or h.positions is None or h.positions[0] is not self.positions:
+            return None
+        return h.positions[1]
 
     @property
     def n_seqs(self) -> int:

@@ -122,5 +122,6 @@ class DecodeStepper:
         }
         fields = _upload(parts, pos, self.device, self.dtype_index)
         mirror = HostMirror(arrays={k: parts[k] for k in MIRRORED},
-                            of=tuple(fields[k] for k in MIRRORED))
+                            of=tuple(fields[k] for k in MIRRORED),
+                            positions=(fields["positions"], pos))
         return BatchMeta(**fields, page_size=bs, is_prefill=False, host=mirror)

@@ -267,9 +267,12 @@ struct NearShape {
 // to 16 lanes are at most 12 steps (the bf16 dot2, measured over 2^20 random
 // operands of sizes down to 2^-20, is off by 1.7 2^-24 of its terms' magnitudes,
 // less than two roundings), together less than 16 2^-23 of sum |q| times the
-// largest bound; subnormal bf16 bounds and sums may be taken for zero. Not a number or infinite if anything is: then nothing is settled by the
-// 32-bit sums.
+// largest bound; subnormal bf16 bounds and sums may be taken for zero. Infinite
+// where anything is infinite or no number, or where a sum could pass the largest
+// float on its way (none is larger than that product but for its roundings: from
+// half of it on): then nothing is settled by the 32-bit sums.
 __device__ __forceinline__ float near(float q_sum, float b_max) {
+  if (!(q_sum * b_max < 1.7014118e38f)) return INFINITY;
   return q_sum * (b_max * (16.f * 1.1920929e-7f) + 1.1754944e-38f) + 1e-36f;
 }
 

@@ -1,7 +1,7 @@
 """
 The choice of pages whose scores run in 32 bits first: every kernel it is made
-of (query heads a KV head, lists of each size the choice is compiled for): the
-chosen pages are those of the 64-bit scores.
+of (query heads a KV head, lists of each size the choice is compiled for), and
+values that 32-bit sums lose: the chosen pages are those of the 64-bit scores.
 """
 
 from __future__ import annotations
@@ -9,6 +9,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from ._ops64 import chosen64
 from .test_gpu_selection import DEV, Cache
 
 pytestmark = pytest.mark.gpu
@@ -52,3 +53,46 @@ def test_every_kernel_of_the_choice(n_heads, n_kv, d, max_pages, dtype, close):
     out, chosen = c.bk.attend_selected(q, 0, 0.125, c.meta, 30, return_pages=True)
     c.bk.check_device_errors()
     c.check(q, 30, out, chosen)
+
+
+def assert_chosen(c, q, chosen, budget):
+    lo, hi = c.bk.key_bounds[0]
+    for i, s in enumerate(c.seqs[:3]):
+        ids = torch.tensor(s.block_ids, device=DEV)
+        want = chosen64(q[i], lo[ids], hi[ids], len(ids), budget)
+        assert [w[:budget] for w in chosen[i].tolist()] == want, f"seq {i}"
+
+
+@pytest.mark.parametrize("n_heads, n_kv, d", [(64, 4, 64), (16, 4, 128), (4, 4, 64)])
+@pytest.mark.parametrize("first", [1, -1])
+@pytest.mark.parametrize("lanes", [1, 2])
+@pytest.mark.parametrize("size", [2e18, 4e18])
+def test_sums_that_overflow_on_the_way(n_heads, n_kv, d, first, lanes, size):
+    """bf16 products of 2e38 and 5e38 (the largest float is 3.4e38) of both signs:
+    a few pages whose 32-bit sum overflows on its way to a score that does not,
+    the lowest or the highest of all, in one lane's elements and from one lane's
+    to another's; a second query head's scores are small. (The attention's own
+    scores overflow with them: its output is not looked at.)"""
+    print(f"near overflow {n_heads}/{n_kv}/{d} {first} {lanes} {size}", flush=True)
+    c = near_cache(n_heads, n_kv, d, torch.bfloat16, 600)
+    kp, groups = c.bk.k_pool[0], n_heads // n_kv
+    a, b = [0, 1], [2, 3] if lanes == 1 else [8, 9]
+    q = torch.zeros((len(c.seqs), n_heads, d), dtype=torch.bfloat16, device=DEV)
+    q[..., a], q[..., b] = first * 1e20, -first * 1e20
+    if groups > 1:
+        q[:, 1::groups] = c.q()[:, 1::groups]
+    kp.zero_()
+    rand = torch.rand((kp.shape[0], 1, n_kv), generator=c.g, device=DEV)
+    for j in (*a, *b):
+        kp[..., j] = (1e17 * rand.roll(j, 0)).to(kp.dtype)
+    for s in c.seqs[:3]:
+        some = torch.tensor(s.block_ids[3:400:40], device=DEV)
+        big = size * (1 + torch.rand((len(some), 1, 1), generator=c.g, device=DEV) / 4)
+        for j in a:
+            kp[some, ..., j] = big.to(kp.dtype)
+        for j in b:        # the score: 2e20 first (big - this)
+            kp[some, ..., j] = (big * 1.2).to(kp.dtype)
+    c.bk.refresh_page_bounds()
+    _, chosen = c.bk.attend_selected(q, 0, 1e-30, c.meta, 30, return_pages=True)
+    c.bk.check_device_errors()
+    assert_chosen(c, q, chosen, 30)

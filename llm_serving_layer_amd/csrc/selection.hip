@@ -267,13 +267,15 @@ struct NearShape {
 // to 16 lanes are at most 12 steps (the bf16 dot2, measured over 2^20 random
 // operands of sizes down to 2^-20, is off by 1.7 2^-24 of its terms' magnitudes,
 // less than two roundings), together less than 16 2^-23 of sum |q| times the
-// largest bound; subnormal bf16 bounds and sums may be taken for zero. Infinite
+// largest bound; subnormal bf16 operands (of up to D query elements, or bounds)
+// and sums may be taken for zero. Infinite
 // where anything is infinite or no number, or where a sum could pass the largest
 // float on its way (none is larger than that product but for its roundings: from
 // half of it on): then nothing is settled by the 32-bit sums.
-__device__ __forceinline__ float near(float q_sum, float b_max) {
+__device__ __forceinline__ float near(float q_sum, float b_max, int D) {
   if (!(q_sum * b_max < 1.7014118e38f)) return INFINITY;
-  return q_sum * (b_max * (16.f * 1.1920929e-7f) + 1.1754944e-38f) + 1e-36f;
+  constexpr float kTiny = 1.1754944e-38f;
+  return q_sum * (b_max * (16.f * 1.1920929e-7f) + kTiny) + b_max * ((float)D * kTiny) + 1e-36f;
 }
 
 // (fp16: dot2 loses low bits of products below 2^-24 or so, a mixed fma does not)
@@ -760,7 +762,7 @@ __global__ __launch_bounds__(B) void select_rows_kernel(
     }
     const float t = __builtin_bit_cast(
         float, c32.least >> 31 ? c32.least ^ 1u << 31 : ~c32.least);
-    const float e = 2.01f * near(q_sum, b_max) + 4.8e-7f * __builtin_fabsf(t);
+    const float e = 2.01f * near(q_sum, b_max, na.D) + 4.8e-7f * __builtin_fabsf(t);
     uint32_t open = 0;
     int n_sure = 0, n_open = 0;
 #pragma unroll

@@ -96,3 +96,19 @@ def test_sums_that_overflow_on_the_way(n_heads, n_kv, d, first, lanes, size):
     _, chosen = c.bk.attend_selected(q, 0, 1e-30, c.meta, 30, return_pages=True)
     c.bk.check_device_errors()
     assert_chosen(c, q, chosen, 30)
+
+
+@pytest.mark.parametrize("n_heads, n_kv, d", [(64, 4, 64), (16, 4, 128), (4, 4, 64)])
+def test_queries_below_the_smallest_normal(n_heads, n_kv, d):
+    """bf16: one query element of 1e-36, the others subnormal, keys of up to 1e30:
+    what the subnormal elements add decides, far above the sums' roundings."""
+    print(f"near subnormal {n_heads}/{n_kv}/{d}", flush=True)
+    c = near_cache(n_heads, n_kv, d, torch.bfloat16, 600)
+    kp = c.bk.k_pool[0]
+    kp.copy_((kp.float() * 1e30).to(kp.dtype))
+    q = (torch.rand((len(c.seqs), n_heads, d), generator=c.g, device=DEV) * 1e-38).bfloat16()
+    q[..., 0] = 1e-36
+    c.bk.refresh_page_bounds()
+    _, chosen = c.bk.attend_selected(q, 0, 0.125, c.meta, 30, return_pages=True)
+    c.bk.check_device_errors()
+    assert_chosen(c, q, chosen, 30)

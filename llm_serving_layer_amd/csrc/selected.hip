@@ -47,7 +47,8 @@ __global__ __launch_bounds__(kMaxWaves * 64) void selected_stream_kernel(
 }
 
 // Any geometry: one wave a query head, three passes over the chosen pages' keys
-// (maximum, sum, weighted values), as the generic kernel does over all of them.
+// (maximum, sum, weighted values), as the generic kernel does over all of them;
+// probabilities stay in 32 bits, as the products with them are.
 template <typename T>
 __global__ __launch_bounds__(64) void selected_generic_kernel(
     const T* __restrict__ q, T* __restrict__ out, const T* __restrict__ kpool,
@@ -87,7 +88,7 @@ __global__ __launch_bounds__(64) void selected_generic_kernel(
   for (int k0 = 0; k0 < n_keys; k0 += 64) {
     const int key = k0 + lane;
     float p = 0.f;
-    if (key < n_keys) p = Elem<T>::to_f(Elem<T>::from_f(expf(score(key) - m) * inv));
+    if (key < n_keys) p = expf(score(key) - m) * inv;
     __syncthreads();
     pw[lane] = p;
     __syncthreads();

@@ -29,7 +29,7 @@ namespace pkv {
 
 template <typename T> struct SharedArgs {
   const T* q; T* out; T* kp; T* vp;
-  int64_t nb; const int32_t* indices; int32_t Hkv; float sl2; SharedTile sh; int32_t n_tiles;
+  int64_t nb; const int32_t* indices; int32_t Hkv; float sl2; SharedTile sh;
   const int32_t* plan; int32_t stride; const T* kn; const T* vn; const int32_t* slots;
   DecodeWorkspace w; int32_t* status;
   int32_t tiles, pieces, turn;   // workgroups of each kind, and in a row of one kind
@@ -49,7 +49,7 @@ __device__ __forceinline__ int shared_role(int block, int tiles, int pieces, int
 }
 
 // Tiles beside the bins of the streaming decode kernel (four KV heads a bin's
-// workgroup).
+// workgroup, a wave each: bins of fewer run in a launch of their own).
 template <typename T, int D, int G>
 __global__ __launch_bounds__(256, 2) void shared_stream_kernel(SharedArgs<T> a) {
   extern __shared__ __align__(16) unsigned char smem[];
@@ -59,7 +59,6 @@ __global__ __launch_bounds__(256, 2) void shared_stream_kernel(SharedArgs<T> a) 
                                 a.indices, nullptr, nullptr, a.Hkv, a.sl2, a.status, a.sh);
   } else {
     const int groups = a.Hkv / heads_per_wg(a.Hkv), bin = ~role / groups;
-    if ((int)(threadIdx.x >> 6) >= heads_per_wg(a.Hkv)) return;
     decode_stream<T, D, G>(smem, bin, ~role - bin * groups, a.q, a.out, a.kp, a.vp, a.nb, a.plan,
                            a.stride, a.Hkv, a.sl2, a.kn, a.vn, a.slots, a.w.part_o, a.w.part_ml,
                            a.w.o_bytes, a.w.ml_bytes, a.w.counters, a.status);
@@ -119,7 +118,7 @@ static void launch_shared(const SharedLaunch& l, hipStream_t s) {
   const int groups = l.Hkv / heads_per_wg(l.Hkv);
   const bool few = few_pieces(l.n_work, l.stride, l.Hkv, D);
   SharedArgs<T> a{(const T*)l.q, (T*)l.out, (T*)l.kp, (T*)l.vp, l.nb, l.indices, l.Hkv, l.sl2, l.sh,
-                  l.n_tiles, l.plan, l.stride, (const T*)l.kn, (const T*)l.vn, l.slots, l.w,
+                  l.plan, l.stride, (const T*)l.kn, (const T*)l.vn, l.slots, l.w,
                   l.status, l.n_tiles * l.Hkv, few ? l.n_work / groups * l.Hkv : l.n_work,
                   std::max(1, compute_units())};
   // A bin's workgroup has a wave a KV head, four at most. With fewer than four

@@ -233,6 +233,7 @@ class MI355XBackend:
 
     _rows: _Rows | None = None
     _selected: _Selected | None = None
+    _budgets: tuple[_Selected, ...] = ()   # the latest meta's plans, one a page budget
     _shared: _Shared | None = None
     _bounds: torch.Tensor | None = None
 
@@ -1006,7 +1007,7 @@ class MI355XBackend:
                              "are of the largest score")
         p = self._selected
         if p is None or p.meta is not meta or p.asked != pages:
-            p = self._plan_selected(meta, pages)
+            p = self._selected_for(meta, pages)
         self._flush()
         stream = self._enter(p)
         if not (q.dtype is self.dtype and q.get_device() == self.device.index
@@ -1030,6 +1031,17 @@ class MI355XBackend:
             _native.check(rc, "attend_selected")
         self.n_runs += 1
         return (out, ordinals) if return_pages else out
+
+    def _selected_for(self, meta: BatchMeta, pages: int) -> _Selected:
+        """The meta's plan for this budget, made once (a step's layers may differ
+        in theirs)."""
+        known = tuple(p for p in self._budgets if p.meta is meta)
+        p = next((p for p in known if p.asked == pages), None)
+        if p is None:
+            p = self._plan_selected(meta, pages)
+            known += (p,)
+        self._budgets, self._selected = known, p
+        return p
 
     def _plan_selected(self, meta: BatchMeta, pages: int) -> _Selected:
         self._refuse_capture("attend_selected")
@@ -1086,7 +1098,6 @@ class MI355XBackend:
         p.ptr = C.addressof(p.args)
         p.stream = _current_stream(self.device)
         p.meta = meta
-        self._selected = p
         self.n_plans += 1
         return p
 
@@ -1368,6 +1379,7 @@ class MI355XBackend:
         self._planned = None
         self._slot_cache = None
         self._rows = self._selected = self._shared = None
+        self._budgets = ()
 
     # -- misc -------------------------------------------------------------------------
 

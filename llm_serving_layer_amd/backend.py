@@ -850,7 +850,8 @@ class MI355XBackend:
             if p.whole is None:
                 self._plan_whole(p, meta)
             self._enter(p)
-            return self._attend_by(p.whole, q, layer_idx, scale, meta)
+            with self._on_device():
+                return self._attend_by(p.whole, q, layer_idx, scale, meta)
         pend = self._pending
         fused = (pend is not None and pend.layer == layer_idx and pend.meta is meta
                  and pend.stream == _current_stream(self.device) and p.fusable

@@ -215,7 +215,8 @@ class _Rows:
 
 class _Shared:
     """What ``attend_shared`` keeps for one BatchMeta. Where nothing is worth
-    sharing ``n_tiles`` is 0; ``whole`` is how such a batch runs, once it has."""
+    sharing ``n_tiles`` is 0; ``whole`` is the plan ``attend`` ran it by, once it
+    has."""
 
     __slots__ = ("meta", "n", "n_tiles", "n_merges", "tiles", "plan", "indices", "slots", "n_work", "n_slots",
                  "stride", "ws", "fusable", "args", "ptr", "buffers", "stream", "whole")
@@ -551,9 +552,12 @@ class MI355XBackend:
         if self._fuse_append:
             p = self._planned
             if p is None or p.meta is not meta:
+                if _capturing():   # no plan is made here: the rows are appended on their own
+                    slots = self._slots_for(meta)
+                    self._keep(slots)
+                    return self._launch_append(layer_idx, k, v, slots, stream)
                 try:
-                    # (not within a capture: the rows are appended on their own)
-                    p = None if _capturing() else self._ensure_planned(meta)
+                    p = self._ensure_planned(meta)
                 except ValueError:
                     p = None  # inconsistent paging metadata: append now, attend will raise
             if p is not None and p.fusable:
@@ -569,8 +573,6 @@ class MI355XBackend:
                     self._v_ptr[layer_idx], k.data_ptr(), v.data_ptr(), stream)
                 if rc:
                     _native.check(rc, "append_kv")
-                if _capturing():
-                    self._keep(p)
                 return
         if self._bounds is None:
             return self._launch_append(layer_idx, k, v, self._slots_for(meta), stream)
@@ -617,10 +619,11 @@ class MI355XBackend:
         r = self._rows
         if r is None or r.meta is not meta or r.table is not table:
             r = self._rows_for(meta, table)
-        if self._pending is not None:
+        pend = self._pending
+        if pend is not None:
             self._flush()
         q, k, v = self._token_rows(q), self._token_rows(k), self._token_rows(v)
-        stream = self._enter(r)
+        stream = self._enter(r, pend.slots if pend is not None else None)
         out = torch.empty((tokens, self.n_heads, d), dtype=self.dtype, device=self.device)
         lo, hi = self._bounds_ptr[layer_idx] if r.complete is not None else (None, None)
         with self._on_device():
@@ -642,10 +645,10 @@ class MI355XBackend:
             raise ValueError(f"rotary_dim={table.rotary_dim} exceeds head_dim={self.head_dim}")
         pos = meta.host_positions()   # (without them the kernel flags it)
         if pos is not None and pos.shape[0]:
-            for p in (int(pos.max()), int(pos.min())):
-                if not 0 <= p < table.max_positions:
-                    raise ValueError(f"position {p} is outside the rotation table of "
-                                     f"{table.max_positions} positions")
+            far = int(pos.view(np.uint64).max())   # (a negative one is the farthest)
+            if far >= table.max_positions:
+                raise ValueError(f"position {far - (far >> 63 << 64)} is outside the rotation "
+                                 f"table of {table.max_positions} positions")
 
     def _rows_for(self, meta: BatchMeta, table: RotaryTable | None = None) -> _Rows:
         """The meta's slots, positions and completed pages on the device, once
@@ -742,8 +745,6 @@ class MI355XBackend:
             k.shape[0], self.n_kv_heads, self.head_dim, self._code, self._status_ptr,
             stream)
         _native.check(rc, "append_kv")
-        if _capturing():
-            self._keep(slots)
 
     def _check_pending_intact(self, pend: _Pending) -> None:
         if pend.k._version != pend.kver or pend.v._version != pend.vver:
@@ -847,11 +848,13 @@ class MI355XBackend:
         if p is None or p.meta is not meta:
             p = self._plan_shared(meta)
         if not p.n_tiles or not C.c_float(float(scale)).value > 0:   # (as the kernels take it)
-            if p.whole is None:
-                self._plan_whole(p, meta)
-            self._enter(p)
             with self._on_device():
-                return self._attend_by(p.whole, q, layer_idx, scale, meta)
+                if _capturing():
+                    return self._attend_in_graph(p, q, layer_idx, scale, meta)
+                out = self.attend(q, layer_idx, scale, meta)
+            if p.whole is None:
+                p.whole = self._planned
+            return out
         pend = self._pending
         fused = (pend is not None and pend.layer == layer_idx and pend.meta is meta
                  and pend.stream == _current_stream(self.device) and p.fusable
@@ -861,7 +864,7 @@ class MI355XBackend:
             self._pending = None
         elif pend is not None:
             self._flush()
-        stream = self._enter(p)
+        stream = self._enter(p, pend.slots if pend is not None else None)
         if not (q.dtype is self.dtype and q.get_device() == self.device.index
                 and q.is_contiguous()):
             q = self._as_pool(q)
@@ -900,22 +903,22 @@ class MI355XBackend:
         self._shared = p
         return p
 
-    def _plan_whole(self, p: _Shared, meta: BatchMeta) -> None:
-        """The batch as ``attend`` runs it: its plan, kept with ``p``, and a
-        workspace of its own, since other plans' partials in the backend's would
-        meet this one's arrival counters when a graph replays it."""
-        self._refuse_capture("attend_shared")
-        w = copy.copy(self._ensure_planned(meta))
-        self._enter(p)
-        d = w.dec or w
-        n = w.n_seqs if w.dec is None else w.dec.n
-        need = self._lib.pkv_decode_workspace_bytes(n, d.n_slots, self.n_heads, self.n_kv_heads,
-                                                    self.head_dim)
-        ws = self._counted_workspace(need, n)
+    def _attend_in_graph(self, p: _Shared, q, layer_idx, scale, meta) -> torch.Tensor:
+        """``attend`` within a capture, by the plan of its eager call, which stays
+        with ``p``, and a workspace of the graph's own, cleared by it. (In the
+        backend's, which each plan lays out anew, other plans' partials would lie on
+        this one's arrival counters between replays.)"""
+        if p.whole is None:
+            self._refuse_capture("attend_shared")
+        self._keep(p)
+        if self._pending is not None:
+            self._keep(self._pending.slots)
+        w = copy.copy(p.whole)
+        n, d = (w.n_seqs, w) if w.dec is None else (w.dec.n, w.dec)
+        ws = self._counted_workspace(self._lib.pkv_decode_workspace_bytes(
+            n, d.n_slots, self.n_heads, self.n_kv_heads, self.head_dim), n)
         self._describe(w, ws)
-        p.buffers += [t for t in (w.plan, w.indptr, w.indices, w.kv_lens, w.cu_q, w.bidx, w.slots,
-                                  d.plan, ws) if t is not None]
-        p.whole = w
+        return self._attend_by(w, q, layer_idx, scale, meta)
 
     def _fill_shared(self, p: _Shared, meta: BatchMeta, indptr, indices, kvl, last) -> None:
         """Plan the batch's shared runs and own pages (pkv_plan_shared)."""
@@ -1155,13 +1158,15 @@ class MI355XBackend:
             raise RuntimeError(f"{what} has to plan this meta before a graph is captured: call "
                                "it once with the meta (and the same arguments), then capture")
 
-    def _enter(self, p) -> int:
+    def _enter(self, p, slots=None) -> int:
         """The current stream's handle, ordered behind the plan's last launch:
-        launches of one plan share its buffers. A plan that a graph captures
-        stays as long as the backend does."""
+        launches of one plan share its buffers. A plan that a graph captures, and
+        the slots of an append that it landed, stay as long as the backend does."""
         stream = _current_stream(self.device)
         if _capturing():
             self._keep(p)
+            if slots is not None:
+                self._keep(slots)
         elif p.stream != stream:
             cur, ev = torch.cuda.current_stream(self.device), torch.cuda.Event()
             ev.record(torch.cuda.ExternalStream(p.stream, device=self.device))

@@ -31,7 +31,7 @@ def rows(bk, meta, heads):
 @pytest.mark.parametrize("scale", [0.125, -0.125])
 def test_a_batch_that_does_not_share_keeps_its_plan(counts, scale, monkeypatch):
     """attend_shared of a meta that it has seen, after another meta was planned:
-    the plan and workspace of the first call, untouched by the other's."""
+    the first call's plan, kept, and a workspace that the other's does not touch."""
     bk = host_backend(monkeypatch)
     alloc = BlockAllocator(bk.num_blocks, 16)
     a, b = batch(bk, [700, 20, 400], counts, alloc), batch(bk, [3000], None, alloc)
@@ -40,20 +40,22 @@ def test_a_batch_that_does_not_share_keeps_its_plan(counts, scale, monkeypatch):
     name, _, eager = bk._lib.calls[-1]
     assert name == "pkv_attend_batch" and eager.n_slots > 0, "a cut sequence"
     bk.attend(qb, 0, scale, b)
-    other = bk._lib.calls[-1][2]
-    assert other.workspace != eager.workspace, "the other's partials are not its counters"
     plans = bk.n_plans
     monkeypatch.setattr(backend, "_capturing", lambda: True)
     monkeypatch.setattr(bk, "_upload", None)     # nothing is uploaded
     bk.attend_shared(qa, 0, scale, a)
     name, _, held = bk._lib.calls[-1]
-    assert bytes(held) == bytes(eager) and bk.n_plans == plans
-    kept = {t.data_ptr() for p in bk._captured for t in getattr(p, "buffers", [])}
-    for at in (held.decode_plan, held.workspace, held.kv_indices, held.kv_lens, held.kv_indptr,
-               held.cu_query_lens, held.batch_indices, held.slot_mapping):
-        assert at in kept
-    if counts:
-        assert held.prefill_plan in kept
+    assert bk.n_plans == plans and held.workspace != bk._ws_ptr, "a workspace of the graph's"
+    assert held.workspace and held.workspace_bytes < bk._ws_bytes
+    for name, _ in held._fields_:
+        if name not in ("workspace", "workspace_bytes"):
+            assert getattr(held, name) == getattr(eager, name), name
+    (p,) = bk._captured
+    w, d = p.whole, p.whole.dec or p.whole
+    kept = {t.data_ptr() for t in (w.plan, d.plan, w.indptr, w.indices, w.kv_lens, w.cu_q, w.bidx,
+                                   w.slots)}
+    assert {held.prefill_plan, held.decode_plan, held.kv_indptr, held.kv_indices, held.kv_lens,
+            held.cu_query_lens, held.batch_indices, held.slot_mapping} == kept
     monkeypatch.setattr(backend, "_capturing", lambda: False)
     assert bk._planned.meta is b, "eager calls find what they planned"
 
@@ -118,3 +120,21 @@ def test_a_captured_append_plans_nothing_and_keeps_its_slots(monkeypatch):
     monkeypatch.setattr(backend, "_capturing", lambda: False)
     bk.append_kv(0, k, k, a)                       # eager again: planned, fused
     assert bk._planned.meta is a and bk._pending is not None
+
+
+def test_an_append_that_a_captured_call_lands_keeps_its_slots(monkeypatch):
+    """A deferred append of another layer, in slots that were converted for it."""
+    import dataclasses
+
+    bk = host_backend(monkeypatch, layers=2)
+    a = batch(bk, [700, 20, 400])
+    a = dataclasses.replace(a, slot_mapping=a.slot_mapping.long(), host=None)
+    q, k = rows(bk, a, 32), rows(bk, a, 8)
+    bk.append_kv(1, k, k, a)
+    bk.attend_shared(q, 0, 0.125, a)
+    monkeypatch.setattr(backend, "_capturing", lambda: True)
+    bk.append_kv(1, k, k, a)
+    bk.attend_shared(q, 0, 0.125, a)
+    name, args, _ = bk._lib.calls[-2]
+    assert name == "pkv_append_kv"
+    assert any(torch.is_tensor(t) and t.data_ptr() == args[5] for t in bk._captured)

@@ -54,7 +54,7 @@ def test_a_batch_that_does_not_share_replays_among_other_plans(counts, scale, be
     want = step()
     plain = [bk.attend(q[l], l, scale, meta) for l in range(2)]
     assert all(torch.equal(a, b) for a, b in zip(want, plain)), "as attend runs it"
-    assert not bk._shared.n_tiles and (bk._shared.whole.dec or bk._shared.whole).n_slots > 0
+    assert not bk._shared.n_tiles and (bk._planned.dec or bk._planned).n_slots > 0
     rows = bk._pool.clone()
     if between:
         other()

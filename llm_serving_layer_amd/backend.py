@@ -67,16 +67,17 @@ _DTYPES = {torch.float16: _native.DTYPE_F16, torch.bfloat16: _native.DTYPE_BF16,
 
 MAX_PART_PAGES = 64      # a partition's page ids are read by one wavefront
 SELECTED_PART_PAGES = 8  # of chosen pages; what their kernel stages at a time
-# Pieces (of 8 pages) up to which each of them gets a workgroup of its own; the
-# streaming kernel takes more. us a call, workgroups against streaming: 64 pieces
+# Pieces (of 8 pages, were every list as long as the longest) up to which each of
+# them gets a workgroup of its own; the streaming kernel takes more. us a call, workgroups against streaming: 64 pieces
 # 20.4 and 29.7, 512 20.0 and 26.8, 1024 26.9 and 29.3 (head_dim 64) or 36.2 and
 # 36.7 (128), 2048 40.7 and 34.5.
 SELECTED_PIECES = 1024
 # What attend_shared must save to be worth its tiles and its merge: a run of
 # shared pages at least 4 pages long, in bytes a KV head more than 25 KiB a
 # sequence (the part it adds), all runs together 16 MiB. us a call, attend against
-# shared: 6 sequences over 96 pages 10.0 and 10.7, 200 over 8 28.5 and 30.4, 2
-# over 512 15.9 and 14.3, 32 over 32 16.8 and 13.8, 256 over 128 130 and 39.
+# shared (8 KV heads of 64): 6 sequences over 96 pages 10.0 and 10.7, 200 over 8
+# 28.5 and 30.4, 32 over 32 16.8 and 13.8, 256 over 128 130 and 39. The least lies
+# on the side of attend: 2 over 512, 15.9 and 14.3, save 15.6 MiB and run it.
 SHARED_MIN_PAGES, SHARED_PART_BYTES, SHARED_LEAST_BYTES = 4, 25 << 10, 16 << 20
 SHARED_TILES = 256       # workgroups that share the work on a batch's shared pages
 DEFAULT_Q_TILE = 64      # prefill tile when the geometry has no matrix-core kernel
@@ -598,7 +599,8 @@ class MI355XBackend:
         it first, as ``append_kv`` does. A position past the table is refused
         where the meta's host mirror holds it, and else flagged for
         ``check_device_errors`` (its row is not written, its query is zero).
-        To capture a graph, call it once with the meta before.
+        To capture a graph, call it with the meta before, with no other meta's
+        call between.
         """
         if layer_idx is None or not 0 <= layer_idx < self.num_layers:
             self._check_layer(layer_idx)
@@ -831,10 +833,10 @@ class MI355XBackend:
 
         Batches with prompt chunks, geometries without the fast decode path, a
         scale that is not positive and batches that share too little to gain
-        by it run as ``attend`` runs them. To capture a graph, call it once with
-        the meta (and a scale of the same sign) before. Graphs captured with one
-        meta share its buffers: neither their replays nor eager calls with it may
-        overlap.
+        by it run as ``attend`` runs them. To capture a graph, call it with the
+        meta (and a scale of the same sign) before, with no other meta's call
+        between. Graphs captured with one meta share its buffers: neither their
+        replays nor eager calls with it may overlap.
         """
         if layer_idx is None or not 0 <= layer_idx < self.num_layers:
             self._check_layer(layer_idx)
@@ -990,9 +992,9 @@ class MI355XBackend:
         scale. With ``return_pages`` also returns the chosen pages' indices in
         each sequence's page list, int32 ``(n_seqs, n_kv_heads, min(pages,
         longest list))``, ascending, -1 behind a shorter list. To capture a
-        graph, call it once with the meta and ``pages`` before. Graphs captured
-        with one meta share its buffers: neither their replays nor eager calls
-        with it may overlap.
+        graph, call it with the meta and ``pages`` before, with no other meta's
+        call between. Graphs captured with one meta share its buffers: neither
+        their replays nor eager calls with it may overlap.
         """
         if layer_idx is None or not 0 <= layer_idx < self.num_layers:
             self._check_layer(layer_idx)

@@ -15,8 +15,8 @@
 //    whose other parts are the shared ones.
 //  * Both run in one launch, side by side: the tiles are bound by the matrix
 //    cores, the own pages by memory, and a compute unit holds a workgroup of
-//    each. Neither knows when a sequence's parts are complete; a last small
-//    launch merges them.
+//    each. Tiles count no arrivals, so nobody in that launch knows when a
+//    sequence's parts are complete; a last small launch merges them.
 #include <algorithm>
 #include <exception>
 #include <numeric>

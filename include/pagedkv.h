@@ -514,6 +514,77 @@ int pkv_attend_selected_batch(const void* batch, const void* q, void* out, void*
                               float scale, void* stream);
 
 /*
+ * The 4-bit cache — no counterpart in the reference. A block's K (or V) is
+ * pkv_block_bytes_4bit bytes (0 for a geometry that has none: odd head_dim or
+ * above 256), laid out as csrc/fourbit.h says; a pool is a contiguous array of
+ * num_blocks of them, which pkv_copy_blocks, pkv_gather_blocks and
+ * pkv_scatter_blocks move like any other. A row of a KV head is cut into groups
+ * of 64 elements (one group where head_dim is no multiple of 64); a group keeps
+ * a float16 zero, a float16 step and 4-bit codes, and reads as zero + step c.
+ *
+ * pkv_append_4bit: for t < n_tokens, row t of k / v (heads one after another,
+ * rows k_stride / v_stride elements apart, f16, bf16 or f32) goes to slot
+ * slot_mapping[t]. Slots outside the pool are skipped and flagged. No two tokens
+ * may share a slot.
+ *
+ * pkv_read_4bit: row i of k / v (contiguous [n_rows, n_kv_heads, head_dim])
+ * receives what slot slots[i] holds, rounded to dtype once; zeros (and the flag)
+ * for slots outside the pool.
+ */
+int64_t pkv_block_bytes_4bit(int32_t n_kv_heads, int32_t head_dim, int32_t page_size);
+int pkv_append_4bit(void* k_pool, void* v_pool, int64_t num_blocks, const void* k,
+                    int64_t k_stride, const void* v, int64_t v_stride,
+                    const int32_t* slot_mapping, int64_t n_tokens, int32_t n_kv_heads,
+                    int32_t head_dim, int32_t page_size, int32_t dtype, int32_t* status_word,
+                    void* stream);
+int pkv_read_4bit(const void* k_pool, const void* v_pool, int64_t num_blocks,
+                  const int32_t* slots, int64_t n_rows, void* k, void* v, int32_t n_kv_heads,
+                  int32_t head_dim, int32_t page_size, int32_t dtype, int32_t* status_word,
+                  void* stream);
+
+/*
+ * Causal attention over the 4-bit cache, any query lengths: sequence i's query
+ * tokens are the last of its kv_lens[i] tokens. q and out are contiguous
+ * [n_tokens, n_heads, head_dim] in dtype; a batch's arguments are set once and
+ * serve every layer.
+ *
+ * pkv_plan_4bit (host, synchronous) checks the metadata as pkv_plan_decode does
+ * and fills items (capacity ints; *needed of them, PKV_ERR_CAPACITY if there are
+ * fewer) with pieces of 8 ints {sequence, first token, tokens, first tile of 64
+ * keys, tiles, partial slot or -1, the first piece's slot, pieces}, those of
+ * sequences with at most 16 query rows (tokens x query heads a KV head) first,
+ * and the plan fields of *plan. Geometries without a matrix-core kernel (head_dim
+ * other than 64 and 128, f32, pages that are no power of two times 16, more than
+ * 32 query heads a KV head) need no items.
+ *
+ * `workspace` (256-byte aligned, workspace_bytes long): n_slots * n_kv_heads
+ * arrival counters, zero before the first launch and left so by each, then the
+ * partial results; launches that share it must not overlap in time. Page ids
+ * outside [0, num_blocks) read as zeros and are flagged.
+ */
+typedef struct pkv_4bit {
+  int64_t num_blocks, workspace_bytes;
+  const int32_t* cu_query_lens;
+  const int32_t* kv_indptr;
+  const int32_t* kv_indices;
+  const int32_t* kv_lens;
+  const int32_t* batch_indices;
+  const int32_t* items;
+  void* workspace;
+  int32_t* status_word;
+  int32_t n_seqs, n_tokens, n_heads, n_kv_heads, head_dim, page_size, dtype;
+  int32_t n_few, n_wide, few_rows, part_rows, n_slots;   /* the plan's */
+} pkv_4bit;
+
+int pkv_plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr, const int32_t* kv_lens,
+                  const int32_t* kv_last_page_len, int32_t n_seqs, int32_t n_heads,
+                  int32_t n_kv_heads, int32_t head_dim, int32_t page_size, int32_t dtype,
+                  int32_t workgroups, int32_t* items, int64_t capacity, int64_t* needed,
+                  pkv_4bit* plan);
+int pkv_attend_4bit(const void* batch, const void* q, void* out, const void* k_pool,
+                    const void* v_pool, float scale, void* stream);
+
+/*
  * Batched block copy over every layer, K and V — replaces
  * PagedTorchBackend.copy_block (serving/backends/paged_torch.py:181-207),
  * called once per pair by RadixCache.ensure_writable

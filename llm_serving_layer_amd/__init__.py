@@ -9,6 +9,7 @@ hand-written gfx950 kernels (include/pagedkv.h, csrc/):
 * ``assembly``  — ScheduledSeq, build_batch_meta, build_token_tensor;
 * ``backend``   — MI355XBackend (append_kv[_rotated] / attend[_shared, _selected] /
   copy_block[s]);
+* ``fourbit``   — FourBitBackend (the same over a cache held in 4 bits);
 * ``rotary``    — RotaryTable (MI355XBackend.append_kv_rotated);
 * ``swap``      — KVSwapSpace / SwapHandle (preemption swap);
 * ``sizing``    — plan_kv_pool / KVPoolPlan (pool sizing for one MI355X).
@@ -23,7 +24,7 @@ from .rotary import RotaryTable
 
 __all__ = ["AttentionBackend", "BatchMeta", "AllocationError", "BlockAllocator",
            "SequenceBlocks", "build_csr", "ScheduledSeq", "build_batch_meta",
-           "build_token_tensor", "RotaryTable", "MI355XBackend", "KVSwapSpace", "SwapHandle",
+           "build_token_tensor", "RotaryTable", "MI355XBackend", "FourBitBackend", "KVSwapSpace", "SwapHandle",
            "SwapSpaceFull", "is_available", "unavailable_reason"]
 
 
@@ -33,6 +34,9 @@ def __getattr__(name):
     if name in ("MI355XBackend", "is_available", "unavailable_reason"):
         from . import backend
         return getattr(backend, name)
+    if name == "FourBitBackend":
+        from . import fourbit
+        return fourbit.FourBitBackend
     if name in ("KVSwapSpace", "SwapHandle", "SwapSpaceFull"):
         from . import swap
         return getattr(swap, name)

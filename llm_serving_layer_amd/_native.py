@@ -15,7 +15,7 @@ from pathlib import Path
 # PKV_LIBRARY selects another build of the same library (e.g. a tuning variant).
 LIB_PATH = Path(os.environ.get("PKV_LIBRARY") or
                 Path(__file__).resolve().parent / "_native" / "libpagedkv.so")
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
 DECODE_SCRATCH_BYTES = 64 * 1024 * 1024   # PKV_DECODE_SCRATCH_BYTES
@@ -73,6 +73,13 @@ SIGNATURES = {
                                            _p]),
     "pkv_attend_shared_batch": (C.c_int, [_p, _p, _p, _p, _p, _f32, _p, _p, _p]),
     "pkv_attend_selected_batch": (C.c_int, [_p, _p, _p, _p, _p, _p, _p, _p, _f32, _p]),
+    "pkv_block_bytes_4bit": (C.c_int64, [_i32, _i32, _i32]),
+    "pkv_append_4bit": (C.c_int, [_p, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i32, _i32, _i32,
+                                  _i32, _p, _p]),
+    "pkv_read_4bit": (C.c_int, [_p, _p, _i64, _p, _i64, _p, _p, _i32, _i32, _i32, _i32, _p, _p]),
+    "pkv_plan_4bit": (C.c_int, [_p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p,
+                                _i64, _p, _p]),
+    "pkv_attend_4bit": (C.c_int, [_p, _p, _p, _p, _p, _f32, _p]),
     "pkv_copy_blocks": (C.c_int, [_p, _i32, _i64, _i64, _i64, _p, _p, _i32, _p, _p]),
     "pkv_gather_blocks": (C.c_int, [_p, _i32, _i64, _i64, _i64, _p, _i32, _p, _p, _p]),
     "pkv_scatter_blocks": (C.c_int, [_p, _i32, _i64, _i64, _i64, _p, _i32, _p, _p, _p]),
@@ -123,6 +130,17 @@ class Selected(C.Structure):
                 *[(n, _i32) for n in ("n_seqs", "max_pages", "pages", "part_pages", "n_heads",
                                       "n_kv_heads", "head_dim", "page_size", "dtype", "n_work",
                                       "n_slots", "plan_stride")]]
+
+
+class FourBit(C.Structure):
+    """``pkv_4bit``: an attention over the 4-bit cache's arguments, set once per plan."""
+
+    _fields_ = [*[(n, _i64) for n in ("num_blocks", "workspace_bytes")],
+                *[(n, _p) for n in ("cu_query_lens", "kv_indptr", "kv_indices", "kv_lens",
+                                    "batch_indices", "items", "workspace", "status_word")],
+                *[(n, _i32) for n in ("n_seqs", "n_tokens", "n_heads", "n_kv_heads", "head_dim",
+                                      "page_size", "dtype", "n_few", "n_wide", "few_rows",
+                                      "part_rows", "n_slots")]]
 
 
 _LIB = None

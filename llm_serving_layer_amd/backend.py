@@ -230,14 +230,190 @@ class _Selected:
                  "ids", "ordinals", "words", "places", "plan", "part", "ws", "width", "args", "ptr", "buffers", "stream")
 
 
-class MI355XBackend:
+class PagedPool:
+    """What the backends share: one pool ``[num_layers, 2, num_blocks, ...]`` whose
+    blocks move as bytes, the checks of a meta's index fields, and the order of
+    launches on streams and in graphs."""
+
+    _bounds: torch.Tensor | None = None
+
+    def _flush(self) -> None:
+        """Launch what an earlier call left to a later one."""
+
+    def pool_bytes(self) -> int:
+        return self.num_layers * 2 * self._plane_bytes
+
+    def block_bytes(self) -> int:
+        return self.pool_bytes() // self.num_blocks
+
+    def tokens_capacity(self) -> int:
+        return self.num_blocks * self.block_size
+
+    def _check_layer(self, layer_idx) -> None:
+        if layer_idx is None or not 0 <= layer_idx < self.num_layers:
+            raise ValueError(f"layer_idx {layer_idx} out of range [0, {self.num_layers})")
+
+    def _dev_i32(self, t: torch.Tensor) -> torch.Tensor:
+        return t.to(device=self.device, dtype=torch.int32).contiguous()
+
+    def _as_pool(self, x: torch.Tensor) -> torch.Tensor:
+        # (a tensor already in the pool dtype, contiguous and on this device is
+        # used as it is, without a conversion call per launch)
+        if x.dtype is self.dtype and x.get_device() == self.device.index and x.is_contiguous():
+            return x
+        return x.to(device=self.device, dtype=self.dtype).contiguous()
+
+    def check_device_errors(self) -> None:
+        """
+        Declared check point: synchronise and raise if any kernel since the
+        last check skipped an out-of-range slot, page or block id.
+        """
+        self._flush()
+        bits = int(self._status.item())
+        if bits:
+            self._status.zero_()
+            what = []
+            if bits & _native.STATUS_BAD_SLOT:
+                what.append("slot_mapping entry outside the pool")
+            if bits & _native.STATUS_BAD_PAGE:
+                what.append("kv_indices entry outside [0, num_blocks)")
+            if bits & _native.STATUS_BAD_BLOCK:
+                what.append("block id outside [0, num_blocks)")
+            if bits & _native.STATUS_BAD_POSITION:
+                what.append("position outside the rotation table")
+            raise IndexError("device kernels skipped invalid ids: " + "; ".join(what))
+
+    def copy_block(self, src: int, dst: int) -> None:
+        """Duplicate one block's KV in every layer (copy-on-write)."""
+        if not (0 <= src < self.num_blocks and 0 <= dst < self.num_blocks):
+            raise IndexError(f"copy_block({src} -> {dst}) outside [0, {self.num_blocks})")
+        if src == dst:
+            return
+        self.copy_blocks([src], [dst])
+
+    def copy_blocks(self, src, dst) -> None:
+        """
+        Batched ``copy_block``: one launch for every (src, dst) pair, every
+        layer, K and V. Destinations must be distinct and must not appear among
+        the sources (so the result cannot depend on the order of the pairs).
+        """
+        ids = copy_ids(src, dst, self.num_blocks)
+        n = ids.shape[0] // 2
+        if n == 0:
+            return
+        self._flush()
+        # pinned, so the upload queues on the stream without a host wait
+        ids = ids.pin_memory().to(self.device, non_blocking=True)
+        with self._on_device():
+            self._launch_copy(self._pool.data_ptr(), self._plane_bytes, self._block_bytes, ids, n)
+            if self._bounds is not None:
+                row = self._block_bytes // self.block_size
+                self._launch_copy(self._bounds.data_ptr(), self.num_blocks * row, row, ids, n)
+
+    def _launch_copy(self, pool: int, plane: int, block: int, ids: torch.Tensor, n: int) -> None:
+        rc = self._lib.pkv_copy_blocks(pool, self.num_layers, plane, block, self.num_blocks,
+                                       ids.data_ptr(), ids.data_ptr() + 4 * n, n,
+                                       self._status.data_ptr(), _current_stream(self.device))
+        _native.check(rc, "copy_blocks")
+
+    def _token_rows(self, x: torch.Tensor) -> torch.Tensor:
+        """x in the pool dtype on this device, heads contiguous in each token's
+        row, rows any distance apart."""
+        if x.dtype is self.dtype and x.get_device() == self.device.index:
+            _, head, one = x.stride()
+            if one == 1 and head == self.head_dim:
+                return x
+        return x.to(device=self.device, dtype=self.dtype).contiguous()
+
+    def _on_device(self):
+        """Launches go to this backend's device, whichever is current."""
+        if _current_device() == self.device.index:
+            return _HERE
+        return torch.cuda.device(self.device)
+
+    def _counted_workspace(self, need: int, n: int) -> torch.Tensor:
+        """A workspace whose arrival counters (at its front) are zero."""
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        if need:
+            ws[:4 * n * self.n_kv_heads].zero_()
+        return ws
+
+    def _check_pages(self, kvl, indptr, last, n_pages: int) -> None:
+        """Every sequence's page list fits its length (ValueError naming the first
+        that does not)."""
+        ps = self.block_size
+        if int(indptr[0]) != 0 or int(indptr[-1]) != n_pages:
+            raise ValueError(f"kv_indptr spans [{int(indptr[0])}, {int(indptr[-1])}) but "
+                             f"kv_indices holds {n_pages} pages")
+        need = (kvl + ps - 1) // ps
+        bad = (kvl < 1) | (np.diff(indptr) != need) | (last != kvl - (need - 1) * ps)
+        if bad.any():
+            i = int(np.argmax(bad))
+            raise ValueError(f"seq {i}: kv_len={int(kvl[i])} with "
+                             f"{int(indptr[i + 1] - indptr[i])} pages of {ps} and "
+                             f"kv_last_page_len={int(last[i])} disagree")
+
+    def _refuse_capture(self, what: str) -> None:
+        """What a plan uploads while a graph is captured is there only once the
+        graph has run, but the plan stays for eager calls too."""
+        if _capturing():
+            raise RuntimeError(f"{what} has to plan this meta before a graph is captured: call "
+                               "it once with the meta (and the same arguments), then capture")
+
+    def _enter(self, p, slots=None) -> int:
+        """The current stream's handle, ordered behind the plan's last launch:
+        launches of one plan share its buffers. A plan that a graph captures, and
+        the slots of an append that it landed, stay as long as the backend does."""
+        stream = _current_stream(self.device)
+        if _capturing():
+            self._keep(p)
+            if slots is not None:
+                self._keep(slots)
+        elif p.stream != stream:
+            cur, ev = torch.cuda.current_stream(self.device), torch.cuda.Event()
+            ev.record(torch.cuda.ExternalStream(p.stream, device=self.device))
+            cur.wait_event(ev)
+            for t in p.buffers:     # not reused before this stream is done with them
+                t.record_stream(cur)
+            p.stream = stream
+        return stream
+
+    def _keep(self, read) -> None:
+        """What a graph being captured reads stays as long as the backend does."""
+        if not any(c is read for c in self._captured):
+            self._captured.append(read)
+
+    @staticmethod
+    def _host_index(meta: BatchMeta, with_slots: bool) -> tuple:
+        """The meta's index fields on the host: query_lens, cu_query_lens,
+        kv_lens, kv_indptr, kv_last_page_len, kv_indices and, if asked for,
+        slot_mapping (else None)."""
+        names = ["query_lens", "cu_query_lens", "kv_lens", "kv_indptr", "kv_last_page_len",
+                 "kv_indices"] + ["slot_mapping"] * with_slots
+        mirror = meta.host_arrays()
+        if mirror is not None:
+            # the assembler's own host arrays: no device read-back
+            out = [mirror[k] for k in names]
+        else:
+            # ONE device->host transfer for everything the host plan reads.
+            parts = [getattr(meta, k).reshape(-1).to(torch.int64) for k in names]
+            host = torch.cat(parts).cpu().numpy()
+            out = np.split(host, np.cumsum([t.shape[0] for t in parts])[:-1])
+        return (*out, *[None] * (not with_slots))
+
+    def _upload(self, a: np.ndarray) -> torch.Tensor:
+        """Host array to the device through a pinned ring buffer, uploaded by a
+        kernel on the current stream without a host wait (upload.py)."""
+        return uploader(self.device).array(a)
+
+
+class MI355XBackend(PagedPool):
     """Paged KV storage plus attention on gfx950 kernels."""
 
     _rows: _Rows | None = None
     _selected: _Selected | None = None
     _budgets: tuple[_Selected, ...] = ()   # the latest meta's plans, one a page budget
     _shared: _Shared | None = None
-    _bounds: torch.Tensor | None = None
 
     def __init__(self, num_layers: int, num_blocks: int, block_size: int, n_kv_heads: int,
                  n_heads: int, head_dim: int, device: str | torch.device = "cuda:0",
@@ -389,19 +565,10 @@ class MI355XBackend:
     def zeros_like_pool(self) -> torch.Tensor:
         return torch.zeros_like(self._k_pool[0])
 
-    def pool_bytes(self) -> int:
-        return self.num_layers * 2 * self._plane_bytes
-
-    def block_bytes(self) -> int:
-        return self.pool_bytes() // self.num_blocks
-
     def workspace_bytes(self) -> int:
         """Split-K partials and arrival counters; grows with the largest batch
         planned, not with the pool."""
         return self._workspace.numel()
-
-    def tokens_capacity(self) -> int:
-        return self.num_blocks * self.block_size
 
     @staticmethod
     def estimate_pool_bytes(num_layers: int, num_blocks: int, block_size: int,
@@ -411,20 +578,6 @@ class MI355XBackend:
         return num_layers * 2 * num_blocks * block_size * n_kv_heads * head_dim * elem
 
     # -- helpers -----------------------------------------------------------------
-
-    def _check_layer(self, layer_idx) -> None:
-        if layer_idx is None or not 0 <= layer_idx < self.num_layers:
-            raise ValueError(f"layer_idx {layer_idx} out of range [0, {self.num_layers})")
-
-    def _dev_i32(self, t: torch.Tensor) -> torch.Tensor:
-        return t.to(device=self.device, dtype=torch.int32).contiguous()
-
-    def _as_pool(self, x: torch.Tensor) -> torch.Tensor:
-        # (a tensor already in the pool dtype, contiguous and on this device is
-        # used as it is, without a conversion call per launch)
-        if x.dtype is self.dtype and x.get_device() == self.device.index and x.is_contiguous():
-            return x
-        return x.to(device=self.device, dtype=self.dtype).contiguous()
 
     def _set_workspace(self, ws: torch.Tensor) -> None:
         self._workspace = ws
@@ -436,61 +589,7 @@ class MI355XBackend:
         # is zero-filled)
         self._ws_zero = ws.numel()
 
-    def check_device_errors(self) -> None:
-        """
-        Declared check point: synchronise and raise if any kernel since the
-        last check skipped an out-of-range slot, page or block id.
-        """
-        self._flush()
-        bits = int(self._status.item())
-        if bits:
-            self._status.zero_()
-            what = []
-            if bits & _native.STATUS_BAD_SLOT:
-                what.append("slot_mapping entry outside the pool")
-            if bits & _native.STATUS_BAD_PAGE:
-                what.append("kv_indices entry outside [0, num_blocks)")
-            if bits & _native.STATUS_BAD_BLOCK:
-                what.append("block id outside [0, num_blocks)")
-            if bits & _native.STATUS_BAD_POSITION:
-                what.append("position outside the rotation table")
-            raise IndexError("device kernels skipped invalid ids: " + "; ".join(what))
-
     # -- write path -----------------------------------------------------------------
-
-    def copy_block(self, src: int, dst: int) -> None:
-        """Duplicate one block's KV in every layer (copy-on-write)."""
-        if not (0 <= src < self.num_blocks and 0 <= dst < self.num_blocks):
-            raise IndexError(f"copy_block({src} -> {dst}) outside [0, {self.num_blocks})")
-        if src == dst:
-            return
-        self.copy_blocks([src], [dst])
-
-    def copy_blocks(self, src, dst) -> None:
-        """
-        Batched ``copy_block``: one launch for every (src, dst) pair, every
-        layer, K and V. Destinations must be distinct and must not appear among
-        the sources (so the result cannot depend on the order of the pairs).
-        """
-        ids = copy_ids(src, dst, self.num_blocks)
-        n = ids.shape[0] // 2
-        if n == 0:
-            return
-        self._flush()
-        # pinned, so the upload queues on the stream without a host wait
-        ids = ids.pin_memory().to(self.device, non_blocking=True)
-        rc = self._lib.pkv_copy_blocks(self._pool.data_ptr(), self.num_layers,
-                                       self._plane_bytes, self._block_bytes, self.num_blocks,
-                                       ids.data_ptr(), ids.data_ptr() + 4 * n, n,
-                                       self._status.data_ptr(), _current_stream(self.device))
-        _native.check(rc, "copy_blocks")
-        if self._bounds is not None:
-            row = self._block_bytes // self.block_size
-            rc = self._lib.pkv_copy_blocks(self._bounds.data_ptr(), self.num_layers,
-                                           self.num_blocks * row, row, self.num_blocks,
-                                           ids.data_ptr(), ids.data_ptr() + 4 * n, n,
-                                           self._status.data_ptr(), _current_stream(self.device))
-            _native.check(rc, "copy_blocks (page bounds)")
 
     def refresh_page_bounds(self, blocks=None) -> None:
         """
@@ -695,21 +794,6 @@ class MI355XBackend:
             r.ptr = C.addressof(r.args)
         self._rows = r
         return r
-
-    def _token_rows(self, x: torch.Tensor) -> torch.Tensor:
-        """x in the pool dtype on this device, heads contiguous in each token's
-        row, rows any distance apart."""
-        if x.dtype is self.dtype and x.get_device() == self.device.index:
-            _, head, one = x.stride()
-            if one == 1 and head == self.head_dim:
-                return x
-        return x.to(device=self.device, dtype=self.dtype).contiguous()
-
-    def _on_device(self):
-        """Launches go to this backend's device, whichever is current."""
-        if _current_device() == self.device.index:
-            return _HERE
-        return torch.cuda.device(self.device)
 
     def _completed_pages(self, meta: BatchMeta) -> np.ndarray:
         """Pages whose last row this meta's append writes: the bounds of a page
@@ -971,13 +1055,6 @@ class MI355XBackend:
         p.ptr = C.addressof(p.args)
         self.n_plans += 1
 
-    def _counted_workspace(self, need: int, n: int) -> torch.Tensor:
-        """A workspace whose arrival counters (at its front) are zero."""
-        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-        if need:
-            ws[:4 * n * self.n_kv_heads].zero_()
-        return ws
-
     def attend_selected(self, q: torch.Tensor, layer_idx: int, scale: float, meta: BatchMeta,
                         pages: int, return_pages: bool = False):
         """
@@ -1138,51 +1215,6 @@ class MI355XBackend:
         return (plan[:needed.value], places[:places_needed.value], n_work.value, n_slots.value,
                 stride.value, need)
 
-    def _check_pages(self, kvl, indptr, last, n_pages: int) -> None:
-        """Every sequence's page list fits its length (ValueError naming the first
-        that does not)."""
-        ps = self.block_size
-        if int(indptr[0]) != 0 or int(indptr[-1]) != n_pages:
-            raise ValueError(f"kv_indptr spans [{int(indptr[0])}, {int(indptr[-1])}) but "
-                             f"kv_indices holds {n_pages} pages")
-        need = (kvl + ps - 1) // ps
-        bad = (kvl < 1) | (np.diff(indptr) != need) | (last != kvl - (need - 1) * ps)
-        if bad.any():
-            i = int(np.argmax(bad))
-            raise ValueError(f"seq {i}: kv_len={int(kvl[i])} with "
-                             f"{int(indptr[i + 1] - indptr[i])} pages of {ps} and "
-                             f"kv_last_page_len={int(last[i])} disagree")
-
-    def _refuse_capture(self, what: str) -> None:
-        """What a plan uploads while a graph is captured is there only once the
-        graph has run, but the plan stays for eager calls too."""
-        if _capturing():
-            raise RuntimeError(f"{what} has to plan this meta before a graph is captured: call "
-                               "it once with the meta (and the same arguments), then capture")
-
-    def _enter(self, p, slots=None) -> int:
-        """The current stream's handle, ordered behind the plan's last launch:
-        launches of one plan share its buffers. A plan that a graph captures, and
-        the slots of an append that it landed, stay as long as the backend does."""
-        stream = _current_stream(self.device)
-        if _capturing():
-            self._keep(p)
-            if slots is not None:
-                self._keep(slots)
-        elif p.stream != stream:
-            cur, ev = torch.cuda.current_stream(self.device), torch.cuda.Event()
-            ev.record(torch.cuda.ExternalStream(p.stream, device=self.device))
-            cur.wait_event(ev)
-            for t in p.buffers:     # not reused before this stream is done with them
-                t.record_stream(cur)
-            p.stream = stream
-        return stream
-
-    def _keep(self, read) -> None:
-        """What a graph being captured reads stays as long as the backend does."""
-        if not any(c is read for c in self._captured):
-            self._captured.append(read)
-
     # -- planning ---------------------------------------------------------------
 
     def _ensure_planned(self, meta: BatchMeta) -> _Plan:
@@ -1263,24 +1295,6 @@ class MI355XBackend:
         self._planned = p
         self.n_plans += 1
         return p
-
-    @staticmethod
-    def _host_index(meta: BatchMeta, with_slots: bool) -> tuple:
-        """The meta's index fields on the host: query_lens, cu_query_lens,
-        kv_lens, kv_indptr, kv_last_page_len, kv_indices and, if asked for,
-        slot_mapping (else None)."""
-        names = ["query_lens", "cu_query_lens", "kv_lens", "kv_indptr", "kv_last_page_len",
-                 "kv_indices"] + ["slot_mapping"] * with_slots
-        mirror = meta.host_arrays()
-        if mirror is not None:
-            # the assembler's own host arrays: no device read-back
-            out = [mirror[k] for k in names]
-        else:
-            # ONE device->host transfer for everything the host plan reads.
-            parts = [getattr(meta, k).reshape(-1).to(torch.int64) for k in names]
-            host = torch.cat(parts).cpu().numpy()
-            out = np.split(host, np.cumsum([t.shape[0] for t in parts])[:-1])
-        return (*out, *[None] * (not with_slots))
 
     def _describe(self, p: _Plan, ws: torch.Tensor | None = None) -> int:
         """Address of the plan's ``pkv_batch``: the arguments its launches share,
@@ -1375,11 +1389,6 @@ class MI355XBackend:
         plan[at + 7] = (plan[at + 7] & 1) | (rows[plan[at]] << 1)
         d.plan = self._upload(plan)
         return d
-
-    def _upload(self, a: np.ndarray) -> torch.Tensor:
-        """Host array to the device through a pinned ring buffer, uploaded by a
-        kernel on the current stream without a host wait (upload.py)."""
-        return uploader(self.device).array(a)
 
     def invalidate_plan(self) -> None:
         """Force the next ``attend`` to re-plan (and drop the cached meta)."""

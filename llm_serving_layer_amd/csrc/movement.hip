@@ -200,7 +200,7 @@ int pkv_upload_pinned(void* dst, const void* host, int64_t bytes, void* stream) 
   return PKV_OK;
 }
 
-int pkv_abi_version(void) { return 13; }
+int pkv_abi_version(void) { return 14; }
 
 const char* pkv_last_error(void) { return g_err.c_str(); }
 

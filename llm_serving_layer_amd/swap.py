@@ -56,7 +56,7 @@ class SwapHandle:
         self.n_kv_heads = n_kv_heads
         self.head_dim = head_dim
         self.released = False
-        self._host = host          # (2, L, nb, bs, Hkv, d) pinned
+        self._host = host          # (2, L, nb, bs, Hkv, d) pinned; 4 bits: (2, L, nb, bytes)
         self._done = done_event    # D2H completion
         self._staging = staging    # device staging, kept alive until the D2H lands
 
@@ -85,7 +85,7 @@ class SwapHandle:
 
 
 class KVSwapSpace:
-    """Swap space over an ``MI355XBackend``'s fused pool."""
+    """Swap space over an ``MI355XBackend``'s (or ``FourBitBackend``'s) fused pool."""
 
     def __init__(self, backend, max_bytes: int | None = None):
         for attr in ("k_pool", "v_pool", "num_layers", "block_size", "n_kv_heads",
@@ -103,7 +103,7 @@ class KVSwapSpace:
         self.last_swap_out_seconds = 0.0
         self._live: dict[int, SwapHandle] = {}
         self.device = backend.device
-        self.dtype = backend.dtype
+        self.dtype = backend._pool.dtype
         self.pinned = True
         # kernels (gather / scatter) on one side stream, host transfers on
         # another, so one sequence's transfer overlaps the next one's kernel
@@ -129,7 +129,7 @@ class KVSwapSpace:
 
     def _shape(self, nb: int) -> tuple:
         b = self.backend
-        return (2, b.num_layers, nb, b.block_size, b.n_kv_heads, b.head_dim)
+        return (2, b.num_layers, nb, *b._pool.shape[3:])   # (a block as the pool has it)
 
     def swap_out(self, request_id: str, blocks: SequenceBlocks) -> SwapHandle:
         """Copy every block of ``blocks`` to host; the caller frees afterwards."""
@@ -198,6 +198,10 @@ class KVSwapSpace:
         nb = handle.num_blocks
         if nb == 0:
             return
+        if tuple(handle._host.shape) != self._shape(nb) or handle._host.dtype != self.dtype:
+            raise RuntimeError(f"handle holds {handle._host.dtype} blocks of shape "
+                               f"{tuple(handle._host.shape)}, the pool's are {self.dtype} of "
+                               f"{self._shape(nb)}")
         if len(set(blocks.block_ids)) != nb:
             raise RuntimeError("swap_in target block ids must be distinct")
         b = self.backend

@@ -648,6 +648,37 @@ int pkv_scatter_blocks(void* pool_base, int32_t n_layers, int64_t plane_bytes,
 int pkv_argmax_rows(const void* logits, int64_t n_rows, int64_t vocab, int64_t row_stride,
                     int32_t dtype, int64_t* out_ids, void* stream);
 
+/*
+ * Verification of drafted tokens — no counterpart in the reference, which
+ * decodes greedily. Rows of logits (row r at element r * row_stride) belong to
+ * n_seqs sequences, rows cu_query_lens[i] .. cu_query_lens[i + 1] to sequence i
+ * (batch_indices[r]: row r's sequence); tokens[r] is the token that row r
+ * follows, so those behind a sequence's first are its drafts. Draft j, x =
+ * tokens[r + 1] at its row r = cu_query_lens[i] + j, stands if numbers[r] *
+ * q(x) < p(x): p the softmax of row r's logits / temperature, q row r - i of
+ * draft_probs ([n_rows - n_seqs, vocab], row stride probs_stride; NULL: 1 at x).
+ * accepted[i] is how many stand before the first that does not; ids[i] (width
+ * entries, at least a sequence's rows) holds them, one more token, and -1. The
+ * one more is drawn from max(p - q, 0) at the first row whose draft falls (p
+ * without x where draft_probs is NULL; p itself where nothing is left), or from
+ * the last row's p: the first token whose running sum of weights exceeds the
+ * last row's number times their sum. All of it as in 64 bits; weights below
+ * 2^-1000 of a row's largest count as 0. At temperatures of 0 or below a draft
+ * stands if it is the row's pkv_argmax_rows id, which is the token otherwise. In
+ * a row without a distribution (a NaN, +inf, or nothing but -inf) no draft
+ * stands, and that id is taken; a draft outside [0, vocab) does not stand.
+ * temperatures: one a sequence, or NULL: `temperature` for all. `workspace`:
+ * pkv_verify_workspace_bytes, aligned to 16, in any state; calls that overlap in
+ * time need one each.
+ */
+int64_t pkv_verify_workspace_bytes(int64_t n_rows, int64_t n_seqs, int64_t vocab, int32_t dtype);
+int pkv_verify_drafts(const void* logits, int64_t n_rows, int64_t vocab, int64_t row_stride,
+                      int32_t dtype, const int64_t* tokens, const int32_t* cu_query_lens,
+                      const int32_t* batch_indices, int64_t n_seqs, const float* numbers,
+                      const void* draft_probs, int64_t probs_stride, int32_t probs_dtype,
+                      const float* temperatures, float temperature, int64_t* ids, int64_t width,
+                      int64_t* accepted, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

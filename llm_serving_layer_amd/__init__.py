@@ -13,7 +13,7 @@ hand-written gfx950 kernels (include/pagedkv.h, csrc/):
 * ``rotary``    — RotaryTable (MI355XBackend.append_kv_rotated);
 * ``swap``      — KVSwapSpace / SwapHandle (preemption swap);
 * ``sizing``    — plan_kv_pool / KVPoolPlan (pool sizing for one MI355X).
-* ``sampling``  — greedy (argmax on the device), StepTimer, greedy_step (the
+* ``sampling``  — greedy (argmax on the device), verify_drafts, StepTimer, greedy_step (the
   scheduler step's forward-and-sample part, timed with HIP events).
 """
 

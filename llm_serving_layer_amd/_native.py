@@ -84,6 +84,9 @@ SIGNATURES = {
     "pkv_gather_blocks": (C.c_int, [_p, _i32, _i64, _i64, _i64, _p, _i32, _p, _p, _p]),
     "pkv_scatter_blocks": (C.c_int, [_p, _i32, _i64, _i64, _i64, _p, _i32, _p, _p, _p]),
     "pkv_argmax_rows": (C.c_int, [_p, _i64, _i64, _i64, _i32, _p, _p]),
+    "pkv_verify_workspace_bytes": (C.c_int64, [_i64, _i64, _i64, _i32]),
+    "pkv_verify_drafts": (C.c_int, [_p, _i64, _i64, _i64, _i32, _p, _p, _p, _i64, _p, _p, _i64,
+                                    _i32, _p, _f32, _p, _i64, _p, _p, _i64, _p]),
     "pkv_upload_pinned": (C.c_int, [_p, _p, _i64, _p]),
 }
 

@@ -12,6 +12,9 @@ device tensor (docs/ADR.md:954-989, ADR-023). Here:
 * ``StepTimer`` brackets a step with HIP events on torch's current stream
   (where the backend launches) and reads the elapsed time only at a declared
   synchronisation point;
+* ``verify_drafts(logits, tokens, meta, uniforms)`` checks a step's drafted
+  tokens against the target's logits and draws the token behind them (the
+  reference decodes greedily: no counterpart);
 * ``greedy_step`` is the forward-and-sample part of ``Scheduler.step``:
   metadata, tokens, forward, greedy pick, and one device-to-host copy of the
   picked ids, the step's only synchronisation.
@@ -23,9 +26,10 @@ import torch
 
 from . import _native
 from .assembly import ScheduledSeq, build_batch_meta, build_token_tensor
-from .backend import _DTYPES, _current_stream
+from .backend import _DTYPES, _capturing, _current_stream
+from .contract import BatchMeta
 
-__all__ = ["greedy", "StepTimer", "greedy_step"]
+__all__ = ["greedy", "verify_drafts", "StepTimer", "greedy_step"]
 
 
 def rows_for_kernel(logits: torch.Tensor) -> torch.Tensor:
@@ -70,6 +74,106 @@ def greedy(logits: torch.Tensor) -> torch.Tensor:
                              _current_stream(logits.device))
     _native.check(rc, "greedy argmax")
     return out
+
+
+def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, meta: BatchMeta,
+                  uniforms: torch.Tensor, *, draft_probs: torch.Tensor | None = None,
+                  temperature=1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """
+    Verify a step's drafted tokens: each sequence of ``meta`` contributes its
+    last accepted token and its drafts (none or more), ``tokens`` (``(T,)``
+    int64, as ``build_token_tensor`` gives them) are the step's tokens and
+    ``logits`` (``(T, vocab)`` f16, bf16 or f32) the target's for what follows
+    each. Draft x behind row r stands if ``uniforms[r] * q(x) < p(x)``: p the
+    softmax of the row over ``temperature`` (a number, or a float32 tensor of one
+    a sequence), q the drafting distribution (``draft_probs``, ``(T - n_seqs,
+    vocab)``, a row a draft in order; None: 1 at the draft). The first that does
+    not stand ends a sequence's run and is replaced by a token drawn from
+    ``max(p - q, 0)`` (p where that is nothing); behind a run that stands whole
+    one is drawn from the last row's p. Drawn is the first token whose running
+    sum of weights exceeds the sequence's last number times their sum, so the
+    ``(T,)`` float32 ``uniforms`` in [0, 1) serve all decisions once each.
+
+    Returns ``(ids, accepted)``, int64: per sequence the drafts that stand, one
+    more token, -1 behind it (``(n_seqs, max(query_lens))``), and how many stand.
+
+    Decisions are those of 64-bit arithmetic. At a temperature of 0 or below a
+    draft stands if it is the row's ``greedy`` id, which is taken otherwise; a
+    row without a distribution (a NaN, +inf, nothing but -inf) lets no draft
+    stand and gives its ``greedy`` id; a draft outside [0, vocab) falls.
+    Asynchronous on torch's current stream; every call has a workspace of its
+    own, so calls may overlap and be captured. A meta without host arrays is read
+    back from the device (not in a capture).
+    """
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be (n_tokens, vocab), got shape {tuple(logits.shape)}")
+    if logits.device.type != "cuda":
+        raise ValueError(f"logits must be on the GPU, got {logits.device}")
+    if logits.dtype not in _DTYPES:
+        raise ValueError(f"logits dtype {logits.dtype} is not float16, bfloat16 or float32")
+    dev, (rows, vocab), n = logits.device, logits.shape, meta.n_seqs
+    if vocab == 0:
+        raise ValueError("verify_drafts of empty rows: vocab is 0")
+    if meta.n_tokens != rows:
+        raise ValueError(f"meta describes {meta.n_tokens} tokens but logits has {rows} rows")
+    if n == 0 or rows < n:
+        raise ValueError(f"verify_drafts needs a row a sequence, got {rows} for {n}")
+    for name, x, dtype in (("tokens", tokens, torch.int64), ("uniforms", uniforms, torch.float32)):
+        if x.shape != (rows,) or x.dtype is not dtype or x.device != dev:
+            raise ValueError(f"{name} must be ({rows},) {dtype} on {dev}, got "
+                             f"{tuple(x.shape)} {x.dtype} on {x.device}")
+    if draft_probs is not None:
+        if draft_probs.shape != (rows - n, vocab):
+            raise ValueError(f"draft_probs has shape {tuple(draft_probs.shape)}, expected "
+                             f"({rows - n}, {vocab}): one row a draft")
+        if draft_probs.dtype not in _DTYPES or draft_probs.device != dev:
+            raise ValueError(f"draft_probs must be float16, bfloat16 or float32 on {dev}, got "
+                             f"{draft_probs.dtype} on {draft_probs.device}")
+        draft_probs = rows_for_kernel(draft_probs)
+        if rows == n:
+            draft_probs = None
+    temps = None
+    if isinstance(temperature, torch.Tensor):
+        if (temperature.shape != (n,) or temperature.dtype is not torch.float32
+                or temperature.device != dev):
+            raise ValueError(f"temperature must be a number or ({n},) float32 on {dev}, got "
+                             f"{tuple(temperature.shape)} {temperature.dtype} on "
+                             f"{temperature.device}")
+        temps, temperature = temperature.contiguous(), 1.0
+    elif not 0.0 <= float(temperature) < float("inf"):
+        raise ValueError(f"temperature must be finite and not negative, got {temperature}")
+    arrays = meta.host_arrays()
+    if arrays is not None:
+        lens = arrays["query_lens"]
+    elif _capturing():
+        raise RuntimeError("verify_drafts reads a meta without host arrays from the device: not "
+                           "while a graph is captured")
+    else:
+        lens = meta.query_lens.cpu().numpy()
+    if int(lens.min()) < 1 or int(lens.sum()) != rows:
+        raise ValueError(f"query_lens ({int(lens.min())} at least, {int(lens.sum())} in all) do "
+                         f"not make up {rows} rows")
+    width = int(lens.max())
+    logits = rows_for_kernel(logits)
+    tokens, uniforms = tokens.contiguous(), uniforms.contiguous()
+    cu, owner = (t.to(device=dev, dtype=torch.int32).contiguous()
+                 for t in (meta.cu_query_lens, meta.batch_indices))
+    ids = torch.empty((n, width), dtype=torch.int64, device=dev)
+    accepted = torch.empty(n, dtype=torch.int64, device=dev)
+    lib, code = _native.load(), _DTYPES[logits.dtype]
+    ws = torch.empty(lib.pkv_verify_workspace_bytes(rows, n, vocab, code), dtype=torch.uint8,
+                     device=dev)
+    with torch.cuda.device(dev):
+        rc = lib.pkv_verify_drafts(
+            logits.data_ptr(), rows, vocab, logits.stride(0) if rows > 1 else vocab, code,
+            tokens.data_ptr(), cu.data_ptr(), owner.data_ptr(), n, uniforms.data_ptr(),
+            None if draft_probs is None else draft_probs.data_ptr(),
+            vocab if draft_probs is None or rows - n < 2 else draft_probs.stride(0),
+            0 if draft_probs is None else _DTYPES[draft_probs.dtype],
+            None if temps is None else temps.data_ptr(), float(temperature), ids.data_ptr(),
+            width, accepted.data_ptr(), ws.data_ptr(), ws.numel(), _current_stream(dev))
+    _native.check(rc, "verify_drafts")
+    return ids, accepted
 
 
 class StepTimer:

@@ -143,7 +143,7 @@ class FourBit(C.Structure):
                                     "batch_indices", "items", "workspace", "status_word")],
                 *[(n, _i32) for n in ("n_seqs", "n_tokens", "n_heads", "n_kv_heads", "head_dim",
                                       "page_size", "dtype", "n_few", "n_wide", "few_rows",
-                                      "part_rows", "n_slots")]]
+                                      "few_waves", "part_rows", "n_slots")]]
 
 
 _LIB = None

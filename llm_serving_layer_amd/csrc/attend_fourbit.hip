@@ -49,27 +49,44 @@ int run_4bit_any(const pkv_4bit& b, const void* q, void* out, const void* k_pool
                  const void* v_pool, float scale, hipStream_t s);
 
 constexpr int kTile = 64;          // keys
-constexpr int kPieceInts = 8;      // {seq, first token, tokens, tile, tiles, slot | -1, slot 0, pieces}
-constexpr int kWaves = 4;
+// A piece: {first token's row in q, tokens, its position, kv_len, first page in
+// kv_indices, pages, tile, tiles, partial slot | -1, slot 0, pieces, sequence}
+constexpr int kPieceInts = 12;
+
+// Workgroups a compute unit that pieces are made for: four waves for few rows, one
+// wave for few rows, wide rows; the least tiles of a one-wave piece; and from how
+// many rows a compute unit on they are.
+constexpr int kFewResident = 4, kOneResident = 16, kWideResident = 2, kOneLeast = 4,
+              kOneWaveRows = 8;
+
+// Query rows of a piece, and pieces of a cut one at most, four waves and one (what
+// the merge's LDS holds the weights of).
+constexpr int kFewRows = 16, kWideRows = 32, kMostPieces = 128, kMostPieces1 = 32;
 
 struct Attend4 {
   const void* q;
   void* out;
   const unsigned char *kpool, *vpool;
-  const int32_t *items, *cu_q, *indptr, *indices, *kv_lens;
+  const int32_t *items, *indices;
   int32_t* counters;
   float *part_o, *part_ml;
   int32_t* status;
   int64_t num_blocks, block;
   int32_t n_items, n_kv, groups, head_bytes, pairs, shift, part_rows;
+  uint32_t per_group;                // 2^16 / groups, rounded up: r / groups below 64 rows
   float scale_log2;
 };
 
-// Per wave: the steps and zeros of a tile's K and V ([K | V][group][key]).
-template <int D> constexpr int kPairInts = 2 * (D / 64) * kTile;
+// Floats per wave for a tile's steps, zeros of K, steps and middles of V
+// ([4][group][key]).
+template <int D> constexpr int kPairFloats = 4 * (D / 64) * kTile;
 
-template <typename T, int D, int RT, int NCL>
-__global__ __launch_bounds__(64 * kWaves) void attend_4bit_kernel(Attend4 a) {
+// Waves a SIMD the kernel is compiled for.
+template <int D, int RT> constexpr int kSimdWaves = RT == 2 ? 2 : D == 64 ? 4 : 2;
+
+// WPP: waves of a piece's workgroup.
+template <typename T, int D, int RT, int NCL, int WPP>
+__global__ __launch_bounds__(64 * WPP, (kSimdWaves<D, RT>)) void attend_4bit_kernel(Attend4 a) {
   constexpr int NG = D / 64;         // groups
   constexpr int W = D / 32;          // words of codes a lane takes of a unit
   constexpr int NT = D / 16;         // output tiles of 16 dims
@@ -78,10 +95,14 @@ __global__ __launch_bounds__(64 * kWaves) void attend_4bit_kernel(Attend4 a) {
   constexpr int ROWS = RT * 16;      // columns of S^T
   constexpr int OROWS = NCL > 1 ? RC : ROWS;
   constexpr int OP = D + 4;          // floats of a row of the merge's LDS
+  constexpr int NTH = 64 * WPP;
   static_assert(RT == 1 || NCL == 1, "classes are for few rows");
-  __shared__ __align__(16) uint32_t pair_lds[kWaves * kPairInts<D>];
-  __shared__ __align__(16) float o_lds[kWaves * ROWS * OP];
-  __shared__ float m_lds[kWaves * ROWS], l_lds[kWaves * ROWS];
+  static_assert(kPairFloats<D> * WPP >= 4 * NTH &&
+                    OP * WPP >= (WPP == 1 ? kMostPieces1 : kMostPieces),
+                "the merge reuses the LDS");
+  __shared__ __align__(16) float pair_lds[WPP * kPairFloats<D>];
+  __shared__ __align__(16) float o_lds[WPP * ROWS * OP];
+  __shared__ float m_lds[WPP * ROWS], l_lds[WPP * ROWS];
   __shared__ int arrived;
 
   // Eight XCDs take workgroups in turn; a piece's heads go to one of them, where
@@ -90,17 +111,69 @@ __global__ __launch_bounds__(64 * kWaves) void attend_4bit_kernel(Attend4 a) {
   const int item = (y / a.n_kv) * 8 + x, h = y % a.n_kv;
   if (item >= a.n_items) return;
   const int32_t* it = a.items + (int64_t)item * kPieceInts;
-  const int seq = it[0], qs = it[1], qn = it[2], tile0 = it[3], n_tiles = it[4], slot = it[5];
-  const int q0 = a.cu_q[seq], q_len = a.cu_q[seq + 1] - q0;
-  const int kv_len = a.kv_lens[seq], pbase = a.indptr[seq];
-  const int n_pages = a.indptr[seq + 1] - pbase;
-  const int base_pos = kv_len - q_len + qs;      // the piece's first token's position
+  const int q0 = it[0], qn = it[1], base_pos = it[2], kv_len = it[3], pbase = it[4],
+            n_pages = it[5], tile0 = it[6], n_tiles = it[7], slot = it[8];
   const int G = a.groups, Hq = a.n_kv * G;
   const int tid = threadIdx.x;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = WPP == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, g = lane >> 4, n = lane & 15;
   const int cls = NCL > 1 ? n / RC : 0;
 
+  // The tile being computed and the next one share registers: K's are loaded again
+  // once its products are through, V's likewise, so that a tile's K is on its way
+  // during the softmax and V's products of the one before, its V during the rest.
+  uint32_t kc[4][W], vc[4][W];       // codes
+  uint32_t kw[NG], vw[NG];           // the words of key `lane`
+  const int shift = a.shift, mask = (1 << shift) - 1;    // units of a page
+  auto load_id = [&](int t) {      // the page of lane group g's unit of tile t
+    return a.indices[pbase + min((4 * t + g) >> shift, n_pages - 1)];
+  };
+  constexpr uint32_t unit_bytes = 8 * D;
+  const uint32_t k_off = h * a.head_bytes + n * (D / 2) + g * (D / 8);
+  const uint32_t v_off = h * a.head_bytes + lane * (D / 8);
+  const int ps = 16 << shift;
+  typedef uint32_t Words __attribute__((ext_vector_type(W)));
+  int64_t at[4];                     // where the units of the tile being loaded begin
+  auto codes = [&](uint32_t (&to)[4][W], const unsigned char* pool, uint32_t off) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      // (a scalar base and a lane's 32-bit offset)
+      const Words x = __builtin_nontemporal_load(reinterpret_cast<const Words*>(pool + at[u] + off));
+#pragma unroll
+      for (int w = 0; w < W; ++w) to[u][w] = x[w];
+    }
+  };
+  auto load_k = [&](int t, int id) {
+    const int ok = (uint64_t)(int64_t)id < (uint64_t)a.num_blocks ? id : 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      at[u] = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(ok, 16 * u) * (uint32_t)a.block +
+              ((4 * t + u) & mask) * unit_bytes;
+    const uint64_t mine = (uint64_t)(uint32_t)ok * (uint32_t)a.block +
+                          (uint32_t)(a.pairs + ((h * NG) * ps + ((4 * t + g) & mask) * 16 + n) * 4);
+#pragma unroll
+    for (int q = 0; q < NG; ++q) {
+      kw[q] = __builtin_nontemporal_load(
+          reinterpret_cast<const uint32_t*>(a.kpool + mine + q * ps * 4));
+      vw[q] = __builtin_nontemporal_load(
+          reinterpret_cast<const uint32_t*>(a.vpool + mine + q * ps * 4));
+    }
+    codes(kc, a.kpool, k_off);
+  };
+  auto load_v = [&]() { codes(vc, a.vpool, v_off); };   // of load_k's tile
+
+  // the first tile goes out before the queries are read
+  const int end = tile0 + n_tiles;
+  int t = tile0 + wave;
+  int id = 0, id_next = 0;           // of tiles t, t + WPP
+  if (t < end) {
+    id = load_id(t);
+    load_k(t, id);
+    load_v();
+    id_next = load_id(t + WPP);
+  }
+
+  auto token_of = [&](int r) { return (int)((uint32_t)r * a.per_group >> 16); };   // r / G
   // Queries: scaled by a power of two that brings the row's largest element to
   // [1024, 2048), exactly (bf16 too, but for elements 2^-35 of the largest), and
   // turned over for a negative scale; in the order of an operand's codes, where
@@ -111,26 +184,27 @@ __global__ __launch_bounds__(64 * kWaves) void attend_4bit_kernel(Attend4 a) {
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int r = NCL > 1 ? n % RC : rt * 16 + n;
-    const int tok = r / G;
+    const int tok = token_of(r);
     const bool valid = tok < qn;
+    const int head = valid ? r - tok * G : 0;
     qpos[rt] = base_pos + (valid ? tok : qn - 1);
     typedef T TV __attribute__((ext_vector_type(8)));
     const T* row = reinterpret_cast<const T*>(a.q) +
-                   ((int64_t)(q0 + qs + (valid ? tok : 0)) * Hq + h * G + r % G) * D + 16 * g;
+                   ((int64_t)(q0 + (valid ? tok : 0)) * Hq + h * G + head) * D + 16 * g;
     float v[2 * NG][8], mx = 0.f;
 #pragma unroll
     for (int w = 0; w < 2 * NG; ++w) {
       const TV t = *reinterpret_cast<const TV*>(row + (w >> 1) * 64 + (w & 1) * 8);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        v[w][i] = valid ? Elem<T>::to_f(t[i]) : 0.f;
+        v[w][i] = Elem<T>::to_f(t[i]);
         mx = fmaxf(mx, __builtin_fabsf(v[w][i]));
       }
     }
     mx = max_x32(max_x16(mx));
     const bool scaled = mx > 0.f && mx < INFINITY;
     const int k = scaled ? 11 - __builtin_amdgcn_frexp_expf(mx) : 0;
-    const float sign = a.scale_log2 < 0.f ? -1.f : 1.f;
+    const uint32_t turn = a.scale_log2 < 0.f ? 0x80008000u : 0u;
     // (a scale of 0: small enough to change nothing, and no 0 x inf at masks)
     f1[rt] = __builtin_amdgcn_ldexpf(__builtin_fabsf(a.scale_log2), 24 - k);
     f1[rt] = f1[rt] < 0x1p-120f ? 0x1p-120f : f1[rt];
@@ -139,72 +213,38 @@ __global__ __launch_bounds__(64 * kWaves) void attend_4bit_kernel(Attend4 a) {
       float sum = 0.f;
 #pragma unroll
       for (int w = 2 * q; w < 2 * q + 2; ++w) {
-        f16x8 op;
+        u32x4 op;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int e = (i >> 1) + 4 * (i & 1);       // elements 0 4 1 5 2 6 3 7
-          const bool up = (i >> 1) & 1;               // codes four bits up
-          op[i] = (_Float16)(__builtin_amdgcn_ldexpf(v[w][e], k) * sign * (up ? 0.0625f : 1.f));
-          sum += (float)op[i] * (up ? 16.f : 1.f);
+        for (int i = 0; i < 4; ++i) {                 // elements i and i + 4
+          const int down = i & 1 ? 4 : 0;             // their codes lie four bits up
+          const f16x2 two{(_Float16)__builtin_amdgcn_ldexpf(v[w][i], k - down),
+                          (_Float16)__builtin_amdgcn_ldexpf(v[w][i + 4], k - down)};
+          const f16x2 turned = __builtin_bit_cast(f16x2, __builtin_bit_cast(uint32_t, two) ^ turn);
+          sum = __builtin_fmaf((float)turned[0], (float)(1 << down), sum);
+          sum = __builtin_fmaf((float)turned[1], (float)(1 << down), sum);
+          op[i] = __builtin_bit_cast(uint32_t, turned);
         }
 #pragma unroll
-        for (int c = 0; c < NCL; ++c) qop[rt][c][w] = NCL == 1 || c == cls ? op : f16x8{};
+        for (int c = 0; c < NCL; ++c)
+          qop[rt][c][w] = __builtin_bit_cast(
+              f16x8, valid && (NCL == 1 || c == cls) ? op : u32x4{0u, 0u, 0u, 0u});
       }
-      qsum[rt][q] = sum_x32(sum_x16(sum)) * 0x1p-24f;
+      sum = sum_x32(sum_x16(sum)) * 0x1p-24f;
+      qsum[rt][q] = valid ? sum : 0.f;
     }
   }
 
-  // a tile on its way
-  struct Tile {
-    uint32_t k[4][W], v[4][W];
-    uint32_t kp[NG], vp[NG];
-    int id;
-  };
-  const int shift = a.shift, mask = (1 << shift) - 1;    // units of a page
-  auto load_id = [&](int t) {      // the page of lane group g's unit of tile t
-    return a.indices[pbase + min((4 * t + g) >> shift, n_pages - 1)];
-  };
-  const int unit_bytes = 8 * D;
-  const int k_off = h * a.head_bytes + n * (D / 2) + g * (D / 8);
-  const int v_off = h * a.head_bytes + lane * (D / 8);
-  const int ps = 16 << shift;
-  typedef uint32_t Words __attribute__((ext_vector_type(W)));
-  auto load = [&](Tile& x, int t, int id) {
-    x.id = id;
-    const int ok = (uint64_t)(int64_t)id < (uint64_t)a.num_blocks ? id : 0;
-    const int64_t mine = (int64_t)ok * a.block + a.pairs +
-                         ((h * NG) * ps + ((4 * t + g) & mask) * 16 + n) * 4;
-#pragma unroll
-    for (int q = 0; q < NG; ++q) {
-      x.kp[q] = __builtin_nontemporal_load(
-          reinterpret_cast<const uint32_t*>(a.kpool + mine + q * ps * 4));
-      x.vp[q] = __builtin_nontemporal_load(
-          reinterpret_cast<const uint32_t*>(a.vpool + mine + q * ps * 4));
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int64_t at = (int64_t)__builtin_amdgcn_readlane(ok, 16 * u) * a.block +
-                         ((4 * t + u) & mask) * unit_bytes;
-      const Words kw = __builtin_nontemporal_load(
-          reinterpret_cast<const Words*>(a.kpool + at + k_off));
-      const Words vw = __builtin_nontemporal_load(
-          reinterpret_cast<const Words*>(a.vpool + at + v_off));
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        x.k[u][w] = kw[w];
-        x.v[u][w] = vw[w];
-      }
-    }
-  };
-
-  f32x4 o[RT][NT];
+  f32x4 o[RT][NT], pr[RT][NG];
   float ref[RT], l[RT], zo[RT][NG];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) o[rt][i] = f32x4{};
 #pragma unroll
-    for (int q = 0; q < NG; ++q) zo[rt][q] = 0.f;
+    for (int q = 0; q < NG; ++q) {
+      zo[rt][q] = 0.f;
+      pr[rt][q] = f32x4{};
+    }
     ref[rt] = -INFINITY;
     l[rt] = 0.f;
   }
@@ -212,26 +252,29 @@ __global__ __launch_bounds__(64 * kWaves) void attend_4bit_kernel(Attend4 a) {
   int e = 0;
   float limit = 4096.f;              // 2^12 2^e
   uint32_t worst = 0;                // any page id out of range
-  uint32_t* const pw = pair_lds + wave * kPairInts<D>;
+  float* const pw = pair_lds + wave * kPairFloats<D>;
   const uint32_t LO = 0x000f000fu, UP = 0x00f000f0u;
 
-  auto compute = [&](Tile& x, int t) {
+  // Tile t. PART: some row does not see all of its keys; MORE: load the next one.
+  auto compute = [&](auto part, auto more) {
+    constexpr bool PART = decltype(part)::value, MORE = decltype(more)::value;
     // steps and zeros; none for keys past the end and for pages out of range,
     // which read as zeros
-    const bool bad = (uint64_t)(int64_t)x.id >= (uint64_t)a.num_blocks;
-    const bool live = kTile * t + lane < kv_len && !bad;
+    const bool bad = (uint64_t)(int64_t)id >= (uint64_t)a.num_blocks;
+    const bool live = (!PART || kTile * t + lane < kv_len) && !bad;
     worst |= bad;
+    uint32_t top = 0;
 #pragma unroll
     for (int q = 0; q < NG; ++q) {
-      x.kp[q] = live ? x.kp[q] : 0u;
-      x.vp[q] = live ? x.vp[q] : 0u;
-      pw[q * kTile + lane] = x.kp[q];
-      pw[(NG + q) * kTile + lane] = x.vp[q];
+      const uint32_t kp = live ? kw[q] : 0u, vp = live ? vw[q] : 0u;
+      top = max(top, vp);
+      const float step = pair_step(vp);
+      pw[q * kTile + lane] = pair_step(kp);
+      pw[(NG + q) * kTile + lane] = pair_zero(kp);
+      pw[(2 * NG + q) * kTile + lane] = step;
+      pw[(3 * NG + q) * kTile + lane] = __builtin_fmaf(7.5f, step, pair_zero(vp));
     }
     wave_lds_sync();
-    uint32_t top = x.vp[0];
-#pragma unroll
-    for (int q = 1; q < NG; ++q) top = max(top, x.vp[q]);
 
     f32x4 s[UPL][RT][NG];
 #pragma unroll
@@ -244,7 +287,7 @@ __global__ __launch_bounds__(64 * kWaves) void attend_4bit_kernel(Attend4 a) {
     for (int u = 0; u < 4; ++u) {
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        const uint32_t c = x.k[u][w];
+        const uint32_t c = kc[u][w];
         const f16x8 ka = __builtin_bit_cast(
             f16x8, u32x4{c & LO, c & UP, (c >> 8) & LO, (c >> 8) & UP});
 #pragma unroll
@@ -253,32 +296,33 @@ __global__ __launch_bounds__(64 * kWaves) void attend_4bit_kernel(Attend4 a) {
               ka, qop[rt][u % NCL][w], s[u / NCL][rt][w / 2], 0, 0, 0);
       }
     }
+    // (Nothing moves across the phases: the compiler would unpack all of a tile's
+    // codes ahead of their products, and run out of registers.)
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (MORE) load_k(t + WPP, id_next);
+    auto pairs = [&](int kind, int q, int i) {   // of the lane's four keys of unit i
+      return *reinterpret_cast<const f32x4*>(pw + (kind * NG + q) * kTile +
+                                             (cls + NCL * i) * 16 + 4 * g);
+    };
     // scores, in the row's unit (times f1: log2)
     float y[UPL][RT][4];
 #pragma unroll
     for (int i = 0; i < UPL; ++i) {
-      u32x4 kp[NG];
+      asm volatile("" ::: "memory");   // (reads no earlier: registers)
 #pragma unroll
-      for (int q = 0; q < NG; ++q)
-        kp[q] = *reinterpret_cast<const u32x4*>(pw + q * kTile + (cls + NCL * i) * 16 + 4 * g);
+      for (int q = 0; q < NG; ++q) {
+        const f32x4 step = pairs(0, q, i), zero = pairs(1, q, i);
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float v = 0.f;
-#pragma unroll
-          for (int q = 0; q < NG; ++q) {
-            const float z = pair_zero(kp[q][j]) * qsum[rt][q];
-            v = q ? v + z : z;
+          for (int j = 0; j < 4; ++j) {
+            const float z = q ? __builtin_fmaf(zero[j], qsum[rt][q], y[i][rt][j])
+                              : zero[j] * qsum[rt][q];
+            y[i][rt][j] = __builtin_fmaf(step[j], s[i][rt][q][j], z);
           }
-#pragma unroll
-          for (int q = 0; q < NG; ++q)
-            v = __builtin_fmaf(pair_step(kp[q][j]), s[i][rt][q][j], v);
-          y[i][rt][j] = v;
-        }
+      }
     }
-    // keys that a row does not see (also those past the end)
-    if (kTile * t + kTile - 1 > base_pos) {
+    if constexpr (PART) {            // (also keys past the end)
 #pragma unroll
       for (int i = 0; i < UPL; ++i)
 #pragma unroll
@@ -320,7 +364,10 @@ __global__ __launch_bounds__(64 * kWaves) void attend_4bit_kernel(Attend4 a) {
             ref[rt] += (float)(old - e);
             l[rt] *= f;
 #pragma unroll
-            for (int q = 0; q < NG; ++q) zo[rt][q] *= f;
+            for (int q = 0; q < NG; ++q) {
+              zo[rt][q] *= f;
+              pr[rt][q] *= f;
+            }
 #pragma unroll
             for (int i = 0; i < NT; ++i) o[rt][i] *= f;
           }
@@ -341,99 +388,104 @@ __global__ __launch_bounds__(64 * kWaves) void attend_4bit_kernel(Attend4 a) {
         ref[rt] = r;
         l[rt] *= alpha;
 #pragma unroll
-        for (int q = 0; q < NG; ++q) zo[rt][q] *= alpha;
+        for (int q = 0; q < NG; ++q) {
+          zo[rt][q] *= alpha;
+          pr[rt][q] *= alpha;
+        }
 #pragma unroll
         for (int i = 0; i < NT; ++i) o[rt][i] *= alpha;
         probs(rt, r == -INFINITY ? 0.f : r);   // (a row that has seen no key yet)
       }
     }
-    // p step (rounded to float16 for the matrix cores: 2^-12 of each at most, as
-    // for 16-bit pools) and the sums over p and p zero
+    // p step, rounded to float16 for the matrix cores, and the sum over p (zero +
+    // 7.5 step). With the sum of the rounded ones (a product with ones) taken off
+    // 7.5 times at the end, a rounding's error enters with c - 7.5, the value about
+    // the group's middle, as it would with 16-bit values; with c alone the outputs
+    // were off twice as far.
     u32x2 pk[UPL][RT][NG];
 #pragma unroll
-    for (int i = 0; i < UPL; ++i) {
-      u32x4 vp[NG];
+    for (int i = 0; i < UPL; ++i)
 #pragma unroll
-      for (int q = 0; q < NG; ++q)
-        vp[q] = *reinterpret_cast<const u32x4*>(pw + (NG + q) * kTile + (cls + NCL * i) * 16 +
-                                                4 * g);
+      for (int q = 0; q < NG; ++q) {
+        asm volatile("" ::: "memory");
+        const f32x4 step = pairs(2, q, i), mid = pairs(3, q, i);
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int q = 0; q < NG; ++q) {
-          float ps4[4];
+        for (int rt = 0; rt < RT; ++rt) {
+          float w[4], z = zo[rt][q];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            ps4[j] = p[i][rt][j] * pair_step(vp[q][j]);
+            const float pj = p[i][rt][j];
             // (a key that the row does not see may hold NaN)
-            if (kTile * t + kTile - 1 > base_pos && p[i][rt][j] == 0.f) {
-              ps4[j] = 0.f;
-            } else {
-              zo[rt][q] = __builtin_fmaf(p[i][rt][j], pair_zero(vp[q][j]), zo[rt][q]);
-            }
+            const bool none = PART && pj == 0.f;
+            w[j] = none ? 0.f : pj * step[j];
+            z = none ? z : __builtin_fmaf(pj, mid[j], z);
           }
-          const f16x2 a0{(_Float16)ps4[0], (_Float16)ps4[2]}, a1{(_Float16)ps4[1], (_Float16)ps4[3]};
+          zo[rt][q] = z;
+          const f16x2 a0{(_Float16)w[0], (_Float16)w[2]}, a1{(_Float16)w[1], (_Float16)w[3]};
           pk[i][rt][q] = u32x2{__builtin_bit_cast(uint32_t, a0), __builtin_bit_cast(uint32_t, a1)};
         }
-    }
+      }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) l[rt] += ls[rt];
     // O^T += V^T P^T, two units a product
+    const f16x8 ones = __builtin_bit_cast(
+        f16x8, u32x4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u});
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
+      __builtin_amdgcn_sched_barrier(0);
       const int ua = 2 * m, ub = 2 * m + 1;
-      u32x4 pb[RT][NG];
+      f16x8 pb[RT][NG];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int q = 0; q < NG; ++q) {
           const u32x2 pa = pk[ua / NCL][rt][q], pz = pk[ub / NCL][rt][q];
           const bool ina = NCL == 1 || cls == ua % NCL, inb = NCL == 1 || cls == ub % NCL;
-          pb[rt][q] = u32x4{ina ? pa[0] : 0u, ina ? pa[1] : 0u, inb ? pz[0] : 0u,
-                            inb ? pz[1] : 0u};
+          pb[rt][q] = __builtin_bit_cast(
+              f16x8, u32x4{ina ? pa[0] : 0u, ina ? pa[1] : 0u, inb ? pz[0] : 0u,
+                           inb ? pz[1] : 0u});
+          pr[rt][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pb[rt][q], pr[rt][q], 0, 0, 0);
         }
 #pragma unroll
       for (int b = 0; b < W; ++b) {
-        const uint32_t wa = x.v[ua][b], wb = x.v[ub][b];
+        const uint32_t wa = vc[ua][b], wb = vc[ub][b];
         const f16x8 lo = __builtin_bit_cast(
             f16x8, u32x4{wa & LO, (wa >> 8) & LO, wb & LO, (wb >> 8) & LO});
         const f16x8 up = __builtin_bit_cast(
             f16x8, u32x4{wa & UP, (wa >> 8) & UP, wb & UP, (wb >> 8) & UP});
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-          const f16x8 pv = __builtin_bit_cast(f16x8, pb[rt][b / 2]);
-          o[rt][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, pv, o[rt][2 * b], 0, 0, 0);
+          o[rt][2 * b] =
+              __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, pb[rt][b / 2], o[rt][2 * b], 0, 0, 0);
           o[rt][2 * b + 1] =
-              __builtin_amdgcn_mfma_f32_16x16x32_f16(up, pv, o[rt][2 * b + 1], 0, 0, 0);
+              __builtin_amdgcn_mfma_f32_16x16x32_f16(up, pb[rt][b / 2], o[rt][2 * b + 1], 0, 0, 0);
         }
       }
     }
-    // (the next tile's words may overwrite these)
-    wave_lds_sync();
+    t += WPP;
+    if constexpr (MORE) {
+      load_v();
+      id = id_next;
+      id_next = load_id(t + WPP);
+    }
+    wave_lds_sync();                 // (the next tile's words overwrite this one's)
   };
-
-  const int end = tile0 + n_tiles;
-  int t = tile0 + wave;
-  if (t < end) {
-    Tile xa, xb;
-    load(xa, t, load_id(t));
-    int id = load_id(t + kWaves);
-    for (;;) {
-      load(xb, t + kWaves, id);
-      id = load_id(t + 2 * kWaves);
-      compute(xa, t);
-      t += kWaves;
-      if (t >= end) break;
-      load(xa, t + kWaves, id);
-      id = load_id(t + 2 * kWaves);
-      compute(xb, t);
-      t += kWaves;
-      if (t >= end) break;
+  // Whole tiles, then those that some row sees in part, the piece's last ones. (Two
+  // loops: with both kinds in one the compiler kept twice the registers.)
+  const int whole = min(end, (base_pos + 1) / kTile);
+  while (t < whole) compute(std::false_type{}, std::true_type{});
+  while (t < end) {
+    compute(std::true_type{}, std::false_type{});
+    if (t < end) {
+      id = id_next;
+      load_k(t, id);
+      load_v();
+      id_next = load_id(t + WPP);
     }
   }
   if (__builtin_amdgcn_ballot_w64(worst) && lane == 0) flag(a.status, PKV_STATUS_BAD_PAGE);
 
-  // the wave's rows: sums over its lane groups, codes' powers of two, zeros
+  // the wave's rows: sums over its lane groups, codes' powers of two, middles
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const float lr = sum_x32(sum_x16(l[rt]));
@@ -444,7 +496,8 @@ __global__ __launch_bounds__(64 * kWaves) void attend_4bit_kernel(Attend4 a) {
     }
     float z[NG];
 #pragma unroll
-    for (int q = 0; q < NG; ++q) z[q] = sum_x32(sum_x16(zo[rt][q]));
+    for (int q = 0; q < NG; ++q)
+      z[q] = __builtin_fmaf(-7.5f, pr[rt][q][0], sum_x32(sum_x16(zo[rt][q])));
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const float f = i & 1 ? 0x1p20f : 0x1p24f;
@@ -457,20 +510,20 @@ __global__ __launch_bounds__(64 * kWaves) void attend_4bit_kernel(Attend4 a) {
   __syncthreads();
 
   // merge the waves' (and classes') rows: set k of row r
-  constexpr int SETS = kWaves * NCL, CH = D / 4;
+  constexpr int SETS = WPP * NCL, CH = D / 4;
   const int64_t part = ((int64_t)slot * a.n_kv + h) * a.part_rows;
   auto store = [&](int r, int c4, f32x4 v, float lr) {
-    const int tok = r / G;
+    const int tok = token_of(r);
     typedef T TV4 __attribute__((ext_vector_type(4)));
     TV4 w;
     const float inv = 1.f / lr;
 #pragma unroll
     for (int j = 0; j < 4; ++j) w[j] = (T)(v[j] * inv);
     *reinterpret_cast<TV4*>(reinterpret_cast<T*>(a.out) +
-                            ((int64_t)(q0 + qs + tok) * Hq + h * G + r % G) * D + 4 * c4) = w;
+                            ((int64_t)(q0 + tok) * Hq + h * G + r - tok * G) * D + 4 * c4) = w;
   };
   const int live_rows = min(OROWS, qn * G);
-  for (int i = tid; i < live_rows * CH; i += 64 * kWaves) {
+  for (int i = tid; i < live_rows * CH; i += NTH) {
     const int r = i / CH, c4 = i % CH;
     auto at = [&](int k) { return NCL > 1 ? (k / NCL) * ROWS + (k % NCL) * RC + r : k * ROWS + r; };
     float m = -INFINITY;
@@ -481,10 +534,10 @@ __global__ __launch_bounds__(64 * kWaves) void attend_4bit_kernel(Attend4 a) {
 #pragma unroll
     for (int k = 0; k < SETS; ++k) {
       const float mk = m_lds[at(k)];
+      // (a set that saw no key holds zeros)
       const float w = mk == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mk - m);
-      if (w == 0.f) continue;            // (a set that saw no key holds nothing)
       v += *reinterpret_cast<const f32x4*>(o_lds + at(k) * OP + 4 * c4) * w;
-      lr += l_lds[at(k)] * w;
+      lr = __builtin_fmaf(l_lds[at(k)], w, lr);
     }
     if (slot < 0) {
       store(r, c4, v, lr);
@@ -505,33 +558,70 @@ __global__ __launch_bounds__(64 * kWaves) void attend_4bit_kernel(Attend4 a) {
   // the last merges, by loads from there. Counters are zero again afterwards.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  const int slot0 = it[6], pieces = it[7];
+  const int slot0 = it[9], pieces = it[10];
   int32_t* cnt = a.counters + (int64_t)slot0 * a.n_kv + h;
   if (tid == 0) arrived = __hip_atomic_fetch_add(cnt, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
   if (arrived != pieces - 1) return;
   if (tid == 0) __hip_atomic_store(cnt, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  for (int i = tid; i < live_rows * CH; i += 64 * kWaves) {
-    const int r = i / CH, c4 = i % CH;
+  // Every piece's (m, l) and from them its weight: a wave a row, a lane a piece.
+  float* const weights = o_lds;      // [row][piece]
+  const int apart = a.n_kv * a.part_rows;   // rows between two pieces' of this head
+  const int64_t row0 = ((int64_t)slot0 * a.n_kv + h) * a.part_rows;
+  const int reach = (pieces - 1) * apart + live_rows;
+  const __amdgpu_buffer_rsrc_t mls = ws_rsrc(a.part_ml + row0 * 2, reach * 8);
+  const __amdgpu_buffer_rsrc_t os = ws_rsrc(a.part_o + row0 * D, reach * D * 4);
+  constexpr int PL = (WPP == 1 ? kMostPieces1 : kMostPieces) <= 64 ? 1 : 2;
+  for (int r = wave; r < live_rows; r += WPP) {
+    f32x2 ml[PL];
     float m = -INFINITY, lr = 0.f;
-    f32x4 v{};
-    for (int k = 0; k < pieces; ++k) {
-      const int64_t pk = ((int64_t)(slot0 + k) * a.n_kv + h) * a.part_rows;
-      const f32x2 ml = __builtin_bit_cast(
-          f32x2, __builtin_amdgcn_raw_buffer_load_b64(
-                     ws_rsrc(a.part_ml + pk * 2, a.part_rows * 8), r * 8, 0, kSc1));
-      const f32x4 ov = __builtin_bit_cast(
-          f32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                     ws_rsrc(a.part_o + pk * D, a.part_rows * D * 4), (r * D + 4 * c4) * 4, 0,
-                     kSc1));
-      if (ml[0] == -INFINITY) continue;
-      const float mn = fmaxf(m, ml[0]);
-      const float wa = __builtin_amdgcn_exp2f(m - mn), wb = __builtin_amdgcn_exp2f(ml[0] - mn);
-      v = v * wa + ov * wb;
-      lr = lr * wa + ml[1] * wb;
-      m = mn;
+#pragma unroll
+    for (int i = 0; i < PL; ++i) {
+      const int k = lane + 64 * i;
+      ml[i] = __builtin_bit_cast(
+          f32x2, __builtin_amdgcn_raw_buffer_load_b64(mls, (k * apart + r) * 8, 0, kSc1));
+      if (k >= pieces) ml[i] = f32x2{-INFINITY, 0.f};
+      m = fmaxf(m, ml[i][0]);
     }
-    store(r, c4, v, lr);
+    m = wave_max(m);
+#pragma unroll
+    for (int i = 0; i < PL; ++i) {
+      const float w = ml[i][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[i][0] - m);
+      lr = __builtin_fmaf(ml[i][1], w, lr);
+      if (lane + 64 * i < pieces) weights[r * pieces + lane + 64 * i] = w;
+    }
+    lr = wave_sum(lr);
+    if (lane == 0) l_lds[r] = lr;
+  }
+  __syncthreads();
+  // Where there are fewer (row, 4 dims) than threads, several threads share one,
+  // each some of the pieces.
+  const int units = live_rows * CH, share = units >= NTH ? 1 : NTH / units;
+  f32x4* const red = reinterpret_cast<f32x4*>(pair_lds);
+  for (int i0 = 0; i0 < units; i0 += NTH) {
+    const int i = share > 1 ? tid % units : i0 + tid;
+    const int first = share > 1 ? tid / units : 0;
+    const int r = i / CH, c4 = i % CH;
+    f32x4 v{};
+    if (i < units && first < share) {
+#pragma unroll 8
+      for (int k = first; k < pieces; k += share) {
+        const f32x4 ov = __builtin_bit_cast(
+            f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                       os, ((k * apart + r) * D + 4 * c4) * 4, 0, kSc1));
+        v += ov * weights[r * pieces + k];
+      }
+    }
+    if (share > 1) {
+      red[tid] = v;
+      __syncthreads();
+      if (first == 0) {
+        for (int k = 1; k < share; ++k) v += red[tid + k * units];
+        store(r, c4, v, l_lds[r]);
+      }
+    } else if (i < units) {
+      store(r, c4, v, l_lds[r]);
+    }
   }
 }
 
@@ -554,25 +644,29 @@ using namespace pkv;
 extern "C" {
 
 static int plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr, const int32_t* kv_lens,
-                  const int32_t* kv_last_page_len, int32_t n_seqs, int32_t n_heads,
-                  int32_t n_kv_heads, int32_t head_dim, int32_t page_size, int32_t dtype,
-                  int32_t workgroups, int32_t* items, int64_t capacity, int64_t* needed,
-                  pkv_4bit* plan) {
+                     const int32_t* kv_last_page_len, int32_t n_seqs, int32_t n_heads,
+                     int32_t n_kv_heads, int32_t head_dim, int32_t page_size, int32_t dtype,
+                     int32_t compute_units, int32_t* items, int64_t capacity, int64_t* needed,
+                     pkv_4bit* plan) {
   const int rc0 = check_4bit(n_kv_heads, head_dim, page_size);
   if (rc0) return rc0;
-  if (n_seqs <= 0 || n_heads <= 0 || n_heads % n_kv_heads || workgroups <= 0)
-    return fail(PKV_ERR_INVALID, "n_seqs, n_heads and workgroups must be positive, n_heads a "
+  if (n_seqs <= 0 || n_heads <= 0 || n_heads % n_kv_heads || compute_units <= 0)
+    return fail(PKV_ERR_INVALID, "n_seqs, n_heads and compute_units must be positive, n_heads a "
                                  "multiple of n_kv_heads");
   if (cu_query_lens[0] != 0 || kv_indptr[0] != 0)
     return fail(PKV_ERR_INVALID, "cu_query_lens and kv_indptr must start at 0");
   plan->n_few = plan->n_wide = plan->few_rows = plan->n_slots = plan->part_rows = 0;
+  plan->few_waves = 0;
   plan->workspace_bytes = 0;
   *needed = 0;
   const int32_t G = n_heads / n_kv_heads;
   const bool fast = fast_4bit(n_heads, n_kv_heads, head_dim, page_size, dtype);
-  int64_t total = 0;      // tiles, over the KV heads
+  int64_t tiles[2] = {0, 0}, rows_of[2] = {0, 0};    // over the KV heads: few, wide
   int32_t few = 0;
-  bool wide = false;
+  auto step_of = [&](int32_t ql) {
+    return (int64_t)ql * G <= kFewRows ? ql : std::max(1, kWideRows / G);
+  };
+  auto tiles_to = [&](int32_t keys) { return (keys + kTile - 1) / kTile; };
   for (int32_t i = 0; i < n_seqs; ++i) {
     const int rc = check_seq_pages(i, kv_indptr[i + 1] - kv_indptr[i], kv_lens[i],
                                    kv_last_page_len[i], page_size);
@@ -582,47 +676,57 @@ static int plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr, con
       return fail(PKV_ERR_INVALID, "seq %d: query_len=%d outside [1, kv_len=%d]", i, ql,
                   kv_lens[i]);
     if (!fast) continue;
-    const int64_t rows = (int64_t)ql * G;
-    if (rows <= 16) few = std::max(few, (int32_t)rows);
-    else wide = true;
-    const int32_t step = rows <= 16 ? ql : std::max(1, 32 / G);
-    for (int32_t q = 0; q < ql; q += step)
-      total += (kv_lens[i] - ql + std::min(q + step, ql) + kTile - 1) / kTile;
+    const bool wide = (int64_t)ql * G > kFewRows;
+    if (!wide) few = std::max(few, ql * G);
+    const int32_t step = step_of(ql);
+    for (int32_t q = 0; q < ql; q += step) {
+      tiles[wide] += (int64_t)n_kv_heads * tiles_to(kv_lens[i] - ql + std::min(q + step, ql));
+      rows_of[wide] += n_kv_heads;
+    }
   }
   if (!fast) return PKV_OK;
   plan->few_rows = few == 0 ? 0 : few <= 4 ? 4 : few <= 8 ? 8 : 16;
-  plan->part_rows = wide ? 32 : plan->few_rows;
-  // A piece: a tile a wave at least, and about as many pieces as workgroups.
-  const int64_t piece = std::max<int64_t>(kWaves, (total * n_kv_heads + workgroups - 1) / workgroups);
+  plan->part_rows = rows_of[1] ? kWideRows : plan->few_rows;
+  // Many short rows take a wave each, the others four.
+  const bool one = rows_of[0] >= kOneWaveRows * (int64_t)compute_units;
+  plan->few_waves = few ? (one ? 1 : 4) : 0;
   struct Piece { int32_t v[kPieceInts]; };
   std::vector<Piece> out[2];
   int32_t slots = 0;
   for (int32_t i = 0; i < n_seqs; ++i) {
     const int32_t ql = cu_query_lens[i + 1] - cu_query_lens[i];
-    const int64_t rows = (int64_t)ql * G;
-    const int32_t step = rows <= 16 ? ql : std::max(1, 32 / G);
+    const bool wide = (int64_t)ql * G > kFewRows;
+    const int32_t step = step_of(ql);
+    const int waves = !wide && one ? 1 : 4;
+    // A piece: a tile a wave at least, and as many pieces as are resident at once.
+    const int64_t resident = (int64_t)compute_units * (wide ? kWideResident : one ? kOneResident : kFewResident);
+    const int64_t least = one && !wide ? kOneLeast : 4;
+    const int64_t piece = std::max<int64_t>(least, (tiles[wide] + resident - 1) / resident);
+    const int64_t most = waves == 1 ? kMostPieces1 : kMostPieces;
     for (int32_t q = 0; q < ql; q += step) {
       const int32_t qn = std::min(step, ql - q);
-      const int32_t tiles = (kv_lens[i] - ql + q + qn + kTile - 1) / kTile;
+      const int32_t nt = tiles_to(kv_lens[i] - ql + q + qn);
       // (a remainder below half a piece is shared out among the others)
-      const int32_t n = (int32_t)std::max<int64_t>(1, (tiles + piece / 2) / piece);
+      const int32_t n = (int32_t)std::min(most, std::max<int64_t>(1, (nt + piece / 2) / piece));
       const int32_t slot0 = slots;
       if (n > 1) {
-        if ((int64_t)slots + n > 0x7fffffff / 64)
+        if (slots > 0x7fffffff / 64 - n)
           return fail(PKV_ERR_INVALID, "the batch takes too many pieces");
         slots += n;
       }
       int32_t t0 = 0;
       for (int32_t k = 0; k < n; ++k) {
-        const int32_t t1 = (int32_t)((int64_t)tiles * (k + 1) / n);
-        out[rows > 16].push_back({{i, q, qn, t0, t1 - t0, n > 1 ? slot0 + k : -1, slot0, n}});
+        const int32_t t1 = (int32_t)((int64_t)nt * (k + 1) / n);
+        out[wide].push_back({{cu_query_lens[i] + q, qn, kv_lens[i] - ql + q, kv_lens[i],
+                              kv_indptr[i], kv_indptr[i + 1] - kv_indptr[i], t0, t1 - t0,
+                              n > 1 ? slot0 + k : -1, slot0, n, i}});
         t0 = t1;
       }
     }
   }
   for (auto& v : out)
     std::stable_sort(v.begin(), v.end(), [](const Piece& a, const Piece& b) {
-      return a.v[4] > b.v[4];
+      return a.v[7] > b.v[7];
     });
   *needed = (int64_t)(out[0].size() + out[1].size()) * kPieceInts;
   plan->n_few = (int32_t)out[0].size();
@@ -647,14 +751,14 @@ static int plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr, con
 int pkv_plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr, const int32_t* kv_lens,
                   const int32_t* kv_last_page_len, int32_t n_seqs, int32_t n_heads,
                   int32_t n_kv_heads, int32_t head_dim, int32_t page_size, int32_t dtype,
-                  int32_t workgroups, int32_t* items, int64_t capacity, int64_t* needed,
+                  int32_t compute_units, int32_t* items, int64_t capacity, int64_t* needed,
                   pkv_4bit* plan) {
   if (!cu_query_lens || !kv_indptr || !kv_lens || !kv_last_page_len || !needed || !plan ||
       capacity < 0 || (capacity && !items))
     return fail(PKV_ERR_INVALID, "null pointer argument");
   try {
     return plan_4bit(cu_query_lens, kv_indptr, kv_lens, kv_last_page_len, n_seqs, n_heads,
-                     n_kv_heads, head_dim, page_size, dtype, workgroups, items, capacity, needed,
+                     n_kv_heads, head_dim, page_size, dtype, compute_units, items, capacity, needed,
                      plan);
   } catch (const std::exception& e) {
     return fail(PKV_ERR_CAPACITY, "planning failed: %s", e.what());
@@ -695,10 +799,7 @@ int pkv_attend_4bit(const void* batch, const void* q, void* out, const void* k_p
   a.out = out;
   a.kpool = (const unsigned char*)k_pool;
   a.vpool = (const unsigned char*)v_pool;
-  a.cu_q = b.cu_query_lens;
-  a.indptr = b.kv_indptr;
   a.indices = b.kv_indices;
-  a.kv_lens = b.kv_lens;
   a.counters = (int32_t*)b.workspace;
   a.part_o = (float*)((char*)b.workspace + counter_bytes(b.n_slots, b.n_kv_heads));
   a.part_ml = a.part_o + (int64_t)b.n_slots * b.n_kv_heads * b.part_rows * b.head_dim;
@@ -707,31 +808,38 @@ int pkv_attend_4bit(const void* batch, const void* q, void* out, const void* k_p
   a.block = f.block;
   a.n_kv = b.n_kv_heads;
   a.groups = b.n_heads / b.n_kv_heads;
+  a.per_group = (65536u + a.groups - 1) / a.groups;
   a.head_bytes = f.head_bytes;
   a.pairs = f.pairs;
   a.shift = __builtin_ctz(b.page_size / 16);
   a.part_rows = b.part_rows;
   a.scale_log2 = scale * kLog2e;
-  auto go = [&](auto kernel, const int32_t* items, int32_t n) -> int {
+  auto go = [&](auto kernel, const int32_t* items, int32_t n, int waves) -> int {
     a.items = items;
     a.n_items = n;
     const int64_t grid = (int64_t)((n + 7) / 8) * 8 * b.n_kv_heads;
     if (grid > 0x7fffffffLL) return fail(PKV_ERR_INVALID, "too many pieces");
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * kWaves), 0, s, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * waves), 0, s, a);
     PKV_LAUNCH_CHECK();
     return PKV_OK;
   };
   auto by_rows = [&](auto type, auto dim) -> int {
     typedef decltype(type) T;
     constexpr int D = decltype(dim)::value;
+    auto few = [&](auto waves) -> int {
+      constexpr int N = decltype(waves)::value;
+      return b.few_rows == 4   ? go(attend_4bit_kernel<T, D, 1, 4, N>, b.items, b.n_few, N)
+             : b.few_rows == 8 ? go(attend_4bit_kernel<T, D, 1, 2, N>, b.items, b.n_few, N)
+                               : go(attend_4bit_kernel<T, D, 1, 1, N>, b.items, b.n_few, N);
+    };
     if (b.n_few) {
-      const int rc = b.few_rows == 4   ? go(attend_4bit_kernel<T, D, 1, 4>, b.items, b.n_few)
-                     : b.few_rows == 8 ? go(attend_4bit_kernel<T, D, 1, 2>, b.items, b.n_few)
-                                       : go(attend_4bit_kernel<T, D, 1, 1>, b.items, b.n_few);
+      const int rc = b.few_waves == 1 ? few(std::integral_constant<int, 1>{})
+                                      : few(std::integral_constant<int, 4>{});
       if (rc) return rc;
     }
     if (b.n_wide)
-      return go(attend_4bit_kernel<T, D, 2, 1>, b.items + (int64_t)b.n_few * kPieceInts, b.n_wide);
+      return go(attend_4bit_kernel<T, D, 2, 1, 4>, b.items + (int64_t)b.n_few * kPieceInts,
+                b.n_wide, 4);
     return PKV_OK;
   };
   auto by_dim = [&](auto type) -> int {

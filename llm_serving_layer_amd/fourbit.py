@@ -39,10 +39,6 @@ from .contract import BatchMeta
 
 __all__ = ["FourBitBackend"]
 
-# Pieces a batch is cut into, a compute unit (see pkv_plan_4bit).
-PIECES_PER_CU = 4
-
-
 class _Plan:
     """What ``attend`` keeps for one BatchMeta."""
 
@@ -56,7 +52,7 @@ class FourBitBackend(PagedPool):
 
     def __init__(self, num_layers: int, num_blocks: int, block_size: int, n_kv_heads: int,
                  n_heads: int, head_dim: int, device: str | torch.device = "cuda:0",
-                 dtype: torch.dtype = torch.float16, *, pieces: int | None = None):
+                 dtype: torch.dtype = torch.float16, *, compute_units: int | None = None):
         if n_heads % n_kv_heads != 0:
             raise ValueError(
                 f"n_heads={n_heads} must be divisible by n_kv_heads={n_kv_heads}; "
@@ -74,8 +70,8 @@ class FourBitBackend(PagedPool):
             raise ValueError(f"head_dim={head_dim} is odd or > 256: not supported")
         if num_blocks * block_size > 2**31 - 1:
             raise ValueError(f"{num_blocks} blocks of {block_size} rows pass the 32-bit slots")
-        if pieces is not None and pieces < 1:
-            raise ValueError(f"pieces={pieces} must be positive")
+        if compute_units is not None and compute_units < 1:
+            raise ValueError(f"compute_units={compute_units} must be positive")
         try:
             self._lib = _native.load()
         except RuntimeError as exc:
@@ -90,7 +86,8 @@ class FourBitBackend(PagedPool):
         self.n_kv_heads, self.n_heads, self.head_dim = n_kv_heads, n_heads, head_dim
         self.dtype, self.groups = dtype, n_heads // n_kv_heads
         self._code = _DTYPES[dtype]
-        self.pieces = pieces or PIECES_PER_CU * torch.cuda.get_device_properties(
+        # (what long sequences are cut to fill; the device's own by default)
+        self.compute_units = compute_units or torch.cuda.get_device_properties(
             self.device).multi_processor_count
         self._block_bytes = self._bytes_of_block(n_kv_heads, head_dim, block_size)
         self._plane_bytes = num_blocks * self._block_bytes
@@ -260,12 +257,12 @@ class FourBitBackend(PagedPool):
         arrays = [i32(a) for a in (cu, indptr, kvl, last)]
         args = _native.FourBit()
         needed = C.c_int64()
-        cap = 8 * (2 * self.pieces + 2 * n + meta.n_tokens * self.groups // 16)
+        cap = 12 * (16 * self.compute_units + 2 * n + meta.n_tokens * self.groups // 16)
         while True:
             items = np.empty(cap, np.int32)
             rc = self._lib.pkv_plan_4bit(
                 *(a.ctypes.data for a in arrays), n, self.n_heads, self.n_kv_heads,
-                self.head_dim, self.block_size, self._code, self.pieces, items.ctypes.data, cap,
+                self.head_dim, self.block_size, self._code, self.compute_units, items.ctypes.data, cap,
                 C.byref(needed), C.addressof(args))
             if rc != _native.ERR_CAPACITY or needed.value <= cap:
                 break

@@ -38,7 +38,7 @@ def test_block_bytes(n_kv, d, ps, want):
     ((1, 4, 16, 3, 8, 64), {}, "divisible"), ((0, 4, 16, 2, 8, 64), {}, "num_layers"),
     ((1, 4, 0, 2, 8, 64), {}, "block_size"), ((1, 4, 16, 2, 8, 63), {}, "odd"),
     ((1, 4, 16, 2, 8, 258), {}, "256"), ((1, 4, 16, 2, 8, 64), {"dtype": torch.int8}, "float16"),
-    ((1, 2**28, 16, 2, 8, 64), {}, "32-bit"), ((1, 4, 16, 2, 8, 64), {"pieces": 0}, "pieces"),
+    ((1, 2**28, 16, 2, 8, 64), {}, "32-bit"), ((1, 4, 16, 2, 8, 64), {"compute_units": 0}, "compute_units"),
     ((1, 4, 16, 2, 8, 64), {"device": "cpu"}, "GPU")])
 def test_refused_geometries(args, kw, match):
     with pytest.raises(ValueError, match=match):
@@ -46,7 +46,7 @@ def test_refused_geometries(args, kw, match):
 
 
 def plan(kv_lens, query_lens, n_heads=32, n_kv=8, d=64, ps=16, dtype=_native.DTYPE_F16,
-         workgroups=1024, last=None, indptr=None):
+         compute_units=256, last=None, indptr=None):
     n = len(kv_lens)
     i32 = lambda a: np.ascontiguousarray(a, dtype=np.int32)  # noqa: E731
     cu = i32(np.concatenate([[0], np.cumsum(query_lens)]))
@@ -60,26 +60,30 @@ def plan(kv_lens, query_lens, n_heads=32, n_kv=8, d=64, ps=16, dtype=_native.DTY
         items = np.empty(cap, np.int32)
         rc = _native.load().pkv_plan_4bit(
             cu.ctypes.data, indptr.ctypes.data, kvl.ctypes.data, last.ctypes.data, n, n_heads,
-            n_kv, d, ps, dtype, workgroups, items.ctypes.data, cap, C.byref(needed),
+            n_kv, d, ps, dtype, compute_units, items.ctypes.data, cap, C.byref(needed),
             C.addressof(args))
         if rc != _native.ERR_CAPACITY or needed.value <= cap:
             break
         cap = needed.value
     _native.check(rc, "plan")
-    return args, items[:needed.value].reshape(-1, 8).tolist()
+    return args, items[:needed.value].reshape(-1, 12).tolist()
 
 
-@pytest.mark.parametrize("workgroups", [1, 64, 1024, 100000])
+@pytest.mark.parametrize("compute_units", [1, 16, 256, 100000])
 @pytest.mark.parametrize("n_heads,n_kv", [(32, 8), (8, 8), (24, 1), (32, 1), (10, 2)])
-def test_the_plan_covers_every_row_and_tile_once(workgroups, n_heads, n_kv):
-    rng = np.random.default_rng(workgroups + n_heads)
+def test_the_plan_covers_every_row_and_tile_once(compute_units, n_heads, n_kv):
+    rng = np.random.default_rng(compute_units + n_heads)
     kv = [int(x) for x in rng.integers(1, 4000, 40)] + [1, 64, 65, 30000]
     ql = [int(min(k, rng.choice([1, 1, 1, 3, 8, 100]))) for k in kv]
-    args, items = plan(kv, ql, n_heads, n_kv, workgroups=workgroups)
+    args, items = plan(kv, ql, n_heads, n_kv, compute_units=compute_units)
     groups = n_heads // n_kv
     assert args.n_few + args.n_wide == len(items)
     seen, slots = {}, []
-    for i, (seq, q, qn, t0, nt, slot, slot0, n) in enumerate(items):
+    cu, first = np.cumsum([0] + ql), np.cumsum([0] + [-(-k // 16) for k in kv])
+    for i, (row, qn, pos, kvl, page, pages, t0, nt, slot, slot0, n, seq) in enumerate(items):
+        q = row - cu[seq]
+        assert (kvl, page, pages) == (kv[seq], first[seq], -(-kv[seq] // 16))
+        assert pos == kv[seq] - ql[seq] + q
         assert nt >= 1 and 1 <= qn and q + qn <= ql[seq]
         wide = ql[seq] * groups > 16
         assert (i >= args.n_few) == wide
@@ -106,7 +110,7 @@ def test_the_plan_covers_every_row_and_tile_once(workgroups, n_heads, n_kv):
         assert at == ql[seq]
     # longest first, in both parts
     for part in (items[:args.n_few], items[args.n_few:]):
-        assert [p[4] for p in part] == sorted((p[4] for p in part), reverse=True)
+        assert [p[7] for p in part] == sorted((p[7] for p in part), reverse=True)
     need = -(-args.n_slots * n_kv * 4 // 256) * 256 + args.n_slots * n_kv * args.part_rows * 66 * 4
     assert args.workspace_bytes == (need if args.n_slots else 0)
 
@@ -122,7 +126,7 @@ def test_geometries_without_a_plan(kw):
     ({"last": [3, 3]}, "kv_last_page_len"), ({"indptr": [0, 6, 7]}, "pages"),
     ({"query_lens": [0, 1]}, "query_len"), ({"query_lens": [101, 1]}, "query_len"),
     ({"kv_lens": [0, 3], "query_lens": [0, 1], "indptr": [0, 0, 1]}, "kv_len"),
-    ({"n_heads": 9}, "multiple"), ({"workgroups": 0}, "positive"), ({"d": 63}, "odd")])
+    ({"n_heads": 9}, "multiple"), ({"compute_units": 0}, "positive"), ({"d": 63}, "odd")])
 def test_refused_plans(kw, match):
     kw = {"kv_lens": [100, 3], "query_lens": [1, 2], **kw}
     with pytest.raises(ValueError, match=match):

@@ -550,17 +550,18 @@ int pkv_read_4bit(const void* k_pool, const void* v_pool, int64_t num_blocks,
  *
  * pkv_plan_4bit (host, synchronous) checks the metadata as pkv_plan_decode does
  * and fills items (capacity ints; *needed of them, PKV_ERR_CAPACITY if there are
- * fewer) with pieces of 12 ints {first token's row in q, tokens, its position,
+ * fewer) with pieces of 28 ints {first token's row in q, tokens, its position,
  * kv_len, first page in kv_indices, pages, first tile of 64 keys, tiles, partial
- * slot or -1, the first piece's slot, pieces, sequence}, those of sequences with
+ * slot or -1, the first piece's slot, pieces, arrival counter, the pages of the
+ * first 256 keys' 16 units}, those of sequences with
  * at most 16 query rows (tokens x query heads a KV head) first, and the plan
  * fields of *plan; long rows are cut to fill compute_units compute units. Geometries without a matrix-core kernel (head_dim
  * other than 64 and 128, f32, pages that are no power of two times 16, more than
  * 32 query heads a KV head) need no items.
  *
- * `workspace` (256-byte aligned, workspace_bytes long): n_slots * n_kv_heads
- * arrival counters, zero before the first launch and left so by each, then the
- * partial results; launches that share it must not overlap in time. Page ids
+ * `workspace` (256-byte aligned, workspace_bytes long): arrival counters, zero
+ * before the first launch and left so by each (pkv_counter_bytes_4bit from the
+ * front), then the partial results; launches that share it must not overlap in time. Page ids
  * outside [0, num_blocks) read as zeros and are flagged.
  */
 typedef struct pkv_4bit {
@@ -574,14 +575,16 @@ typedef struct pkv_4bit {
   void* workspace;
   int32_t* status_word;
   int32_t n_seqs, n_tokens, n_heads, n_kv_heads, head_dim, page_size, dtype;
-  int32_t n_few, n_wide, few_rows, few_waves, part_rows, n_slots;   /* the plan's */
+  int32_t n_few, n_wide, few_rows, few_waves, part_rows, n_slots, n_cuts;   /* the plan's */
 } pkv_4bit;
 
-int pkv_plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr, const int32_t* kv_lens,
+int pkv_plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr,
+                  const int32_t* kv_indices, const int32_t* kv_lens,
                   const int32_t* kv_last_page_len, int32_t n_seqs, int32_t n_heads,
                   int32_t n_kv_heads, int32_t head_dim, int32_t page_size, int32_t dtype,
                   int32_t compute_units, int32_t* items, int64_t capacity, int64_t* needed,
                   pkv_4bit* plan);
+int64_t pkv_counter_bytes_4bit(int32_t n_cuts, int32_t n_kv_heads);
 int pkv_attend_4bit(const void* batch, const void* q, void* out, const void* k_pool,
                     const void* v_pool, float scale, void* stream);
 

@@ -77,7 +77,8 @@ SIGNATURES = {
     "pkv_append_4bit": (C.c_int, [_p, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i32, _i32, _i32,
                                   _i32, _p, _p]),
     "pkv_read_4bit": (C.c_int, [_p, _p, _i64, _p, _i64, _p, _p, _i32, _i32, _i32, _i32, _p, _p]),
-    "pkv_plan_4bit": (C.c_int, [_p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p,
+    "pkv_counter_bytes_4bit": (C.c_int64, [_i32, _i32]),
+    "pkv_plan_4bit": (C.c_int, [_p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p,
                                 _i64, _p, _p]),
     "pkv_attend_4bit": (C.c_int, [_p, _p, _p, _p, _p, _f32, _p]),
     "pkv_copy_blocks": (C.c_int, [_p, _i32, _i64, _i64, _i64, _p, _p, _i32, _p, _p]),
@@ -143,7 +144,7 @@ class FourBit(C.Structure):
                                     "batch_indices", "items", "workspace", "status_word")],
                 *[(n, _i32) for n in ("n_seqs", "n_tokens", "n_heads", "n_kv_heads", "head_dim",
                                       "page_size", "dtype", "n_few", "n_wide", "few_rows",
-                                      "few_waves", "part_rows", "n_slots")]]
+                                      "few_waves", "part_rows", "n_slots", "n_cuts")]]
 
 
 _LIB = None

@@ -50,17 +50,17 @@ int run_4bit_any(const pkv_4bit& b, const void* q, void* out, const void* k_pool
 
 constexpr int kTile = 64;          // keys
 // A piece: {first token's row in q, tokens, its position, kv_len, first page in
-// kv_indices, pages, tile, tiles, partial slot | -1, slot 0, pieces, sequence}
-constexpr int kPieceInts = 12;
+// kv_indices, pages, tile, tiles, partial slot | -1, slot 0, pieces, counter}, then
+// the pages of the first four tiles' units.
+constexpr int kPieceInts = 28;
 
 // Workgroups a compute unit that pieces are made for: four waves for few rows, one
 // wave for few rows, wide rows; the least tiles of a one-wave piece; and from how
 // many rows a compute unit on they are.
-constexpr int kFewResident = 4, kOneResident = 16, kWideResident = 2, kOneLeast = 4,
-              kOneWaveRows = 8;
+constexpr int kFewResident = 2, kOneResident = 16, kWideResident = 2, kOneLeast = 4,
+              kOneWaveRows = 8, kJoin = 4;
 
-// Query rows of a piece, and pieces of a cut one at most, four waves and one (what
-// the merge's LDS holds the weights of).
+// Query rows of a piece, and pieces of a cut one at most, four waves and one.
 constexpr int kFewRows = 16, kWideRows = 32, kMostPieces = 128, kMostPieces1 = 32;
 
 struct Attend4 {
@@ -72,7 +72,7 @@ struct Attend4 {
   float *part_o, *part_ml;
   int32_t* status;
   int64_t num_blocks, block;
-  int32_t n_items, n_kv, groups, head_bytes, pairs, shift, part_rows;
+  int32_t n_items, n_kv, groups, head_bytes, pairs, shift, part_rows, count_step;
   uint32_t per_group;                // 2^16 / groups, rounded up: r / groups below 64 rows
   float scale_log2;
 };
@@ -84,38 +84,54 @@ template <int D> constexpr int kPairFloats = 4 * (D / 64) * kTile;
 // Waves a SIMD the kernel is compiled for.
 template <int D, int RT> constexpr int kSimdWaves = RT == 2 ? 2 : D == 64 ? 4 : 2;
 
-// WPP: waves of a piece's workgroup.
+// WPP: waves of a piece (its team). A workgroup has four waves at least: one-wave
+// teams share none but the dispatch (2840 of them began within 0.6 us of each
+// other, 2.0 us as workgroups of their own).
 template <typename T, int D, int RT, int NCL, int WPP>
-__global__ __launch_bounds__(64 * WPP, (kSimdWaves<D, RT>)) void attend_4bit_kernel(Attend4 a) {
+__global__ __launch_bounds__(WPP < 4 ? 256 : 64 * WPP, (kSimdWaves<D, RT>))
+void attend_4bit_kernel(Attend4 a) {
   constexpr int NG = D / 64;         // groups
   constexpr int W = D / 32;          // words of codes a lane takes of a unit
   constexpr int NT = D / 16;         // output tiles of 16 dims
   constexpr int RC = 16 / NCL;       // rows of a class
-  constexpr int UPL = 4 / NCL;       // units of a tile whose scores a lane holds
+  constexpr int PASSES = RT;         // of a tile: 4 / PASSES units each (registers)
+  constexpr int UPP = 4 / PASSES;    // units of a pass
+  constexpr int UPL = UPP / NCL;     // those whose scores a lane holds
   constexpr int ROWS = RT * 16;      // columns of S^T
   constexpr int OROWS = NCL > 1 ? RC : ROWS;
   constexpr int OP = D + 4;          // floats of a row of the merge's LDS
-  constexpr int NTH = 64 * WPP;
+  constexpr int NTH = 64 * WPP;      // threads of a team
+  constexpr int TEAMS = WPP < 4 ? 4 / WPP : 1;
   static_assert(RT == 1 || NCL == 1, "classes are for few rows");
-  static_assert(kPairFloats<D> * WPP >= 4 * NTH &&
-                    OP * WPP >= (WPP == 1 ? kMostPieces1 : kMostPieces),
-                "the merge reuses the LDS");
-  __shared__ __align__(16) float pair_lds[WPP * kPairFloats<D>];
-  __shared__ __align__(16) float o_lds[WPP * ROWS * OP];
-  __shared__ float m_lds[WPP * ROWS], l_lds[WPP * ROWS];
+  static_assert(WPP == 1 || TEAMS == 1, "a team is a wave or a workgroup");
+  // steps and zeros of a tile; then the merges' sums
+  constexpr int PAIR_F = WPP * kPairFloats<D>, RED_F = NTH * 6;
+  __shared__ __align__(16) float pair_all[TEAMS][PAIR_F > RED_F ? PAIR_F : RED_F];
+  __shared__ __align__(16) float o_all[TEAMS][WPP * ROWS * OP];
+  __shared__ float m_all[TEAMS][WPP * ROWS], l_all[TEAMS][WPP * ROWS];
   __shared__ int arrived;
+
+  const int wave_of_block = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int team = WPP == 1 ? wave_of_block : 0, wave = WPP == 1 ? 0 : wave_of_block;
+  const int tid = WPP == 1 ? threadIdx.x & 63 : threadIdx.x;
+  float* const pair_lds = pair_all[team];
+  float* const o_lds = o_all[team];
+  float* const m_lds = m_all[team];
+  float* const l_lds = l_all[team];
+  auto team_sync = [&]() {
+    if constexpr (WPP == 1) wave_lds_sync();
+    else __syncthreads();
+  };
 
   // Eight XCDs take workgroups in turn; a piece's heads go to one of them, where
   // they share the lines that hold steps and zeros of two heads.
-  const int x = blockIdx.x & 7, y = blockIdx.x >> 3;
+  const int x = blockIdx.x & 7, y = (blockIdx.x >> 3) * TEAMS + team;
   const int item = (y / a.n_kv) * 8 + x, h = y % a.n_kv;
   if (item >= a.n_items) return;
   const int32_t* it = a.items + (int64_t)item * kPieceInts;
   const int q0 = it[0], qn = it[1], base_pos = it[2], kv_len = it[3], pbase = it[4],
             n_pages = it[5], tile0 = it[6], n_tiles = it[7], slot = it[8];
   const int G = a.groups, Hq = a.n_kv * G;
-  const int tid = threadIdx.x;
-  const int wave = WPP == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, g = lane >> 4, n = lane & 15;
   const int cls = NCL > 1 ? n / RC : 0;
 
@@ -167,7 +183,12 @@ __global__ __launch_bounds__(64 * WPP, (kSimdWaves<D, RT>)) void attend_4bit_ker
   int t = tile0 + wave;
   int id = 0, id_next = 0;           // of tiles t, t + WPP
   if (t < end) {
-    id = load_id(t);
+    if constexpr (WPP <= 4) {        // (its pages came with the piece)
+      const int32_t* first = it + 12 + 4 * wave;
+      id = g == 0 ? first[0] : g == 1 ? first[1] : g == 2 ? first[2] : first[3];
+    } else {
+      id = load_id(t);
+    }
     load_k(t, id);
     load_v();
     id_next = load_id(t + WPP);
@@ -276,6 +297,12 @@ __global__ __launch_bounds__(64 * WPP, (kSimdWaves<D, RT>)) void attend_4bit_ker
     }
     wave_lds_sync();
 
+    auto pairs = [&](int kind, int q, int u) {   // of the lane's four keys of unit u
+      return *reinterpret_cast<const f32x4*>(pw + (kind * NG + q) * kTile + (cls + u) * 16 + 4 * g);
+    };
+#pragma unroll
+    for (int ps = 0; ps < PASSES; ++ps) {
+    const int u0 = ps * UPP;         // the pass's first unit
     f32x4 s[UPL][RT][NG];
 #pragma unroll
     for (int i = 0; i < UPL; ++i)
@@ -284,10 +311,10 @@ __global__ __launch_bounds__(64 * WPP, (kSimdWaves<D, RT>)) void attend_4bit_ker
 #pragma unroll
         for (int q = 0; q < NG; ++q) s[i][rt][q] = f32x4{};
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < UPP; ++u) {
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        const uint32_t c = kc[u][w];
+        const uint32_t c = kc[u0 + u][w];
         const f16x8 ka = __builtin_bit_cast(
             f16x8, u32x4{c & LO, c & UP, (c >> 8) & LO, (c >> 8) & UP});
 #pragma unroll
@@ -299,11 +326,9 @@ __global__ __launch_bounds__(64 * WPP, (kSimdWaves<D, RT>)) void attend_4bit_ker
     // (Nothing moves across the phases: the compiler would unpack all of a tile's
     // codes ahead of their products, and run out of registers.)
     __builtin_amdgcn_sched_barrier(0);
-    if constexpr (MORE) load_k(t + WPP, id_next);
-    auto pairs = [&](int kind, int q, int i) {   // of the lane's four keys of unit i
-      return *reinterpret_cast<const f32x4*>(pw + (kind * NG + q) * kTile +
-                                             (cls + NCL * i) * 16 + 4 * g);
-    };
+    if (ps == PASSES - 1) {
+      if constexpr (MORE) load_k(t + WPP, id_next);
+    }
     // scores, in the row's unit (times f1: log2)
     float y[UPL][RT][4];
 #pragma unroll
@@ -311,7 +336,7 @@ __global__ __launch_bounds__(64 * WPP, (kSimdWaves<D, RT>)) void attend_4bit_ker
       asm volatile("" ::: "memory");   // (reads no earlier: registers)
 #pragma unroll
       for (int q = 0; q < NG; ++q) {
-        const f32x4 step = pairs(0, q, i), zero = pairs(1, q, i);
+        const f32x4 step = pairs(0, q, u0 + NCL * i), zero = pairs(1, q, u0 + NCL * i);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -329,7 +354,7 @@ __global__ __launch_bounds__(64 * WPP, (kSimdWaves<D, RT>)) void attend_4bit_ker
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (kTile * t + (cls + NCL * i) * 16 + 4 * g + j > qpos[rt]) y[i][rt][j] = -INFINITY;
+            if (kTile * t + (u0 + cls + NCL * i) * 16 + 4 * g + j > qpos[rt]) y[i][rt][j] = -INFINITY;
     }
     float p[UPL][RT][4], ls[RT];
     auto probs = [&](int rt, float r) {
@@ -342,7 +367,7 @@ __global__ __launch_bounds__(64 * WPP, (kSimdWaves<D, RT>)) void attend_4bit_ker
           ls[rt] += p[i][rt][j];
         }
     };
-    bool past = top > cap;
+    bool past = ps == 0 && top > cap;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       probs(rt, ref[rt]);
@@ -350,7 +375,7 @@ __global__ __launch_bounds__(64 * WPP, (kSimdWaves<D, RT>)) void attend_4bit_ker
     }
     if (__builtin_amdgcn_ballot_w64(past)) {
       // 2^e for the largest step yet: its product below 1, up to 8 allowed
-      if (__builtin_amdgcn_ballot_w64(top > cap)) {
+      if (ps == 0 && __builtin_amdgcn_ballot_w64(top > cap)) {
         uint32_t w = top;
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) w = max(w, (uint32_t)__shfl_xor((int)w, off, 64));
@@ -408,7 +433,7 @@ __global__ __launch_bounds__(64 * WPP, (kSimdWaves<D, RT>)) void attend_4bit_ker
 #pragma unroll
       for (int q = 0; q < NG; ++q) {
         asm volatile("" ::: "memory");
-        const f32x4 step = pairs(2, q, i), mid = pairs(3, q, i);
+        const f32x4 step = pairs(2, q, u0 + NCL * i), mid = pairs(3, q, u0 + NCL * i);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
           float w[4], z = zo[rt][q];
@@ -431,9 +456,9 @@ __global__ __launch_bounds__(64 * WPP, (kSimdWaves<D, RT>)) void attend_4bit_ker
     const f16x8 ones = __builtin_bit_cast(
         f16x8, u32x4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u});
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
+    for (int m = 0; m < UPP / 2; ++m) {
       __builtin_amdgcn_sched_barrier(0);
-      const int ua = 2 * m, ub = 2 * m + 1;
+      const int ua = 2 * m, ub = 2 * m + 1;      // of the pass
       f16x8 pb[RT][NG];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
@@ -448,7 +473,7 @@ __global__ __launch_bounds__(64 * WPP, (kSimdWaves<D, RT>)) void attend_4bit_ker
         }
 #pragma unroll
       for (int b = 0; b < W; ++b) {
-        const uint32_t wa = vc[ua][b], wb = vc[ub][b];
+        const uint32_t wa = vc[u0 + ua][b], wb = vc[u0 + ub][b];
         const f16x8 lo = __builtin_bit_cast(
             f16x8, u32x4{wa & LO, (wa >> 8) & LO, wb & LO, (wb >> 8) & LO});
         const f16x8 up = __builtin_bit_cast(
@@ -461,6 +486,7 @@ __global__ __launch_bounds__(64 * WPP, (kSimdWaves<D, RT>)) void attend_4bit_ker
               __builtin_amdgcn_mfma_f32_16x16x32_f16(up, pb[rt][b / 2], o[rt][2 * b + 1], 0, 0, 0);
         }
       }
+    }
     }
     t += WPP;
     if constexpr (MORE) {
@@ -507,7 +533,7 @@ __global__ __launch_bounds__(64 * WPP, (kSimdWaves<D, RT>)) void attend_4bit_ker
       *reinterpret_cast<f32x4*>(o_lds + row * OP + 16 * i + 4 * g) = v;
     }
   }
-  __syncthreads();
+  team_sync();
 
   // merge the waves' (and classes') rows: set k of row r
   constexpr int SETS = WPP * NCL, CH = D / 4;
@@ -554,73 +580,89 @@ __global__ __launch_bounds__(64 * WPP, (kSimdWaves<D, RT>)) void attend_4bit_ker
   if (slot < 0) return;
 
   // Publish: the stores above are performed beyond the XCD's cache (sc1), and
-  // every wave waits for its own before the count; the workgroup whose count is
-  // the last merges, by loads from there. Counters are zero again afterwards.
+  // every wave waits for its own before the count; the team whose count is the
+  // last merges, by loads from there. Counters are zero again afterwards.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
   const int slot0 = it[9], pieces = it[10];
-  int32_t* cnt = a.counters + (int64_t)slot0 * a.n_kv + h;
-  if (tid == 0) arrived = __hip_atomic_fetch_add(cnt, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  if (arrived != pieces - 1) return;
+  int32_t* cnt = a.counters + ((int64_t)it[11] * a.n_kv + h) * a.count_step;
+  int count = 0;
+  if constexpr (WPP == 1) {
+    if (lane == 0)
+      count = __hip_atomic_fetch_add(cnt, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    count = __builtin_amdgcn_readfirstlane(count);
+  } else {
+    __syncthreads();
+    if (tid == 0)
+      arrived = __hip_atomic_fetch_add(cnt, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    count = arrived;
+  }
+  if (count != pieces - 1) return;
   if (tid == 0) __hip_atomic_store(cnt, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // Every piece's (m, l) and from them its weight: a wave a row, a lane a piece.
-  float* const weights = o_lds;      // [row][piece]
+  // A thread per (row, 4 dims), or several, each some of the pieces, where there
+  // are fewer; eight pieces' loads are in flight together (none past the last).
   const int apart = a.n_kv * a.part_rows;   // rows between two pieces' of this head
   const int64_t row0 = ((int64_t)slot0 * a.n_kv + h) * a.part_rows;
   const int reach = (pieces - 1) * apart + live_rows;
   const __amdgpu_buffer_rsrc_t mls = ws_rsrc(a.part_ml + row0 * 2, reach * 8);
   const __amdgpu_buffer_rsrc_t os = ws_rsrc(a.part_o + row0 * D, reach * D * 4);
-  constexpr int PL = (WPP == 1 ? kMostPieces1 : kMostPieces) <= 64 ? 1 : 2;
-  for (int r = wave; r < live_rows; r += WPP) {
-    f32x2 ml[PL];
-    float m = -INFINITY, lr = 0.f;
-#pragma unroll
-    for (int i = 0; i < PL; ++i) {
-      const int k = lane + 64 * i;
-      ml[i] = __builtin_bit_cast(
-          f32x2, __builtin_amdgcn_raw_buffer_load_b64(mls, (k * apart + r) * 8, 0, kSc1));
-      if (k >= pieces) ml[i] = f32x2{-INFINITY, 0.f};
-      m = fmaxf(m, ml[i][0]);
-    }
-    m = wave_max(m);
-#pragma unroll
-    for (int i = 0; i < PL; ++i) {
-      const float w = ml[i][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[i][0] - m);
-      lr = __builtin_fmaf(ml[i][1], w, lr);
-      if (lane + 64 * i < pieces) weights[r * pieces + lane + 64 * i] = w;
-    }
-    lr = wave_sum(lr);
-    if (lane == 0) l_lds[r] = lr;
-  }
-  __syncthreads();
-  // Where there are fewer (row, 4 dims) than threads, several threads share one,
-  // each some of the pieces.
   const int units = live_rows * CH, share = units >= NTH ? 1 : NTH / units;
-  f32x4* const red = reinterpret_cast<f32x4*>(pair_lds);
   for (int i0 = 0; i0 < units; i0 += NTH) {
     const int i = share > 1 ? tid % units : i0 + tid;
     const int first = share > 1 ? tid / units : 0;
     const int r = i / CH, c4 = i % CH;
+    const bool mine = i < units && first < share;
     f32x4 v{};
-    if (i < units && first < share) {
-#pragma unroll 8
-      for (int k = first; k < pieces; k += share) {
-        const f32x4 ov = __builtin_bit_cast(
-            f32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                       os, ((k * apart + r) * D + 4 * c4) * 4, 0, kSc1));
-        v += ov * weights[r * pieces + k];
+    float m = -INFINITY, lr = 0.f;
+    for (int k0 = first; k0 < pieces; k0 += 8 * share) {
+      f32x2 ml[8];
+      f32x4 ov[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int k = k0 + j * share;
+        const int at = mine && k < pieces ? k * apart + r : reach;
+        ml[j] = __builtin_bit_cast(f32x2,
+                                   __builtin_amdgcn_raw_buffer_load_b64(mls, at * 8, 0, kSc1));
+        ov[j] = __builtin_bit_cast(
+            f32x4, __builtin_amdgcn_raw_buffer_load_b128(os, (at * D + 4 * c4) * 4, 0, kSc1));
+      }
+      float mn = m;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (k0 + j * share >= pieces) ml[j][0] = -INFINITY;
+        mn = fmaxf(mn, ml[j][0]);
+      }
+      const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      v *= f;
+      lr *= f;
+      m = mn;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float w = ml[j][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[j][0] - m);
+        v += ov[j] * w;
+        lr = __builtin_fmaf(ml[j][1], w, lr);
       }
     }
     if (share > 1) {
+      f32x4* const red = reinterpret_cast<f32x4*>(pair_lds);
+      f32x2* const red2 = reinterpret_cast<f32x2*>(red + NTH);
       red[tid] = v;
-      __syncthreads();
+      red2[tid] = f32x2{m, lr};
+      team_sync();
       if (first == 0) {
-        for (int k = 1; k < share; ++k) v += red[tid + k * units];
-        store(r, c4, v, l_lds[r]);
+        for (int k = 1; k < share; ++k) {
+          const f32x2 other = red2[tid + k * units];
+          if (other[0] == -INFINITY) continue;
+          const float mn = fmaxf(m, other[0]);
+          const float f = __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(other[0] - mn);
+          v = v * f + red[tid + k * units] * w;
+          lr = lr * f + other[1] * w;
+          m = mn;
+        }
+        store(r, c4, v, lr);
       }
-    } else if (i < units) {
-      store(r, c4, v, l_lds[r]);
+    } else if (mine) {
+      store(r, c4, v, lr);
     }
   }
 }
@@ -633,8 +675,12 @@ static bool fast_4bit(int32_t n_heads, int32_t n_kv, int32_t d, int32_t ps, int3
          ps % 16 == 0 && units > 0 && (units & (units - 1)) == 0 && n_heads / n_kv <= 32;
 }
 
-static int64_t counter_bytes(int64_t slots, int32_t n_kv) {
-  return (slots * n_kv * 4 + 255) / 256 * 256;
+// Arrival counters lie 128 bytes apart where they are few and their pieces may be
+// many: counts of one line are taken one after another, 10 ns each.
+static int32_t count_step(int64_t counters) { return counters <= 4096 ? 32 : 1; }
+static int64_t counter_bytes(int64_t cuts, int32_t n_kv) {
+  const int64_t n = cuts * n_kv;
+  return (n * count_step(n) * 4 + 255) / 256 * 256;
 }
 
 }  // namespace pkv
@@ -643,7 +689,8 @@ using namespace pkv;
 
 extern "C" {
 
-static int plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr, const int32_t* kv_lens,
+static int plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr,
+                     const int32_t* kv_indices, const int32_t* kv_lens,
                      const int32_t* kv_last_page_len, int32_t n_seqs, int32_t n_heads,
                      int32_t n_kv_heads, int32_t head_dim, int32_t page_size, int32_t dtype,
                      int32_t compute_units, int32_t* items, int64_t capacity, int64_t* needed,
@@ -656,70 +703,91 @@ static int plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr, con
   if (cu_query_lens[0] != 0 || kv_indptr[0] != 0)
     return fail(PKV_ERR_INVALID, "cu_query_lens and kv_indptr must start at 0");
   plan->n_few = plan->n_wide = plan->few_rows = plan->n_slots = plan->part_rows = 0;
-  plan->few_waves = 0;
+  plan->few_waves = plan->n_cuts = 0;
   plan->workspace_bytes = 0;
   *needed = 0;
   const int32_t G = n_heads / n_kv_heads;
   const bool fast = fast_4bit(n_heads, n_kv_heads, head_dim, page_size, dtype);
-  int64_t tiles[2] = {0, 0}, rows_of[2] = {0, 0};    // over the KV heads: few, wide
+  struct Row { int32_t seq, q, n, tiles; };      // n tokens of a sequence from its q-th
+  std::vector<Row> rows[2];                       // few, wide
+  int64_t tiles[2] = {0, 0};
   int32_t few = 0;
-  auto step_of = [&](int32_t ql) {
-    return (int64_t)ql * G <= kFewRows ? ql : std::max(1, kWideRows / G);
-  };
-  auto tiles_to = [&](int32_t keys) { return (keys + kTile - 1) / kTile; };
   for (int32_t i = 0; i < n_seqs; ++i) {
-    const int rc = check_seq_pages(i, kv_indptr[i + 1] - kv_indptr[i], kv_lens[i],
-                                   kv_last_page_len[i], page_size);
+    const int32_t kv = kv_lens[i], ql = cu_query_lens[i + 1] - cu_query_lens[i];
+    const int rc = check_seq_pages(i, kv_indptr[i + 1] - kv_indptr[i], kv, kv_last_page_len[i],
+                                   page_size);
     if (rc) return rc;
-    const int32_t ql = cu_query_lens[i + 1] - cu_query_lens[i];
-    if (ql < 1 || ql > kv_lens[i])
-      return fail(PKV_ERR_INVALID, "seq %d: query_len=%d outside [1, kv_len=%d]", i, ql,
-                  kv_lens[i]);
+    if (ql < 1 || ql > kv)
+      return fail(PKV_ERR_INVALID, "seq %d: query_len=%d outside [1, kv_len=%d]", i, ql, kv);
     if (!fast) continue;
     const bool wide = (int64_t)ql * G > kFewRows;
     if (!wide) few = std::max(few, ql * G);
-    const int32_t step = step_of(ql);
+    const int32_t step = wide ? std::max(1, kWideRows / G) : ql;
     for (int32_t q = 0; q < ql; q += step) {
-      tiles[wide] += (int64_t)n_kv_heads * tiles_to(kv_lens[i] - ql + std::min(q + step, ql));
-      rows_of[wide] += n_kv_heads;
+      const int32_t n = std::min(step, ql - q);
+      rows[wide].push_back({i, q, n, (kv - ql + q + n + kTile - 1) / kTile});
+      tiles[wide] += rows[wide].back().tiles;
     }
   }
   if (!fast) return PKV_OK;
+  // Beside wide rows few rows run as wide ones do, unless theirs are most tiles: one
+  // launch, with one ramp and one tail.
+  if (!rows[1].empty() && tiles[0] <= kJoin * tiles[1]) {
+    rows[1].insert(rows[1].end(), rows[0].begin(), rows[0].end());
+    rows[0].clear();
+    few = 0;
+  }
   plan->few_rows = few == 0 ? 0 : few <= 4 ? 4 : few <= 8 ? 8 : 16;
-  plan->part_rows = rows_of[1] ? kWideRows : plan->few_rows;
+  plan->part_rows = !rows[1].empty() ? kWideRows : plan->few_rows;
   // Many short rows take a wave each, the others four.
-  const bool one = rows_of[0] >= kOneWaveRows * (int64_t)compute_units;
+  const bool one = (int64_t)rows[0].size() * n_kv_heads >= kOneWaveRows * (int64_t)compute_units;
   plan->few_waves = few ? (one ? 1 : 4) : 0;
   struct Piece { int32_t v[kPieceInts]; };
   std::vector<Piece> out[2];
-  int32_t slots = 0;
-  for (int32_t i = 0; i < n_seqs; ++i) {
-    const int32_t ql = cu_query_lens[i + 1] - cu_query_lens[i];
-    const bool wide = (int64_t)ql * G > kFewRows;
-    const int32_t step = step_of(ql);
-    const int waves = !wide && one ? 1 : 4;
-    // A piece: a tile a wave at least, and as many pieces as are resident at once.
-    const int64_t resident = (int64_t)compute_units * (wide ? kWideResident : one ? kOneResident : kFewResident);
-    const int64_t least = one && !wide ? kOneLeast : 4;
-    const int64_t piece = std::max<int64_t>(least, (tiles[wide] + resident - 1) / resident);
-    const int64_t most = waves == 1 ? kMostPieces1 : kMostPieces;
-    for (int32_t q = 0; q < ql; q += step) {
-      const int32_t qn = std::min(step, ql - q);
-      const int32_t nt = tiles_to(kv_lens[i] - ql + q + qn);
-      // (a remainder below half a piece is shared out among the others)
-      const int32_t n = (int32_t)std::min(most, std::max<int64_t>(1, (nt + piece / 2) / piece));
+  const int32_t units = page_size / 16;      // of a page
+  int32_t slots = 0, cuts = 0;
+  for (int wide = 0; wide < 2; ++wide) {
+    // The shortest piece (a tile a wave at least) with which all of them are
+    // resident at once: none waits for another to end.
+    const bool alone = !wide && one;
+    const int64_t resident =
+        (int64_t)compute_units * (wide ? kWideResident : alone ? kOneResident : kFewResident);
+    const int64_t most = alone ? kMostPieces1 : kMostPieces;
+    auto pieces = [&](const Row& r, int64_t piece) {
+      return std::min<int64_t>(most, (r.tiles + piece - 1) / piece);
+    };
+    auto fits = [&](int64_t piece) {
+      int64_t n = 0;
+      for (const Row& r : rows[wide]) n += pieces(r, piece);
+      return n * n_kv_heads <= resident;
+    };
+    int64_t lo = alone ? kOneLeast : 4, hi = lo;
+    for (const Row& r : rows[wide]) hi = std::max<int64_t>(hi, r.tiles);
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) / 2;
+      if (fits(mid)) hi = mid;
+      else lo = mid + 1;
+    }
+    for (const Row& r : rows[wide]) {
+      const int32_t i = r.seq, q = r.q, qn = r.n, nt = r.tiles;
+      const int32_t ql = cu_query_lens[i + 1] - cu_query_lens[i];
+      const int32_t n = (int32_t)pieces(r, lo);
       const int32_t slot0 = slots;
       if (n > 1) {
         if (slots > 0x7fffffff / 64 - n)
           return fail(PKV_ERR_INVALID, "the batch takes too many pieces");
         slots += n;
+        ++cuts;
       }
       int32_t t0 = 0;
       for (int32_t k = 0; k < n; ++k) {
         const int32_t t1 = (int32_t)((int64_t)nt * (k + 1) / n);
-        out[wide].push_back({{cu_query_lens[i] + q, qn, kv_lens[i] - ql + q, kv_lens[i],
-                              kv_indptr[i], kv_indptr[i + 1] - kv_indptr[i], t0, t1 - t0,
-                              n > 1 ? slot0 + k : -1, slot0, n, i}});
+        Piece p{{cu_query_lens[i] + q, qn, kv_lens[i] - ql + q, kv_lens[i], kv_indptr[i],
+                 kv_indptr[i + 1] - kv_indptr[i], t0, t1 - t0, n > 1 ? slot0 + k : -1, slot0, n,
+                 cuts - 1}};
+        for (int32_t u = 0; u < 16; ++u)
+          p.v[12 + u] = kv_indices[kv_indptr[i] + std::min((4 * t0 + u) / units, p.v[5] - 1)];
+        out[wide].push_back(p);
         t0 = t1;
       }
     }
@@ -732,8 +800,9 @@ static int plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr, con
   plan->n_few = (int32_t)out[0].size();
   plan->n_wide = (int32_t)out[1].size();
   plan->n_slots = slots;
+  plan->n_cuts = cuts;
   plan->workspace_bytes =
-      slots ? counter_bytes(slots, n_kv_heads) +
+      slots ? counter_bytes(cuts, n_kv_heads) +
                   (int64_t)slots * n_kv_heads * plan->part_rows * (head_dim + 2) * 4
             : 0;
   if (*needed > capacity)
@@ -748,21 +817,26 @@ static int plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr, con
   return PKV_OK;
 }
 
-int pkv_plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr, const int32_t* kv_lens,
+int pkv_plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr,
+                  const int32_t* kv_indices, const int32_t* kv_lens,
                   const int32_t* kv_last_page_len, int32_t n_seqs, int32_t n_heads,
                   int32_t n_kv_heads, int32_t head_dim, int32_t page_size, int32_t dtype,
                   int32_t compute_units, int32_t* items, int64_t capacity, int64_t* needed,
                   pkv_4bit* plan) {
-  if (!cu_query_lens || !kv_indptr || !kv_lens || !kv_last_page_len || !needed || !plan ||
+  if (!cu_query_lens || !kv_indptr || !kv_indices || !kv_lens || !kv_last_page_len || !needed || !plan ||
       capacity < 0 || (capacity && !items))
     return fail(PKV_ERR_INVALID, "null pointer argument");
   try {
-    return plan_4bit(cu_query_lens, kv_indptr, kv_lens, kv_last_page_len, n_seqs, n_heads,
-                     n_kv_heads, head_dim, page_size, dtype, compute_units, items, capacity, needed,
+    return plan_4bit(cu_query_lens, kv_indptr, kv_indices, kv_lens, kv_last_page_len, n_seqs,
+                     n_heads, n_kv_heads, head_dim, page_size, dtype, compute_units, items, capacity, needed,
                      plan);
   } catch (const std::exception& e) {
     return fail(PKV_ERR_CAPACITY, "planning failed: %s", e.what());
   }
+}
+
+int64_t pkv_counter_bytes_4bit(int32_t n_cuts, int32_t n_kv_heads) {
+  return n_cuts > 0 && n_kv_heads > 0 ? counter_bytes(n_cuts, n_kv_heads) : 0;
 }
 
 int pkv_attend_4bit(const void* batch, const void* q, void* out, const void* k_pool,
@@ -787,7 +861,7 @@ int pkv_attend_4bit(const void* batch, const void* q, void* out, const void* k_p
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool) % 16)
     return fail(PKV_ERR_INVALID, "q, out and the pools have to be aligned to 16 bytes");
   const FourBit f = four_bit(b.n_kv_heads, b.head_dim, b.page_size);
-  const int64_t need = b.n_slots ? counter_bytes(b.n_slots, b.n_kv_heads) +
+  const int64_t need = b.n_slots ? counter_bytes(b.n_cuts, b.n_kv_heads) +
                                        (int64_t)b.n_slots * b.n_kv_heads * b.part_rows *
                                            (b.head_dim + 2) * 4
                                  : 0;
@@ -801,7 +875,8 @@ int pkv_attend_4bit(const void* batch, const void* q, void* out, const void* k_p
   a.vpool = (const unsigned char*)v_pool;
   a.indices = b.kv_indices;
   a.counters = (int32_t*)b.workspace;
-  a.part_o = (float*)((char*)b.workspace + counter_bytes(b.n_slots, b.n_kv_heads));
+  a.part_o = (float*)((char*)b.workspace + counter_bytes(b.n_cuts, b.n_kv_heads));
+  a.count_step = count_step((int64_t)b.n_cuts * b.n_kv_heads);
   a.part_ml = a.part_o + (int64_t)b.n_slots * b.n_kv_heads * b.part_rows * b.head_dim;
   a.status = b.status_word;
   a.num_blocks = b.num_blocks;
@@ -817,9 +892,11 @@ int pkv_attend_4bit(const void* batch, const void* q, void* out, const void* k_p
   auto go = [&](auto kernel, const int32_t* items, int32_t n, int waves) -> int {
     a.items = items;
     a.n_items = n;
-    const int64_t grid = (int64_t)((n + 7) / 8) * 8 * b.n_kv_heads;
+    // (of each XCD: its pieces' heads, four to a workgroup where a wave takes one)
+    const int64_t per_xcd = (int64_t)((n + 7) / 8) * b.n_kv_heads;
+    const int64_t grid = (waves == 1 ? (per_xcd + 3) / 4 : per_xcd) * 8;
     if (grid > 0x7fffffffLL) return fail(PKV_ERR_INVALID, "too many pieces");
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * waves), 0, s, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(waves == 1 ? 256 : 64 * waves), 0, s, a);
     PKV_LAUNCH_CHECK();
     return PKV_OK;
   };

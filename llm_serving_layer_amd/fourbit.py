@@ -254,10 +254,10 @@ class FourBitBackend(PagedPool):
                              f"for {meta.n_tokens} tokens")
         self._check_pages(kvl, indptr, last, int(indices.shape[0]))
         i32 = lambda a: np.ascontiguousarray(a, dtype=np.int32)  # noqa: E731
-        arrays = [i32(a) for a in (cu, indptr, kvl, last)]
+        arrays = [i32(a) for a in (cu, indptr, indices, kvl, last)]
         args = _native.FourBit()
         needed = C.c_int64()
-        cap = 12 * (16 * self.compute_units + 2 * n + meta.n_tokens * self.groups // 16)
+        cap = 28 * (16 * self.compute_units + 2 * n + meta.n_tokens * self.groups // 16)
         while True:
             items = np.empty(cap, np.int32)
             rc = self._lib.pkv_plan_4bit(
@@ -278,7 +278,7 @@ class FourBitBackend(PagedPool):
          args.items) = at
         if args.workspace_bytes:   # (the plan's own: its counters stay zero between launches)
             ws = torch.empty(args.workspace_bytes, dtype=torch.uint8, device=self.device)
-            ws[:4 * args.n_slots * self.n_kv_heads].zero_()
+            ws[:self._lib.pkv_counter_bytes_4bit(args.n_cuts, self.n_kv_heads)].zero_()
             args.workspace = ws.data_ptr()
             p.buffers.append(ws)
         args.num_blocks, args.status_word = self.num_blocks, self._status_ptr

@@ -54,19 +54,20 @@ def plan(kv_lens, query_lens, n_heads=32, n_kv=8, d=64, ps=16, dtype=_native.DTY
         indptr = np.concatenate([[0], np.cumsum([-(-k // ps) for k in kv_lens])])
     indptr, kvl = i32(indptr), i32(kv_lens)
     last = i32([k % ps or ps for k in kv_lens] if last is None else last)
+    ids = np.arange(int(indptr[-1]) if indptr[-1] > 0 else 1, dtype=np.int32) * 3
     args, needed = _native.FourBit(), C.c_int64()
     cap = 8
     for _ in range(2):
         items = np.empty(cap, np.int32)
         rc = _native.load().pkv_plan_4bit(
-            cu.ctypes.data, indptr.ctypes.data, kvl.ctypes.data, last.ctypes.data, n, n_heads,
+            cu.ctypes.data, indptr.ctypes.data, ids.ctypes.data, kvl.ctypes.data, last.ctypes.data, n, n_heads,
             n_kv, d, ps, dtype, compute_units, items.ctypes.data, cap, C.byref(needed),
             C.addressof(args))
         if rc != _native.ERR_CAPACITY or needed.value <= cap:
             break
         cap = needed.value
     _native.check(rc, "plan")
-    return args, items[:needed.value].reshape(-1, 12).tolist()
+    return args, items[:needed.value].reshape(-1, 28).tolist()
 
 
 @pytest.mark.parametrize("compute_units", [1, 16, 256, 100000])
@@ -80,18 +81,23 @@ def test_the_plan_covers_every_row_and_tile_once(compute_units, n_heads, n_kv):
     assert args.n_few + args.n_wide == len(items)
     seen, slots = {}, []
     cu, first = np.cumsum([0] + ql), np.cumsum([0] + [-(-k // 16) for k in kv])
-    for i, (row, qn, pos, kvl, page, pages, t0, nt, slot, slot0, n, seq) in enumerate(items):
+    counters = {}
+    for i, (row, qn, pos, kvl, page, pages, t0, nt, slot, slot0, n, counter, *ids) in \
+            enumerate(items):
+        seq = int(np.searchsorted(cu, row, side="right")) - 1
         q = row - cu[seq]
+        assert ids == [3 * (page + min(4 * t0 + u, pages - 1)) for u in range(16)]
         assert (kvl, page, pages) == (kv[seq], first[seq], -(-kv[seq] // 16))
         assert pos == kv[seq] - ql[seq] + q
         assert nt >= 1 and 1 <= qn and q + qn <= ql[seq]
-        wide = ql[seq] * groups > 16
-        assert (i >= args.n_few) == wide
+        wide = i >= args.n_few
+        assert wide or ql[seq] * groups <= 16
         assert qn * groups <= (32 if wide else args.few_rows) <= args.part_rows * (1 if wide else 9)
         assert (slot < 0) == (n == 1)
         if n > 1:
             assert slot0 <= slot < slot0 + n <= args.n_slots
             slots.append(slot)
+            assert 0 <= counter < args.n_cuts and counters.setdefault(counter, slot0) == slot0
         seen.setdefault((seq, q, qn), []).append((t0, nt))
     assert sorted(slots) == list(range(args.n_slots))
     rows = {i: [] for i in range(len(kv))}
@@ -111,7 +117,8 @@ def test_the_plan_covers_every_row_and_tile_once(compute_units, n_heads, n_kv):
     # longest first, in both parts
     for part in (items[:args.n_few], items[args.n_few:]):
         assert [p[7] for p in part] == sorted((p[7] for p in part), reverse=True)
-    need = -(-args.n_slots * n_kv * 4 // 256) * 256 + args.n_slots * n_kv * args.part_rows * 66 * 4
+    assert len(counters) == len(set(counters.values())) == args.n_cuts
+    need = _native.load().pkv_counter_bytes_4bit(args.n_cuts, n_kv) + args.n_slots * n_kv * args.part_rows * 66 * 4
     assert args.workspace_bytes == (need if args.n_slots else 0)
 
 

@@ -6,6 +6,7 @@ block copies, swaps, streams and graphs.
 
 from __future__ import annotations
 
+import dataclasses
 import math
 import random
 
@@ -341,6 +342,7 @@ def test_pages_outside_the_pool_read_as_zeros():
     c = Cache([200], F16, 2, 8, 64)
     meta = c.append([1])
     meta.kv_indices[3] = c.bk.num_blocks + 5
+    meta = dataclasses.replace(meta, host=None)      # (its host arrays hold the old page)
     q = c.q([1])
     out = c.bk.attend(q.to(DEV), 0, 0.125, meta).cpu()
     keep = torch.ones(201, dtype=torch.bool)

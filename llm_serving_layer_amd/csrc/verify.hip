@@ -29,9 +29,18 @@
 namespace pkv {
 
 constexpr int kVT = 256;            // threads of a workgroup
-constexpr int kMaxSplits = 64;
+constexpr int kMaxSplits = 64;      // of a row: a lane each
+constexpr int kChunks = 4;          // of 16 bytes a thread and round, in the first kernel
 
 struct RowStats { float m, z; int32_t arg, pad; };
+
+// A sequence's decision: how many drafts stand, and the row that follows.
+struct Decision {
+  int32_t run, row, token;   // token: taken as it is, or -1: drawn from the row
+  int32_t banned;            // the draft that fell, without draft probabilities; -1
+  int32_t rest, pad;         // drawn from max(p - q, 0)
+  double m, c;               // the row's largest logit, log2 e / temperature
+};
 
 struct Verify {
   const void* logits;
@@ -40,6 +49,7 @@ struct Verify {
   const int32_t *cu, *owner;
   const float *numbers, *temps;
   RowStats* stats;
+  Decision* decisions;
   double *sums, *rest;              // of a sequence's parts: 2^x, max(2^x - q z, 0)
   int32_t* counters;                // two a sequence; cleared by the first kernel
   int64_t *ids, *accepted;
@@ -61,7 +71,7 @@ __device__ __forceinline__ void part_of(const T* row, int vocab, int s, int n, i
 
 template <typename T>
 __global__ __launch_bounds__(kVT) void verify_stats_kernel(Verify a) {
-  constexpr int E = 16 / (int)sizeof(T), U = 8;
+  constexpr int E = 16 / (int)sizeof(T), U = kChunks;
   typedef T TV __attribute__((ext_vector_type(E)));
   const int r = blockIdx.x / a.splits, s = blockIdx.x - r * a.splits;
   const int tid = threadIdx.x;
@@ -97,8 +107,10 @@ __global__ __launch_bounds__(kVT) void verify_stats_kernel(Verify a) {
         for (int e = 0; e < E; ++e) w[u][e] = (T)-INFINITY;
     }
     float top = m;
+    const int live = min(U, (chunks - c0 + kVT - 1) / kVT);   // of the U, uniform
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      if (u >= live) break;
       TV x = w[u];
       float cm = Elem<T>::to_f(x[0]);
 #pragma unroll
@@ -113,16 +125,20 @@ __global__ __launch_bounds__(kVT) void verify_stats_kernel(Verify a) {
     m = top;
     if (__builtin_fabsf(rc) < 0x1p80f) {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        if (u >= live) break;
 #pragma unroll
         for (int e = 0; e < E; ++e)
           z += __builtin_amdgcn_exp2f(__builtin_fmaf(Elem<T>::to_f(w[u][e]), c, rc));
+      }
     } else {                         // (far from 1: the products may overflow)
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        if (u >= live) break;
 #pragma unroll
         for (int e = 0; e < E; ++e)
           z += __builtin_amdgcn_exp2f((Elem<T>::to_f(w[u][e]) - ref) * c);
+      }
     }
   }
   const int tail = body + chunks * E;
@@ -191,6 +207,16 @@ __device__ __forceinline__ double wave_sum64(double v) {
   for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
   return v;
 }
+// v plus the lower lanes' values
+__device__ __forceinline__ double wave_scan64(double v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const double o = __shfl_up(v, off, 64);
+    v += lane >= off ? o : 0.0;
+  }
+  return v;
+}
 // the sum over the workgroup, in every thread (4 doubles of LDS)
 __device__ __forceinline__ double block_sum64(double v, double* lds) {
   v = wave_sum64(v);
@@ -203,125 +229,170 @@ __device__ __forceinline__ double block_sum64(double v, double* lds) {
   return s;
 }
 
-// f(index, logit) over elements [begin, end) of a row, 16 bytes at a time; the
-// inner borders lie on 16-byte boundaries.
-template <typename T, typename F>
-__device__ __forceinline__ void each(const T* row, int begin, int end, F&& f) {
-  constexpr int E = 16 / (int)sizeof(T);
-  typedef T TV __attribute__((ext_vector_type(E)));
-  const int head = min((int)((-(uintptr_t)(row + begin) & 15) / sizeof(T)), end - begin);
-  const int body = begin + head, chunks = (end - body) / E, tail = body + chunks * E;
-  if ((int)threadIdx.x < head) f(begin + threadIdx.x, Elem<T>::to_f(row[begin + threadIdx.x]));
-  for (int k = threadIdx.x; k < chunks; k += kVT) {
-    const TV w = *reinterpret_cast<const TV*>(row + body + (int64_t)k * E);
-#pragma unroll
-    for (int e = 0; e < E; ++e) f(body + k * E + e, Elem<T>::to_f(w[e]));
+// Elements [begin, end) of a row as cells: cell 0 those before the first 16-byte
+// boundary (none where begin lies on one), then 16 bytes each, the last one what is
+// left (maybe none).
+template <typename T> struct Cells {
+  static constexpr int E = 16 / (int)sizeof(T);
+  int begin, body, chunks, end;
+  __device__ Cells(const T* row, int b, int e) : begin(b), end(e) {
+    body = b + min((int)((-(uintptr_t)(row + b) & 15) / sizeof(T)), e - b);
+    chunks = (e - body) / E;
   }
-  if (tail + (int)threadIdx.x < end)
-    f(tail + threadIdx.x, Elem<T>::to_f(row[tail + threadIdx.x]));
+  __device__ int count() const { return chunks + 2; }
+  __device__ int first(int c) const { return c == 0 ? begin : body + (c - 1) * E; }
+  __device__ int size(int c) const {
+    return c == 0 ? body - begin : c <= chunks ? E : c == chunks + 1 ? end - body - chunks * E : 0;
+  }
+};
+// N values from wherever they lie
+template <int N, typename Q> __device__ __forceinline__ void loose(const Q* p, float (&x)[N]) {
+  typedef Q QV __attribute__((ext_vector_type(N)));
+  struct __attribute__((packed, aligned(sizeof(Q)))) Loose { QV v; };
+  const QV v = reinterpret_cast<const Loose*>(p)->v;
+#pragma unroll
+  for (int e = 0; e < N; ++e) x[e] = Elem<Q>::to_f(v[e]);
 }
 
-// A sequence's decision: how many drafts stand, and the row that follows.
-struct Decision {
-  int run, row, token;     // token: taken as it is, or -1: drawn from the row
-  int banned;              // the draft that fell, without draft probabilities; -1
-  bool rest;               // drawn from max(p - q, 0)
-  double m, c;             // the row's largest logit, log2 e / temperature
+// f(index, logit, probability) over elements [begin, end) of a row and, from the
+// same indices, one of probabilities (or none): four cells' loads at a time.
+template <typename T, typename Q, typename F>
+__device__ __forceinline__ void each(const T* row, const Q* qrow, int begin, int end, F&& f) {
+  constexpr int E = Cells<T>::E, U = 4;
+  const Cells<T> cells(row, begin, end);
+  auto edge = [&](int c) {
+    if ((int)threadIdx.x < cells.size(c)) {
+      const int i = cells.first(c) + threadIdx.x;
+      f(i, Elem<T>::to_f(row[i]), qrow ? Elem<Q>::to_f(qrow[i]) : 0.f);
+    }
+  };
+  edge(0);
+  edge(cells.chunks + 1);
+  for (int k0 = threadIdx.x; k0 < cells.chunks; k0 += U * kVT) {
+    float l[U][E], q[U][E];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * kVT, i = cells.body + (k < cells.chunks ? k : k0) * E;
+      loose(row + i, l[u]);
+      if (qrow) loose(qrow + i, q[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * kVT;
+      if (k < cells.chunks) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) f(cells.body + k * E + e, l[u][e], qrow ? q[u][e] : 0.f);
+      }
+    }
+  }
+}
+
+struct DrawLds {
+  double table[256];
+  double sums[kMaxSplits], waves[kVT / 64];
+  RowStats rows[64];
+  int flags[64];
+  int last, found, any;
 };
 
-// (uniform over the workgroup; lds: 4 doubles, flags: kVT ints)
+// Decides a sequence (uniform over the workgroup).
 template <typename T, typename Q>
-__device__ Decision decide(const Verify& a, int seq, const double* table, double* lds, int* flags) {
+__device__ Decision decide(const Verify& a, int seq, DrawLds& lds) {
   const int r0 = a.cu[seq], n = a.cu[seq + 1] - r0;
   const float t = a.temps ? a.temps[seq] : a.temp;
   const bool greedy = !(t > 0.f);
   const double c = 1.44269504088896340736 / (greedy ? 1.0 : (double)t);
+  const float cf = fminf((float)c, 0x1p100f);
   const T* logits = reinterpret_cast<const T*>(a.logits);
-  const int tid = threadIdx.x;
-  auto whole = [&](int r) {          // a row's statistics
-    const RowStats* st = a.stats + (int64_t)r * a.splits;
-    RowStats b = st[0];
-    for (int s = 1; s < a.splits; ++s) b.m = fmaxf(b.m, st[s].m);
-    b.z = 0.f;
-    b.arg = 0x7fffffff;
-    const float ref = b.m == -INFINITY ? 0.f : b.m;
-    for (int s = 0; s < a.splits; ++s) {
-      b.z += st[s].z * __builtin_amdgcn_exp2f((st[s].m - ref) * fminf((float)c, 0x1p100f));
-      if (st[s].m == b.m) b.arg = min(b.arg, st[s].arg);
-    }
-    return b;
+  const int tid = threadIdx.x, lane = tid & 63;
+  auto prob = [&](int r, int64_t x) {
+    return a.probs ? (double)Elem<Q>::to_f(
+                         reinterpret_cast<const Q*>(a.probs)[(int64_t)(r - seq) * a.probs_stride + x])
+                   : 1.0;
   };
   Decision d;
   d.c = c;
   d.run = n - 1;
-  for (int j0 = 0; j0 < n - 1; j0 += kVT) {
-    const int j = j0 + tid;
-    int state = 1;                   // 0: falls, 1: stands, 2: too close to tell
-    if (j < n - 1) {
-      const int r = r0 + j;
-      const int64_t x = a.tokens[r + 1];
-      const RowStats b = whole(r);
-      if (x < 0 || x >= a.vocab) {
-        state = 0;
-      } else if (greedy) {
-        state = b.z == b.z && b.arg == x;
-      } else {
-        const double qx =
-            a.probs ? (double)Elem<Q>::to_f(
-                          reinterpret_cast<const Q*>(a.probs)[(int64_t)(r - seq) * a.probs_stride + x])
-                    : 1.0;
-        const double ex = exp2_64(
-            ((double)Elem<T>::to_f(logits[r * a.row_stride + x]) - (double)b.m) * c, table);
-        const double need = (double)a.numbers[r] * qx * (double)b.z;
-        // the sum's error, relative: its terms' and their sums' (a.error), and what
-        // the rounding of m c does to every exponent
-        const double error = (double)a.error + fmin(fabs((double)b.m * c), 0x1p80) * 0x1p-23;
-        state = need < ex;
-        if (fabs(need - ex) <= error * fabs(need)) state = 2;
-        if (!(b.z == b.z)) state = 0;
-      }
+  RowStats b{};
+  // 64 rows at a time: a wave a row for its statistics, a lane a part (there are at
+  // most 64); then a thread a row for its test.
+  for (int j0 = 0; j0 < n; j0 += 64) {
+    const int m = min(64, n - j0);
+    for (int j = tid >> 6; j < m; j += kVT / 64) {
+      const RowStats st = lane < a.splits ? a.stats[(int64_t)(r0 + j0 + j) * a.splits + lane]
+                                          : RowStats{-INFINITY, 0.f, 0x7fffffff, 0};
+      const float top = wave_max(st.m), ref = top == -INFINITY ? 0.f : top;
+      const float z = wave_sum(st.z * __builtin_amdgcn_exp2f((st.m - ref) * cf));
+      int arg = st.m == top ? st.arg : 0x7fffffff;
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) arg = min(arg, __shfl_xor(arg, off, 64));
+      if (lane == 0) lds.rows[j] = RowStats{top, z, arg, 0};
     }
-    flags[tid] = state;
     __syncthreads();
-    int stop = min(kVT, n - 1 - j0);
-    for (int i = 0; i < stop; ++i) {
-      int s = flags[i];
+    if (tid < m) {
+      const int j = j0 + tid, r = r0 + j;
+      const RowStats s = lds.rows[tid];
+      int state = 0;                 // 0: falls, 1: stands, 2: too close to tell
+      if (j < n - 1) {
+        const int64_t x = a.tokens[r + 1];
+        if (x < 0 || x >= a.vocab || !(s.z == s.z)) {
+          state = 0;
+        } else if (greedy) {
+          state = s.arg == x;
+        } else {
+          const double ex = exp2_64(
+              ((double)Elem<T>::to_f(logits[r * a.row_stride + x]) - (double)s.m) * c, lds.table);
+          const double need = (double)a.numbers[r] * prob(r, x) * (double)s.z;
+          // the sum's error, relative: its terms' and their sums' (a.error), and what
+          // the rounding of m c does to every exponent
+          const double error = (double)a.error + fmin(fabs((double)s.m * c), 0x1p80) * 0x1p-23;
+          state = need < ex;
+          if (fabs(need - ex) <= error * fabs(need)) state = 2;
+        }
+      }
+      lds.flags[tid] = state;
+    }
+    __syncthreads();
+    int at = -1;                     // the run's end in these rows
+    for (int i = 0; i < m; ++i) {
+      const int s = lds.flags[i];
       if (s == 1) continue;
       if (s == 2) {                  // the row's sum in 64 bits
         const int r = r0 + j0 + i;
         const T* row = logits + r * a.row_stride;
-        const RowStats b = whole(r);
+        const double top = (double)lds.rows[i].m;
         double z = 0.0;
-        each(row, 0, a.vocab, [&](int, float l) { z += exp2_64(((double)l - (double)b.m) * c, table); });
-        z = block_sum64(z, lds);
+        each(row, (const Q*)nullptr, 0, a.vocab, [&](int, float l, float) {
+          z += exp2_64(((double)l - top) * c, lds.table);
+        });
+        z = block_sum64(z, lds.waves);
         const int64_t x = a.tokens[r + 1];
-        const double qx =
-            a.probs ? (double)Elem<Q>::to_f(
-                          reinterpret_cast<const Q*>(a.probs)[(int64_t)(r - seq) * a.probs_stride + x])
-                    : 1.0;
-        const double ex = exp2_64(((double)Elem<T>::to_f(row[x]) - (double)b.m) * c, table);
-        if ((double)a.numbers[r] * qx < ex / z) continue;
+        const double ex = exp2_64(((double)Elem<T>::to_f(row[x]) - top) * c, lds.table);
+        if ((double)a.numbers[r] * prob(r, x) < ex / z) continue;
       }
-      d.run = j0 + i;
+      at = i;
       break;
     }
-    __syncthreads();                 // flags are free again
-    if (d.run < n - 1) break;
+    if (at >= 0) {
+      d.run = j0 + at;
+      b = lds.rows[at];
+    }
+    __syncthreads();                 // rows and flags are free again
+    if (at >= 0) break;
   }
   d.row = r0 + d.run;
-  const RowStats b = whole(d.row);
   d.m = b.m;
   d.token = -1;
   const bool none = !(b.z == b.z) || b.m == -INFINITY;   // no distribution
   if (greedy || none) d.token = b.arg;
   if (!(b.z == b.z)) {               // a NaN, or +inf: torch's order, the first NaN first
-    if (tid == 0) flags[0] = 0x7fffffff;
+    if (tid == 0) lds.found = 0x7fffffff;
     __syncthreads();
-    each(logits + d.row * a.row_stride, 0, a.vocab, [&](int i, float l) {
-      if (l != l) atomicMin(&flags[0], i);
+    each(logits + d.row * a.row_stride, (const Q*)nullptr, 0, a.vocab, [&](int i, float l, float) {
+      if (l != l) atomicMin(&lds.found, i);
     });
     __syncthreads();
-    if (flags[0] != 0x7fffffff) d.token = flags[0];
+    if (lds.found != 0x7fffffff) d.token = lds.found;
     __syncthreads();
   }
   d.rest = d.run < n - 1 && a.probs;
@@ -333,189 +404,208 @@ __device__ Decision decide(const Verify& a, int seq, const double* table, double
   return d;
 }
 
-struct DrawLds {
-  double table[256];
-  double sums[kVT];
-  double four[kVT / 64];
-  int flags[kVT];
-  int last, found, any;
-};
-
-// The token of a sequence from its parts' sums (sums[0 .. parts)), in the
-// workgroup that arrived last: the part, then the thread, then the element whose
-// running sum passes the target. weight(index): an element's weight.
-template <typename T, typename F>
-__device__ int pick(const Verify& a, int seq, const T* row, const double* sums, DrawLds& lds,
+// The token of a sequence from its parts' sums (sums[0 .. parts) in LDS), in the
+// workgroup that arrived last: the part whose running sum passes the target, in it
+// the thread, of that thread's cells (now a lane each) the lane, and its element.
+// weight(index, logit, probability): an element's.
+template <typename T, typename Q, typename F>
+__device__ int pick(const Verify& a, int seq, const T* row, const Q* qrow, DrawLds& lds,
                     F&& weight) {
-  const int tid = threadIdx.x;
+  constexpr int E = Cells<T>::E;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float u = a.numbers[a.cu[seq + 1] - 1];
-  double total = 0.0;
-  for (int s = 0; s < a.parts; ++s) total += sums[s];
-  const double target = (double)u * total;
-  double base = 0.0;
-  int part = -1, lastp = 0;
-  for (int s = 0; s < a.parts; ++s) {
-    if (sums[s] > 0.0) lastp = s;
-    if (base + sums[s] > target) { part = s; break; }
-    base += sums[s];
-  }
-  if (part < 0) {                    // (a number of 1, or the last sum's rounding)
-    part = lastp;
-    base = INFINITY;
-  }
+  // (every wave the same: a lane a part)
+  const double own = lane < a.parts ? lds.sums[lane] : 0.0;
+  const double upto = wave_scan64(own);
+  const double target = (double)u * __shfl(upto, 63, 64);
+  const uint64_t past = __builtin_amdgcn_ballot_w64(own > 0.0 && upto > target);
+  const uint64_t some = __builtin_amdgcn_ballot_w64(own > 0.0);
+  // (a number of 1, or the last sum's rounding: the last weight of all)
+  const int part = past ? __builtin_ctzll(past) : some ? 63 - __builtin_clzll(some) : 0;
+  const double base = past ? __shfl(upto - own, part, 64) : INFINITY;
   int begin, end;
   part_of(row, a.vocab, part, a.parts, begin, end);
-  const int per = (end - begin + kVT - 1) / kVT;
-  const int b = min(begin + tid * per, end), e = min(b + per, end);
-  double mine = 0.0;
-  for (int i = b; i < e; ++i) mine += weight(i);
+  const Cells<T> cells(row, begin, end);
+  auto weights = [&](int c, double (&w)[E]) {
+    const int i = cells.first(c), n = cells.size(c);
+    float l[E] = {}, q[E] = {};
+    if (n == E) {
+      loose(row + i, l);
+      if (qrow) loose(qrow + i, q);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (e < n) {
+          l[e] = Elem<T>::to_f(row[i + e]);
+          if (qrow) q[e] = Elem<Q>::to_f(qrow[i + e]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) w[e] = e < n ? weight(i + e, l[e], q[e]) : 0.0;
+  };
+  auto sum_of = [&](int c0, int c1) {
+    double sum = 0.0;
+#pragma unroll 4
+    for (int c = c0; c < c1; ++c) {
+      double w[E];
+      weights(c, w);
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum += w[e];
+    }
+    return sum;
+  };
+  const int per = (cells.count() + kVT - 1) / kVT;
+  const double mine = sum_of(min(tid * per, cells.count()), min((tid + 1) * per, cells.count()));
+  const double scan = wave_scan64(mine);
   __syncthreads();
-  lds.sums[tid] = mine;
+  if (lane == 63) lds.waves[wave] = scan;
   if (tid == 0) {
     lds.found = 0x7fffffff;
     lds.any = -1;
   }
   __syncthreads();
-  double before = base;
-  for (int i = 0; i < tid; ++i) before += lds.sums[i];
-  if (before + mine > target && base < INFINITY) atomicMin(&lds.found, tid);
+  double before = base + (scan - mine);
+  for (int w = 0; w < wave; ++w) before += lds.waves[w];
+  if (past && mine > 0.0 && before + mine > target) atomicMin(&lds.found, tid);
   if (mine > 0.0) atomicMax(&lds.any, tid);
   __syncthreads();
   // (where rounding leaves no thread past the target: the part's last weight)
-  const bool exact = lds.found != 0x7fffffff;
-  const int owner = exact ? lds.found : lds.any;
+  const int owner = lds.found != 0x7fffffff ? lds.found : lds.any;
+  if (owner < 0) return -1;
+  if (tid == owner) lds.sums[0] = before;
   __syncthreads();
-  if (tid == owner) {
-    int got = -1;
-    double run = before;
-    for (int i = b; i < e; ++i) {
-      const double w = weight(i);
-      run += w;
-      if (w > 0.0) got = i;
-      if (exact && run > target && w > 0.0) break;
+  const double from = lds.sums[0];
+  const int c0 = owner * per, c1 = min(c0 + per, cells.count()), each_lane = (per + 63) / 64;
+  const int l0 = min(c0 + lane * each_lane, c1), l1 = min(l0 + each_lane, c1);
+  const double part_sum = sum_of(l0, l1);
+  const double up = wave_scan64(part_sum);
+  const uint64_t over = __builtin_amdgcn_ballot_w64(part_sum > 0.0 && from + up > target);
+  const uint64_t any = __builtin_amdgcn_ballot_w64(part_sum > 0.0);
+  const int at = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any);
+  int got = -1;
+  if (lane == at) {
+    double run = from + (up - part_sum);
+    bool done = false;
+    for (int c = l0; c < l1 && !done; ++c) {
+      double w[E];
+      weights(c, w);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (done) continue;
+        run += w[e];
+        if (w[e] > 0.0) {
+          got = cells.first(c) + e;
+          done = over && run > target;
+        }
+      }
     }
-    lds.found = got;
   }
-  __syncthreads();
-  const int out = owner < 0 ? -1 : lds.found;
-  __syncthreads();
-  return out;
+  return __shfl(got, at, 64);
 }
 
 // Whether this workgroup is the last of its sequence to arrive at counter k; its
-// part's sum is stored where the last one reads all of them. (Stores and loads
-// beyond the XCDs' caches; the wait before the count.)
-__device__ __forceinline__ bool arrive(const Verify& a, int seq, int k, double* at, double sum,
-                                       DrawLds& lds) {
+// part's sum is stored where the last one reads all of them, into lds.sums. (Stores
+// and loads beyond the XCDs' caches; the wait before the count.)
+__device__ __forceinline__ bool arrive(const Verify& a, int seq, int k, int s, double* sums,
+                                       double sum, DrawLds& lds) {
   if (threadIdx.x == 0) {
-    __hip_atomic_store(at, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(sums + s, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     lds.last = __hip_atomic_fetch_add(a.counters + 2 * seq + k, 1, __ATOMIC_RELAXED,
                                       __HIP_MEMORY_SCOPE_AGENT) == a.parts - 1;
   }
   __syncthreads();
-  return lds.last;
-}
-// a sequence's sums into lds.sums, by the last one to arrive
-__device__ __forceinline__ void read_sums(const Verify& a, const double* sums, DrawLds& lds) {
+  if (!lds.last) return false;
+  if ((int)threadIdx.x < a.parts)
+    lds.sums[threadIdx.x] =
+        __hip_atomic_load(sums + threadIdx.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
-  for (int s = threadIdx.x; s < a.parts; s += kVT)
-    lds.sums[s] = __hip_atomic_load(sums + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
+  return true;
 }
 
 template <typename T, typename Q>
 __global__ __launch_bounds__(kVT) void verify_draw_kernel(Verify a) {
   __shared__ DrawLds lds;
-  __shared__ double parts[kMaxSplits];
   const int seq = blockIdx.x / a.parts, s = blockIdx.x - seq * a.parts, tid = threadIdx.x;
   fill_table(lds.table);
-  const Decision d = decide<T, Q>(a, seq, lds.table, lds.four, lds.flags);
+  const Decision d = decide<T, Q>(a, seq, lds);
   int64_t* ids = a.ids + seq * a.width;
   if (s == 0) {
     const int r0 = a.cu[seq];
     for (int j = tid; j < a.width; j += kVT)
-      if (j != d.run || d.token >= 0) ids[j] = j < d.run ? a.tokens[r0 + 1 + j] : j == d.run ? d.token : -1;
-    if (tid == 0) a.accepted[seq] = d.run;
+      if (j != d.run || d.token >= 0)
+        ids[j] = j < d.run ? a.tokens[r0 + 1 + j] : j == d.run ? d.token : -1;
+    if (tid == 0) {
+      a.accepted[seq] = d.run;
+      a.decisions[seq] = d;
+    }
   }
   if (d.token >= 0) return;
   const T* row = reinterpret_cast<const T*>(a.logits) + d.row * a.row_stride;
   int begin, end;
   part_of(row, a.vocab, s, a.parts, begin, end);
   double sum = 0.0;
-  each(row, begin, end, [&](int i, float l) {
+  auto weight = [&](int i, float l, float) {
     const double w = exp2_64(((double)l - d.m) * d.c, lds.table);
-    sum += i == d.banned ? 0.0 : w;
-  });
-  sum = block_sum64(sum, lds.four);
+    return i == d.banned ? 0.0 : w;
+  };
+  const Q* const no_probs = nullptr;
+  each(row, no_probs, begin, end, [&](int i, float l, float q) { sum += weight(i, l, q); });
+  sum = block_sum64(sum, lds.waves);
   double* const sums = a.sums + (int64_t)seq * a.parts;
   if (d.rest) {                      // the row's whole sum, for the next kernel
     if (tid == 0) sums[s] = sum;
     return;
   }
-  if (!arrive(a, seq, 0, sums + s, sum, lds)) return;
-  read_sums(a, sums, lds);
-  for (int i = tid; i < a.parts; i += kVT) parts[i] = lds.sums[i];
-  __syncthreads();
-  const int got = pick(a, seq, row, parts, lds, [&](int i) {
-    return i == d.banned ? 0.0
-                         : exp2_64(((double)Elem<T>::to_f(row[i]) - d.m) * d.c, lds.table);
-  });
+  if (!arrive(a, seq, 0, s, sums, sum, lds)) return;
+  const int got = pick(a, seq, row, no_probs, lds, weight);
   if (tid == 0) ids[d.run] = got < 0 ? d.banned : got;   // (the draft is all there is)
 }
 
 template <typename T, typename Q>
 __global__ __launch_bounds__(kVT) void verify_rest_kernel(Verify a) {
   __shared__ DrawLds lds;
-  __shared__ double parts[kMaxSplits];
   const int seq = blockIdx.x / a.parts, s = blockIdx.x - seq * a.parts, tid = threadIdx.x;
-  fill_table(lds.table);
-  const Decision d = decide<T, Q>(a, seq, lds.table, lds.four, lds.flags);
+  const Decision d = a.decisions[seq];
   if (d.token >= 0 || !d.rest) return;
+  fill_table(lds.table);
   const T* row = reinterpret_cast<const T*>(a.logits) + d.row * a.row_stride;
   const Q* qrow = reinterpret_cast<const Q*>(a.probs) + (int64_t)(d.row - seq) * a.probs_stride;
   const double* const all = a.sums + (int64_t)seq * a.parts;
-  double z = 0.0;
-  for (int i = 0; i < a.parts; ++i) z += all[i];
-  const double iz = 1.0 / z;
-  auto weight = [&](int i, float l) {
-    const double w = exp2_64(((double)l - d.m) * d.c, lds.table) * iz - (double)Elem<Q>::to_f(qrow[i]);
+  const double own = (tid & 63) < a.parts ? all[tid & 63] : 0.0;   // (every wave the same)
+  const double iz = 1.0 / wave_sum64(own);
+  auto weight = [&](int, float l, float q) {
+    const double w = exp2_64(((double)l - d.m) * d.c, lds.table) * iz - (double)q;
     return w > 0.0 ? w : 0.0;
   };
   int begin, end;
   part_of(row, a.vocab, s, a.parts, begin, end);
   double sum = 0.0;
-  each(row, begin, end, [&](int i, float l) { sum += weight(i, l); });
-  sum = block_sum64(sum, lds.four);
-  double* const rest = a.rest + (int64_t)seq * a.parts;
-  if (!arrive(a, seq, 1, rest + s, sum, lds)) return;
-  read_sums(a, rest, lds);
-  for (int i = tid; i < a.parts; i += kVT) parts[i] = lds.sums[i];
-  __syncthreads();
-  double total = 0.0;
-  for (int i = 0; i < a.parts; ++i) total += parts[i];
+  each(row, qrow, begin, end, [&](int i, float l, float q) { sum += weight(i, l, q); });
+  sum = block_sum64(sum, lds.waves);
+  if (!arrive(a, seq, 1, s, a.rest + (int64_t)seq * a.parts, sum, lds)) return;
+  const bool some = __builtin_amdgcn_ballot_w64((tid & 63) < a.parts && lds.sums[tid & 63] > 0.0);
   int got;
-  if (total > 0.0) {
-    got = pick(a, seq, row, parts, lds,
-               [&](int i) { return weight(i, Elem<T>::to_f(row[i])); });
+  if (some) {
+    got = pick(a, seq, row, qrow, lds, weight);
   } else {                           // q covers p: from p
     __syncthreads();
-    for (int i = tid; i < a.parts; i += kVT) parts[i] = all[i];
+    if (tid < a.parts) lds.sums[tid] = all[tid];
     __syncthreads();
-    got = pick(a, seq, row, parts, lds, [&](int i) {
-      return exp2_64(((double)Elem<T>::to_f(row[i]) - d.m) * d.c, lds.table);
+    got = pick(a, seq, row, (const Q*)nullptr, lds, [&](int, float l, float) {
+      return exp2_64(((double)l - d.m) * d.c, lds.table);
     });
   }
   if (tid == 0) a.ids[seq * a.width + d.run] = got;
 }
 
-// Workgroups a row of the first kernel: about 2048 of them, at most 8 chunks of 16
-// bytes a thread (one round of loads) where there are enough rows, at least one.
+// Workgroups a row of the first kernel: one round of loads where that makes a thousand workgroups, fewer otherwise, at least one.
 static int32_t row_splits(int64_t n_rows, int64_t vocab, int eb) {
   const int64_t chunks = vocab * eb / 16;
-  const int64_t want = std::max<int64_t>((2048 + n_rows - 1) / n_rows, 1);
+  const int64_t round = (chunks + kChunks * kVT - 1) / (kChunks * kVT);
+  const int64_t want = std::max<int64_t>((1024 + n_rows - 1) / n_rows, round);
   const int64_t most = std::max<int64_t>(chunks / kVT, 1);
-  return (int32_t)std::min<int64_t>({want, most, kMaxSplits});
+  return (int32_t)std::max<int64_t>(std::min<int64_t>({want, most, kMaxSplits}), 1);
 }
 // Parts of a drawn row: about 1024 workgroups, at least 8 elements a thread.
 static int32_t seq_parts(int64_t n_seqs, int64_t vocab) {
@@ -524,12 +614,13 @@ static int32_t seq_parts(int64_t n_seqs, int64_t vocab) {
   return (int32_t)std::min<int64_t>({want, most, kMaxSplits});
 }
 
-struct VerifySpace { int64_t stats, sums, rest, counters, bytes; };
+struct VerifySpace { int64_t stats, decisions, sums, rest, counters, bytes; };
 static VerifySpace verify_space(int64_t rows, int64_t seqs, int64_t vocab, int eb) {
   VerifySpace s;
   const int64_t parts = seq_parts(seqs, vocab);
   s.stats = 0;
-  s.sums = rows * row_splits(rows, vocab, eb) * (int64_t)sizeof(RowStats);
+  s.decisions = rows * row_splits(rows, vocab, eb) * (int64_t)sizeof(RowStats);
+  s.sums = s.decisions + seqs * (int64_t)sizeof(Decision);
   s.rest = s.sums + seqs * parts * 8;
   s.counters = s.rest + seqs * parts * 8;
   s.bytes = s.counters + seqs * 2 * 4;
@@ -586,6 +677,7 @@ int pkv_verify_drafts(const void* logits, int64_t n_rows, int64_t vocab, int64_t
   a.numbers = numbers;
   a.temps = temperatures;
   a.stats = (RowStats*)workspace;
+  a.decisions = (Decision*)((char*)workspace + sp.decisions);
   a.sums = (double*)((char*)workspace + sp.sums);
   a.rest = (double*)((char*)workspace + sp.rest);
   a.counters = (int32_t*)((char*)workspace + sp.counters);

@@ -183,7 +183,7 @@ __global__ __launch_bounds__(kVT) void verify_stats_kernel(Verify a) {
 
 // 2^(j / 256)
 __device__ __forceinline__ void fill_table(double* table) {
-  for (int j = threadIdx.x; j < 256; j += kVT) table[j] = exp2((double)j / 256.0);
+  for (int j = threadIdx.x; j < 256; j += blockDim.x) table[j] = exp2((double)j / 256.0);
   __syncthreads();
 }
 // 2^x for x <= 0, 0 below -1000 (and for NaN): x = n / 256 + f, |f| <= 2^-9, the
@@ -217,7 +217,35 @@ __device__ __forceinline__ double wave_scan64(double v) {
   }
   return v;
 }
-// the sum over the workgroup, in every thread (4 doubles of LDS)
+// The drawing kernels' cells: eight elements of a row, a thread's step. (These
+// kernels run their code once or twice, so its length counts as well, by the
+// instruction cache's misses: their loops are rolled.)
+constexpr int kDT = 512, kCell = 8, kPart = kDT * kCell;
+
+// Eight values from wherever they lie, read where they are used.
+template <typename Q> struct Eight {
+  typedef Q QV __attribute__((ext_vector_type(8)));
+  struct __attribute__((packed, aligned(sizeof(Q)))) Loose { QV v; };
+  QV v;
+  __device__ __forceinline__ void load(const Q* row, int i, int n) {
+    if (i + 8 <= n) {
+      v = reinterpret_cast<const Loose*>(row + i)->v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = row[min(i + e, n - 1)];
+    }
+  }
+};
+
+struct DrawLds {
+  double table[256];
+  double sums[kMaxSplits], waves[kDT / 64];
+  RowStats rows[64];
+  int flags[64];
+  int last, found;
+};
+
+// The sum over the workgroup, in every thread.
 __device__ __forceinline__ double block_sum64(double v, double* lds) {
   v = wave_sum64(v);
   __syncthreads();
@@ -225,75 +253,56 @@ __device__ __forceinline__ double block_sum64(double v, double* lds) {
   __syncthreads();
   double s = 0.0;
 #pragma unroll
-  for (int w = 0; w < kVT / 64; ++w) s += lds[w];
+  for (int w = 0; w < kDT / 64; ++w) s += lds[w];
   return s;
 }
 
-// Elements [begin, end) of a row as cells: cell 0 those before the first 16-byte
-// boundary (none where begin lies on one), then 16 bytes each, the last one what is
-// left (maybe none).
-template <typename T> struct Cells {
-  static constexpr int E = 16 / (int)sizeof(T);
-  int begin, body, chunks, end;
-  __device__ Cells(const T* row, int b, int e) : begin(b), end(e) {
-    body = b + min((int)((-(uintptr_t)(row + b) & 15) / sizeof(T)), e - b);
-    chunks = (e - body) / E;
-  }
-  __device__ int count() const { return chunks + 2; }
-  __device__ int first(int c) const { return c == 0 ? begin : body + (c - 1) * E; }
-  __device__ int size(int c) const {
-    return c == 0 ? body - begin : c <= chunks ? E : c == chunks + 1 ? end - body - chunks * E : 0;
-  }
-};
-// N values from wherever they lie
-template <int N, typename Q> __device__ __forceinline__ void loose(const Q* p, float (&x)[N]) {
-  typedef Q QV __attribute__((ext_vector_type(N)));
-  struct __attribute__((packed, aligned(sizeof(Q)))) Loose { QV v; };
-  const QV v = reinterpret_cast<const Loose*>(p)->v;
+// The weights 2^((l - m) c), or, with probabilities p, max(2^((l - m) c) iz - p, 0),
+// of cells; none at `banned` and past the vocabulary.
+struct Weigh {
+  const double* table;
+  double m, c, iz;
+  int banned, vocab;
+  template <typename T, typename Q>
+  __device__ __forceinline__ double operator()(const Eight<T>& l, const Eight<Q>& p, bool rest, int i,
+                                               double (&w)[kCell]) const {
+    double sum = 0.0;
 #pragma unroll
-  for (int e = 0; e < N; ++e) x[e] = Elem<Q>::to_f(v[e]);
-}
-
-// f(index, logit, probability) over elements [begin, end) of a row and, from the
-// same indices, one of probabilities (or none): four cells' loads at a time.
-template <typename T, typename Q, typename F>
-__device__ __forceinline__ void each(const T* row, const Q* qrow, int begin, int end, F&& f) {
-  constexpr int E = Cells<T>::E, U = 4;
-  const Cells<T> cells(row, begin, end);
-  auto edge = [&](int c) {
-    if ((int)threadIdx.x < cells.size(c)) {
-      const int i = cells.first(c) + threadIdx.x;
-      f(i, Elem<T>::to_f(row[i]), qrow ? Elem<Q>::to_f(qrow[i]) : 0.f);
-    }
-  };
-  edge(0);
-  edge(cells.chunks + 1);
-  for (int k0 = threadIdx.x; k0 < cells.chunks; k0 += U * kVT) {
-    float l[U][E], q[U][E];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = k0 + u * kVT, i = cells.body + (k < cells.chunks ? k : k0) * E;
-      loose(row + i, l[u]);
-      if (qrow) loose(qrow + i, q[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = k0 + u * kVT;
-      if (k < cells.chunks) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) f(cells.body + k * E + e, l[u][e], qrow ? q[u][e] : 0.f);
+    for (int e = 0; e < kCell; ++e) {
+      double x = exp2_64(((double)Elem<T>::to_f(l.v[e]) - m) * c, table);
+      if (rest) {
+        x = x * iz - (double)Elem<Q>::to_f(p.v[e]);
+        x = x > 0.0 ? x : 0.0;
       }
+      w[e] = i + e < vocab && i + e != banned ? x : 0.0;
+      sum += w[e];
     }
+    return sum;
   }
-}
-
-struct DrawLds {
-  double table[256];
-  double sums[kMaxSplits], waves[kVT / 64];
-  RowStats rows[64];
-  int flags[64];
-  int last, found, any;
 };
+
+// The sum of a thread's cells, from element `at` on, `step` elements apart, `count`
+// of them; the next one is on its way while one is weighed. w: the last one's.
+template <typename T, typename Q>
+__device__ __forceinline__ double weigh_run(const T* row, const Q* q, int at, int step, int count,
+                                            const Weigh& weigh, double (&w)[kCell]) {
+  Eight<T> l, l2;
+  Eight<Q> p{}, p2{};
+  const int n = weigh.vocab, last = n - 1;
+  l.load(row, min(at, last), n);
+  if (q) p.load(q, min(at, last), n);
+  double sum = 0.0;
+#pragma unroll 1
+  for (int r = 0; r < count; ++r, at += step) {
+    const int next = min(r + 1 < count ? at + step : at, last);
+    l2.load(row, next, n);
+    if (q) p2.load(q, next, n);
+    sum += weigh(l, p, q != nullptr, at, w);
+    l = l2;
+    p = p2;
+  }
+  return sum;
+}
 
 // Decides a sequence (uniform over the workgroup).
 template <typename T, typename Q>
@@ -305,20 +314,30 @@ __device__ Decision decide(const Verify& a, int seq, DrawLds& lds) {
   const float cf = fminf((float)c, 0x1p100f);
   const T* logits = reinterpret_cast<const T*>(a.logits);
   const int tid = threadIdx.x, lane = tid & 63;
-  auto prob = [&](int r, int64_t x) {
-    return a.probs ? (double)Elem<Q>::to_f(
-                         reinterpret_cast<const Q*>(a.probs)[(int64_t)(r - seq) * a.probs_stride + x])
-                   : 1.0;
-  };
   Decision d;
   d.c = c;
   d.run = n - 1;
   RowStats b{};
-  // 64 rows at a time: a wave a row for its statistics, a lane a part (there are at
-  // most 64); then a thread a row for its test.
+  // 64 rows at a time: a thread a row reads what its test needs, a wave a row its
+  // statistics, a lane a part (there are at most 64); then the threads test.
   for (int j0 = 0; j0 < n; j0 += 64) {
     const int m = min(64, n - j0);
-    for (int j = tid >> 6; j < m; j += kVT / 64) {
+    int64_t x = -1;
+    float u = 0.f, lx = 0.f, qx = 1.f;
+    if (tid < m && j0 + tid < n - 1) {
+      const int r = r0 + j0 + tid;
+      x = a.tokens[r + 1];
+      u = a.numbers[r];
+      if (x >= 0 && x < a.vocab) {
+        lx = Elem<T>::to_f(logits[r * a.row_stride + x]);
+        if (a.probs)
+          qx = Elem<Q>::to_f(
+              reinterpret_cast<const Q*>(a.probs)[(int64_t)(r - seq) * a.probs_stride + x]);
+      } else {
+        x = -1;
+      }
+    }
+    for (int j = tid >> 6; j < m; j += kDT / 64) {
       const RowStats st = lane < a.splits ? a.stats[(int64_t)(r0 + j0 + j) * a.splits + lane]
                                           : RowStats{-INFINITY, 0.f, 0x7fffffff, 0};
       const float top = wave_max(st.m), ref = top == -INFINITY ? 0.f : top;
@@ -329,25 +348,21 @@ __device__ Decision decide(const Verify& a, int seq, DrawLds& lds) {
       if (lane == 0) lds.rows[j] = RowStats{top, z, arg, 0};
     }
     __syncthreads();
+    double ex = 0.0, need = 0.0;
     if (tid < m) {
-      const int j = j0 + tid, r = r0 + j;
       const RowStats s = lds.rows[tid];
       int state = 0;                 // 0: falls, 1: stands, 2: too close to tell
-      if (j < n - 1) {
-        const int64_t x = a.tokens[r + 1];
-        if (x < 0 || x >= a.vocab || !(s.z == s.z)) {
-          state = 0;
-        } else if (greedy) {
+      if (x >= 0 && s.z == s.z) {
+        if (greedy) {
           state = s.arg == x;
         } else {
-          const double ex = exp2_64(
-              ((double)Elem<T>::to_f(logits[r * a.row_stride + x]) - (double)s.m) * c, lds.table);
-          const double need = (double)a.numbers[r] * prob(r, x) * (double)s.z;
+          ex = exp2_64(((double)lx - (double)s.m) * c, lds.table);
+          need = (double)u * (double)qx;
+          const double sum = need * (double)s.z;
           // the sum's error, relative: its terms' and their sums' (a.error), and what
           // the rounding of m c does to every exponent
           const double error = (double)a.error + fmin(fabs((double)s.m * c), 0x1p80) * 0x1p-23;
-          state = need < ex;
-          if (fabs(need - ex) <= error * fabs(need)) state = 2;
+          state = fabs(sum - ex) <= error * fabs(sum) ? 2 : sum < ex;
         }
       }
       lds.flags[tid] = state;
@@ -358,17 +373,17 @@ __device__ Decision decide(const Verify& a, int seq, DrawLds& lds) {
       const int s = lds.flags[i];
       if (s == 1) continue;
       if (s == 2) {                  // the row's sum in 64 bits
-        const int r = r0 + j0 + i;
-        const T* row = logits + r * a.row_stride;
         const double top = (double)lds.rows[i].m;
-        double z = 0.0;
-        each(row, (const Q*)nullptr, 0, a.vocab, [&](int, float l, float) {
-          z += exp2_64(((double)l - top) * c, lds.table);
-        });
-        z = block_sum64(z, lds.waves);
-        const int64_t x = a.tokens[r + 1];
-        const double ex = exp2_64(((double)Elem<T>::to_f(row[x]) - top) * c, lds.table);
-        if ((double)a.numbers[r] * prob(r, x) < ex / z) continue;
+        double w[kCell];
+        const double z = block_sum64(
+            weigh_run(logits + (r0 + j0 + i) * a.row_stride, (const Q*)nullptr, tid * kCell, kPart,
+                      (a.vocab + kPart - 1) / kPart, Weigh{lds.table, top, c, 1.0, -1, a.vocab}, w),
+            lds.waves);
+        if (tid == i) lds.last = need < ex / z;
+        __syncthreads();
+        const bool stands = lds.last;
+        __syncthreads();
+        if (stands) continue;
       }
       at = i;
       break;
@@ -388,9 +403,10 @@ __device__ Decision decide(const Verify& a, int seq, DrawLds& lds) {
   if (!(b.z == b.z)) {               // a NaN, or +inf: torch's order, the first NaN first
     if (tid == 0) lds.found = 0x7fffffff;
     __syncthreads();
-    each(logits + d.row * a.row_stride, (const Q*)nullptr, 0, a.vocab, [&](int i, float l, float) {
+    for (int i = tid; i < a.vocab; i += kDT) {
+      const float l = Elem<T>::to_f(logits[d.row * a.row_stride + i]);
       if (l != l) atomicMin(&lds.found, i);
-    });
+    }
     __syncthreads();
     if (lds.found != 0x7fffffff) d.token = lds.found;
     __syncthreads();
@@ -404,127 +420,101 @@ __device__ Decision decide(const Verify& a, int seq, DrawLds& lds) {
   return d;
 }
 
-// The token of a sequence from its parts' sums (sums[0 .. parts) in LDS), in the
-// workgroup that arrived last: the part whose running sum passes the target, in it
-// the thread, of that thread's cells (now a lane each) the lane, and its element.
-// weight(index, logit, probability): an element's.
-template <typename T, typename Q, typename F>
-__device__ int pick(const Verify& a, int seq, const T* row, const Q* qrow, DrawLds& lds,
-                    F&& weight) {
-  constexpr int E = Cells<T>::E;
+// Sums part s of the row that a sequence draws from; the workgroup that is the last
+// to (counter k) finds the token: the part whose running sum passes the target, in
+// it the thread, its element. Returns it there (-1: no weight at all, and then
+// none_left is set), -2 in the others. sums: the parts', beyond the XCDs' caches.
+enum DrawMode { kSumOnly, kCounted, kKnown };   // kKnown: sums hold all parts' already
+
+template <typename T, typename Q>
+__device__ int draw(const Verify& a, int seq, int s, const Decision& d, const T* row, const Q* q,
+                    double iz, int k, double* sums, DrawMode mode, DrawLds& lds) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const float u = a.numbers[a.cu[seq + 1] - 1];
-  // (every wave the same: a lane a part)
-  const double own = lane < a.parts ? lds.sums[lane] : 0.0;
-  const double upto = wave_scan64(own);
-  const double target = (double)u * __shfl(upto, 63, 64);
-  const uint64_t past = __builtin_amdgcn_ballot_w64(own > 0.0 && upto > target);
-  const uint64_t some = __builtin_amdgcn_ballot_w64(own > 0.0);
-  // (a number of 1, or the last sum's rounding: the last weight of all)
-  const int part = past ? __builtin_ctzll(past) : some ? 63 - __builtin_clzll(some) : 0;
-  const double base = past ? __shfl(upto - own, part, 64) : INFINITY;
-  int begin, end;
-  part_of(row, a.vocab, part, a.parts, begin, end);
-  const Cells<T> cells(row, begin, end);
-  auto weights = [&](int c, double (&w)[E]) {
-    const int i = cells.first(c), n = cells.size(c);
-    float l[E] = {}, q[E] = {};
-    if (n == E) {
-      loose(row + i, l);
-      if (qrow) loose(qrow + i, q);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (e < n) {
-          l[e] = Elem<T>::to_f(row[i + e]);
-          if (qrow) q[e] = Elem<Q>::to_f(qrow[i + e]);
-        }
+  // kDT cells a part, or, where the vocabulary takes more, runs of cells a thread
+  const int per = (a.vocab + a.parts * kPart - 1) / (a.parts * kPart);
+  const Weigh weigh{lds.table, d.m, d.c, iz, d.banned, a.vocab};
+  int part = s;
+  double target = 0.0, base = 0.0;
+  bool past = false, found = false;
+  for (;;) {                         // first the part's sum, then (the last one) the token
+    const int first = (part * kDT + tid) * per * kCell;
+    const int count = first < a.vocab ? min(per, (a.vocab - first + kCell - 1) / kCell) : 0;
+    double w[kCell] = {}, mine = 0.0;
+    if (found || mode != kKnown) mine = weigh_run(row, q, first, kCell, count, weigh, w);
+    if (!found) {
+      const double sum = mode == kKnown ? 0.0 : block_sum64(mine, lds.waves);
+      if (mode == kSumOnly) {
+        if (tid == 0) sums[s] = sum;
+        return -2;
+      }
+      if (mode == kCounted && tid == 0) {
+        __hip_atomic_store(sums + s, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        lds.last = __hip_atomic_fetch_add(a.counters + 2 * seq + k, 1, __ATOMIC_RELAXED,
+                                          __HIP_MEMORY_SCOPE_AGENT) == a.parts - 1;
+      }
+      __syncthreads();
+      if (mode == kCounted && !lds.last) return -2;
+      // (every wave the same: a lane a part)
+      const double own =
+          lane < a.parts
+              ? __hip_atomic_load(sums + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+              : 0.0;
+      const double upto = wave_scan64(own);
+      target = (double)a.numbers[a.cu[seq + 1] - 1] * __shfl(upto, 63, 64);
+      const uint64_t over = __builtin_amdgcn_ballot_w64(own > 0.0 && upto > target);
+      const uint64_t some = __builtin_amdgcn_ballot_w64(own > 0.0);
+      if (!some) return -1;
+      // (a number of 1, or the last sum's rounding: the last weight of all)
+      past = over;
+      part = past ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
+      base = past ? __shfl(upto - own, part, 64) : 0.0;
+      found = true;
+      continue;
     }
-#pragma unroll
-    for (int e = 0; e < E; ++e) w[e] = e < n ? weight(i + e, l[e], q[e]) : 0.0;
-  };
-  auto sum_of = [&](int c0, int c1) {
-    double sum = 0.0;
-#pragma unroll 4
-    for (int c = c0; c < c1; ++c) {
-      double w[E];
-      weights(c, w);
-#pragma unroll
-      for (int e = 0; e < E; ++e) sum += w[e];
+    const double scan = wave_scan64(mine);
+    __syncthreads();
+    if (lane == 63) lds.waves[wave] = scan;
+    __syncthreads();
+    double run = base + (scan - mine);
+    for (int v = 0; v < wave; ++v) run += lds.waves[v];
+    const uint64_t over = __builtin_amdgcn_ballot_w64(past && mine > 0.0 && run + mine > target);
+    const uint64_t any = __builtin_amdgcn_ballot_w64(mine > 0.0);
+    if (lane == 0) {
+      lds.flags[wave] = over ? tid + __builtin_ctzll(over) : -1;
+      lds.flags[kDT / 64 + wave] = any ? tid + 63 - __builtin_clzll(any) : -1;
     }
-    return sum;
-  };
-  const int per = (cells.count() + kVT - 1) / kVT;
-  const double mine = sum_of(min(tid * per, cells.count()), min((tid + 1) * per, cells.count()));
-  const double scan = wave_scan64(mine);
-  __syncthreads();
-  if (lane == 63) lds.waves[wave] = scan;
-  if (tid == 0) {
-    lds.found = 0x7fffffff;
-    lds.any = -1;
-  }
-  __syncthreads();
-  double before = base + (scan - mine);
-  for (int w = 0; w < wave; ++w) before += lds.waves[w];
-  if (past && mine > 0.0 && before + mine > target) atomicMin(&lds.found, tid);
-  if (mine > 0.0) atomicMax(&lds.any, tid);
-  __syncthreads();
-  // (where rounding leaves no thread past the target: the part's last weight)
-  const int owner = lds.found != 0x7fffffff ? lds.found : lds.any;
-  if (owner < 0) return -1;
-  if (tid == owner) lds.sums[0] = before;
-  __syncthreads();
-  const double from = lds.sums[0];
-  const int c0 = owner * per, c1 = min(c0 + per, cells.count()), each_lane = (per + 63) / 64;
-  const int l0 = min(c0 + lane * each_lane, c1), l1 = min(l0 + each_lane, c1);
-  const double part_sum = sum_of(l0, l1);
-  const double up = wave_scan64(part_sum);
-  const uint64_t over = __builtin_amdgcn_ballot_w64(part_sum > 0.0 && from + up > target);
-  const uint64_t any = __builtin_amdgcn_ballot_w64(part_sum > 0.0);
-  const int at = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any);
-  int got = -1;
-  if (lane == at) {
-    double run = from + (up - part_sum);
-    bool done = false;
-    for (int c = l0; c < l1 && !done; ++c) {
-      double w[E];
-      weights(c, w);
+    __syncthreads();
+    // (where rounding leaves no thread past the target: the part's last weight)
+    int owner = -1, latest = -1;
+    for (int v = kDT / 64 - 1; v >= 0; --v) {
+      owner = lds.flags[v] >= 0 ? lds.flags[v] : owner;
+      latest = max(latest, lds.flags[kDT / 64 + v]);
+    }
+    const bool exact = owner >= 0;
+    if (tid == (exact ? owner : latest)) {
+      int got = -1;
+      bool done = false;
+      for (int r = 0; r < count && !done; ++r) {
+        if (count > 1) weigh_run(row, q, first + r * kCell, kCell, 1, weigh, w);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        if (done) continue;
-        run += w[e];
-        if (w[e] > 0.0) {
-          got = cells.first(c) + e;
-          done = over && run > target;
+        for (int e = 0; e < kCell; ++e) {
+          run += done ? 0.0 : w[e];
+          if (!done && w[e] > 0.0) {
+            got = first + r * kCell + e;
+            done = exact && run > target;
+          }
         }
       }
+      lds.found = got;
     }
+    __syncthreads();
+    return lds.found;
   }
-  return __shfl(got, at, 64);
-}
-
-// Whether this workgroup is the last of its sequence to arrive at counter k; its
-// part's sum is stored where the last one reads all of them, into lds.sums. (Stores
-// and loads beyond the XCDs' caches; the wait before the count.)
-__device__ __forceinline__ bool arrive(const Verify& a, int seq, int k, int s, double* sums,
-                                       double sum, DrawLds& lds) {
-  if (threadIdx.x == 0) {
-    __hip_atomic_store(sums + s, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    lds.last = __hip_atomic_fetch_add(a.counters + 2 * seq + k, 1, __ATOMIC_RELAXED,
-                                      __HIP_MEMORY_SCOPE_AGENT) == a.parts - 1;
-  }
-  __syncthreads();
-  if (!lds.last) return false;
-  if ((int)threadIdx.x < a.parts)
-    lds.sums[threadIdx.x] =
-        __hip_atomic_load(sums + threadIdx.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  return true;
 }
 
 template <typename T, typename Q>
-__global__ __launch_bounds__(kVT) void verify_draw_kernel(Verify a) {
+__global__ __launch_bounds__(kDT) void verify_draw_kernel(Verify a) {
   __shared__ DrawLds lds;
   const int seq = blockIdx.x / a.parts, s = blockIdx.x - seq * a.parts, tid = threadIdx.x;
   fill_table(lds.table);
@@ -532,7 +522,7 @@ __global__ __launch_bounds__(kVT) void verify_draw_kernel(Verify a) {
   int64_t* ids = a.ids + seq * a.width;
   if (s == 0) {
     const int r0 = a.cu[seq];
-    for (int j = tid; j < a.width; j += kVT)
+    for (int j = tid; j < a.width; j += kDT)
       if (j != d.run || d.token >= 0)
         ids[j] = j < d.run ? a.tokens[r0 + 1 + j] : j == d.run ? d.token : -1;
     if (tid == 0) {
@@ -541,61 +531,29 @@ __global__ __launch_bounds__(kVT) void verify_draw_kernel(Verify a) {
     }
   }
   if (d.token >= 0) return;
-  const T* row = reinterpret_cast<const T*>(a.logits) + d.row * a.row_stride;
-  int begin, end;
-  part_of(row, a.vocab, s, a.parts, begin, end);
-  double sum = 0.0;
-  auto weight = [&](int i, float l, float) {
-    const double w = exp2_64(((double)l - d.m) * d.c, lds.table);
-    return i == d.banned ? 0.0 : w;
-  };
-  const Q* const no_probs = nullptr;
-  each(row, no_probs, begin, end, [&](int i, float l, float q) { sum += weight(i, l, q); });
-  sum = block_sum64(sum, lds.waves);
-  double* const sums = a.sums + (int64_t)seq * a.parts;
-  if (d.rest) {                      // the row's whole sum, for the next kernel
-    if (tid == 0) sums[s] = sum;
-    return;
-  }
-  if (!arrive(a, seq, 0, s, sums, sum, lds)) return;
-  const int got = pick(a, seq, row, no_probs, lds, weight);
-  if (tid == 0) ids[d.run] = got < 0 ? d.banned : got;   // (the draft is all there is)
+  // (d.rest: the row's whole sum alone, for the next kernel)
+  const int got = draw(a, seq, s, d, reinterpret_cast<const T*>(a.logits) + d.row * a.row_stride,
+                       (const Q*)nullptr, 1.0, 0, a.sums + (int64_t)seq * a.parts, d.rest ? kSumOnly : kCounted,
+                       lds);
+  if (got > -2 && tid == 0) ids[d.run] = got < 0 ? d.banned : got;   // (the draft is all there is)
 }
 
 template <typename T, typename Q>
-__global__ __launch_bounds__(kVT) void verify_rest_kernel(Verify a) {
+__global__ __launch_bounds__(kDT) void verify_rest_kernel(Verify a) {
   __shared__ DrawLds lds;
   const int seq = blockIdx.x / a.parts, s = blockIdx.x - seq * a.parts, tid = threadIdx.x;
   const Decision d = a.decisions[seq];
   if (d.token >= 0 || !d.rest) return;
   fill_table(lds.table);
   const T* row = reinterpret_cast<const T*>(a.logits) + d.row * a.row_stride;
-  const Q* qrow = reinterpret_cast<const Q*>(a.probs) + (int64_t)(d.row - seq) * a.probs_stride;
+  const Q* q = reinterpret_cast<const Q*>(a.probs) + (int64_t)(d.row - seq) * a.probs_stride;
   const double* const all = a.sums + (int64_t)seq * a.parts;
   const double own = (tid & 63) < a.parts ? all[tid & 63] : 0.0;   // (every wave the same)
-  const double iz = 1.0 / wave_sum64(own);
-  auto weight = [&](int, float l, float q) {
-    const double w = exp2_64(((double)l - d.m) * d.c, lds.table) * iz - (double)q;
-    return w > 0.0 ? w : 0.0;
-  };
-  int begin, end;
-  part_of(row, a.vocab, s, a.parts, begin, end);
-  double sum = 0.0;
-  each(row, qrow, begin, end, [&](int i, float l, float q) { sum += weight(i, l, q); });
-  sum = block_sum64(sum, lds.waves);
-  if (!arrive(a, seq, 1, s, a.rest + (int64_t)seq * a.parts, sum, lds)) return;
-  const bool some = __builtin_amdgcn_ballot_w64((tid & 63) < a.parts && lds.sums[tid & 63] > 0.0);
-  int got;
-  if (some) {
-    got = pick(a, seq, row, qrow, lds, weight);
-  } else {                           // q covers p: from p
-    __syncthreads();
-    if (tid < a.parts) lds.sums[tid] = all[tid];
-    __syncthreads();
-    got = pick(a, seq, row, (const Q*)nullptr, lds, [&](int, float l, float) {
-      return exp2_64(((double)l - d.m) * d.c, lds.table);
-    });
-  }
+  int got = draw(a, seq, s, d, row, q, 1.0 / wave_sum64(own), 1, a.rest + (int64_t)seq * a.parts,
+                 kCounted, lds);
+  if (got == -2) return;
+  if (got == -1)                     // q covers p: from p, by the sums of before
+    got = draw(a, seq, s, d, row, (const Q*)nullptr, 1.0, 0, const_cast<double*>(all), kKnown, lds);
   if (tid == 0) a.ids[seq * a.width + d.run] = got;
 }
 
@@ -607,10 +565,10 @@ static int32_t row_splits(int64_t n_rows, int64_t vocab, int eb) {
   const int64_t most = std::max<int64_t>(chunks / kVT, 1);
   return (int32_t)std::max<int64_t>(std::min<int64_t>({want, most, kMaxSplits}), 1);
 }
-// Parts of a drawn row: about 1024 workgroups, at least 8 elements a thread.
+// Parts of a drawn row: about 512 workgroups (two a compute unit; each repeats the
+// decision, which takes as long as two cells), a cell a thread at least.
 static int32_t seq_parts(int64_t n_seqs, int64_t vocab) {
-  const int64_t want = std::max<int64_t>((1024 + n_seqs - 1) / n_seqs, 1);
-  const int64_t most = std::max<int64_t>(vocab / (8 * kVT), 1);
+  const int64_t want = (512 + n_seqs - 1) / n_seqs, most = (vocab + 4095) / 4096;
   return (int32_t)std::min<int64_t>({want, most, kMaxSplits});
 }
 
@@ -702,10 +660,10 @@ int pkv_verify_drafts(const void* logits, int64_t n_rows, int64_t vocab, int64_t
     typedef decltype(probs) Q;
     hipLaunchKernelGGL(verify_stats_kernel<T>, dim3(rows), dim3(kVT), 0, s, a);
     PKV_LAUNCH_CHECK();
-    hipLaunchKernelGGL((verify_draw_kernel<T, Q>), dim3(seqs), dim3(kVT), 0, s, a);
+    hipLaunchKernelGGL((verify_draw_kernel<T, Q>), dim3(seqs), dim3(kDT), 0, s, a);
     PKV_LAUNCH_CHECK();
     if (a.probs) {
-      hipLaunchKernelGGL((verify_rest_kernel<T, Q>), dim3(seqs), dim3(kVT), 0, s, a);
+      hipLaunchKernelGGL((verify_rest_kernel<T, Q>), dim3(seqs), dim3(kDT), 0, s, a);
       PKV_LAUNCH_CHECK();
     }
     return PKV_OK;

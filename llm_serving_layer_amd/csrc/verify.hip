@@ -186,18 +186,19 @@ __device__ __forceinline__ void fill_table(double* table) {
   for (int j = threadIdx.x; j < 256; j += blockDim.x) table[j] = exp2((double)j / 256.0);
   __syncthreads();
 }
-// 2^x for x <= 0, 0 below -1000 (and for NaN): x = n / 256 + f, |f| <= 2^-9, the
-// polynomial's rest below 2^-55.
+// 2^x for x <= 0, 0 below -1000 (and for NaN): x = n / 256 + g, |g| <= 2^-9; 2^g =
+// e^(g ln 2) by its series, the rest below 2^-54.
 __device__ __forceinline__ double exp2_64(double x, const double* table) {
   constexpr double kMagic = 6755399441055744.0 / 256.0;   // 1.5 2^52 / 256: adds round to n / 256
+  constexpr double kLn2 = 0.693147180559945309417;
   const double at = x + kMagic;
-  const double f = (x - (at - kMagic)) * 0.693147180559945309417;
+  const double g = x - (at - kMagic);
   const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, at);
-  double p = __builtin_fma(f, 1.0 / 24.0, 1.0 / 6.0);
-  p = __builtin_fma(f, p, 0.5);
-  p = __builtin_fma(f, p, 1.0);
+  double p = __builtin_fma(g, kLn2 * kLn2 * kLn2 * kLn2 / 24.0, kLn2 * kLn2 * kLn2 / 6.0);
+  p = __builtin_fma(g, p, kLn2 * kLn2 / 2.0);
+  p = __builtin_fma(g, p, kLn2);
   const double base = table[n & 255];
-  const double y = __builtin_fma(base * f, p, base);
+  const double y = __builtin_fma(base * g, p, base);
   const uint64_t bits = __builtin_bit_cast(uint64_t, y) + ((uint64_t)(uint32_t)(n >> 8) << 52);
   return x >= -1000.0 ? __builtin_bit_cast(double, bits) : 0.0;
 }
@@ -274,9 +275,15 @@ struct Weigh {
         x = x * iz - (double)Elem<Q>::to_f(p.v[e]);
         x = x > 0.0 ? x : 0.0;
       }
-      w[e] = i + e < vocab && i + e != banned ? x : 0.0;
-      sum += w[e];
+      w[e] = x;
     }
+    if (i + kCell > vocab || (unsigned)(banned - i) < (unsigned)kCell) {
+#pragma unroll
+      for (int e = 0; e < kCell; ++e)
+        if (i + e >= vocab || i + e == banned) w[e] = 0.0;
+    }
+#pragma unroll
+    for (int e = 0; e < kCell; ++e) sum += w[e];
     return sum;
   }
 };
@@ -492,24 +499,39 @@ __device__ int draw(const Verify& a, int seq, int s, const Decision& d, const T*
       latest = max(latest, lds.flags[kDT / 64 + v]);
     }
     const bool exact = owner >= 0;
-    if (tid == (exact ? owner : latest)) {
-      int got = -1;
+    owner = exact ? owner : latest;
+    if (tid == owner) {
+      lds.waves[0] = run;
+      lds.last = count;
+    }
+    __syncthreads();
+    // the thread's cells, now a lane each (a run of them where they are more)
+    const double from = lds.waves[0];
+    const int cells = lds.last, each = (cells + 63) / 64;
+    const int at = (part * kDT + owner) * per * kCell + lane * each * kCell;
+    const int here = max(0, min(each, cells - lane * each));
+    const double sum = weigh_run(row, q, at, kCell, here, weigh, w);
+    const double up = wave_scan64(sum);
+    const uint64_t in = __builtin_amdgcn_ballot_w64(sum > 0.0 && exact && from + up > target);
+    const uint64_t weighty = __builtin_amdgcn_ballot_w64(sum > 0.0);
+    const int of = in ? __builtin_ctzll(in) : 63 - __builtin_clzll(weighty);
+    int got = -1;
+    if (lane == of) {
+      double r0 = from + (up - sum);
       bool done = false;
-      for (int r = 0; r < count && !done; ++r) {
-        if (count > 1) weigh_run(row, q, first + r * kCell, kCell, 1, weigh, w);
+      for (int r = 0; r < here && !done; ++r) {
+        if (here > 1) weigh_run(row, q, at + r * kCell, kCell, 1, weigh, w);
 #pragma unroll
         for (int e = 0; e < kCell; ++e) {
-          run += done ? 0.0 : w[e];
+          r0 += done ? 0.0 : w[e];
           if (!done && w[e] > 0.0) {
-            got = first + r * kCell + e;
-            done = exact && run > target;
+            got = at + r * kCell + e;
+            done = in && r0 > target;
           }
         }
       }
-      lds.found = got;
     }
-    __syncthreads();
-    return lds.found;
+    return __shfl(got, of, 64);
   }
 }
 

@@ -26,7 +26,7 @@ import torch
 
 from . import _native
 from .assembly import ScheduledSeq, build_batch_meta, build_token_tensor
-from .backend import _DTYPES, _capturing, _current_stream
+from .backend import _DTYPES, _HERE, _capturing, _current_device, _current_stream
 from .contract import BatchMeta
 
 __all__ = ["greedy", "verify_drafts", "StepTimer", "greedy_step"]
@@ -150,20 +150,23 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, meta: BatchMeta,
                            "while a graph is captured")
     else:
         lens = meta.query_lens.cpu().numpy()
-    if int(lens.min()) < 1 or int(lens.sum()) != rows:
+    if lens.min() < 1 or lens.sum() != rows:
         raise ValueError(f"query_lens ({int(lens.min())} at least, {int(lens.sum())} in all) do "
                          f"not make up {rows} rows")
     width = int(lens.max())
     logits = rows_for_kernel(logits)
     tokens, uniforms = tokens.contiguous(), uniforms.contiguous()
-    cu, owner = (t.to(device=dev, dtype=torch.int32).contiguous()
-                 for t in (meta.cu_query_lens, meta.batch_indices))
+    cu, owner = meta.cu_query_lens, meta.batch_indices
+    if not (cu.dtype is owner.dtype is torch.int32 and cu.device == owner.device == dev
+            and cu.is_contiguous() and owner.is_contiguous()):
+        cu, owner = (t.to(device=dev, dtype=torch.int32).contiguous() for t in (cu, owner))
     ids = torch.empty((n, width), dtype=torch.int64, device=dev)
     accepted = torch.empty(n, dtype=torch.int64, device=dev)
     lib, code = _native.load(), _DTYPES[logits.dtype]
     ws = torch.empty(lib.pkv_verify_workspace_bytes(rows, n, vocab, code), dtype=torch.uint8,
                      device=dev)
-    with torch.cuda.device(dev):
+    here = _HERE if _current_device() == dev.index else torch.cuda.device(dev)
+    with here:
         rc = lib.pkv_verify_drafts(
             logits.data_ptr(), rows, vocab, logits.stride(0) if rows > 1 else vocab, code,
             tokens.data_ptr(), cu.data_ptr(), owner.data_ptr(), n, uniforms.data_ptr(),

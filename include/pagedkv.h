@@ -553,8 +553,9 @@ int pkv_read_4bit(const void* k_pool, const void* v_pool, int64_t num_blocks,
  * fewer) with pieces of 28 ints {first token's row in q, tokens, its position,
  * kv_len, first page in kv_indices, pages, first tile of 64 keys, tiles, partial
  * slot or -1, the first piece's slot, pieces, arrival counter, the pages of the
- * first 256 keys' 16 units}, those of sequences with
- * at most 16 query rows (tokens x query heads a KV head) first, and the plan
+ * first 256 keys' 16 units}, n_few those of sequences with
+ * at most 16 query rows (tokens x query heads a KV head), n_wide of 32 rows, n_tall
+ * of 128, and the plan
  * fields of *plan; long rows are cut to fill compute_units compute units. Geometries without a matrix-core kernel (head_dim
  * other than 64 and 128, f32, pages that are no power of two times 16, more than
  * 32 query heads a KV head) need no items.
@@ -575,7 +576,7 @@ typedef struct pkv_4bit {
   void* workspace;
   int32_t* status_word;
   int32_t n_seqs, n_tokens, n_heads, n_kv_heads, head_dim, page_size, dtype;
-  int32_t n_few, n_wide, few_rows, few_waves, part_rows, n_slots, n_cuts;   /* the plan's */
+  int32_t n_few, n_wide, n_tall, few_rows, few_waves, part_rows, n_slots, n_cuts;   /* the plan's */
 } pkv_4bit;
 
 int pkv_plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr,

@@ -143,7 +143,7 @@ class FourBit(C.Structure):
                 *[(n, _p) for n in ("cu_query_lens", "kv_indptr", "kv_indices", "kv_lens",
                                     "batch_indices", "items", "workspace", "status_word")],
                 *[(n, _i32) for n in ("n_seqs", "n_tokens", "n_heads", "n_kv_heads", "head_dim",
-                                      "page_size", "dtype", "n_few", "n_wide", "few_rows",
+                                      "page_size", "dtype", "n_few", "n_wide", "n_tall", "few_rows",
                                       "few_waves", "part_rows", "n_slots", "n_cuts")]]
 
 

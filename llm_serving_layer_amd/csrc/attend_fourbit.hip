@@ -39,7 +39,7 @@
 #include <exception>
 #include <vector>
 
-#include "fourbit.h"
+#include "attend_fourbit.h"
 
 namespace pkv {
 
@@ -48,34 +48,14 @@ int check_4bit(int32_t n_kv, int32_t d, int32_t ps);
 int run_4bit_any(const pkv_4bit& b, const void* q, void* out, const void* k_pool,
                  const void* v_pool, float scale, hipStream_t s);
 
-constexpr int kTile = 64;          // keys
-// A piece: {first token's row in q, tokens, its position, kv_len, first page in
-// kv_indices, pages, tile, tiles, partial slot | -1, slot 0, pieces, counter}, then
-// the pages of the first four tiles' units.
-constexpr int kPieceInts = 28;
-
+// Query rows of a piece (few, wide; more than kTallFrom of a sequence are tall), and
+// pieces of a cut row at most, four waves and one.
+constexpr int kFewRows = 16, kWideRows = 32, kTallFrom = 64, kMostPieces = 128, kMostPieces1 = 32;
 // Workgroups a compute unit that pieces are made for: four waves for few rows, one
 // wave for few rows, wide rows; the least tiles of a one-wave piece; and from how
 // many rows a compute unit on they are.
 constexpr int kFewResident = 2, kOneResident = 16, kWideResident = 2, kOneLeast = 4,
               kOneWaveRows = 8, kJoin = 4;
-
-// Query rows of a piece, and pieces of a cut one at most, four waves and one.
-constexpr int kFewRows = 16, kWideRows = 32, kMostPieces = 128, kMostPieces1 = 32;
-
-struct Attend4 {
-  const void* q;
-  void* out;
-  const unsigned char *kpool, *vpool;
-  const int32_t *items, *indices;
-  int32_t* counters;
-  float *part_o, *part_ml;
-  int32_t* status;
-  int64_t num_blocks, block;
-  int32_t n_items, n_kv, groups, head_bytes, pairs, shift, part_rows, count_step;
-  uint32_t per_group;                // 2^16 / groups, rounded up: r / groups below 64 rows
-  float scale_log2;
-};
 
 // Floats per wave for a tile's steps, zeros of K, steps and middles of V
 // ([4][group][key]).
@@ -702,14 +682,14 @@ static int plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr,
                                  "multiple of n_kv_heads");
   if (cu_query_lens[0] != 0 || kv_indptr[0] != 0)
     return fail(PKV_ERR_INVALID, "cu_query_lens and kv_indptr must start at 0");
-  plan->n_few = plan->n_wide = plan->few_rows = plan->n_slots = plan->part_rows = 0;
+  plan->n_few = plan->n_wide = plan->n_tall = plan->few_rows = plan->n_slots = plan->part_rows = 0;
   plan->few_waves = plan->n_cuts = 0;
   plan->workspace_bytes = 0;
   *needed = 0;
   const int32_t G = n_heads / n_kv_heads;
   const bool fast = fast_4bit(n_heads, n_kv_heads, head_dim, page_size, dtype);
   struct Row { int32_t seq, q, n, tiles; };      // n tokens of a sequence from its q-th
-  std::vector<Row> rows[2];                       // few, wide
+  std::vector<Row> rows[3];                       // few, wide, tall
   int64_t tiles[2] = {0, 0};
   int32_t few = 0;
   for (int32_t i = 0; i < n_seqs; ++i) {
@@ -720,13 +700,14 @@ static int plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr,
     if (ql < 1 || ql > kv)
       return fail(PKV_ERR_INVALID, "seq %d: query_len=%d outside [1, kv_len=%d]", i, ql, kv);
     if (!fast) continue;
-    const bool wide = (int64_t)ql * G > kFewRows;
-    if (!wide) few = std::max(few, ql * G);
-    const int32_t step = wide ? std::max(1, kWideRows / G) : ql;
+    const int64_t qr = (int64_t)ql * G;
+    const int kind = qr <= kFewRows ? 0 : qr <= kTallFrom ? 1 : 2;
+    if (kind == 0) few = std::max(few, ql * G);
+    const int32_t step = kind == 0 ? ql : std::max(1, (kind == 1 ? kWideRows : kTallRows) / G);
     for (int32_t q = 0; q < ql; q += step) {
       const int32_t n = std::min(step, ql - q);
-      rows[wide].push_back({i, q, n, (kv - ql + q + n + kTile - 1) / kTile});
-      tiles[wide] += rows[wide].back().tiles;
+      rows[kind].push_back({i, q, n, (kv - ql + q + n + kTile - 1) / kTile});
+      if (kind < 2) tiles[kind] += rows[kind].back().tiles;
     }
   }
   if (!fast) return PKV_OK;
@@ -743,16 +724,16 @@ static int plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr,
   const bool one = (int64_t)rows[0].size() * n_kv_heads >= kOneWaveRows * (int64_t)compute_units;
   plan->few_waves = few ? (one ? 1 : 4) : 0;
   struct Piece { int32_t v[kPieceInts]; };
-  std::vector<Piece> out[2];
+  std::vector<Piece> out[3];
   const int32_t units = page_size / 16;      // of a page
   int32_t slots = 0, cuts = 0;
-  for (int wide = 0; wide < 2; ++wide) {
+  for (int wide = 0; wide < 3; ++wide) {
     // The shortest piece (a tile a wave at least) with which all of them are
     // resident at once: none waits for another to end.
     const bool alone = !wide && one;
     const int64_t resident =
         (int64_t)compute_units * (wide ? kWideResident : alone ? kOneResident : kFewResident);
-    const int64_t most = alone ? kMostPieces1 : kMostPieces;
+    const int64_t most = wide == 2 ? 1 : alone ? kMostPieces1 : kMostPieces;
     auto pieces = [&](const Row& r, int64_t piece) {
       return std::min<int64_t>(most, (r.tiles + piece - 1) / piece);
     };
@@ -796,9 +777,10 @@ static int plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr,
     std::stable_sort(v.begin(), v.end(), [](const Piece& a, const Piece& b) {
       return a.v[7] > b.v[7];
     });
-  *needed = (int64_t)(out[0].size() + out[1].size()) * kPieceInts;
+  *needed = (int64_t)(out[0].size() + out[1].size() + out[2].size()) * kPieceInts;
   plan->n_few = (int32_t)out[0].size();
   plan->n_wide = (int32_t)out[1].size();
+  plan->n_tall = (int32_t)out[2].size();
   plan->n_slots = slots;
   plan->n_cuts = cuts;
   plan->workspace_bytes =
@@ -856,7 +838,8 @@ int pkv_attend_4bit(const void* batch, const void* q, void* out, const void* k_p
     if (!b.batch_indices) return fail(PKV_ERR_INVALID, "null pointer argument");
     return run_4bit_any(b, q, out, k_pool, v_pool, scale, s);
   }
-  if (!b.items || b.n_few + b.n_wide <= 0 || b.n_few < 0 || b.n_wide < 0)
+  if (!b.items || b.n_few < 0 || b.n_wide < 0 || b.n_tall < 0 ||
+      (int64_t)b.n_few + b.n_wide + b.n_tall <= 0)
     return fail(PKV_ERR_INVALID, "the batch has no plan");
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool) % 16)
     return fail(PKV_ERR_INVALID, "q, out and the pools have to be aligned to 16 bytes");
@@ -914,9 +897,14 @@ int pkv_attend_4bit(const void* batch, const void* q, void* out, const void* k_p
                                       : few(std::integral_constant<int, 4>{});
       if (rc) return rc;
     }
-    if (b.n_wide)
-      return go(attend_4bit_kernel<T, D, 2, 1, 4>, b.items + (int64_t)b.n_few * kPieceInts,
-                b.n_wide, 4);
+    if (b.n_wide) {
+      const int rc = go(attend_4bit_kernel<T, D, 2, 1, 4>,
+                        b.items + (int64_t)b.n_few * kPieceInts, b.n_wide, 4);
+      if (rc) return rc;
+    }
+    if (b.n_tall)
+      return run_4bit_tall(a, D, b.dtype, b.items + ((int64_t)b.n_few + b.n_wide) * kPieceInts,
+                           b.n_tall, s);
     return PKV_OK;
   };
   auto by_dim = [&](auto type) -> int {

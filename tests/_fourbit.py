@@ -44,16 +44,18 @@ def held64(x):
     return (zero[..., None] + codes * step[..., None]).flatten(-2)
 
 
-def attend64(q, k, v, scale, dtype):
+def attend64(q, k, v, scale, dtype, tall=False):
     """
     Causal attention of the last n of N tokens: q (n, Hq, D); k, v (N, Hkv, D)
     rows before they are quantised. Returns (out, bound), (n, Hq, D) in 64 bits.
 
-    The kernels compute sum_t (p step) c + sum_t p zero, p the softmax's weights.
-    With u = eps / 2 of the output's type, v16 = 2^-11 (p step is rounded to
-    float16), B = sum_t p_t (step_t c_t + |zero_t|), per output element:
+    The kernels compute sum_t r_t c_t + sum_t p_t (zero_t + 7.5 step_t) - 7.5
+    sum_t r_t, p the softmax's weights and r_t = p_t step_t rounded to float16,
+    so that r_t's error enters times c_t - 7.5 (the plain ones sum_t p_t (zero_t +
+    step_t c_t)). With u = eps / 2 of the output's type, v16 = 2^-11, B = sum_t
+    p_t (step_t c_t + |zero_t + 7.5 step_t| + 7.5 step_t), per output element:
       u |out|                          the output's rounding
-      v16 sum_t p_t step_t c_t         each product's rounding
+      v16 sum_t p_t step_t |c_t - 7.5| each product's rounding
       (2 delta + 2 (N + 64) 2^-24) B   32 bits: delta bounds a score's error
                                        (terms of magnitude |q| (step c + |zero|):
                                        D + 8 roundings of the sum, the factors
@@ -65,6 +67,11 @@ def attend64(q, k, v, scale, dtype):
                                        sequence is below 2 and the row's largest
                                        p at least 1 / 2: up to 4 units a code,
                                        hence 4 times that
+    and where many rows share a tile (``tall``), whose keys and values are rounded
+    to float16 (2^-11 of each, or 2^-25 where that is more) and whose weights are
+    rounded without their step:
+      2 2^-11 sum_t p_t |v_t|          values and weights
+      2 kappa sum_t p_t |v_t|          kappa = 2^-11 |scale| max sum |q| |k|, as delta
     """
     n, hq, d = q.shape
     total, hkv = k.shape[0], k.shape[1]
@@ -73,20 +80,25 @@ def attend64(q, k, v, scale, dtype):
     kk, kb = ((kz[..., None] + kc * ks[..., None]).flatten(-2),
               (kz.abs()[..., None] + kc * ks[..., None]).flatten(-2))
     vv, vb = ((vz[..., None] + vc * vs[..., None]).flatten(-2),
-              (vz.abs()[..., None] + vc * vs[..., None]).flatten(-2))
-    vr = (vc * vs[..., None]).flatten(-2)
+              ((vz + 7.5 * vs).abs()[..., None] + (vc + 7.5) * vs[..., None]).flatten(-2))
+    vr = ((vc - 7.5).abs() * vs[..., None]).flatten(-2)
     u = torch.finfo(dtype).eps / 2
     qq = q.detach().cpu().double()
     see = torch.arange(total) <= torch.arange(total - n, total)[:, None]
     out, bound = torch.empty_like(qq), torch.empty_like(qq)
     for h in range(hq):
         of = h // gr
+        extra = 0.0
         s = qq[:, h] @ kk[:, of].t() * scale
         p = torch.softmax(s.masked_fill(~see, -math.inf), dim=-1)
         delta = ((d + 8) * 2.0 ** -24 * abs(scale)
                  * (qq[:, h].abs() @ kb[:, of].t()).masked_fill(~see, 0).amax(1, keepdim=True))
         out[:, h] = p @ vv[:, of]
+        if tall:
+            kappa = ((qq[:, h].abs() @ (kk[:, of].abs().t() * 2.0 ** -11 + 2.0 ** -25))
+                     * abs(scale)).masked_fill(~see, 0).amax(1, keepdim=True)
+            extra = (2 * 2.0 ** -11 + 2 * kappa) * (p @ vv[:, of].abs()) + 2.0 ** -24
         bound[:, h] = (u * out[:, h].abs() + 2.0 ** -11 * (p @ vr[:, of])
                        + (2 * delta + 2 * (total + 64) * 2.0 ** -24) * (p @ vb[:, of])
-                       + total * 2.0 ** -23 * 15 * vs[:, of].max())
+                       + total * 2.0 ** -23 * 15 * vs[:, of].max() + extra)
     return out, bound * 1.001 + torch.finfo(dtype).tiny

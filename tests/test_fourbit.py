@@ -78,7 +78,7 @@ def test_the_plan_covers_every_row_and_tile_once(compute_units, n_heads, n_kv):
     ql = [int(min(k, rng.choice([1, 1, 1, 3, 8, 100]))) for k in kv]
     args, items = plan(kv, ql, n_heads, n_kv, compute_units=compute_units)
     groups = n_heads // n_kv
-    assert args.n_few + args.n_wide == len(items)
+    assert args.n_few + args.n_wide + args.n_tall == len(items)
     seen, slots = {}, []
     cu, first = np.cumsum([0] + ql), np.cumsum([0] + [-(-k // 16) for k in kv])
     counters = {}
@@ -91,8 +91,12 @@ def test_the_plan_covers_every_row_and_tile_once(compute_units, n_heads, n_kv):
         assert pos == kv[seq] - ql[seq] + q
         assert nt >= 1 and 1 <= qn and q + qn <= ql[seq]
         wide = i >= args.n_few
+        tall = i >= args.n_few + args.n_wide
         assert wide or ql[seq] * groups <= 16
-        assert qn * groups <= (32 if wide else args.few_rows) <= args.part_rows * (1 if wide else 9)
+        assert tall == (ql[seq] * groups > 64)
+        assert qn * groups <= (128 if tall else 32 if wide else args.few_rows)
+        assert tall or args.part_rows >= min(32 if wide else 16, qn * groups)
+        assert not tall or n == 1
         assert (slot < 0) == (n == 1)
         if n > 1:
             assert slot0 <= slot < slot0 + n <= args.n_slots
@@ -115,7 +119,8 @@ def test_the_plan_covers_every_row_and_tile_once(compute_units, n_heads, n_kv):
             at += qn
         assert at == ql[seq]
     # longest first, in both parts
-    for part in (items[:args.n_few], items[args.n_few:]):
+    for part in (items[:args.n_few], items[args.n_few:args.n_few + args.n_wide],
+                 items[args.n_few + args.n_wide:]):
         assert [p[7] for p in part] == sorted((p[7] for p in part), reverse=True)
     assert len(counters) == len(set(counters.values())) == args.n_cuts
     need = _native.load().pkv_counter_bytes_4bit(args.n_cuts, n_kv) + args.n_slots * n_kv * args.part_rows * 66 * 4

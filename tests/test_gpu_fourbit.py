@@ -77,11 +77,18 @@ class Cache:
         g = torch.Generator().manual_seed(self.seed + 77)
         return (torch.randn((sum(counts), hq, d), generator=g) * factor).to(self.dtype)
 
+    def tall(self, n):
+        """Whether n tokens run as many rows of the matrix-core kernels."""
+        n_kv, hq, d = self.dims
+        return (self.dtype != F32 and d in (64, 128) and self.ps in (16, 32, 64)
+                and hq // n_kv <= 32 and n * (hq // n_kv) > 64)
+
     def check(self, got, q, counts, scale, label=""):
         got, at = got.cpu(), 0
         for i, n in enumerate(counts):
             if n:
-                want, bound = attend64(q[at:at + n], self.k[i], self.v[i], scale, self.dtype)
+                want, bound = attend64(q[at:at + n], self.k[i], self.v[i], scale, self.dtype,
+                                       self.tall(n))
                 assert_within(got[at:at + n], want, bound, f"{label} seq {i}")
             at += n
 
@@ -332,10 +339,58 @@ def test_rows_that_no_token_sees(d, hq):
     out = c.bk.attend(q.to(DEV), 0, d ** -0.5, meta).cpu()
     at = 0
     for n in counts:
-        want, bound = attend64(q[at:at + n - 1], k[at:at + n - 1], v[at:at + n - 1], d ** -0.5, F16)
+        want, bound = attend64(q[at:at + n - 1], k[at:at + n - 1], v[at:at + n - 1], d ** -0.5, F16,
+                               c.tall(n))
         assert_within(out[at:at + n - 1], want, bound)
         assert out[at + n - 1].isnan().all()
         at += n
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("counts", [[150, 1], [33, 200], [17, 129]])
+def test_prompt_chunks(d, counts):
+    """Many rows: chunks that end inside tiles of keys and of rows, over histories
+    that do, beside other rows."""
+    for n_kv, hq in ((2, 8), (1, 3), (1, 32)):
+        print(f"chunks {d} {counts} {hq}", flush=True)
+        c = Cache([130, 5], BF16 if n_kv == 2 else F16, n_kv, hq, d, room=300)
+        meta = c.append(counts)
+        q = c.q(counts)
+        c.check(c.bk.attend(q.to(DEV), 0, d ** -0.5, meta), q, counts, d ** -0.5)
+        c.check(c.bk.attend(q.to(DEV), 0, -0.1, meta), q, counts, -0.1)
+
+
+@pytest.mark.parametrize("new", [1, 5, 40])
+def test_values_next_to_the_largest_float16(new):
+    """A group's values may reach past 65504 by a step's rounding."""
+    c = Cache([0], BF16, 1, 4, 64)
+    n = 70
+    c.seqs[0].append(n)
+    k = rows((n, 1, 64), BF16, 1)
+    v = (torch.rand((n, 1, 64), generator=torch.Generator().manual_seed(2)) * 65000).to(BF16)
+    v[:, 0, 0], v[:, 0, 1] = 65280.0, 0.0
+    c.k, c.v = [k], [v]
+    c.bk.append_kv(0, k.to(DEV), v.to(DEV), make_meta(c.seqs, [n], 16, device=DEV))
+    counts = [new]
+    meta = c.append(counts)
+    q = c.q(counts)
+    c.check(c.bk.attend(q.to(DEV), 0, 0.125, meta), q, counts, 0.125)
+
+
+@pytest.mark.parametrize("n", [3, 40])
+def test_pages_outside_the_pool_among_many_rows(n):
+    c = Cache([200], F16, 2, 8, 64)
+    meta = c.append([n])
+    meta.kv_indices[3] = -1
+    meta = dataclasses.replace(meta, host=None)
+    q = c.q([n])
+    out = c.bk.attend(q.to(DEV), 0, 0.125, meta).cpu()
+    k, v = c.k[0].clone(), c.v[0].clone()
+    k[48:64], v[48:64] = 0, 0
+    want, bound = attend64(q, k, v, 0.125, F16, c.tall(n))
+    assert_within(out, want, bound)
+    with pytest.raises(IndexError, match="kv_indices"):
+        c.bk.check_device_errors()
 
 
 def test_pages_outside_the_pool_read_as_zeros():

@@ -48,14 +48,28 @@ int check_4bit(int32_t n_kv, int32_t d, int32_t ps);
 int run_4bit_any(const pkv_4bit& b, const void* q, void* out, const void* k_pool,
                  const void* v_pool, float scale, hipStream_t s);
 
-// Query rows of a piece (few, wide; more than kTallFrom of a sequence are tall), and
-// pieces of a cut row at most, four waves and one.
-constexpr int kFewRows = 16, kWideRows = 32, kTallFrom = 64, kMostPieces = 128, kMostPieces1 = 32;
-// Workgroups a compute unit that pieces are made for: four waves for few rows, one
-// wave for few rows, wide rows; the least tiles of a one-wave piece; and from how
-// many rows a compute unit on they are.
-constexpr int kFewResident = 2, kOneResident = 16, kWideResident = 2, kOneLeast = 4,
-              kOneWaveRows = 8, kJoin = 4;
+// Query rows of a piece (few, wide; a sequence of more than kTallFrom may be tall).
+constexpr int kFewRows = 16, kWideRows = 32, kTallFrom = 64;
+// Pieces of a cut row at most, four waves and one: what the last of them joins.
+constexpr int kMostPieces = 128, kMostPieces1 = 32;
+// Workgroups a compute unit that pieces are cut for. Few rows, four waves: 2 (one
+// sequence of 16384: 13.0 us; 1 took 12.4, 4 16.6; 16 of 32768: 115, 163 and 116).
+// Wide rows: 2 (32 drafts of 5 over 4096: 79; 1 took 88, 4 81).
+constexpr int kFewResident = 2, kWideResident = 2;
+// From kOneWaveRows rows (x KV heads) a compute unit on, a piece of few rows is one
+// wave's, of kOneLeast tiles at least, 16 a compute unit: 256 sequences of 16 to 1024
+// tokens take 14.4 us, as four waves' 18.0; pieces from 3 tiles 15.3, from 10 18.9.
+constexpr int kOneResident = 16, kOneLeast = 4, kOneWaveRows = 8;
+// Few rows beside wide ones run as wide ones up to kJoin times their tiles: one launch
+// with one ramp and tail, for a row of them at least half idle in the matrix cores.
+constexpr int kJoin = 4;
+// A sequence is tall where kTallAlong tiles x compute units <= kTallWork work (tiles of
+// all wide pieces): a tile takes a tall piece by itself 1.2 us at head_dim 64, a wide
+// one 1.3 us / 4 of a compute unit (1.8 and 1.9 / 4 at 128). Measured, head_dim 64,
+// 4 query heads each of 8, tall and wide: one chunk of 2000 tokens 46 and 50 us, of 512
+// over 30000 571 and 297; 8 of 128 over 1000 30 and 33, over 4000 92 and 86; 64 of 20
+// over 300 17 and 23; 8 of 512 over 1536 94 and 152.
+constexpr int64_t kTallAlong = 7, kTallWork = 2;
 
 // Floats per wave for a tile's steps, zeros of K, steps and middles of V
 // ([4][group][key]).
@@ -690,8 +704,23 @@ static int plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr,
   const bool fast = fast_4bit(n_heads, n_kv_heads, head_dim, page_size, dtype);
   struct Row { int32_t seq, q, n, tiles; };      // n tokens of a sequence from its q-th
   std::vector<Row> rows[3];                       // few, wide, tall
-  int64_t tiles[2] = {0, 0};
+  std::vector<int32_t> many;                      // wide or tall sequences
+  int64_t tiles[2] = {0, 0}, work = 0;
   int32_t few = 0;
+  // Sequence i's rows in parts of a kind; their tiles.
+  auto part = [&](int32_t i, int kind, bool keep) {
+    const int32_t kv = kv_lens[i], ql = cu_query_lens[i + 1] - cu_query_lens[i];
+    const int32_t step = kind == 0 ? ql : std::max(1, (kind == 1 ? kWideRows : kTallRows) / G);
+    int64_t sum = 0;
+    for (int32_t q = 0; q < ql; q += step) {
+      const int32_t n = std::min(step, ql - q);
+      const int32_t nt = (kv - ql + q + n + kTile - 1) / kTile;
+      if (keep) rows[kind].push_back({i, q, n, nt});
+      sum += nt;
+    }
+    if (keep && kind < 2) tiles[kind] += sum;
+    return sum;
+  };
   for (int32_t i = 0; i < n_seqs; ++i) {
     const int32_t kv = kv_lens[i], ql = cu_query_lens[i + 1] - cu_query_lens[i];
     const int rc = check_seq_pages(i, kv_indptr[i + 1] - kv_indptr[i], kv, kv_last_page_len[i],
@@ -701,14 +730,21 @@ static int plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr,
       return fail(PKV_ERR_INVALID, "seq %d: query_len=%d outside [1, kv_len=%d]", i, ql, kv);
     if (!fast) continue;
     const int64_t qr = (int64_t)ql * G;
-    const int kind = qr <= kFewRows ? 0 : qr <= kTallFrom ? 1 : 2;
-    if (kind == 0) few = std::max(few, ql * G);
-    const int32_t step = kind == 0 ? ql : std::max(1, (kind == 1 ? kWideRows : kTallRows) / G);
-    for (int32_t q = 0; q < ql; q += step) {
-      const int32_t n = std::min(step, ql - q);
-      rows[kind].push_back({i, q, n, (kv - ql + q + n + kTile - 1) / kTile});
-      if (kind < 2) tiles[kind] += rows[kind].back().tiles;
+    if (qr > kTallFrom) {
+      many.push_back(i);
+      work += part(i, 1, false) * n_kv_heads;
+      continue;
     }
+    const int kind = qr <= kFewRows ? 0 : 1;
+    if (kind == 0) few = std::max(few, ql * G);
+    part(i, kind, true);
+  }
+  // A tall piece runs along all its keys by itself, so a sequence is tall only where
+  // its tiles one after the other take no longer than all of the work does, shared
+  // out as wide pieces.
+  for (const int32_t i : many) {
+    const int64_t along = (kv_lens[i] + kTile - 1) / kTile;
+    part(i, kTallAlong * along * compute_units <= kTallWork * work ? 2 : 1, true);
   }
   if (!fast) return PKV_OK;
   // Beside wide rows few rows run as wide ones do, unless theirs are most tiles: one

@@ -11,7 +11,8 @@
 //    of a tile passes 2^12.
 // K and V are rounded to float16 here (2^-12 of a value at most, what a 16-bit cache
 // holds of it); with exact codes and the steps applied to the scores and weights, as
-// for few rows, 8 x 512 tokens over 1536 (head_dim 64) took 152 us, as here 88.
+// for few rows, 8 x 512 tokens over 1536 (head_dim 64) took 152 us, as here 95
+// (640 TFLOP/s).
 // Rows of 144 bytes (272 for K at head_dim 128) put the 16 lanes of a 16-byte read on
 // different banks.
 #include "attend_fourbit.h"
@@ -200,10 +201,12 @@ __global__ __launch_bounds__(256, 2) void attend_4bit_tall_kernel(Attend4 a) {
   f32x16 o[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) o[b] = f32x16{};
-  float ref = -INFINITY, l = 0.f;
+  float ref = -INFINITY, l = 0.f, none[NG] = {};
 
   stage(0);
-  if (n_tiles > 1) load(1, page(1));
+  int next = page(1);                // (read a tile ahead of its use)
+  if (n_tiles > 1) load(1, next);
+  next = page(2);
   __syncthreads();
   for (int t = 0; t < n_tiles; ++t) {
     const unsigned char* buf = smem + (t & 1) * BUF;
@@ -239,26 +242,30 @@ __global__ __launch_bounds__(256, 2) void attend_4bit_tall_kernel(Attend4 a) {
           pb[2 * hf + (e >> 3)][(e & 4) + ((e & 1) << 1 | (e >> 1 & 1))] = (_Float16)p;
         }
     };
-    probs(ref);
-    if (__builtin_amdgcn_ballot_w64(!(ls <= 4096.f))) {
+    // (one copy of the weights' code: two took 31 registers more, a third of the waves)
+    float m = ref;
+    for (int again = 0;; ++again) {
+      probs(m);
+      if (again || !__builtin_amdgcn_ballot_w64(!(ls <= 4096.f))) break;
       float mx = -INFINITY;
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
         for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[hf][e]);
-      const float m = fmaxf(ref, max_x32(mx) * f1);
+      m = fmaxf(ref, max_x32(mx) * f1);
       const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref - m);
       ref = m;
+      m = m == -INFINITY ? 0.f : m;
       l *= alpha;
 #pragma unroll
       for (int b = 0; b < NB; ++b) o[b] *= alpha;
-      probs(m == -INFINITY ? 0.f : m);
     }
     l += ls;
     // the next tile into the other buffer, the one after it on its way
     if (t + 1 < n_tiles) {
       stage((t + 1) & 1);
-      if (t + 2 < n_tiles) load(t + 2, page(t + 2));
+      if (t + 2 < n_tiles) load(t + 2, next);
+      next = page(t + 3);
     }
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb)
@@ -267,15 +274,14 @@ __global__ __launch_bounds__(256, 2) void attend_4bit_tall_kernel(Attend4 a) {
         o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
             *reinterpret_cast<const f16x8*>(buf + KB + (32 * b + n) * VS + 32 * kb + 16 * g), pb[kb],
             o[b], 0, 0, 0);
-    // a row that sees a key whose V is NaN gets NaN
+    // a row that sees a key whose V is NaN gets NaN, at the end
 #pragma unroll
     for (int q = 0; q < NG; ++q) {
       const uint64_t keys = *reinterpret_cast<const uint64_t*>(nan_keys[t & 1][q]);
-      if (__builtin_amdgcn_ballot_w64(keys != 0)) {
+      if (__builtin_amdgcn_readfirstlane((uint32_t)keys | (uint32_t)(keys >> 32))) {
         const int seen = qpos - kTile * t;     // the last one
         const uint64_t mine = seen < 0 ? 0 : seen >= 63 ? keys : keys & ((2ull << seen) - 1);
-        if (mine) o[2 * q] += NAN;
-        if (mine) o[2 * q + 1] += NAN;
+        none[q] = mine ? NAN : none[q];
       }
     }
     __syncthreads();
@@ -292,7 +298,7 @@ __global__ __launch_bounds__(256, 2) void attend_4bit_tall_kernel(Attend4 a) {
     for (int j = 0; j < 4; ++j) {
       TV4 v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (T)(o[b][4 * j + e] * inv);
+      for (int e = 0; e < 4; ++e) v[e] = (T)__builtin_fmaf(o[b][4 * j + e], inv, none[b / 2]);
       *reinterpret_cast<TV4*>(row + 32 * b + 8 * j) = v;
     }
 }

@@ -82,6 +82,12 @@ def test_the_plan_covers_every_row_and_tile_once(compute_units, n_heads, n_kv):
     seen, slots = {}, []
     cu, first = np.cumsum([0] + ql), np.cumsum([0] + [-(-k // 16) for k in kv])
     counters = {}
+    # tall: the tiles along the sequence within the share of all as wide pieces
+    step = max(1, 32 // groups)
+    work = n_kv * sum(-(-(k - n + min(n, at + step)) // 64) for k, n in zip(kv, ql)
+                      if n * groups > 64 for at in range(0, n, step))
+    tall_seqs = {i for i, (k, n) in enumerate(zip(kv, ql)) if n * groups > 64
+                 and 7 * -(-k // 64) * compute_units <= 2 * work}
     for i, (row, qn, pos, kvl, page, pages, t0, nt, slot, slot0, n, counter, *ids) in \
             enumerate(items):
         seq = int(np.searchsorted(cu, row, side="right")) - 1
@@ -93,7 +99,7 @@ def test_the_plan_covers_every_row_and_tile_once(compute_units, n_heads, n_kv):
         wide = i >= args.n_few
         tall = i >= args.n_few + args.n_wide
         assert wide or ql[seq] * groups <= 16
-        assert tall == (ql[seq] * groups > 64)
+        assert tall == (seq in tall_seqs)
         assert qn * groups <= (128 if tall else 32 if wide else args.few_rows)
         assert tall or args.part_rows >= min(32 if wide else 16, qn * groups)
         assert not tall or n == 1

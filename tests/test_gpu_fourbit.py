@@ -78,10 +78,11 @@ class Cache:
         return (torch.randn((sum(counts), hq, d), generator=g) * factor).to(self.dtype)
 
     def tall(self, n):
-        """Whether n tokens run as many rows of the matrix-core kernels."""
+        """Whether n tokens of the last batch may have run as a tall piece."""
         n_kv, hq, d = self.dims
         return (self.dtype != F32 and d in (64, 128) and self.ps in (16, 32, 64)
-                and hq // n_kv <= 32 and n * (hq // n_kv) > 64)
+                and hq // n_kv <= 32 and n * (hq // n_kv) > 64
+                and self.bk._planned.args.n_tall > 0)
 
     def check(self, got, q, counts, scale, label=""):
         got, at = got.cpu(), 0
@@ -312,11 +313,12 @@ def test_values_that_grow_along_the_sequence(grow, new):
     c.check(c.bk.attend(q.to(DEV), 0, 0.125, meta), q, counts, 0.125)
 
 
+@pytest.mark.parametrize("units", [None, 1])
 @pytest.mark.parametrize("d,hq", [(64, 8), (128, 2), (64, 32), (80, 4)])
-def test_rows_that_no_token_sees(d, hq):
+def test_rows_that_no_token_sees(d, hq, units):
     """What lies behind a sequence's end in its last page, and keys behind a
     token's position, may hold NaN."""
-    c = Cache([0, 0], F16, 2, hq, d)
+    c = Cache([0, 0], F16, 2, hq, d, compute_units=units)
     whole = [64 + 16, 32]
     for s, n in zip(c.seqs, whole):
         s.append(n)
@@ -348,22 +350,26 @@ def test_rows_that_no_token_sees(d, hq):
 
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("counts", [[150, 1], [33, 200], [17, 129]])
-def test_prompt_chunks(d, counts):
+@pytest.mark.parametrize("units", [None, 1])
+def test_prompt_chunks(d, counts, units):
     """Many rows: chunks that end inside tiles of keys and of rows, over histories
-    that do, beside other rows."""
+    that do, beside other rows; as wide pieces of a whole card, as tall ones of a
+    compute unit."""
     for n_kv, hq in ((2, 8), (1, 3), (1, 32)):
         print(f"chunks {d} {counts} {hq}", flush=True)
-        c = Cache([130, 5], BF16 if n_kv == 2 else F16, n_kv, hq, d, room=300)
+        c = Cache([130, 5], BF16 if n_kv == 2 else F16, n_kv, hq, d, room=300,
+                  compute_units=units)
         meta = c.append(counts)
         q = c.q(counts)
         c.check(c.bk.attend(q.to(DEV), 0, d ** -0.5, meta), q, counts, d ** -0.5)
         c.check(c.bk.attend(q.to(DEV), 0, -0.1, meta), q, counts, -0.1)
+        assert (c.bk._planned.args.n_tall > 0) == (units == 1)
 
 
-@pytest.mark.parametrize("new", [1, 5, 40])
-def test_values_next_to_the_largest_float16(new):
+@pytest.mark.parametrize("new,units", [(1, None), (5, None), (40, None), (40, 1)])
+def test_values_next_to_the_largest_float16(new, units):
     """A group's values may reach past 65504 by a step's rounding."""
-    c = Cache([0], BF16, 1, 4, 64)
+    c = Cache([0], BF16, 1, 4, 64, compute_units=units)
     n = 70
     c.seqs[0].append(n)
     k = rows((n, 1, 64), BF16, 1)
@@ -377,9 +383,9 @@ def test_values_next_to_the_largest_float16(new):
     c.check(c.bk.attend(q.to(DEV), 0, 0.125, meta), q, counts, 0.125)
 
 
-@pytest.mark.parametrize("n", [3, 40])
-def test_pages_outside_the_pool_among_many_rows(n):
-    c = Cache([200], F16, 2, 8, 64)
+@pytest.mark.parametrize("n,units", [(3, None), (40, None), (40, 1)])
+def test_pages_outside_the_pool_among_many_rows(n, units):
+    c = Cache([200], F16, 2, 8, 64, compute_units=units)
     meta = c.append([n])
     meta.kv_indices[3] = -1
     meta = dataclasses.replace(meta, host=None)

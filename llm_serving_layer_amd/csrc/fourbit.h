@@ -50,6 +50,23 @@ __host__ __device__ inline FourBit four_bit(int32_t n_kv, int32_t d, int32_t ps)
   return f;
 }
 
+// n / d for n < 2^31 as a product: with 2^s >= d and m = 2^(31 + s) / d rounded up (by
+// less than 2^s / d), n m exceeds n 2^(31 + s) / d by less than 2^(31 + s) / d.
+struct Div {
+  uint32_t d, m;
+  int32_t s;
+};
+inline Div div_by(uint32_t d) {
+  int s = 0;
+  while ((1ull << s) < d) ++s;
+  return {d, (uint32_t)(((1ull << (31 + s)) + d - 1) / d), 31 + s};
+}
+__device__ __forceinline__ uint32_t divide(uint32_t n, const Div& v, uint32_t& rest) {
+  const uint32_t q = (uint32_t)((uint64_t)n * v.m >> v.s);
+  rest = n - q * v.d;
+  return q;
+}
+
 // Where row r's element e lies among a head's codes: byte and half.
 __device__ __forceinline__ int k_byte(const FourBit& f, int r, int e) {
   if (!f.tiled) return r * (f.d / 2) + e / 2;
@@ -86,16 +103,16 @@ __device__ __forceinline__ _Float16 next_f16(_Float16 h, bool up) {
 constexpr float kF16Max = 65504.f;
 constexpr uint32_t kNanPair = 0x7e007e00u;
 
-// A group's word, from its least and largest element (finite, in range). The
-// quotient in 64 bits, where the difference of two elements and the quotient's
-// order against a float16 are right.
+// A group's word, from its least and largest element (finite, in range). The nearest
+// float16 to the quotient (in 32 bits: off by 2^-22 of it) is the step or the one
+// below it: 15 steps, exact in 32 bits, against the difference in 64 decide.
 __device__ __forceinline__ uint32_t group_pair(float lo, float hi) {
   _Float16 z = (_Float16)lo;
   if ((float)z > lo) z = next_f16(z, false);
-  const double need = ((double)hi - (double)(float)z) / 15.0;
-  _Float16 s = (_Float16)(float)need;
-  if ((double)(float)s < need) s = next_f16(s, true);
-  return (uint32_t)__builtin_bit_cast(uint16_t, s) << 16 | __builtin_bit_cast(uint16_t, z);
+  const double need = (double)hi - (double)(float)z;
+  uint32_t s = __builtin_bit_cast(uint16_t, (_Float16)((float)need * (1.f / 15.f)));
+  s += (double)(15.f * (float)f16_bits(s)) < need;
+  return s << 16 | __builtin_bit_cast(uint16_t, z);
 }
 
 // Element x's code. In 32 bits with an error below 2^-17 steps; next to a

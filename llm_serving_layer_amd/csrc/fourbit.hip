@@ -1,6 +1,7 @@
 // The 4-bit cache's rows: append (quantise), read (the values held), and
 // attention over it for any geometry. The format is fourbit.h's.
 #include <algorithm>
+#include <type_traits>
 
 #include "fourbit.h"
 
@@ -8,47 +9,36 @@ namespace pkv {
 
 // ----------------------------------------------------------------- append ---
 
-// A tiled row group (64 elements) by 8 lanes of 8 elements: 16-byte loads, a
-// minimum and maximum over the 8 lanes, and each lane's codes: K one word, V four
-// bytes. HBM-bound by its inputs (4 of 5 bytes); small launches by their chain:
-// slot and row read together, then two reductions of three steps.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  typedef T TV __attribute__((ext_vector_type(8)));
-  const TV v = *reinterpret_cast<const TV*>(p);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = Elem<T>::to_f(v[i]);
-}
-
-__device__ __forceinline__ uint32_t dpp_u(uint32_t v, int) {   // quad_perm [2,3,0,1]
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false);
-}
-
+// A tiled row group (64 elements) by 8 lanes of 8 elements: 16-byte loads, a minimum
+// and maximum over the 8 lanes, then each lane's codes: K one word, V four bytes.
+// HBM-bound by its inputs (4 of 5 bytes) if the vector work is short: a group's
+// elements next to a border between codes are looked for together and all decided in
+// 64 bits where there is one (a wave in 16), codes are packed as sums in float.
 template <typename T>
 __global__ __launch_bounds__(256) void append_4bit_kernel(
     unsigned char* __restrict__ kpool, unsigned char* __restrict__ vpool, int64_t num_slots,
-    FourBit f, const T* __restrict__ k, int64_t k_stride, const T* __restrict__ v,
-    int64_t v_stride, const int32_t* __restrict__ slots, int64_t n_tokens, int32_t* status) {
-  const int per_token = f.n_kv * f.groups;               // groups of a token's K or V
-  const int64_t unit = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
-  const int64_t total = n_tokens * 2 * per_token;
+    FourBit f, Div by_row, Div by_group, Div by_page, const T* __restrict__ k, int64_t k_stride,
+    const T* __restrict__ v, int64_t v_stride, const int32_t* __restrict__ slots, uint32_t total,
+    int32_t* status) {
+  const uint32_t unit = blockIdx.x * 32 + (threadIdx.x >> 3);
   const bool live = unit < total;
-  const int64_t u = live ? unit : total - 1;
-  const int64_t row = u / per_token;                      // (token, K or V)
-  const int hq = (int)(u - row * per_token);
-  const int64_t t = row >> 1;
+  uint32_t hq, r;
+  const uint32_t row = divide(live ? unit : total - 1, by_row, hq);   // (token, K or V)
+  const uint32_t t = row >> 1;
   const bool is_v = row & 1;
-  const int h = hq / f.groups, q = hq - h * f.groups;
   const int l = threadIdx.x & 7;
-  const int64_t slot = slots[t];
-  float x[8];
-  load8((is_v ? v + t * v_stride : k + t * k_stride) + (int64_t)h * f.d + q * 64 + l * 8, x);
-  float lo = INFINITY, hi = -INFINITY;
-  bool odd = false;                                       // a NaN or an infinity
+  const int32_t slot = slots[t];
+  typedef T TV __attribute__((ext_vector_type(8)));
+  // (heads lie one after another, so group hq of the row starts at 64 hq)
+  const TV in = *reinterpret_cast<const TV*>((is_v ? v + t * v_stride : k + t * k_stride) +
+                                             hq * 64 + l * 8);
+  float x[8], lo = INFINITY, hi = -INFINITY, finite = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    odd |= !(__builtin_fabsf(x[i]) < INFINITY);
-    x[i] = fminf(fmaxf(x[i], -kF16Max), kF16Max);
+    x[i] = Elem<T>::to_f(in[i]);
+    finite = __builtin_fmaf(x[i], 0.f, finite);           // (NaN of an infinity or NaN)
+    if constexpr (!std::is_same<T, _Float16>::value)
+      x[i] = __builtin_amdgcn_fmed3f(x[i], -kF16Max, kF16Max);
     lo = fminf(lo, x[i]);
     hi = fmaxf(hi, x[i]);
   }
@@ -58,43 +48,63 @@ __global__ __launch_bounds__(256) void append_4bit_kernel(
   hi = fmaxf(hi, dpp<0x4E>(hi));
   lo = fminf(lo, dpp<0x141>(lo));    // row_half_mirror: the 8 lanes
   hi = fmaxf(hi, dpp<0x141>(hi));
-  const uint64_t odds = __builtin_amdgcn_ballot_w64(odd);
+  const uint64_t odds = __builtin_amdgcn_ballot_w64(finite != 0.f);
   const bool none = (odds >> (threadIdx.x & 56)) & 0xffu;
-  const uint32_t pair = none ? kNanPair : group_pair(lo, hi);
-  const float step = none ? 0.f : pair_step(pair), zero = pair_zero(pair), inv = 1.f / step;
-  uint32_t c[8];
+  const uint32_t pair = none ? kNanPair : group_pair(none ? 0.f : lo, none ? 0.f : hi);
+  const float step = none ? 0.f : pair_step(pair), zero = none ? 0.f : pair_zero(pair);
+  const float inv = step > 0.f ? 1.f / step : 0.f;
+  // Codes: off by less than 2^-17 of a step, so wrong only next to a border; 15 steps
+  // reach the largest element, so none passes 15.
+  float c[8], far = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) c[i] = code_of(x[i], step, inv, zero);
-  // (V: dims 32 b + n and 32 b + 16 + n share a byte: lanes two apart)
-  uint32_t mine[2] = {c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24,
-                      c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24};
-  const uint32_t other0 = dpp_u(mine[0], 0), other1 = dpp_u(mine[1], 0);
-  if (!live) return;
-  if (slot < 0 || slot >= num_slots) {
-    if (hq == 0 && l == 0) flag(status, PKV_STATUS_BAD_SLOT);
-    return;
+  for (int i = 0; i < 8; ++i) {
+    const float w = (x[i] - zero) * inv;
+    c[i] = __builtin_rintf(w);
+    far = fmaxf(far, __builtin_fabsf(w - c[i]));
   }
-  const int64_t block = slot / f.ps;
-  const int r = (int)(slot - block * f.ps);
-  unsigned char* base = (is_v ? vpool : kpool) + block * f.block;
-  unsigned char* codes = base + h * f.head_bytes;
-  if (l == 0)
-    reinterpret_cast<uint32_t*>(base + f.pairs)[(h * f.groups + q) * f.ps + r] = pair;
+  if (__builtin_amdgcn_ballot_w64(far > 0.5f - 0x1p-14f)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = (float)code_of(x[i], step, inv, zero);
+  }
+  if (none) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = 0.f;
+  }
+  const uint32_t block = divide((uint32_t)slot, by_page, r);
+  const bool write = live && slot >= 0 && slot < num_slots;
+  if (live && !write && hq == 0 && l == 0) flag(status, PKV_STATUS_BAD_SLOT);
+  unsigned char* const base = (is_v ? vpool : kpool) + (int64_t)block * f.block;
+  uint32_t q;
+  const uint32_t h = divide(hq, by_group, q);
+  unsigned char* const codes = base + h * f.head_bytes;
+  if (write && l == 0) reinterpret_cast<uint32_t*>(base + f.pairs)[hq * f.ps + r] = pair;
   if (!is_v) {
     uint32_t w = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w |= c[i] << (4 * i);
-    *reinterpret_cast<uint32_t*>(codes + k_byte(f, r, q * 64 + l * 8)) = w;
-    return;
+    for (int i = 0; i < 8; i += 4) {
+      const float four = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(c[i + 3], 16.f, c[i + 2]),
+                                                       16.f, c[i + 1]), 16.f, c[i]);
+      w |= (uint32_t)four << (4 * i);
+    }
+    if (write) *reinterpret_cast<uint32_t*>(codes + k_byte(f, r, q * 64 + l * 8)) = w;
   }
-  // lanes (l & 2) == 0 hold dims n, the others n + 16; each writes four of the
-  // pair's eight bytes
-  const bool upper = l & 2;
-  const uint32_t low = upper ? other1 : mine[0], high = upper ? mine[1] : other0;
-  const uint32_t bytes = low | high << 4;
-  const int e = q * 64 + (l >> 2) * 32 + (l & 1) * 8 + (upper ? 4 : 0);
+  if (__builtin_amdgcn_ballot_w64(is_v)) {
+    // Dims 32 b + n and 32 b + 16 + n share a byte: lanes two apart. Lanes (l & 2) == 0
+    // hold dims n, the others n + 16; each writes four of the pair's eight bytes.
+    const bool upper = l & 2;
+    uint32_t bytes = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) codes[v_byte(f, r, e + i)] = (unsigned char)(bytes >> (8 * i));
+    for (int i = 0; i < 4; ++i) {
+      const float own = upper ? c[4 + i] : c[i], sent = dpp<0x4E>(upper ? c[i] : c[4 + i]);
+      const float byte = upper ? __builtin_fmaf(own, 16.f, sent) : __builtin_fmaf(sent, 16.f, own);
+      bytes = __builtin_amdgcn_cvt_pk_u8_f32(byte, i, bytes);
+    }
+    if (!write || !is_v) return;
+    unsigned char* const to =
+        codes + v_byte(f, r, q * 64 + (l >> 2) * 32 + (l & 1) * 8 + (upper ? 4 : 0));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[i * (f.d / 8)] = (unsigned char)(bytes >> (8 * i));
+  }
 }
 
 // Any geometry: a wave per (token, K or V, head), one group.
@@ -154,42 +164,100 @@ __global__ __launch_bounds__(64) void append_4bit_any_kernel(
 
 // ------------------------------------------------------------------- read ---
 
-// The values that slots hold, 8 elements a thread (2 where the layout is not
-// tiled), rounded once to the pool's type.
-template <typename T, int N>
+// The values that slots hold, rounded once to the pool's type. Tiled: 16 elements a
+// thread, K's as two words, V's as the bytes of dims 32 b + n .. + 7 with those 16
+// further. Bound by what it writes where there are many rows.
+template <typename T>
 __global__ __launch_bounds__(256) void read_4bit_kernel(
     const unsigned char* __restrict__ kpool, const unsigned char* __restrict__ vpool,
-    int64_t num_slots, FourBit f, const int32_t* __restrict__ slots, int64_t n_rows,
-    T* __restrict__ k, T* __restrict__ v, int32_t* status) {
-  typedef T TV __attribute__((ext_vector_type(N)));
-  const int per_row = f.n_kv * f.d / N;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n_rows * 2 * per_row) return;
-  const int64_t row = i / per_row;
-  const int at = (int)(i - row * per_row) * N;
-  const int64_t t = row >> 1;
+    int64_t num_slots, FourBit f, Div by_row, Div by_head, Div by_page,
+    const int32_t* __restrict__ slots, uint32_t total, T* __restrict__ k, T* __restrict__ v,
+    int32_t* status) {
+  typedef T TV __attribute__((ext_vector_type(8)));
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  uint32_t at, part, r;                                   // of a row, of a head
+  const uint32_t row = divide(i, by_row, at), h = divide(at, by_head, part);
+  const uint32_t t = row >> 1;
   const bool is_v = row & 1;
-  const int h = at / f.d, e = at - h * f.d;
-  const int64_t slot = slots[t];
+  const int32_t slot = slots[t];
+  TV lo{}, hi{};
+  if (slot < 0 || slot >= num_slots) {
+    if (at == 0) flag(status, PKV_STATUS_BAD_SLOT);
+  } else {
+    const uint32_t block = divide((uint32_t)slot, by_page, r);
+    const unsigned char* base = (is_v ? vpool : kpool) + (int64_t)block * f.block;
+    const unsigned char* codes = base + h * f.head_bytes;
+    const uint32_t pair =
+        reinterpret_cast<const uint32_t*>(base + f.pairs)[(h * f.groups + (part >> 2)) * f.ps + r];
+    uint32_t low[2], up[2];       // bytes of the first 8 elements, of the others
+    if (is_v) {
+      const unsigned char* from = codes + v_byte(f, r, 32 * (part >> 1) + 8 * (part & 1));
+      low[0] = low[1] = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) low[j >> 2] |= (uint32_t)from[j * (f.d / 8)] << (8 * (j & 3));
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        up[j] = low[j] >> 4 & 0x0f0f0f0fu;
+        low[j] &= 0x0f0f0f0fu;
+      }
+    } else {
+      const uint32_t* from = reinterpret_cast<const uint32_t*>(codes + k_byte(f, r, 16 * part));
+      auto bytes = [](uint32_t w, uint32_t (&of)[2]) {
+        const uint32_t even = w & 0x0f0f0f0fu, odd = w >> 4 & 0x0f0f0f0fu;
+        of[0] = __builtin_amdgcn_perm(odd, even, 0x05010400u);
+        of[1] = __builtin_amdgcn_perm(odd, even, 0x07030602u);
+      };
+      bytes(from[0], low);
+      bytes(from[1], up);
+    }
+    const float step = pair_step(pair), zero = pair_zero(pair);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      lo[j] = Elem<T>::from_f(
+          __builtin_fmaf((float)(low[j >> 2] >> (8 * (j & 3)) & 0xffu), step, zero));
+      hi[j] = Elem<T>::from_f(
+          __builtin_fmaf((float)(up[j >> 2] >> (8 * (j & 3)) & 0xffu), step, zero));
+    }
+  }
+  // (K: 16 elements in a row; V: 8 and the 8 that lie 16 further)
+  T* to = (is_v ? v : k) + (int64_t)t * f.n_kv * f.d + h * f.d +
+          (is_v ? 32 * (part >> 1) + 8 * (part & 1) : 16 * part);
+  *reinterpret_cast<TV*>(to) = lo;
+  *reinterpret_cast<TV*>(to + (is_v ? 16 : 8)) = hi;
+}
+
+// Any geometry: two elements a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void read_4bit_any_kernel(
+    const unsigned char* __restrict__ kpool, const unsigned char* __restrict__ vpool,
+    int64_t num_slots, FourBit f, Div by_row, Div by_head, Div by_page,
+    const int32_t* __restrict__ slots, uint32_t total, T* __restrict__ k, T* __restrict__ v,
+    int32_t* status) {
+  typedef T TV __attribute__((ext_vector_type(2)));
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  uint32_t at, e, r;
+  const uint32_t row = divide(i, by_row, at), h = divide(at, by_head, e);
+  const uint32_t t = row >> 1;
+  const bool is_v = row & 1;
+  e *= 2;
+  const int32_t slot = slots[t];
   TV out{};
   if (slot < 0 || slot >= num_slots) {
     if (at == 0) flag(status, PKV_STATUS_BAD_SLOT);
   } else {
-    const int64_t block = slot / f.ps;
-    const int r = (int)(slot - block * f.ps);
-    const unsigned char* base = (is_v ? vpool : kpool) + block * f.block;
+    const uint32_t block = divide((uint32_t)slot, by_page, r);
+    const unsigned char* base = (is_v ? vpool : kpool) + (int64_t)block * f.block;
     const unsigned char* codes = base + h * f.head_bytes;
     const uint32_t pair =
         reinterpret_cast<const uint32_t*>(base + f.pairs)[(h * f.groups + group_of(f, e)) * f.ps + r];
     const float step = pair_step(pair), zero = pair_zero(pair);
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int b = codes[is_v ? v_byte(f, r, e + j) : k_byte(f, r, e + j)];
-      const int half = is_v ? v_half(f, e + j) : k_half(f, e + j);
-      out[j] = Elem<T>::from_f(__builtin_fmaf((float)(b >> (4 * half) & 15), step, zero));
-    }
+    const int b = codes[is_v ? v_byte(f, r, e) : k_byte(f, r, e)];
+    out[0] = Elem<T>::from_f(__builtin_fmaf((float)(b & 15), step, zero));
+    out[1] = Elem<T>::from_f(__builtin_fmaf((float)(b >> 4), step, zero));
   }
-  *reinterpret_cast<TV*>((is_v ? v : k) + t * f.n_kv * f.d + at) = out;
+  *reinterpret_cast<TV*>((is_v ? v : k) + (int64_t)t * f.n_kv * f.d + 2 * at) = out;
 }
 
 // ------------------------------------------------ attention, any geometry ---
@@ -319,18 +387,18 @@ int pkv_append_4bit(void* k_pool, void* v_pool, int64_t num_blocks, const void* 
   hipStream_t s = (hipStream_t)stream;
   const bool wide = f.tiled && ((uintptr_t)k | (uintptr_t)v | (uint64_t)(k_stride * eb) |
                                 (uint64_t)(v_stride * eb)) % 16 == 0;
-  const int64_t work = wide ? (n_tokens * 2 * f.n_kv * f.groups + 31) / 32 : n_tokens * 2 * f.n_kv;
-  if (n_tokens > (1ll << 40) || work > 0x7fffffffLL)
-    return fail(PKV_ERR_INVALID, "too many rows in one append");
+  const int64_t work = n_tokens > 0x7fffffffLL ? n_tokens : n_tokens * 2 * f.n_kv * f.groups;
+  if (work > 0x7fffffffLL) return fail(PKV_ERR_INVALID, "too many rows in one append");
   auto go = [&](auto type) {
     typedef decltype(type) T;
     if (wide)
-      hipLaunchKernelGGL(append_4bit_kernel<T>, dim3((unsigned)work), dim3(256), 0, s,
+      hipLaunchKernelGGL(append_4bit_kernel<T>, dim3((unsigned)((work + 31) / 32)), dim3(256), 0, s,
                          (unsigned char*)k_pool, (unsigned char*)v_pool, num_blocks * page_size, f,
-                         (const T*)k, k_stride, (const T*)v, v_stride, slot_mapping, n_tokens,
-                         status_word);
+                         div_by(f.n_kv * f.groups), div_by(f.groups), div_by(page_size),
+                         (const T*)k, k_stride,
+                         (const T*)v, v_stride, slot_mapping, (uint32_t)work, status_word);
     else
-      hipLaunchKernelGGL(append_4bit_any_kernel<T>, dim3((unsigned)work), dim3(64), 0, s,
+      hipLaunchKernelGGL(append_4bit_any_kernel<T>, dim3((unsigned)(n_tokens * 2 * f.n_kv)), dim3(64), 0, s,
                          (unsigned char*)k_pool, (unsigned char*)v_pool, num_blocks * page_size, f,
                          (const T*)k, k_stride, (const T*)v, v_stride, slot_mapping, status_word);
   };
@@ -355,26 +423,27 @@ int pkv_read_4bit(const void* k_pool, const void* v_pool, int64_t num_blocks,
     return fail(PKV_ERR_INVALID, "null pointer argument");
   const FourBit f = four_bit(n_kv_heads, head_dim, page_size);
   hipStream_t s = (hipStream_t)stream;
-  const int n = f.tiled ? 8 : 2;
-  if (((uintptr_t)k | (uintptr_t)v) % (n * eb))
-    return fail(PKV_ERR_INVALID, "k and v have to be aligned to %d bytes", n * eb);
-  const int64_t threads = n_rows > (1ll << 40) ? INT64_MAX - 255
-                                               : n_rows * 2 * (n_kv_heads * head_dim / n);
-  const int64_t blocks = (threads + 255) / 256;
-  if (blocks > 0x7fffffffLL) return fail(PKV_ERR_INVALID, "too many rows in one read");
-  auto go = [&](auto type, auto width) {
+  const int n = f.tiled ? 16 : 2;                  // elements of a thread
+  if (((uintptr_t)k | (uintptr_t)v) % (std::min(n, 8) * eb))
+    return fail(PKV_ERR_INVALID, "k and v have to be aligned to %d bytes", std::min(n, 8) * eb);
+  const int per_head = head_dim / n, per_row = n_kv_heads * per_head;
+  const int64_t total = n_rows > 0x7fffffffLL ? n_rows : n_rows * 2 * per_row;
+  if (total > 0x7fffffffLL) return fail(PKV_ERR_INVALID, "too many rows in one read");
+  auto go = [&](auto kernel, auto type) {
     typedef decltype(type) T;
-    hipLaunchKernelGGL((read_4bit_kernel<T, decltype(width)::value>), dim3((unsigned)blocks),
-                       dim3(256), 0, s, (const unsigned char*)k_pool, (const unsigned char*)v_pool,
-                       num_blocks * page_size, f, slots, n_rows, (T*)k, (T*)v, status_word);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s,
+                       (const unsigned char*)k_pool, (const unsigned char*)v_pool,
+                       num_blocks * page_size, f, div_by(per_row), div_by(per_head),
+                       div_by(page_size), slots, (uint32_t)total, (T*)k, (T*)v, status_word);
   };
-  auto by_type = [&](auto width) {
-    if (dtype == PKV_DTYPE_F16) go(_Float16{}, width);
-    else if (dtype == PKV_DTYPE_BF16) go(__bf16{}, width);
-    else go(float{}, width);
+  auto by_type = [&](auto type) {
+    typedef decltype(type) T;
+    if (f.tiled) go(read_4bit_kernel<T>, type);
+    else go(read_4bit_any_kernel<T>, type);
   };
-  if (f.tiled) by_type(std::integral_constant<int, 8>{});
-  else by_type(std::integral_constant<int, 2>{});
+  if (dtype == PKV_DTYPE_F16) by_type(_Float16{});
+  else if (dtype == PKV_DTYPE_BF16) by_type(__bf16{});
+  else by_type(float{});
   PKV_LAUNCH_CHECK();
   return PKV_OK;
 }

@@ -254,6 +254,9 @@ class PagedPool:
             raise ValueError(f"layer_idx {layer_idx} out of range [0, {self.num_layers})")
 
     def _dev_i32(self, t: torch.Tensor) -> torch.Tensor:
+        # (as it is, without conversion calls, where nothing is to be done)
+        if t.dtype is torch.int32 and t.get_device() == self.device.index and t.is_contiguous():
+            return t
         return t.to(device=self.device, dtype=torch.int32).contiguous()
 
     def _as_pool(self, x: torch.Tensor) -> torch.Tensor:

@@ -63,13 +63,13 @@ constexpr int kOneResident = 16, kOneLeast = 4, kOneWaveRows = 8;
 // Few rows beside wide ones run as wide ones up to kJoin times their tiles: one launch
 // with one ramp and tail, for a row of them at least half idle in the matrix cores.
 constexpr int kJoin = 4;
-// A sequence is tall where kTallAlong tiles x compute units <= kTallWork work (tiles of
-// all wide pieces): a tile takes a tall piece by itself 1.2 us at head_dim 64, a wide
-// one 1.3 us / 4 of a compute unit (1.8 and 1.9 / 4 at 128). Measured, head_dim 64,
-// 4 query heads each of 8, tall and wide: one chunk of 2000 tokens 46 and 50 us, of 512
-// over 30000 571 and 297; 8 of 128 over 1000 30 and 33, over 4000 92 and 86; 64 of 20
-// over 300 17 and 23; 8 of 512 over 1536 94 and 152.
-constexpr int64_t kTallAlong = 7, kTallWork = 2;
+// A sequence is tall where kTallAlong tiles x compute units <= work (tiles of all wide
+// pieces): a tile takes a tall piece by itself 1.7 us at head_dim 64, a wide one 1.3 us
+// / 4 of a compute unit (2.9 and 1.9 / 4 at 128). Measured, 4 query heads each of 8, tall
+// and wide: 8 chunks of 512 over 1536 153 and 177 us (head_dim 128: 267 and 318), 16 of
+// 512 over 100 67 and 117, 64 of 20 over 300 30 and 43 (128); one of 2000 tokens 57 and
+// 46, 8 of 128 over 1000 35 and 30.
+constexpr int64_t kTallAlong = 5;
 
 // Floats per wave for a tile's steps, zeros of K, steps and middles of V
 // ([4][group][key]).
@@ -744,7 +744,7 @@ static int plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr,
   // out as wide pieces.
   for (const int32_t i : many) {
     const int64_t along = (kv_lens[i] + kTile - 1) / kTile;
-    part(i, kTallAlong * along * compute_units <= kTallWork * work ? 2 : 1, true);
+    part(i, kTallAlong * along * compute_units <= work ? 2 : 1, true);
   }
   if (!fast) return PKV_OK;
   // Beside wide rows few rows run as wide ones do, unless theirs are most tiles: one

@@ -1,18 +1,23 @@
 // Attention over the 4-bit cache for many query rows a sequence (prompt chunks): a
 // workgroup of four waves takes 128 rows (tokens x heads of a KV head) over all the
-// keys they see, 64 at a time. The matrix cores bound it, and beside them the
-// softmax's vector work, so a tile's codes become float16 values once for all rows:
+// keys they see, 64 at a time. The softmax's vector work bounds it, and beside it the
+// matrix cores, so a tile's codes become operands once for all rows:
 //  * each wave takes one unit of 16 keys from memory into registers a tile ahead
-//    (a lane its operand's codes, its keys' steps and zeros) and writes zero +
-//    step c to LDS: K row by row, V dim by dim, so that both are read as operands
-//    16 bytes a lane. Two tiles' buffers, one barrier a tile;
-//  * S^T = K Q^T and O^T += V^T P^T by 32x32x16 products, 32 rows a wave; the
-//    softmax of a row in its two lanes, its reference moved only when a lane's sum
-//    of a tile passes 2^12.
-// K and V are rounded to float16 here (2^-12 of a value at most, what a 16-bit cache
-// holds of it); with exact codes and the steps applied to the scores and weights, as
-// for few rows, 8 x 512 tokens over 1536 (head_dim 64) took 152 us, as here 95
-// (640 TFLOP/s).
+//    (a lane its operand's codes, its keys' words) and writes to LDS: K's codes as
+//    float16 numbers c 2^-24, row by row, V's as (c - 7.5) 2^-9, dim by dim, so that
+//    both are read as operands 16 bytes a lane; and the words. Two tiles' buffers, one
+//    barrier a tile;
+//  * S^T = K Q^T and O^T += V^T P^T by 32x32x16 products, 32 rows a wave; a score is
+//    sum_g step_g (q . c)_g + zero_g sum q, exact but for 32-bit sums; the softmax of a
+//    row in its two lanes, its reference moved only when a lane's sum of a tile passes
+//    2^12;
+//  * P is p step, rounded to float16 once (2^-11 of it), against c - 7.5, and in 32
+//    bits p zero + 7.5 p step. With 2^E at least the largest step so far (the same for
+//    all rows), p counts 2^-E more, so that p step stays within float16.
+// (With the values zero + step c rounded to float16 in LDS and p beside them, 8 x 512
+// tokens over 1536, head_dim 64, take 95 us, here 122
+// (490 TFLOP/s; as wide pieces 155), but the three roundings of
+// 2^-11 are, together, 1.5 times the output's own; these are as large as it.)
 // Rows of 144 bytes (272 for K at head_dim 128) put the 16 lanes of a 16-byte read on
 // different banks.
 #include "attend_fourbit.h"
@@ -21,22 +26,21 @@ namespace pkv {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-// 1024 + c (or 1024 + 16 c) in the halves of w, as numbers less 1024
-__device__ __forceinline__ f16x2 code_pair(uint32_t w, uint32_t mask) {
-  const f16x2 k{(_Float16)1024.f, (_Float16)1024.f};
-  return __builtin_bit_cast(f16x2, (w & mask) | 0x64006400u) - k;
-}
-__device__ __forceinline__ f16x2 fma2(f16x2 a, f16x2 b, f16x2 c) {
-  return __builtin_elementwise_fma(a, b, c);
-}
+__device__ __forceinline__ float step_of(uint32_t w) { return (float)f16_bits(w >> 16); }
+__device__ __forceinline__ float zero_of(uint32_t w) { return (float)f16_bits(w & 0xffffu); }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void attend_4bit_tall_kernel(Attend4 a) {
+__global__ __launch_bounds__(256, (D == 64 ? 3 : 2)) void attend_4bit_tall_kernel(Attend4 a) {
   constexpr int NG = D / 64, W = D / 32, NC = D / 16, NB = D / 32;
+  // keys of a step, in 32: all of a tile's, or half where the registers hold no more
+  // (head_dim 64 in halves: 131 us for 122; 128 in whole tiles: 298 for 267)
+  constexpr int NH = D == 64 ? 2 : 1;
   constexpr int KS = 2 * D + 16, VS = 2 * kTile + 16;    // bytes of an LDS row
   constexpr int KB = kTile * KS, BUF = KB + D * VS;
   constexpr uint32_t LO = 0x000f000fu, UP = 0x00f000f0u;
   __shared__ __align__(16) unsigned char smem[2 * BUF];
+  __shared__ __align__(16) uint32_t words[2][2][NG][kTile];   // a tile's, of K and of V
+  __shared__ __align__(16) uint32_t tops[2][4];          // its units' largest words of V
   __shared__ __align__(8) uint16_t nan_keys[2][NG][4];   // a tile's keys whose V is NaN
 
   // (as in the pieces' kernel: a tile's heads on one XCD)
@@ -92,86 +96,76 @@ __global__ __launch_bounds__(256, 2) void attend_4bit_tall_kernel(Attend4 a) {
       }
     }
   };
-  auto halves = [](uint32_t lo, uint32_t hi) {
-    return __builtin_bit_cast(f16x2, (lo & 0xffffu) | hi << 16);
-  };
-  const f16x2 sixteenth{(_Float16)0.0625f, (_Float16)0.0625f};
-  // The unit's values into tile buffer `of`. RARE: steps of 4096 on, whose values may
-  // round past the largest float16, or NaN: a NaN of V is left out, and its key noted.
-  auto stage_as = [&](int of, auto rare) {
-    constexpr bool RARE = decltype(rare)::value;
+  // The unit into tile buffer `of`. A word of V that is NaN is left out, its key noted.
+  auto stage = [&](int of) {
     unsigned char* const buf = smem + of * BUF;
-    auto held = [&](f16x2 code, f16x2 step, f16x2 zero) {
-      f16x2 v = fma2(code, step, zero);
-      if constexpr (RARE) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (__builtin_bit_cast(uint16_t, (_Float16)v[i]) == 0x7c00u) v[i] = (_Float16)kF16Max;
-      }
-      return __builtin_bit_cast(uint32_t, v);
-    };
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const uint32_t p = kw[w / 2], c = kc[w], c8 = c >> 8;
-      const f16x2 step = halves(p >> 16, p >> 16), zero = halves(p, p), s16 = step * sixteenth;
-      // elements (0, 4) (1, 5) (2, 6) (3, 7), as Q has them
-      const u32x4 v{held(code_pair(c, LO), step, zero), held(code_pair(c, UP), s16, zero),
-                    held(code_pair(c8, LO), step, zero), held(code_pair(c8, UP), s16, zero)};
+      // elements (0, 4) (1, 5) (2, 6) (3, 7), as Q has them; the second and fourth
+      // pair 16 times as large
+      const uint32_t c = kc[w], c8 = c >> 8;
       const int dim = 64 * (w / 2) + 16 * kg + 8 * (w & 1);
-      *reinterpret_cast<u32x4*>(buf + (16 * wave + kn) * KS + 2 * dim) = v;
+      *reinterpret_cast<u32x4*>(buf + (16 * wave + kn) * KS + 2 * dim) =
+          u32x4{c & LO, c & UP, c8 & LO, c8 & UP};
     }
-    // V: keys (0, 2), (1, 3) of a quartet; of 16 keys the quartets lie 0 2 1 3, so
-    // that a lane's two of a product are neighbours
-    const int at = KB + 32 * wave + (kg & 1) * 16 + (kg >> 1) * 8;
-#pragma unroll
-    for (int q = 0; q < NG; ++q) {
-      uint32_t p[4];
-      uint32_t none = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        p[j] = vw[q][j];
-        if constexpr (RARE) {
-          const bool nan = p[j] >= 0x7c010000u;
-          // (bit 4 kg + j of the unit's keys, from the lanes kn = 0)
-          const uint64_t b = __builtin_amdgcn_ballot_w64(nan);
-          none |= (uint32_t)((b & 1) << j | (b >> 16 & 1) << (4 + j) | (b >> 32 & 1) << (8 + j) |
-                             (b >> 48 & 1) << (12 + j));
-          p[j] = nan ? 0u : p[j];
-        }
-      }
-      if (lane == 0) nan_keys[of][q][wave] = (uint16_t)none;
-      const f16x2 sa = halves(p[0] >> 16, p[2] >> 16), sb = halves(p[1] >> 16, p[3] >> 16);
-      const f16x2 za = halves(p[0], p[2]), zb = halves(p[1], p[3]);
-      const f16x2 sa16 = sa * sixteenth, sb16 = sb * sixteenth;
-#pragma unroll
-      for (int b = 2 * q; b < 2 * q + 2; ++b) {
-        const uint32_t c = vc[b], c8 = c >> 8;
-        const u32x2 lo{held(code_pair(c, LO), sa, za), held(code_pair(c8, LO), sb, zb)};
-        const u32x2 up{held(code_pair(c, UP), sa16, za), held(code_pair(c8, UP), sb16, zb)};
-        *reinterpret_cast<u32x2*>(buf + at + (32 * b + kn) * VS) = lo;
-        *reinterpret_cast<u32x2*>(buf + at + (32 * b + 16 + kn) * VS) = up;
-      }
-    }
-  };
-  auto stage = [&](int of) {
     uint32_t top = 0;
 #pragma unroll
     for (int q = 0; q < NG; ++q)
-      top = max(top, max(max(kw[q], max(vw[q][0], vw[q][1])), max(vw[q][2], vw[q][3])));
-    if (__builtin_amdgcn_ballot_w64(top >= 0x6c000000u)) stage_as(of, std::true_type{});
-    else stage_as(of, std::false_type{});
+      top = max(top, max(max(vw[q][0], vw[q][1]), max(vw[q][2], vw[q][3])));
+    uint32_t none[NG] = {};
+    if (__builtin_amdgcn_ballot_w64(top >= 0x7c000000u)) {
+      top = 0;
+#pragma unroll
+      for (int q = 0; q < NG; ++q)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool nan = vw[q][j] >= 0x7c000000u;
+          // (bit 4 kg + j of the unit's keys, from the lanes kn = 0)
+          const uint64_t b = __builtin_amdgcn_ballot_w64(nan);
+          none[q] |= (uint32_t)((b & 1) << j | (b >> 16 & 1) << (4 + j) | (b >> 32 & 1) << (8 + j) |
+                                (b >> 48 & 1) << (12 + j));
+          vw[q][j] = nan ? 0u : vw[q][j];
+          top = max(top, vw[q][j]);
+        }
+    }
+    const uint32_t unit_top = max(max(__builtin_amdgcn_readlane(top, 0), __builtin_amdgcn_readlane(top, 16)),
+                                  max(__builtin_amdgcn_readlane(top, 32), __builtin_amdgcn_readlane(top, 48)));
+#pragma unroll
+    for (int q = 0; q < NG; ++q) {
+      if (lane < 16) words[of][0][q][16 * wave + kn] = kw[q];
+      if (kn == 0) *reinterpret_cast<u32x4*>(&words[of][1][q][16 * wave + 4 * kg]) = vw[q];
+      if (lane == 0) nan_keys[of][q][wave] = (uint16_t)none[q];
+    }
+    if (lane == 0) tops[of][wave] = unit_top;
+    // V: keys (0, 2), (1, 3) of a quartet; of 16 keys the quartets lie 0 2 1 3, so
+    // that a lane's two of a product are neighbours
+    const int at = KB + 32 * wave + (kg & 1) * 16 + (kg >> 1) * 8;
+    auto middle = [](uint32_t codes, float unit) {    // (c - 7.5) 2^-9 of c unit 2^-24
+      const _Float16 f = (_Float16)(0x1p15f / unit), m = (_Float16)(-7.5f * 0x1p-9f);
+      return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(
+          __builtin_bit_cast(f16x2, codes), f16x2{f, f}, f16x2{m, m}));
+    };
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const uint32_t c = vc[b], c8 = c >> 8;
+      *reinterpret_cast<u32x2*>(buf + at + (32 * b + kn) * VS) =
+          u32x2{middle(c & LO, 1.f), middle(c8 & LO, 1.f)};
+      *reinterpret_cast<u32x2*>(buf + at + (32 * b + 16 + kn) * VS) =
+          u32x2{middle(c & UP, 16.f), middle(c8 & UP, 16.f)};
+    }
   };
   load(0, page(0));
 
   // Q^T as the B operand: lane (row, g) holds dims 16 c + 8 g .. + 7, scaled by a
   // power of two to a largest element in [128, 256) (a product of 256 elements of
-  // +-65504 stays finite), the scale's sign with it.
+  // +-65504 stays finite), the scale's sign with it; the elements whose codes count 16
+  // times as much a 16th. qs: a group's sum, in a product's unit of 2^-24.
   const int r = wave * 32 + n;
   const int tok = (int)((uint32_t)r * a.per_group >> 16);
   const bool valid = tok < qn;
   const int qpos = base_pos + (valid ? tok : qn - 1);
   f16x8 qb[NC];
-  float f1;
+  float f1, qs[NG] = {};
   {
     typedef T TV __attribute__((ext_vector_type(8)));
     const T* row = reinterpret_cast<const T*>(a.q) +
@@ -194,14 +188,21 @@ __global__ __launch_bounds__(256, 2) void attend_4bit_tall_kernel(Attend4 a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float e = __builtin_amdgcn_ldexpf(Elem<T>::to_f(v[c][(i >> 1) + 4 * (i & 1)]), k);
-        qb[c][i] = (_Float16)(!valid ? 0.f : turn ? -e : e);
+        const _Float16 x = (_Float16)(!valid ? 0.f : turn ? -e : e);
+        qs[c / 4] += (float)x;
+        qb[c][i] = (i & 2) ? x * (_Float16)0.0625f : x;
       }
+    f1 *= 0x1p24f;
+#pragma unroll
+    for (int q = 0; q < NG; ++q) qs[q] = sum_x32(qs[q]) * 0x1p-24f;
   }
 
   f32x16 o[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) o[b] = f32x16{};
   float ref = -INFINITY, l = 0.f, none[NG] = {};
+  float zeros[NG] = {}, steps[NG] = {};   // sums of p zero, p step
+  int top = -30;                     // E
 
   stage(0);
   int next = page(1);                // (read a tile ahead of its use)
@@ -210,70 +211,119 @@ __global__ __launch_bounds__(256, 2) void attend_4bit_tall_kernel(Attend4 a) {
   __syncthreads();
   for (int t = 0; t < n_tiles; ++t) {
     const unsigned char* buf = smem + (t & 1) * BUF;
-    // S^T: s[hf][e] = the row's score with key 64 t + 32 hf + 8 (e / 4) + 4 g + e % 4
-    f32x16 s[2];
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) s[hf] = f32x16{};
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
-        s[hf] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-            *reinterpret_cast<const f16x8*>(buf + (32 * hf + n) * KS + 32 * c + 16 * g), qb[c], s[hf],
-            0, 0, 0);
-    if (kTile * t + kTile - 1 > base_pos) {
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (kTile * t + 32 * hf + 8 * (e >> 2) + 4 * g + (e & 3) > qpos) s[hf][e] = -INFINITY;
+    const auto& wk = words[t & 1][0];
+    const auto& wv = words[t & 1][1];
+    // a larger step than any before: the sums in its unit
+    const u32x4 tile_tops = *reinterpret_cast<const u32x4*>(tops[t & 1]);
+    const uint32_t word = __builtin_amdgcn_readfirstlane(
+        max(max(tile_tops[0], tile_tops[1]), max(tile_tops[2], tile_tops[3])));
+    const int now = word >= 0x10000u ? __builtin_amdgcn_frexp_expf(step_of(word)) : top;
+    float by = 1.f;                  // what the sums so far count now
+    bool less = now > top;
+    if (less) {
+      by = __builtin_amdgcn_ldexpf(1.f, top - now);
+      ref += (float)(now - top);
+      top = now;
     }
-    float ls;
-    f16x8 pb[4];
-    auto probs = [&](float m) {
-      ls = 0.f;
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
+    for (int h0 = 0; h0 < 2; h0 += NH) {
+      // s[hf][e] = the row's score with key 64 t + 32 (h0 + hf) + 8 (e / 4) + 4 g + e % 4
+      f32x16 s[NH];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[hf][e], f1, -m));
-          ls += p;
-          // (quartets as V has them: 0 2 1 3)
-          pb[2 * hf + (e >> 3)][(e & 4) + ((e & 1) << 1 | (e >> 1 & 1))] = (_Float16)p;
-        }
-    };
-    // (one copy of the weights' code: two took 31 registers more, a third of the waves)
-    float m = ref;
-    for (int again = 0;; ++again) {
-      probs(m);
-      if (again || !__builtin_amdgcn_ballot_w64(!(ls <= 4096.f))) break;
+      for (int hf = 0; hf < NH; ++hf) {
+        f32x16 acc[NG];
+#pragma unroll
+        for (int q = 0; q < NG; ++q) acc[q] = f32x16{};
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          acc[c / 4] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+              *reinterpret_cast<const f16x8*>(buf + (32 * (h0 + hf) + n) * KS + 32 * c + 16 * g),
+              qb[c], acc[c / 4], 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int q = 0; q < NG; ++q) {
+            const u32x4 w = *reinterpret_cast<const u32x4*>(&wk[q][32 * (h0 + hf) + 8 * j + 4 * g]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int e = 4 * j + i;
+              const float z = __builtin_fmaf(zero_of(w[i]), qs[q], q ? s[hf][e] : 0.f);
+              s[hf][e] = __builtin_fmaf(step_of(w[i]), acc[q][e], z);
+            }
+          }
+      }
+      const int key = kTile * t + 32 * h0;
+      if (key + 32 * NH - 1 > base_pos) {
+#pragma unroll
+        for (int hf = 0; hf < NH; ++hf)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (key + 32 * hf + 8 * (e >> 2) + 4 * g + (e & 3) > qpos) s[hf][e] = -INFINITY;
+      }
+      // (looking at the largest score first keeps the scores' registers for the weights)
       float mx = -INFINITY;
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
+      for (int hf = 0; hf < NH; ++hf)
 #pragma unroll
         for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[hf][e]);
-      m = fmaxf(ref, max_x32(mx) * f1);
-      const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref - m);
-      ref = m;
-      m = m == -INFINITY ? 0.f : m;
-      l *= alpha;
+      mx = __builtin_fmaf(mx, f1, (float)top);
+      if (__builtin_amdgcn_ballot_w64(!(mx - ref <= 12.f))) {
+        const float m = fmaxf(ref, max_x32(mx));
+        by *= m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref - m);
+        less = true;
+        ref = m;
+      }
+      if (less) {
+        l *= by;
 #pragma unroll
-      for (int b = 0; b < NB; ++b) o[b] *= alpha;
+        for (int q = 0; q < NG; ++q) {
+          zeros[q] *= by;
+          steps[q] *= by;
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) o[b] *= by;
+        less = false;
+        by = 1.f;
+      }
+      f16x8 pb[NG][2 * NH];
+      const float m = ref == -INFINITY ? 0.f : ref;
+#pragma unroll
+      for (int hf = 0; hf < NH; ++hf)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float p[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[hf][4 * j + i], f1, -m));
+            l += p[i];
+          }
+#pragma unroll
+          for (int q = 0; q < NG; ++q) {
+            const u32x4 w = *reinterpret_cast<const u32x4*>(&wv[q][32 * (h0 + hf) + 8 * j + 4 * g]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              zeros[q] = __builtin_fmaf(p[i], zero_of(w[i]), zeros[q]);
+              steps[q] = __builtin_fmaf(p[i], step_of(w[i]), steps[q]);
+              // (quartets as V has them: 0 2 1 3)
+              pb[q][2 * hf + (j >> 1)][(4 * j & 4) + ((i & 1) << 1 | (i >> 1 & 1))] =
+                  (_Float16)__builtin_fmaf(p[i], step_of(w[i]), 0.f);
+            }
+          }
+        }
+      // the next tile into the other buffer, the one after it on its way
+      if (h0 == 0 && t + 1 < n_tiles) {
+        stage((t + 1) & 1);
+        if (t + 2 < n_tiles) load(t + 2, next);
+        next = page(t + 3);
+      }
+#pragma unroll
+      for (int kb = 0; kb < 2 * NH; ++kb)
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+              *reinterpret_cast<const f16x8*>(buf + KB + (32 * b + n) * VS + 64 * h0 + 32 * kb + 16 * g),
+              pb[b / 2][kb], o[b], 0, 0, 0);
     }
-    l += ls;
-    // the next tile into the other buffer, the one after it on its way
-    if (t + 1 < n_tiles) {
-      stage((t + 1) & 1);
-      if (t + 2 < n_tiles) load(t + 2, next);
-      next = page(t + 3);
-    }
-#pragma unroll
-    for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-            *reinterpret_cast<const f16x8*>(buf + KB + (32 * b + n) * VS + 32 * kb + 16 * g), pb[kb],
-            o[b], 0, 0, 0);
     // a row that sees a key whose V is NaN gets NaN, at the end
 #pragma unroll
     for (int q = 0; q < NG; ++q) {
@@ -288,8 +338,10 @@ __global__ __launch_bounds__(256, 2) void attend_4bit_tall_kernel(Attend4 a) {
   }
   if (worst && lane == 0) flag(a.status, PKV_STATUS_BAD_PAGE);
   l = sum_x32(l);
+#pragma unroll
+  for (int q = 0; q < NG; ++q) none[q] += sum_x32(__builtin_fmaf(7.5f, steps[q], zeros[q])) / l;
   if (!valid) return;
-  const float inv = 1.f / l;
+  const float inv = 512.f / l;
   typedef T TV4 __attribute__((ext_vector_type(4)));
   T* row = reinterpret_cast<T*>(a.out) + ((int64_t)(q0 + tok) * Hq + h * G + r - tok * G) * D + 4 * g;
 #pragma unroll

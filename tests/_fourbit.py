@@ -44,7 +44,7 @@ def held64(x):
     return (zero[..., None] + codes * step[..., None]).flatten(-2)
 
 
-def attend64(q, k, v, scale, dtype, tall=False):
+def attend64(q, k, v, scale, dtype):
     """
     Causal attention of the last n of N tokens: q (n, Hq, D); k, v (N, Hkv, D)
     rows before they are quantised. Returns (out, bound), (n, Hq, D) in 64 bits.
@@ -67,11 +67,6 @@ def attend64(q, k, v, scale, dtype, tall=False):
                                        sequence is below 2 and the row's largest
                                        p at least 1 / 2: up to 4 units a code,
                                        hence 4 times that
-    and where many rows share a tile (``tall``), whose keys and values are rounded
-    to float16 (2^-11 of each, or 2^-25 where that is more) and whose weights are
-    rounded without their step:
-      2 2^-11 sum_t p_t |v_t|          values and weights
-      2 kappa sum_t p_t |v_t|          kappa = 2^-11 |scale| max sum |q| |k|, as delta
     """
     n, hq, d = q.shape
     total, hkv = k.shape[0], k.shape[1]
@@ -88,17 +83,12 @@ def attend64(q, k, v, scale, dtype, tall=False):
     out, bound = torch.empty_like(qq), torch.empty_like(qq)
     for h in range(hq):
         of = h // gr
-        extra = 0.0
         s = qq[:, h] @ kk[:, of].t() * scale
         p = torch.softmax(s.masked_fill(~see, -math.inf), dim=-1)
         delta = ((d + 8) * 2.0 ** -24 * abs(scale)
                  * (qq[:, h].abs() @ kb[:, of].t()).masked_fill(~see, 0).amax(1, keepdim=True))
         out[:, h] = p @ vv[:, of]
-        if tall:
-            kappa = ((qq[:, h].abs() @ (kk[:, of].abs().t() * 2.0 ** -11 + 2.0 ** -25))
-                     * abs(scale)).masked_fill(~see, 0).amax(1, keepdim=True)
-            extra = (2 * 2.0 ** -11 + 2 * kappa) * (p @ vv[:, of].abs()) + 2.0 ** -24
         bound[:, h] = (u * out[:, h].abs() + 2.0 ** -11 * (p @ vr[:, of])
                        + (2 * delta + 2 * (total + 64) * 2.0 ** -24) * (p @ vb[:, of])
-                       + total * 2.0 ** -23 * 15 * vs[:, of].max() + extra)
+                       + total * 2.0 ** -23 * 15 * vs[:, of].max())
     return out, bound * 1.001 + torch.finfo(dtype).tiny

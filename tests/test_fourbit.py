@@ -87,7 +87,7 @@ def test_the_plan_covers_every_row_and_tile_once(compute_units, n_heads, n_kv):
     work = n_kv * sum(-(-(k - n + min(n, at + step)) // 64) for k, n in zip(kv, ql)
                       if n * groups > 64 for at in range(0, n, step))
     tall_seqs = {i for i, (k, n) in enumerate(zip(kv, ql)) if n * groups > 64
-                 and 7 * -(-k // 64) * compute_units <= 2 * work}
+                 and 5 * -(-k // 64) * compute_units <= work}
     for i, (row, qn, pos, kvl, page, pages, t0, nt, slot, slot0, n, counter, *ids) in \
             enumerate(items):
         seq = int(np.searchsorted(cu, row, side="right")) - 1

@@ -77,19 +77,11 @@ class Cache:
         g = torch.Generator().manual_seed(self.seed + 77)
         return (torch.randn((sum(counts), hq, d), generator=g) * factor).to(self.dtype)
 
-    def tall(self, n):
-        """Whether n tokens of the last batch may have run as a tall piece."""
-        n_kv, hq, d = self.dims
-        return (self.dtype != F32 and d in (64, 128) and self.ps in (16, 32, 64)
-                and hq // n_kv <= 32 and n * (hq // n_kv) > 64
-                and self.bk._planned.args.n_tall > 0)
-
     def check(self, got, q, counts, scale, label=""):
         got, at = got.cpu(), 0
         for i, n in enumerate(counts):
             if n:
-                want, bound = attend64(q[at:at + n], self.k[i], self.v[i], scale, self.dtype,
-                                       self.tall(n))
+                want, bound = attend64(q[at:at + n], self.k[i], self.v[i], scale, self.dtype)
                 assert_within(got[at:at + n], want, bound, f"{label} seq {i}")
             at += n
 
@@ -341,8 +333,7 @@ def test_rows_that_no_token_sees(d, hq, units):
     out = c.bk.attend(q.to(DEV), 0, d ** -0.5, meta).cpu()
     at = 0
     for n in counts:
-        want, bound = attend64(q[at:at + n - 1], k[at:at + n - 1], v[at:at + n - 1], d ** -0.5, F16,
-                               c.tall(n))
+        want, bound = attend64(q[at:at + n - 1], k[at:at + n - 1], v[at:at + n - 1], d ** -0.5, F16)
         assert_within(out[at:at + n - 1], want, bound)
         assert out[at + n - 1].isnan().all()
         at += n
@@ -393,7 +384,7 @@ def test_pages_outside_the_pool_among_many_rows(n, units):
     out = c.bk.attend(q.to(DEV), 0, 0.125, meta).cpu()
     k, v = c.k[0].clone(), c.v[0].clone()
     k[48:64], v[48:64] = 0, 0
-    want, bound = attend64(q, k, v, 0.125, F16, c.tall(n))
+    want, bound = attend64(q, k, v, 0.125, F16)
     assert_within(out, want, bound)
     with pytest.raises(IndexError, match="kv_indices"):
         c.bk.check_device_errors()

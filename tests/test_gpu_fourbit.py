@@ -277,21 +277,22 @@ def test_other_scales(d, hq, scale):
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("factor", [1e-4, 30.0])
-def test_peaked_and_flat_weights(dtype, factor):
+@pytest.mark.parametrize("counts,units,d", [([1, 6], None, 64), ([40, 30], 1, 64), ([40, 30], 1, 128)])
+def test_peaked_and_flat_weights(dtype, factor, counts, units, d):
     """Queries so large that one key takes all, and so small that none does."""
-    c = Cache([900, 333], dtype, 2, 8, 64)
-    counts = [1, 6]
+    print(f"peaked {dtype} {factor} {counts} {d}", flush=True)
+    c = Cache([900, 333], dtype, 2, 8, d, compute_units=units)
     meta = c.append(counts)
     q = c.q(counts, factor)
     c.check(c.bk.attend(q.to(DEV), 0, 0.125, meta), q, counts, 0.125)
 
 
 @pytest.mark.parametrize("grow", [2.0 ** -9, 2.0 ** 9])
-@pytest.mark.parametrize("new", [1, 9])
-def test_values_that_grow_along_the_sequence(grow, new):
+@pytest.mark.parametrize("new,units", [(1, None), (9, None), (40, None), (40, 1)])
+def test_values_that_grow_along_the_sequence(grow, new, units):
     """Steps of V that rise or fall by 2^9 between tiles: what keeps p step in
     range follows them."""
-    c = Cache([0], F16, 2, 8, 64, room=700)
+    c = Cache([0], F16, 2, 8, 64, room=700, compute_units=units)
     c.seqs[0].append(640)
     n = 640
     k = rows((n, 2, 64), F16, 1)
@@ -303,6 +304,51 @@ def test_values_that_grow_along_the_sequence(grow, new):
     meta = c.append(counts)
     q = c.q(counts)
     c.check(c.bk.attend(q.to(DEV), 0, 0.125, meta), q, counts, 0.125)
+
+
+@pytest.mark.parametrize("new,units", [(1, None), (9, None), (40, 1)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_groups_without_a_step(d, new, units):
+    """Constant groups have a step of 0: all of V's, then V's of the first tiles alone."""
+    for last in (False, True):
+        c = Cache([0], F16, 2, 8, d, room=400, compute_units=units)
+        n = 200
+        c.seqs[0].append(n)
+        k = rows((n, 2, d), F16, 1)
+        v = rows((n, 2, 1), F16, 2).expand(n, 2, d).contiguous()
+        if last:
+            v[-30:] = rows((30, 2, d), F16, 3) * 2.0 ** -12
+        c.k, c.v = [k], [v]
+        c.bk.append_kv(0, k.to(DEV), v.to(DEV), make_meta(c.seqs, [n], 16, device=DEV))
+        s = c.seqs[0]
+        meta = make_meta(c.seqs, [new], 16, device=DEV)      # (the last rows' queries)
+        q = c.q([new])
+        c.check(c.bk.attend(q.to(DEV), 0, 0.125, meta), q, [new], 0.125, f"last {last}")
+        assert s.num_tokens == n
+
+
+def test_blocks_past_32_bits():
+    """Block ids whose bytes lie beyond 2^32."""
+    n_kv, d, blocks = 8, 128, 2**32 // 36864 + 40
+    bk = FourBitBackend(1, blocks, 16 * 4, n_kv, 32, d, device=DEV)
+    assert bk._block_bytes * (blocks - 20) > 2**32
+    alloc = BlockAllocator(blocks, 64)
+    low = alloc.allocate(blocks - 20)
+    s = SequenceBlocks(alloc, seq_id=0)
+    meta = grow_and_assemble([s], [300], 64, device=DEV)
+    assert min(s.block_ids) >= blocks - 20 and len(low) == blocks - 20
+    k, v = rows((300, n_kv, d), F16, 5), rows((300, n_kv, d), F16, 6)
+    bk.append_kv(0, k.to(DEV), v.to(DEV), meta)
+    gk, gv = bk.read_kv(0, meta.slot_mapping)
+    same_bits(gk, held64(k), F16)
+    same_bits(gv, held64(v), F16)
+    g = torch.Generator().manual_seed(1)
+    q = torch.randn((300, 32, d), generator=g).to(F16)
+    for n in (1, 4, 300):
+        part = make_meta([s], [n], 64, device=DEV)
+        out = bk.attend(q[:n].to(DEV), 0, d ** -0.5, part).cpu()
+        want, bound = attend64(q[:n], k, v, d ** -0.5, F16)
+        assert_within(out, want, bound, f"{n} tokens")
 
 
 @pytest.mark.parametrize("units", [None, 1])

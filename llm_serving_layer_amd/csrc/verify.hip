@@ -53,11 +53,11 @@ struct Verify {
   const float *numbers, *temps;
   RowStats* stats;
   Decision* decisions;
-  double *sums, *rest;              // of a sequence's parts: 2^x, max(2^x - q z, 0)
+  double *sums, *rest;              // of a sequence's units: 2^x, max(2^x - q z, 0)
   int32_t* counters;                // two a sequence; cleared by the first kernel
   int64_t *ids, *accepted;
   int64_t row_stride, probs_stride, width;
-  int32_t n_rows, n_seqs, vocab, splits, parts;
+  int32_t n_rows, n_seqs, vocab, splits, parts, units, cells;
   float temp, error;                // error: of a row's 32-bit sum, relative
 };
 
@@ -243,7 +243,7 @@ template <typename Q> struct Eight {
 
 struct DrawLds {
   double table[256];
-  double sums[kMaxSplits], waves[kDT / 64];
+  double sums[kMaxSplits][kDT / 64], waves[kDT / 64];   // of units by wave
   RowStats rows[64];
   int flags[64];
   int last, found;
@@ -312,6 +312,38 @@ __device__ __forceinline__ double weigh_run(const T* row, const Q* q, int at, in
     p = p2;
   }
   return sum;
+}
+
+// The sums of units [u0, u1) by wave, into lds: `cells` of a thread's a unit, the next
+// one on its way while one is weighed.
+template <typename T, typename Q>
+__device__ __forceinline__ void weigh_units(const T* row, const Q* q, int u0, int u1, int cells,
+                                            const Weigh& weigh, double (&lds)[kMaxSplits][kDT / 64]) {
+  const int n = weigh.vocab, last = n - 1, tid = threadIdx.x;
+  Eight<T> l, l2;
+  Eight<Q> p{}, p2{};
+  int at = (u0 * kDT + tid) * cells * kCell;
+  l.load(row, min(at, last), n);
+  if (q) p.load(q, min(at, last), n);
+  double sum = 0.0;
+  int u = 0;
+#pragma unroll 1
+  for (int j = 1; u < u1 - u0; ++j) {
+    const int next = at + (j < cells ? 1 : (kDT - 1) * cells + 1) * kCell;
+    l2.load(row, min(next, last), n);
+    if (q) p2.load(q, min(next, last), n);
+    double w[kCell];
+    sum += weigh(l, p, q != nullptr, at, w);
+    at = next;
+    l = l2;
+    p = p2;
+    if (j < cells) continue;
+    sum = wave_sum64(sum);
+    if ((tid & 63) == 0) lds[u][tid >> 6] = sum;
+    sum = 0.0;
+    j = 0;
+    ++u;
+  }
 }
 
 // Decides a sequence (uniform over the workgroup).
@@ -430,58 +462,59 @@ __device__ Decision decide(const Verify& a, int seq, DrawLds& lds) {
   return d;
 }
 
-// Sums part s of the row that a sequence draws from; the workgroup that is the last
-// to (counter k) finds the token: the part whose running sum passes the target, in
-// it the thread, its element. Returns it there (-1: no weight at all, and then
-// none_left is set), -2 in the others. sums: the parts', beyond the XCDs' caches.
-enum DrawMode { kSumOnly, kCounted, kKnown };   // kKnown: sums hold all parts' already
+// Sums the units of part s of the row that a sequence draws from; the workgroup that is
+// the last to (counter k) finds the token: the unit whose running sum passes the
+// target, in it the thread, its element. Returns it there (-1: no weight at all), -2
+// in the others. sums: the units', beyond the XCDs' caches.
+enum DrawMode { kSumOnly, kCounted, kKnown };   // kKnown: sums hold all units' already
 
 template <typename T, typename Q>
 __device__ int draw(const Verify& a, int seq, int s, const Decision& d, const T* row, const Q* q,
                     double iz, int k, double* sums, DrawMode mode, DrawLds& lds) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  // kDT cells a part, or, where the vocabulary takes more, runs of cells a thread
-  const int per = (a.vocab + a.parts * kPart - 1) / (a.parts * kPart);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, per = a.cells;
   const Weigh weigh{lds.table, d.m, d.c, iz, d.banned, a.vocab};
-  int part = s;
-  double target = 0.0, base = 0.0;
-  bool past = false, found = false;
-  for (;;) {                         // first the part's sum, then (the last one) the token
-    const int first = (part * kDT + tid) * per * kCell;
-    const int count = first < a.vocab ? min(per, (a.vocab - first + kCell - 1) / kCell) : 0;
-    double w[kCell] = {}, mine = 0.0;
-    if (found || mode != kKnown) mine = weigh_run(row, q, first, kCell, count, weigh, w);
-    if (!found) {
-      const double sum = mode == kKnown ? 0.0 : block_sum64(mine, lds.waves);
+  if (mode != kKnown) {
+    const int u0 = s * a.units / a.parts, u1 = (s + 1) * a.units / a.parts;
+    weigh_units(row, q, u0, u1, per, weigh, lds.sums);
+    __syncthreads();
+    if (wave == 0) {
+      double sum = 0.0;
+      if (tid < u1 - u0)
+#pragma unroll
+        for (int w = 0; w < kDT / 64; ++w) sum += lds.sums[tid][w];
       if (mode == kSumOnly) {
-        if (tid == 0) sums[s] = sum;
-        return -2;
-      }
-      if (mode == kCounted && tid == 0) {
-        __hip_atomic_store(sums + s, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (tid < u1 - u0) sums[u0 + tid] = sum;
+      } else {
+        if (tid < u1 - u0)
+          __hip_atomic_store(sums + u0 + tid, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        lds.last = __hip_atomic_fetch_add(a.counters + 2 * seq + k, 1, __ATOMIC_RELAXED,
-                                          __HIP_MEMORY_SCOPE_AGENT) == a.parts - 1;
+        if (tid == 0)
+          lds.last = __hip_atomic_fetch_add(a.counters + 2 * seq + k, 1, __ATOMIC_RELAXED,
+                                            __HIP_MEMORY_SCOPE_AGENT) == a.parts - 1;
       }
-      __syncthreads();
-      if (mode == kCounted && !lds.last) return -2;
-      // (every wave the same: a lane a part)
-      const double own =
-          lane < a.parts
-              ? __hip_atomic_load(sums + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
-              : 0.0;
-      const double upto = wave_scan64(own);
-      target = (double)a.numbers[a.cu[seq + 1] - 1] * __shfl(upto, 63, 64);
-      const uint64_t over = __builtin_amdgcn_ballot_w64(own > 0.0 && upto > target);
-      const uint64_t some = __builtin_amdgcn_ballot_w64(own > 0.0);
-      if (!some) return -1;
-      // (a number of 1, or the last sum's rounding: the last weight of all)
-      past = over;
-      part = past ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
-      base = past ? __shfl(upto - own, part, 64) : 0.0;
-      found = true;
-      continue;
     }
+    if (mode == kSumOnly) return -2;
+    __syncthreads();
+    if (!lds.last) return -2;
+  }
+  // (every wave the same: a lane a unit)
+  const double own =
+      lane < a.units ? __hip_atomic_load(sums + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+                     : 0.0;
+  const double upto = wave_scan64(own);
+  const double target = (double)a.numbers[a.cu[seq + 1] - 1] * __shfl(upto, 63, 64);
+  const uint64_t passed = __builtin_amdgcn_ballot_w64(own > 0.0 && upto > target);
+  const uint64_t some = __builtin_amdgcn_ballot_w64(own > 0.0);
+  if (!some) return -1;
+  // (a number of 1, or the last sum's rounding: the last weight of all)
+  const bool past = passed;
+  const int unit = past ? __builtin_ctzll(passed) : 63 - __builtin_clzll(some);
+  const double base = past ? __shfl(upto - own, unit, 64) : 0.0;
+  {
+    const int first = (unit * kDT + tid) * per * kCell;
+    const int count = first < a.vocab ? min(per, (a.vocab - first + kCell - 1) / kCell) : 0;
+    double w[kCell] = {};
+    const double mine = weigh_run(row, q, first, kCell, count, weigh, w);
     const double scan = wave_scan64(mine);
     __syncthreads();
     if (lane == 63) lds.waves[wave] = scan;
@@ -503,6 +536,23 @@ __device__ int draw(const Verify& a, int seq, int s, const Decision& d, const T*
     }
     const bool exact = owner >= 0;
     owner = exact ? owner : latest;
+    if (per == 1) {                  // the thread's one cell is at hand
+      if (tid == owner) {
+        int got = -1;
+        bool done = false;
+#pragma unroll
+        for (int e = 0; e < kCell; ++e) {
+          run += done ? 0.0 : w[e];
+          if (!done && w[e] > 0.0) {
+            got = first + e;
+            done = exact && run > target;
+          }
+        }
+        lds.found = got;
+      }
+      __syncthreads();
+      return lds.found;
+    }
     if (tid == owner) {
       lds.waves[0] = run;
       lds.last = count;
@@ -511,7 +561,7 @@ __device__ int draw(const Verify& a, int seq, int s, const Decision& d, const T*
     // the thread's cells, now a lane each (a run of them where they are more)
     const double from = lds.waves[0];
     const int cells = lds.last, each = (cells + 63) / 64;
-    const int at = (part * kDT + owner) * per * kCell + lane * each * kCell;
+    const int at = (unit * kDT + owner) * per * kCell + lane * each * kCell;
     const int here = max(0, min(each, cells - lane * each));
     const double sum = weigh_run(row, q, at, kCell, here, weigh, w);
     const double up = wave_scan64(sum);
@@ -558,7 +608,7 @@ __global__ __launch_bounds__(kDT) void verify_draw_kernel(Verify a) {
   if (d.token >= 0) return;
   // (d.rest: the row's whole sum alone, for the next kernel)
   const int got = draw(a, seq, s, d, reinterpret_cast<const T*>(a.logits) + d.row * a.row_stride,
-                       (const Q*)nullptr, 1.0, 0, a.sums + (int64_t)seq * a.parts, d.rest ? kSumOnly : kCounted,
+                       (const Q*)nullptr, 1.0, 0, a.sums + (int64_t)seq * a.units, d.rest ? kSumOnly : kCounted,
                        lds);
   if (got > -2 && tid == 0) ids[d.run] = got < 0 ? d.banned : got;   // (the draft is all there is)
 }
@@ -572,9 +622,9 @@ __global__ __launch_bounds__(kDT) void verify_rest_kernel(Verify a) {
   fill_table(lds.table);
   const T* row = reinterpret_cast<const T*>(a.logits) + d.row * a.row_stride;
   const Q* q = reinterpret_cast<const Q*>(a.probs) + (int64_t)(d.row - seq) * a.probs_stride;
-  const double* const all = a.sums + (int64_t)seq * a.parts;
-  const double own = (tid & 63) < a.parts ? all[tid & 63] : 0.0;   // (every wave the same)
-  int got = draw(a, seq, s, d, row, q, 1.0 / wave_sum64(own), 1, a.rest + (int64_t)seq * a.parts,
+  const double* const all = a.sums + (int64_t)seq * a.units;
+  const double own = (tid & 63) < a.units ? all[tid & 63] : 0.0;   // (every wave the same)
+  int got = draw(a, seq, s, d, row, q, 1.0 / wave_sum64(own), 1, a.rest + (int64_t)seq * a.units,
                  kCounted, lds);
   if (got == -2) return;
   if (got == -1)                     // q covers p: from p, by the sums of before
@@ -590,22 +640,30 @@ static int32_t row_splits(int64_t n_rows, int64_t vocab, int eb) {
   const int64_t most = std::max<int64_t>(chunks / kVT, 1);
   return (int32_t)std::max<int64_t>(std::min<int64_t>({want, most, kMaxSplits}), 1);
 }
+// A drawn row's units, at most a lane each: a cell a thread of a workgroup, or as many
+// as that takes.
+static int32_t unit_cells(int64_t vocab) {
+  return (int32_t)((vocab + (int64_t)kMaxSplits * kPart - 1) / ((int64_t)kMaxSplits * kPart));
+}
+static int32_t row_units(int64_t vocab) {
+  const int64_t unit = (int64_t)unit_cells(vocab) * kPart;
+  return (int32_t)((vocab + unit - 1) / unit);
+}
 // Parts of a drawn row: about 512 workgroups (two a compute unit; each repeats the
-// decision, which takes as long as two cells), a cell a thread at least.
+// decision, which takes as long as two cells), a unit each at least.
 static int32_t seq_parts(int64_t n_seqs, int64_t vocab) {
-  const int64_t want = (512 + n_seqs - 1) / n_seqs, most = (vocab + 4095) / 4096;
-  return (int32_t)std::min<int64_t>({want, most, kMaxSplits});
+  return (int32_t)std::min<int64_t>((512 + n_seqs - 1) / n_seqs, row_units(vocab));
 }
 
 struct VerifySpace { int64_t stats, decisions, sums, rest, counters, bytes; };
 static VerifySpace verify_space(int64_t rows, int64_t seqs, int64_t vocab, int eb) {
   VerifySpace s;
-  const int64_t parts = seq_parts(seqs, vocab);
+  const int64_t units = row_units(vocab);
   s.stats = 0;
   s.decisions = rows * row_splits(rows, vocab, eb) * (int64_t)sizeof(RowStats);
   s.sums = s.decisions + seqs * (int64_t)sizeof(Decision);
-  s.rest = s.sums + seqs * parts * 8;
-  s.counters = s.rest + seqs * parts * 8;
+  s.rest = s.sums + seqs * units * 8;
+  s.counters = s.rest + seqs * units * 8;
   s.bytes = s.counters + seqs * 2 * 4;
   return s;
 }
@@ -674,6 +732,8 @@ int pkv_verify_drafts(const void* logits, int64_t n_rows, int64_t vocab, int64_t
   a.vocab = (int32_t)vocab;
   a.splits = row_splits(n_rows, vocab, eb);
   a.parts = seq_parts(n_seqs, vocab);
+  a.units = row_units(vocab);
+  a.cells = unit_cells(vocab);
   a.temp = temperature;
   // terms: an exponent down to -60 (smaller ones add nothing) rounds three times by
   // 2^-24 of itself, the exponential by 2^-22; sums: one rounding a term

@@ -15,16 +15,16 @@
 //    max) c), c = log2 e / temperature, in 32 bits.
 //  * verify_draw_kernel: each workgroup of a sequence repeats its tests on those
 //    statistics (a few loads; no launch of its own). A test closer than the sum's
-//    error takes the row's sum in 64 bits. The workgroups then sum their part of
+//    error takes the row's sum in 64 bits. The workgroups then sum their units of
 //    the one row that a token is drawn from in 64 bits: an exponential is a table
 //    of 256 entries in LDS and a polynomial of degree 4, some 20 instructions, on
 //    n rows instead of all. The last one to arrive finds the token, except where
 //    the row's whole sum is needed first:
 //  * verify_rest_kernel, with draft probabilities: the same over max(p - q, 0).
 //    In 32 bits the sum's error would move the border of every token behind it.
-// 64 sequences of 2 to 6 rows of 128256 bf16 logits, fp32 draft probabilities: 18.9 (64
-// MB, 3.4 TB/s) + 24.0 + 29.7 us; 24 of 9 rows in fp32 21.8 (5.1 TB/s) + 15.5 + 18.6; one
-// sequence of 5 rows 4.8 + 5.9 + 11.4, a chain of waits.
+// 64 sequences of 2 to 6 rows of 128256 bf16 logits, fp32 draft probabilities: 19.3 (64
+// MB, 3.3 TB/s) + 18.2 + 18.5 us; 24 of 9 rows in fp32 21.6 (5.1 TB/s) + 14.1 + 14.5; one
+// sequence of 5 rows 4.7 + 5.7 + 9.1, a chain of waits.
 #include <algorithm>
 
 #include "mfma.h"

@@ -144,18 +144,17 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, meta: BatchMeta,
         raise ValueError(f"temperature must be finite and not negative, got {temperature}")
     arrays = meta.host_arrays()
     if arrays is not None:
-        lens = arrays["query_lens"]
+        lens = arrays["query_lens"].tolist()     # (a list: numpy's reductions cost 1 us each)
     elif _capturing():
         raise RuntimeError("verify_drafts reads a meta without host arrays from the device: not "
                            "while a graph is captured")
     else:
-        lens = meta.query_lens.cpu().numpy()
-    if lens.min() < 1 or lens.sum() != rows:
-        raise ValueError(f"query_lens ({int(lens.min())} at least, {int(lens.sum())} in all) do "
+        lens = meta.query_lens.tolist()
+    if min(lens) < 1 or sum(lens) != rows:
+        raise ValueError(f"query_lens ({min(lens)} at least, {sum(lens)} in all) do "
                          f"not make up {rows} rows")
-    width = int(lens.max())
-    logits = rows_for_kernel(logits)
-    tokens, uniforms = tokens.contiguous(), uniforms.contiguous()
+    width = max(lens)
+    logits, tokens, uniforms = rows_for_kernel(logits), tokens.contiguous(), uniforms.contiguous()
     cu, owner = meta.cu_query_lens, meta.batch_indices
     if not (cu.dtype is owner.dtype is torch.int32 and cu.device == owner.device == dev
             and cu.is_contiguous() and owner.is_contiguous()):
@@ -175,7 +174,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, meta: BatchMeta,
             0 if draft_probs is None else _DTYPES[draft_probs.dtype],
             None if temps is None else temps.data_ptr(), float(temperature), ids.data_ptr(),
             width, accepted.data_ptr(), ws.data_ptr(), ws.numel(), _current_stream(dev))
-    _native.check(rc, "verify_drafts")
+    if rc:
+        _native.check(rc, "verify_drafts")
     return ids, accepted
 
 

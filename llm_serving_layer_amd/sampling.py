@@ -22,6 +22,8 @@ device tensor (docs/ADR.md:954-989, ADR-023). Here:
 
 from __future__ import annotations
 
+from itertools import accumulate
+
 import torch
 
 from . import _native
@@ -150,6 +152,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, meta: BatchMeta,
                            "while a graph is captured")
     else:
         lens = meta.query_lens.tolist()
+        if meta.cu_query_lens.tolist() != [0, *accumulate(lens)]:
+            raise ValueError("cu_query_lens are not the sums of query_lens")
     if min(lens) < 1 or sum(lens) != rows:
         raise ValueError(f"query_lens ({min(lens)} at least, {sum(lens)} in all) do "
                          f"not make up {rows} rows")

@@ -327,6 +327,24 @@ def test_groups_without_a_step(d, new, units):
         assert s.num_tokens == n
 
 
+@pytest.mark.parametrize("d,hq,counts,units", [(64, 8, [1, 3], None), (64, 16, [1, 1], None),
+                                               (128, 2, [4, 16], None), (64, 8, [9, 14], None),
+                                               (64, 8, [60, 40], 1), (128, 8, [60, 40], 1),
+                                               (80, 4, [2, 5], None)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_a_query_that_is_not_finite_is_alone(d, hq, counts, units, bad):
+    print(f"query {d} {hq} {counts} {bad}", flush=True)
+    c = Cache([150, 90], F16, 2, hq, d, compute_units=units)
+    meta = c.append(counts)
+    q = c.q(counts)
+    spoilt = q.clone()
+    spoilt[1, 1, 3] = bad
+    out = c.bk.attend(spoilt.to(DEV), 0, d ** -0.5, meta)
+    assert out[1, 1].isnan().all()
+    out[1, 1] = c.bk.attend(q.to(DEV), 0, d ** -0.5, meta)[1, 1]
+    c.check(out, q, counts, d ** -0.5)
+
+
 def test_blocks_past_32_bits():
     """Block ids whose bytes lie beyond 2^32."""
     n_kv, d, blocks = 8, 128, 2**32 // 36864 + 40

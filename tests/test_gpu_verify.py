@@ -233,6 +233,15 @@ def test_without_host_arrays_and_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(out + two, eager + other))
 
 
+def test_lengths_that_do_not_sum_up_are_refused():
+    lens = [4, 1, 3]
+    logits, tokens, numbers, _ = (x.to(DEV) for x in inputs(lens, 301, F16, seed=13))
+    bare = meta_to_device(meta_of(lens, "cpu"), DEV, mirror=False)
+    bare.cu_query_lens[2] = 7
+    with pytest.raises(ValueError, match="sums"):
+        verify_drafts(logits, tokens, bare, numbers)
+
+
 def test_calls_on_two_streams_at_once():
     lens = [3] * 50
     a = [x.to(DEV) for x in inputs(lens, 20011, F16, seed=30)]

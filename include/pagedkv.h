@@ -558,7 +558,7 @@ int pkv_read_4bit(const void* k_pool, const void* v_pool, int64_t num_blocks,
  * of 128, and the plan
  * fields of *plan; long rows are cut to fill compute_units compute units. Geometries without a matrix-core kernel (head_dim
  * other than 64 and 128, f32, pages that are no power of two times 16, more than
- * 32 query heads a KV head) need no items.
+ * 32 query heads a KV head, 256 KV heads) need no items.
  *
  * `workspace` (256-byte aligned, workspace_bytes long): arrival counters, zero
  * before the first launch and left so by each (pkv_counter_bytes_4bit from the

@@ -184,12 +184,8 @@ void attend_4bit_kernel(Attend4 a) {
   int t = tile0 + wave;
   int id = 0, id_next = 0;           // of tiles t, t + WPP
   if (t < end) {
-    if constexpr (WPP <= 4) {        // (its pages came with the piece)
-      const int32_t* first = it + 12 + 4 * wave;
-      id = g == 0 ? first[0] : g == 1 ? first[1] : g == 2 ? first[2] : first[3];
-    } else {
-      id = load_id(t);
-    }
+    const int32_t* first = it + 12 + 4 * wave;         // (its pages came with the piece)
+    id = g == 0 ? first[0] : g == 1 ? first[1] : g == 2 ? first[2] : first[3];
     load_k(t, id);
     load_v();
     id_next = load_id(t + WPP);
@@ -670,10 +666,12 @@ void attend_4bit_kernel(Attend4 a) {
 
 // ------------------------------------------------------------------- plan ---
 
+// (KV heads: 128 pieces' parts of 32 rows lie within 2^31 bytes of each other)
 static bool fast_4bit(int32_t n_heads, int32_t n_kv, int32_t d, int32_t ps, int32_t dtype) {
   const int32_t units = ps / 16;
   return (dtype == PKV_DTYPE_F16 || dtype == PKV_DTYPE_BF16) && (d == 64 || d == 128) &&
-         ps % 16 == 0 && units > 0 && (units & (units - 1)) == 0 && n_heads / n_kv <= 32;
+         ps % 16 == 0 && units > 0 && (units & (units - 1)) == 0 && n_heads / n_kv <= 32 &&
+         n_kv <= 256;
 }
 
 // Arrival counters lie 128 bytes apart where they are few and their pieces may be
@@ -871,7 +869,7 @@ int pkv_attend_4bit(const void* batch, const void* q, void* out, const void* k_p
   const int rc = check_4bit(b.n_kv_heads, b.head_dim, b.page_size);
   if (rc) return rc;
   if (b.n_heads <= 0 || b.n_heads % b.n_kv_heads || b.n_seqs <= 0 || b.n_tokens <= 0 ||
-      b.num_blocks < 0 || !elem_bytes(b.dtype))
+      b.num_blocks <= 0 || !elem_bytes(b.dtype))
     return fail(PKV_ERR_INVALID, "the batch's geometry is invalid");
   if (!q || !out || !k_pool || !v_pool || !b.cu_query_lens || !b.kv_indptr || !b.kv_indices ||
       !b.kv_lens)

@@ -22,7 +22,7 @@ The same calls in the same order as ``MI355XBackend`` (``append_kv`` then
 word; ``copy_block(s)`` and ``KVSwapSpace`` move its blocks. ``k_pool`` /
 ``v_pool`` are the blocks' bytes; ``read_kv`` gives the values that slots hold.
 Matrix-core kernels for head_dim 64 and 128, float16 and bfloat16, pages of 16
-rows times a power of two and up to 32 query heads a KV head; other geometries
+rows times a power of two, up to 32 query heads a KV head and 256 KV heads; others
 (any even head_dim up to 256, float32, any page size) run generic ones.
 """
 

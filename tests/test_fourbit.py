@@ -134,7 +134,7 @@ def test_the_plan_covers_every_row_and_tile_once(compute_units, n_heads, n_kv):
 
 
 @pytest.mark.parametrize("kw", [{"d": 80}, {"dtype": _native.DTYPE_F32}, {"ps": 8}, {"ps": 48},
-                                {"n_heads": 33, "n_kv": 1}])
+                                {"n_heads": 33, "n_kv": 1}, {"n_heads": 257, "n_kv": 257}])
 def test_geometries_without_a_plan(kw):
     args, items = plan([100, 3], [1, 2], **kw)
     assert not items and args.n_few == args.n_wide == args.workspace_bytes == 0
@@ -169,7 +169,7 @@ def test_the_entry_refuses_before_it_launches(change, match):
 
 @pytest.mark.parametrize("change,match", [
     ({"items": None}, "no plan"), ({"n_few": -1, "n_wide": 2}, "no plan"),
-    ({"n_slots": 2, "workspace_bytes": 8}, "workspace"), ({"n_tokens": 0}, "geometry"),
+    ({"n_slots": 2, "workspace_bytes": 8}, "workspace"), ({"n_tokens": 0}, "geometry"), ({"num_blocks": 0}, "geometry"),
     ({"kv_lens": None}, "null"), ({"head_dim": 80, "batch_indices": None}, "null")])
 def test_attend_refuses_before_it_launches(change, match):
     b = _native.FourBit(num_blocks=4, n_seqs=1, n_tokens=1, n_heads=8, n_kv_heads=2, head_dim=64,

@@ -22,9 +22,9 @@
 //    the row's whole sum is needed first:
 //  * verify_rest_kernel, with draft probabilities: the same over max(p - q, 0).
 //    In 32 bits the sum's error would move the border of every token behind it.
-// 64 sequences of 2 to 6 rows of 128256 bf16 logits, fp32 draft probabilities: 19.3 (64
-// MB, 3.3 TB/s) + 18.2 + 18.5 us; 24 of 9 rows in fp32 21.6 (5.1 TB/s) + 14.1 + 14.5; one
-// sequence of 5 rows 4.7 + 5.7 + 9.1, a chain of waits.
+// 64 sequences of 2 to 6 rows of 128256 bf16 logits, fp32 draft probabilities: 17.4 (64
+// MB, 3.7 TB/s) + 18.2 + 18.0 us; 24 of 9 rows in fp32 21.5 (5.1 TB/s) + 14.1 + 14.4; one
+// sequence of 5 rows 4.5 + 5.7 + 9.0, a chain of waits.
 #include <algorithm>
 
 #include "mfma.h"
@@ -33,7 +33,8 @@ namespace pkv {
 
 constexpr int kVT = 256;            // threads of a workgroup
 constexpr int kMaxSplits = 64;      // of a row: a lane each
-constexpr int kChunks = 4;          // of 16 bytes a thread and round, in the first kernel
+constexpr int kChunks = 8;          // of 16 bytes a thread and round, in the first kernel
+                                    // (249 rows of 128256 in bf16: 17.4 us; 4 take 18.7)
 
 struct RowStats { float m, z; int32_t arg, pad; };
 
@@ -173,9 +174,13 @@ __global__ __launch_bounds__(kVT) void verify_stats_kernel(Verify a) {
     if (sm[w] == bm) ba = min(ba, sa[w]);
   }
   if (ba < end) {
-    const int stop = min(ba + E, end);
-    for (int i = ba; i < stop; ++i)
-      if (Elem<T>::to_f(row[i]) == bm) { ba = i; break; }
+    if (ba >= body && ba < tail) {   // (a chunk's start, read again in one load)
+      const TV w = *reinterpret_cast<const TV*>(row + ba);
+      int place = 0;
+#pragma unroll
+      for (int e = E - 1; e > 0; --e) place = Elem<T>::to_f(w[e]) == bm ? e : place;
+      ba += Elem<T>::to_f(w[0]) == bm ? 0 : place;
+    }
   } else {
     ba = begin;                      // (nothing but NaN, or an empty part)
   }

@@ -34,7 +34,9 @@
 //
 // The running reference of the softmax moves lazily: only when a lane's sum of a
 // tile's probabilities passes 2^12, or when a step of V outgrows the power of two
-// 2^e that keeps p step within float16 (p 2^e against the reference).
+// 2^e that keeps p step within float16 (p 2^e against the reference). e is a row's
+// own and follows the steps of the keys that it sees, those of NaN groups left out:
+// what a later token holds leaves an earlier one's weights their bits.
 //
 // 16 sequences of 20000 to 60000 tokens, head_dim 128 (643 MB), take 113 us: HBM, 5.7
 // TB/s. 256 of 1 to 2048, head_dim 64 (40 MB), 13.5: starting, one tile's latency and
@@ -81,6 +83,21 @@ constexpr int64_t kTallAlong = 5;
 // Floats per wave for a tile's steps, zeros of K, steps and middles of V
 // ([4][group][key]).
 template <int D> constexpr int kPairFloats = 4 * (D / 64) * kTile;
+
+// Words from here on are a NaN group's.
+constexpr uint32_t kNoStep = 0x7c000000u;
+
+// The largest of the lanes up to this one's.
+__device__ __forceinline__ uint32_t scan_max(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false));  // row_shr
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false));
+  // row_bcast:15 into rows 1 and 3, row_bcast:31 into 2 and 3
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));
+  return v;
+}
 
 // Waves a SIMD the kernel is compiled for.
 template <int D, int RT> constexpr int kSimdWaves = RT == 2 ? 2 : D == 64 ? 4 : 2;
@@ -266,9 +283,17 @@ void attend_4bit_kernel(Attend4 a) {
     ref[rt] = -INFINITY;
     l[rt] = 0.f;
   }
-  uint32_t cap = 0;                  // the largest step (a word's) that 2^e allows
-  int e = 0;
-  float limit = 4096.f;              // 2^12 2^e
+  // of each row: the largest step (a word's) that 2^e allows, e, 2^12 2^e. (The same
+  // in all rows, and in scalar registers, until a tile is seen in part.)
+  uint32_t cap[RT];
+  int e[RT];
+  float limit[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    cap[rt] = 0;
+    e[rt] = 0;
+    limit[rt] = 4096.f;
+  }
   uint32_t worst = 0;                // any page id out of range
   float* const pw = pair_lds + wave * kPairFloats<D>;
   const uint32_t LO = 0x000f000fu, UP = 0x00f000f0u;
@@ -281,11 +306,11 @@ void attend_4bit_kernel(Attend4 a) {
     const bool bad = (uint64_t)(int64_t)id >= (uint64_t)a.num_blocks;
     const bool live = (!PART || kTile * t + lane < kv_len) && !bad;
     worst |= bad;
-    uint32_t top = 0;
+    uint32_t top = 0;                // the key's largest step, then that of keys up to it
 #pragma unroll
     for (int q = 0; q < NG; ++q) {
       const uint32_t kp = live ? kw[q] : 0u, vp = live ? vw[q] : 0u;
-      top = max(top, vp);
+      top = max(top, vp < kNoStep ? vp : 0u);
       const float step = pair_step(vp);
       pw[q * kTile + lane] = pair_step(kp);
       pw[(NG + q) * kTile + lane] = pair_zero(kp);
@@ -293,6 +318,16 @@ void attend_4bit_kernel(Attend4 a) {
       pw[(3 * NG + q) * kTile + lane] = __builtin_fmaf(7.5f, step, pair_zero(vp));
     }
     wave_lds_sync();
+    uint32_t seen[RT];               // the largest step among a row's keys of the tile
+    if constexpr (PART) {
+      top = scan_max(top);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const int last = qpos[rt] - kTile * t;
+        const uint32_t w = (uint32_t)__shfl((int)top, min(max(last, 0), kTile - 1), 64);
+        seen[rt] = last < 0 ? 0u : w;
+      }
+    }
 
     auto pairs = [&](int kind, int q, int u) {   // of the lane's four keys of unit u
       return *reinterpret_cast<const f32x4*>(pw + (kind * NG + q) * kTile + (cls + u) * 16 + 4 * g);
@@ -364,37 +399,39 @@ void attend_4bit_kernel(Attend4 a) {
           ls[rt] += p[i][rt][j];
         }
     };
-    bool past = ps == 0 && top > cap;
+    bool past = false, more_step = false;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
+      if (ps == 0) more_step = more_step || (PART ? seen[rt] : top) > cap[rt];
       probs(rt, ref[rt]);
-      past = past || !(ls[rt] <= limit);
+      past = past || !(ls[rt] <= limit[rt]);
     }
-    if (__builtin_amdgcn_ballot_w64(past)) {
+    if (__builtin_amdgcn_ballot_w64(past || more_step)) {
       // 2^e for the largest step yet: its product below 1, up to 8 allowed
-      if (ps == 0 && __builtin_amdgcn_ballot_w64(top > cap)) {
-        uint32_t w = top;
+      if (ps == 0 && __builtin_amdgcn_ballot_w64(more_step)) {
+        if constexpr (!PART) {
+          const uint32_t w = (uint32_t)__builtin_amdgcn_readlane((int)scan_max(top), 63);
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) w = max(w, (uint32_t)__shfl_xor((int)w, off, 64));
-        const int ex = min((int)(w >> 26 & 31u), 30);
-        if (cap == 0 || 14 - ex < e) {
-          const int old = cap ? e : 14 - ex;
-          e = 14 - ex;
-          const float f = __builtin_amdgcn_ldexpf(1.f, e - old);
+          for (int rt = 0; rt < RT; ++rt) seen[rt] = w;
+        }
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            ref[rt] += (float)(old - e);
-            l[rt] *= f;
+        for (int rt = 0; rt < RT; ++rt) {
+          const int ex = (int)(seen[rt] >> 26);
+          const bool moves = seen[rt] > cap[rt];
+          const int old = cap[rt] ? e[rt] : 14 - ex, now = moves ? 14 - ex : e[rt];
+          const float f = moves ? __builtin_amdgcn_ldexpf(1.f, now - old) : 1.f;
+          ref[rt] += moves ? (float)(old - now) : 0.f;
+          l[rt] *= f;
 #pragma unroll
-            for (int q = 0; q < NG; ++q) {
-              zo[rt][q] *= f;
-              pr[rt][q] *= f;
-            }
-#pragma unroll
-            for (int i = 0; i < NT; ++i) o[rt][i] *= f;
+          for (int q = 0; q < NG; ++q) {
+            zo[rt][q] *= f;
+            pr[rt][q] *= f;
           }
-          cap = (uint32_t)min(ex + 3, 30) << 26 | 0x03ffffffu;
-          limit = __builtin_amdgcn_ldexpf(4096.f, e);
+#pragma unroll
+          for (int i = 0; i < NT; ++i) o[rt][i] *= f;
+          e[rt] = now;
+          if (moves) cap[rt] = (uint32_t)min(ex + 3, 30) << 26 | 0x03ffffffu;
+          limit[rt] = __builtin_amdgcn_ldexpf(4096.f, now);
         }
       }
 #pragma unroll
@@ -404,7 +441,7 @@ void attend_4bit_kernel(Attend4 a) {
         for (int i = 0; i < UPL; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j) mx = fmaxf(mx, y[i][rt][j]);
-        mx = max_x32(max_x16(mx)) * f1[rt] - (float)e;
+        mx = max_x32(max_x16(mx)) * f1[rt] - (float)e[rt];
         const float r = fmaxf(ref[rt], mx);
         const float alpha = r == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref[rt] - r);
         ref[rt] = r;

@@ -1,0 +1,67 @@
+"""
+Attention over the 4-bit cache where keys differ in scale, or hold what is not
+finite: a token's output depends on the keys that it sees alone.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from ._fourbit import attend64
+from ._ops64 import assert_within
+from ._util import make_meta
+from .test_gpu_fourbit import DEV, F16, Cache, rows
+
+pytestmark = pytest.mark.gpu
+
+
+def fill(c, k, v):
+    """The rows of sequence 0, all at once."""
+    n = k.shape[0]
+    if not c.seqs[0].num_tokens:
+        c.seqs[0].append(n)
+    c.k, c.v = [k], [v]
+    c.bk.append_kv(0, k.to(DEV), v.to(DEV), make_meta(c.seqs, [n], c.ps, device=DEV))
+
+
+def attend_last(c, new, scale, q=None):
+    """(queries, outputs) of the last ``new`` tokens."""
+    q = c.q([new]) if q is None else q
+    out = c.bk.attend(q.to(DEV), 0, scale, make_meta(c.seqs, [new], c.ps, device=DEV))
+    return q, out.cpu()
+
+
+# (query heads of 2 KV heads, new tokens, compute units): rows in four, two and one
+# classes, wide rows twice
+FORMS = [(4, 2, None), (8, 2, None), (8, 4, None), (8, 6, None), (16, 8, None)]
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,new,units", FORMS)
+@pytest.mark.parametrize("history", [0, 100, 300])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, 60000.0])
+@pytest.mark.parametrize("spread", [0.5, 0.02])
+def test_a_later_value_leaves_earlier_tokens_as_they_are(d, hq, new, units, history, bad, spread):
+    """The last token's V is not finite, or a thousand times the others: the tokens
+    before it stay within the bound of a call without it."""
+    print(f"later {d} {hq} {new} {history} {bad} {spread}", flush=True)
+    n = history + new
+    c = Cache([0], F16, 2, hq, d, room=400, compute_units=units)
+    k, v = rows((n, 2, d), F16, 1), rows((n, 2, d), F16, 2).mul(spread)
+    v[-1, :, 3] = bad                # (of the first group)
+    fill(c, k, v)
+    q, out = attend_last(c, new, d ** -0.5)
+    want, bound = attend64(q[:-1], k[:-1], v[:-1], d ** -0.5, F16)
+    assert_within(out[:-1], want, bound, "earlier tokens")
+    if math.isfinite(bad):
+        want, bound = attend64(q[-1:], k, v, d ** -0.5, F16)
+        assert_within(out[-1:], want, bound, "the token itself")
+        return
+    assert out[-1, :, :64].isnan().all()
+    if d == 128:                     # the other group is finite
+        v[-1, :, :64] = 0
+        want, bound = attend64(q[-1:], k, v, d ** -0.5, F16)
+        assert_within(out[-1:, :, 64:], want[..., 64:], bound[..., 64:], "the other group")

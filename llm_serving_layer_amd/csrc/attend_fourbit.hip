@@ -84,21 +84,6 @@ constexpr int64_t kTallAlong = 5;
 // ([4][group][key]).
 template <int D> constexpr int kPairFloats = 4 * (D / 64) * kTile;
 
-// Words from here on are a NaN group's.
-constexpr uint32_t kNoStep = 0x7c000000u;
-
-// The largest of the lanes up to this one's.
-__device__ __forceinline__ uint32_t scan_max(uint32_t v) {
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false));  // row_shr
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false));
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false));
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false));
-  // row_bcast:15 into rows 1 and 3, row_bcast:31 into 2 and 3
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));
-  return v;
-}
-
 // Waves a SIMD the kernel is compiled for.
 template <int D, int RT> constexpr int kSimdWaves = RT == 2 ? 2 : D == 64 ? 4 : 2;
 

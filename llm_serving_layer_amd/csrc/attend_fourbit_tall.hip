@@ -11,8 +11,8 @@
 //    sum_g step_g (q . c)_g + zero_g sum q, exact but for 32-bit sums; the softmax of a
 //    row in its two lanes, its reference moved only when a score passes it by 2^12;
 //  * P is p step, rounded to float16 once (2^-11 of it), against c - 7.5, and in 32
-//    bits p zero + 7.5 p step. With 2^E at least the largest step so far (the same for
-//    all rows), p counts 2^-E more, so that p step stays within float16.
+//    bits p zero + 7.5 p step. With 2^E at least the largest step that the row has seen,
+//    p counts 2^-E more, so that p step stays within float16.
 // 8 x 512 tokens over 1536, head_dim 64, 8 KV heads of 4: 122 us, 490 TFLOP/s (as wide
 // pieces 155). With keys and values rounded to float16 in LDS and p beside them it took
 // 95, but three roundings of 2^-11 added 1.4 times the output's own error; this one adds
@@ -40,6 +40,7 @@ __global__ __launch_bounds__(256, (D == 64 ? 3 : 2)) void attend_4bit_tall_kerne
   __shared__ __align__(16) unsigned char smem[2 * BUF];
   __shared__ __align__(16) uint32_t words[2][2][NG][kTile];   // a tile's, of K and of V
   __shared__ __align__(16) uint32_t tops[2][4];          // its units' largest words of V
+  __shared__ float row_top[256];     // a lane's row's E, from the first tile seen in part
   __shared__ __align__(8) uint16_t nan_keys[2][NG][4];   // a tile's keys whose V is NaN
 
   // (as in the pieces' kernel: a tile's heads on one XCD)
@@ -112,13 +113,13 @@ __global__ __launch_bounds__(256, (D == 64 ? 3 : 2)) void attend_4bit_tall_kerne
     for (int q = 0; q < NG; ++q)
       top = max(top, max(max(vw[q][0], vw[q][1]), max(vw[q][2], vw[q][3])));
     uint32_t none[NG] = {};
-    if (__builtin_amdgcn_ballot_w64(top >= 0x7c000000u)) {
+    if (__builtin_amdgcn_ballot_w64(top >= kNoStep)) {
       top = 0;
 #pragma unroll
       for (int q = 0; q < NG; ++q)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const bool nan = vw[q][j] >= 0x7c000000u;
+          const bool nan = vw[q][j] >= kNoStep;
           // (bit 4 kg + j of the unit's keys, from the lanes kn = 0)
           const uint64_t b = __builtin_amdgcn_ballot_w64(nan);
           none[q] |= (uint32_t)((b & 1) << j | (b >> 16 & 1) << (4 + j) | (b >> 32 & 1) << (8 + j) |
@@ -201,7 +202,7 @@ __global__ __launch_bounds__(256, (D == 64 ? 3 : 2)) void attend_4bit_tall_kerne
   for (int b = 0; b < NB; ++b) o[b] = f32x16{};
   float ref = -INFINITY, l = 0.f, none[NG] = {};
   float zeros[NG] = {}, steps[NG] = {};   // sums of p zero, p step
-  int top = -30;                     // E
+  int whole_top = -30;               // E, all rows' until a tile is seen in part
 
   stage(0);
   int next = page(1);                // (read a tile ahead of its use)
@@ -212,17 +213,19 @@ __global__ __launch_bounds__(256, (D == 64 ? 3 : 2)) void attend_4bit_tall_kerne
     const unsigned char* buf = smem + (t & 1) * BUF;
     const auto& wk = words[t & 1][0];
     const auto& wv = words[t & 1][1];
-    // a larger step than any before: the sums in its unit
+    // a larger step than any that the rows have seen: the sums in its unit
+    const bool in_part = kTile * t + kTile - 1 > base_pos;     // (by some row)
     const u32x4 tile_tops = *reinterpret_cast<const u32x4*>(tops[t & 1]);
     const uint32_t word = __builtin_amdgcn_readfirstlane(
         max(max(tile_tops[0], tile_tops[1]), max(tile_tops[2], tile_tops[3])));
-    const int now = word >= 0x10000u ? __builtin_amdgcn_frexp_expf(step_of(word)) : top;
+    const int now =
+        word >= 0x10000u && !in_part ? __builtin_amdgcn_frexp_expf(step_of(word)) : whole_top;
     float by = 1.f;                  // what the sums so far count now
-    bool less = now > top;
+    bool less = now > whole_top;
     if (less) {
-      by = __builtin_amdgcn_ldexpf(1.f, top - now);
-      ref += (float)(now - top);
-      top = now;
+      by = __builtin_amdgcn_ldexpf(1.f, whole_top - now);
+      ref += (float)(now - whole_top);
+      whole_top = now;
     }
 #pragma unroll
     for (int h0 = 0; h0 < 2; h0 += NH) {
@@ -251,13 +254,32 @@ __global__ __launch_bounds__(256, (D == 64 ? 3 : 2)) void attend_4bit_tall_kerne
             }
           }
       }
-      const int key = kTile * t + 32 * h0;
-      if (key + 32 * NH - 1 > base_pos) {
+      float top = (float)whole_top;
+      if (in_part) {
+        const int key = kTile * t + 32 * h0;
 #pragma unroll
         for (int hf = 0; hf < NH; ++hf)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             if (key + 32 * hf + 8 * (e >> 2) + 4 * g + (e & 3) > qpos) s[hf][e] = -INFINITY;
+        // (the row's E, from its own keys in such tiles)
+        if (h0 || (t > 0 && kTile * t - 1 > base_pos)) top = row_top[threadIdx.x];
+        if (h0 == 0) {
+          uint32_t seen = 0;
+#pragma unroll
+          for (int q = 0; q < NG; ++q) seen = max(seen, wv[q][lane]);
+          const int last = qpos - kTile * t;
+          seen = (uint32_t)__shfl((int)scan_max(seen), min(max(last, 0), kTile - 1), 64);
+          const float more =
+              last < 0 || seen < 0x10000u
+                  ? 0.f
+                  : fmaxf((float)__builtin_amdgcn_frexp_expf(step_of(seen)) - top, 0.f);
+          by = __builtin_amdgcn_exp2f(-more);
+          ref += more;
+          top += more;
+          row_top[threadIdx.x] = top;
+          less = true;
+        }
       }
       // (looking at the largest score first keeps the scores' registers for the weights)
       float mx = -INFINITY;
@@ -265,7 +287,7 @@ __global__ __launch_bounds__(256, (D == 64 ? 3 : 2)) void attend_4bit_tall_kerne
       for (int hf = 0; hf < NH; ++hf)
 #pragma unroll
         for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[hf][e]);
-      mx = __builtin_fmaf(mx, f1, (float)top);
+      mx = __builtin_fmaf(mx, f1, top);
       if (__builtin_amdgcn_ballot_w64(!(mx - ref <= 12.f))) {
         const float m = fmaxf(ref, max_x32(mx));
         by *= m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref - m);

@@ -35,8 +35,8 @@ def attend_last(c, new, scale, q=None):
 
 
 # (query heads of 2 KV heads, new tokens, compute units): rows in four, two and one
-# classes, wide rows twice
-FORMS = [(4, 2, None), (8, 2, None), (8, 4, None), (8, 6, None), (16, 8, None)]
+# classes, wide rows twice, tall ones
+FORMS = [(4, 2, None), (8, 2, None), (8, 4, None), (8, 6, None), (16, 8, None), (8, 40, 1)]
 
 
 @pytest.mark.parametrize("d", [64, 128])

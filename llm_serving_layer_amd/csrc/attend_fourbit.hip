@@ -403,9 +403,9 @@ void attend_4bit_kernel(Attend4 a) {
         for (int rt = 0; rt < RT; ++rt) {
           const int ex = (int)(seen[rt] >> 26);
           const bool moves = seen[rt] > cap[rt];
-          const int old = cap[rt] ? e[rt] : 14 - ex, now = moves ? 14 - ex : e[rt];
-          const float f = moves ? __builtin_amdgcn_ldexpf(1.f, now - old) : 1.f;
-          ref[rt] += moves ? (float)(old - now) : 0.f;
+          const int now = moves ? 14 - ex : e[rt];
+          const float f = __builtin_amdgcn_ldexpf(1.f, now - e[rt]);
+          ref[rt] += (float)(e[rt] - now);
           l[rt] *= f;
 #pragma unroll
           for (int q = 0; q < NG; ++q) {

@@ -13,7 +13,7 @@ import torch
 from ._fourbit import attend64
 from ._ops64 import assert_within
 from ._util import make_meta
-from .test_gpu_fourbit import DEV, F16, Cache, rows
+from .test_gpu_fourbit import BF16, DEV, F16, Cache, rows
 
 pytestmark = pytest.mark.gpu
 
@@ -65,3 +65,20 @@ def test_a_later_value_leaves_earlier_tokens_as_they_are(d, hq, new, units, hist
         v[-1, :, :64] = 0
         want, bound = attend64(q[-1:], k, v, d ** -0.5, F16)
         assert_within(out[-1:, :, 64:], want[..., 64:], bound[..., 64:], "the other group")
+
+
+@pytest.mark.parametrize("hq,new", [f[:2] for f in FORMS])
+def test_small_steps_behind_tiles_without_one(hq, new):
+    """V of the first tiles is nothing; the first steps that come are the least
+    there are. (One piece: its first wave takes tiles 0 and 4.)"""
+    n = 256 + 8
+    c = Cache([0], BF16, 2, hq, 64, room=400, compute_units=1)
+    k = rows((n, 2, 64), BF16, 1)
+    v = torch.zeros((n, 2, 64), dtype=BF16)
+    g = torch.Generator().manual_seed(3)
+    v[256:] = (torch.randint(0, 16, (8, 2, 64), generator=g).float() * 2.0 ** -24).to(BF16)
+    v[256:, :, 0], v[256:, :, 1] = 0.0, 15 * 2.0 ** -24
+    fill(c, k, v)
+    q, out = attend_last(c, new, 0.125)
+    want, bound = attend64(q, k, v, 0.125, BF16)
+    assert_within(out, want, bound)

@@ -346,6 +346,9 @@ void attend_4bit_kernel(Attend4 a) {
     if (ps == PASSES - 1) {
       if constexpr (MORE) load_k(t + WPP, id_next);
     }
+    auto unseen = [&](int rt, int i, int j) {    // key j of the lane's unit i of the pass
+      return kTile * t + (u0 + cls + NCL * i) * 16 + 4 * g + j > qpos[rt];
+    };
     // scores, in the row's unit (times f1: log2)
     float y[UPL][RT][4];
 #pragma unroll
@@ -371,7 +374,7 @@ void attend_4bit_kernel(Attend4 a) {
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (kTile * t + (u0 + cls + NCL * i) * 16 + 4 * g + j > qpos[rt]) y[i][rt][j] = -INFINITY;
+            if (unseen(rt, i, j)) y[i][rt][j] = -INFINITY;
     }
     float p[UPL][RT][4], ls[RT];
     auto probs = [&](int rt, float r) {
@@ -459,8 +462,9 @@ void attend_4bit_kernel(Attend4 a) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float pj = p[i][rt][j];
-            // (a key that the row does not see may hold NaN)
-            const bool none = PART && pj == 0.f;
+            // (a key that the row does not see may hold NaN; one that it sees counts
+            // however small its weight)
+            const bool none = PART && unseen(rt, i, j);
             w[j] = none ? 0.f : pj * step[j];
             z = none ? z : __builtin_fmaf(pj, mid[j], z);
           }

@@ -1,6 +1,7 @@
 """
 Attention over the 4-bit cache where keys differ in scale, or hold what is not
-finite: a token's output depends on the keys that it sees alone.
+finite: a token's output depends on the keys that it sees alone, and is NaN where
+one of them is.
 """
 
 from __future__ import annotations
@@ -82,3 +83,19 @@ def test_small_steps_behind_tiles_without_one(hq, new):
     q, out = attend_last(c, new, 0.125)
     want, bound = attend64(q, k, v, 0.125, BF16)
     assert_within(out, want, bound)
+
+
+@pytest.mark.parametrize("d", [64, 128, 80])
+@pytest.mark.parametrize("n", [20, 300])
+@pytest.mark.parametrize("hq,new,units", FORMS)
+def test_a_seen_nan_of_hardly_any_weight(d, n, hq, new, units):
+    """A weight of e^-300 is not nothing: a token that sees the key gets NaN."""
+    n += new
+    c = Cache([0], F16, 2, hq, d, room=400, compute_units=units)
+    k, v = rows((n, 2, d), F16, 1, centre=0.0), rows((n, 2, d), F16, 2)
+    q = torch.full((new, hq, d), 4.0, dtype=F16)
+    k[3] = -300.0 / (4 * d * 0.125)
+    v[3] = math.nan
+    fill(c, k, v)
+    _, out = attend_last(c, new, 0.125, q)
+    assert out.isnan().all()

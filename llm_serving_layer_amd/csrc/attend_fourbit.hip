@@ -675,9 +675,10 @@ void attend_4bit_kernel(Attend4 a) {
       if (first == 0) {
         for (int k = 1; k < share; ++k) {
           const f32x2 other = red2[tid + k * units];
-          if (other[0] == -INFINITY) continue;
           const float mn = fmaxf(m, other[0]);
-          const float f = __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(other[0] - mn);
+          // (at -inf: no key, and zeros, or NaN scores alone, and NaN)
+          const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+          const float w = other[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(other[0] - mn);
           v = v * f + red[tid + k * units] * w;
           lr = lr * f + other[1] * w;
           m = mn;

@@ -99,3 +99,24 @@ def test_a_seen_nan_of_hardly_any_weight(d, n, hq, new, units):
     fill(c, k, v)
     _, out = attend_last(c, new, 0.125, q)
     assert out.isnan().all()
+
+
+@pytest.mark.parametrize("d,hq", [(64, 4), (64, 8), (128, 4)])
+@pytest.mark.parametrize("units", [2, 4, 8])
+def test_pieces_whose_scores_are_all_nan(d, hq, units):
+    """K of all of one piece of a cut sequence is NaN: it has no finite score, and the
+    output is NaN."""
+    n = 3000
+    c = Cache([0], F16, 2, hq, d, room=3100, compute_units=units)
+    k, v = rows((n, 2, d), F16, 1), rows((n, 2, d), F16, 2)
+    fill(c, k, v)
+    _, out = attend_last(c, 1, d ** -0.5)
+    assert torch.isfinite(out).all()
+    pieces = c.bk._planned.buffers[5].view(-1, 28)[:, 6:8].tolist()
+    assert len(pieces) == units and sum(tiles for _, tiles in pieces) == 47
+    for first, tiles in pieces:
+        spoilt = k.clone()
+        spoilt[64 * first:64 * (first + tiles)] = math.nan
+        fill(c, spoilt, v)
+        _, out = attend_last(c, 1, d ** -0.5)
+        assert out.isnan().all(), (first, tiles)

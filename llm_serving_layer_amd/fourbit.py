@@ -34,7 +34,7 @@ import numpy as np
 import torch
 
 from . import _native
-from .backend import _DTYPES, PagedPool, _current_stream
+from .backend import _DTYPES, PagedPool, _capturing, _current_stream
 from .contract import BatchMeta
 
 __all__ = ["FourBitBackend"]
@@ -130,6 +130,7 @@ class FourBitBackend(PagedPool):
         Quantise this step's K/V into the pool through ``meta.slot_mapping`` (no
         two tokens may share a slot). ``k`` and ``v`` may be slices of one
         projection's output: any stride between tokens, heads one after another.
+        Slots that a captured append reads stay as long as the backend does.
         """
         if layer_idx is None or not 0 <= layer_idx < self.num_layers:
             self._check_layer(layer_idx)
@@ -152,6 +153,8 @@ class FourBitBackend(PagedPool):
             k = k.clone(memory_format=torch.contiguous_format)
         if v.data_ptr() % 16:
             v = v.clone(memory_format=torch.contiguous_format)
+        if _capturing():
+            self._keep(meta.slot_mapping)
         row = self.n_kv_heads * self.head_dim   # (a single row's stride may be anything)
         with self._on_device():
             rc = self._lib.pkv_append_4bit(
@@ -178,6 +181,8 @@ class FourBitBackend(PagedPool):
                 or slots.dtype is torch.bool:
             raise ValueError(f"slots must be a 1-d tensor of whole numbers, got {slots.dtype} of "
                              f"shape {tuple(slots.shape)}")
+        if _capturing():
+            self._keep(slots)
         if slots.dtype is torch.int64:   # (beyond 32 bits: no pool has such a slot)
             slots = slots.clamp(-1, 2**31 - 1)
         slots = self._dev_i32(slots)

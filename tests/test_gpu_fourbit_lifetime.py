@@ -1,0 +1,45 @@
+"""Graphs of the 4-bit cache's calls: what they read stays."""
+
+from __future__ import annotations
+
+import dataclasses
+import gc
+
+import pytest
+import torch
+
+from ._fourbit import held64
+from .test_gpu_fourbit import DEV, F16, Cache, rows, same_bits
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_a_captured_append_keeps_its_slots(dtype):
+    """The meta goes once the graph is captured, and its memory is written over."""
+    c = Cache([30, 7], F16, 2, 8, 64)
+    meta = c.append([3, 2])
+    slots = meta.slot_mapping.tolist()
+    meta = dataclasses.replace(meta, slot_mapping=meta.slot_mapping.to(dtype).clone(), host=None)
+    k, v = rows((5, 2, 64), F16, 50).to(DEV), rows((5, 2, 64), F16, 51).to(DEV)
+    asked = torch.tensor(slots, dtype=dtype, device=DEV)
+    c.bk.append_kv(0, k, v, meta)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.bk.append_kv(0, k, v, meta)
+        held = c.bk.read_kv(0, asked)
+    del meta, asked
+    gc.collect()
+    over = [torch.zeros(n, dtype=t, device=DEV) for t in (torch.int32, torch.int64)
+            for n in (1, 2, 3, 5, 8) for _ in range(40)]
+    torch.cuda.synchronize()
+    for i in range(3):
+        k.copy_(rows((5, 2, 64), F16, 60 + i))
+        v.copy_(rows((5, 2, 64), F16, 70 + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, want in ((held[0], k), (held[1], v), (c.bk.read_kv(0, slots)[0], k)):
+            same_bits(got, held64(want), F16)
+    assert len(over) == 400
+    c.bk.check_device_errors()

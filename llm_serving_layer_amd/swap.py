@@ -202,9 +202,13 @@ class KVSwapSpace:
             raise RuntimeError(f"handle holds {handle._host.dtype} blocks of shape "
                                f"{tuple(handle._host.shape)}, the pool's are {self.dtype} of "
                                f"{self._shape(nb)}")
+        b = self.backend
+        if (handle.n_kv_heads, handle.head_dim) != (b.n_kv_heads, b.head_dim):
+            # (4-bit blocks of other heads may have as many bytes)
+            raise RuntimeError(f"handle holds rows of {handle.n_kv_heads} KV heads of "
+                               f"{handle.head_dim}, the pool's are {b.n_kv_heads} of {b.head_dim}")
         if len(set(blocks.block_ids)) != nb:
             raise RuntimeError("swap_in target block ids must be distinct")
-        b = self.backend
         b._flush()
         main = torch.cuda.current_stream(self.device)
         ids = self._ids(blocks.block_ids)

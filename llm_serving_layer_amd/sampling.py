@@ -78,6 +78,30 @@ def greedy(logits: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def _step_lengths(meta: BatchMeta, rows: int) -> list[int]:
+    """Every sequence's rows of a step, checked against what the kernels read of the
+    meta on the device."""
+    n = meta.n_seqs
+    if meta.cu_query_lens.shape != (n + 1,) or meta.batch_indices.shape != (rows,):
+        raise ValueError(f"cu_query_lens has shape {tuple(meta.cu_query_lens.shape)} and "
+                         f"batch_indices {tuple(meta.batch_indices.shape)} for {n} sequences "
+                         f"and {rows} tokens")
+    arrays = meta.host_arrays()
+    if arrays is not None:
+        lens = arrays["query_lens"].tolist()     # (a list: numpy's reductions cost 1 us each)
+    elif _capturing():
+        raise RuntimeError("verify_drafts reads a meta without host arrays from the device: not "
+                           "while a graph is captured")
+    else:
+        lens = meta.query_lens.tolist()
+        if meta.cu_query_lens.tolist() != [0, *accumulate(lens)]:
+            raise ValueError("cu_query_lens are not the sums of query_lens")
+    if min(lens) < 1 or sum(lens) != rows:
+        raise ValueError(f"query_lens ({min(lens)} at least, {sum(lens)} in all) do "
+                         f"not make up {rows} rows")
+    return lens
+
+
 def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, meta: BatchMeta,
                   uniforms: torch.Tensor, *, draft_probs: torch.Tensor | None = None,
                   temperature=1.0) -> tuple[torch.Tensor, torch.Tensor]:
@@ -144,19 +168,7 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, meta: BatchMeta,
         temps, temperature = temperature.contiguous(), 1.0
     elif not 0.0 <= float(temperature) < float("inf"):
         raise ValueError(f"temperature must be finite and not negative, got {temperature}")
-    arrays = meta.host_arrays()
-    if arrays is not None:
-        lens = arrays["query_lens"].tolist()     # (a list: numpy's reductions cost 1 us each)
-    elif _capturing():
-        raise RuntimeError("verify_drafts reads a meta without host arrays from the device: not "
-                           "while a graph is captured")
-    else:
-        lens = meta.query_lens.tolist()
-        if meta.cu_query_lens.tolist() != [0, *accumulate(lens)]:
-            raise ValueError("cu_query_lens are not the sums of query_lens")
-    if min(lens) < 1 or sum(lens) != rows:
-        raise ValueError(f"query_lens ({min(lens)} at least, {sum(lens)} in all) do "
-                         f"not make up {rows} rows")
+    lens = _step_lengths(meta, rows)
     width = max(lens)
     logits, tokens, uniforms = rows_for_kernel(logits), tokens.contiguous(), uniforms.contiguous()
     cu, owner = meta.cu_query_lens, meta.batch_indices

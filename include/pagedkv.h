@@ -672,7 +672,8 @@ int pkv_argmax_rows(const void* logits, int64_t n_rows, int64_t vocab, int64_t r
  * stands if it is the row's pkv_argmax_rows id, which is the token otherwise. In
  * a row without a distribution (a NaN, +inf, or nothing but -inf) no draft
  * stands, and that id is taken; a draft outside [0, vocab) does not stand.
- * temperatures: one a sequence, or NULL: `temperature` for all. `workspace`:
+ * temperatures: one a sequence, or NULL: `temperature` for all; one above the
+ * largest finite float (and +inf) counts as that. `workspace`:
  * pkv_verify_workspace_bytes, aligned to 16, in any state; calls that overlap in
  * time need one each.
  */

@@ -73,6 +73,10 @@ __device__ __forceinline__ void part_of(const T* row, int vocab, int s, int n, i
   end = s == n - 1 ? vocab : head + min((s + 1) * per, chunks) * E;
 }
 
+// What a temperature divides by: 1 for greedy rows; at most the largest finite float,
+// so that log2 e / temperature is not 0, and a logit of -inf keeps no weight.
+__device__ __forceinline__ float divisor(float t) { return t > 0.f ? fminf(t, 0x1.fffffep127f) : 1.f; }
+
 template <typename T>
 __global__ __launch_bounds__(kVT) void verify_stats_kernel(Verify a) {
   constexpr int E = 16 / (int)sizeof(T), U = kChunks;
@@ -85,7 +89,7 @@ __global__ __launch_bounds__(kVT) void verify_stats_kernel(Verify a) {
   part_of(row, a.vocab, s, a.splits, begin, end);
   const int seq = a.owner[r];
   const float t = a.temps ? (seq >= 0 && seq < a.n_seqs ? a.temps[seq] : 1.f) : a.temp;
-  const float c = fminf(kLog2e / (t > 0.f ? t : 1.f), 0x1p100f);
+  const float c = fminf(kLog2e / divisor(t), 0x1p100f);
   float m = -INFINITY, z = 0.f;
   int arg = 0x7fffffff;             // the thread's first place of m, or its chunk's start
   auto scalar = [&](int i) {
@@ -357,7 +361,7 @@ __device__ Decision decide(const Verify& a, int seq, DrawLds& lds) {
   const int r0 = a.cu[seq], n = a.cu[seq + 1] - r0;
   const float t = a.temps ? a.temps[seq] : a.temp;
   const bool greedy = !(t > 0.f);
-  const double c = 1.44269504088896340736 / (greedy ? 1.0 : (double)t);
+  const double c = 1.44269504088896340736 / (double)divisor(t);
   const float cf = fminf((float)c, 0x1p100f);
   const T* logits = reinterpret_cast<const T*>(a.logits);
   const int tid = threadIdx.x, lane = tid & 63;

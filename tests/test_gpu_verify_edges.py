@@ -1,0 +1,38 @@
+"""``verify_drafts`` at the ends of its ranges, against its definition in 64 bits."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from .test_gpu_verify import BF16, F16, F32, check, inputs
+
+pytestmark = pytest.mark.gpu
+MOST = torch.finfo(F32).max
+
+
+def below(temps):
+    """Temperatures as the definition has them: past the largest float, that."""
+    return [min(t, MOST) for t in temps]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("vocab", [37, 4099, 16384, 50021])
+@pytest.mark.parametrize("probs", [None, F32])
+def test_a_temperature_without_end(dtype, vocab, probs, monkeypatch):
+    """Every token as likely as the others, but for those at -inf."""
+    from . import test_gpu_verify as t
+    lens = [3, 2, 1, 4]
+    logits, tokens, numbers, q = inputs(lens, vocab, dtype, seed=vocab, probs=probs, near=0.05)
+    logits[:, 5:9] = -math.inf
+    logits[:, -2:] = -math.inf
+    tokens[1] = 6                    # (a draft that cannot be)
+    oracle = t.verify64
+    monkeypatch.setattr(t, "verify64",
+                        lambda *a: oracle(*a[:5], below(a[5]) if isinstance(a[5], list) else min(a[5], MOST)))
+    check(lens, logits, tokens, numbers, q, temps=[math.inf, 1.0, math.inf, math.inf])
+    check(lens, logits, tokens, numbers, q, temps=[0.5, math.inf, 0.0, MOST])
+    check(lens, logits, tokens, numbers, q, temps=MOST)
+    check(lens, logits, tokens, numbers, q, temps=1e39)

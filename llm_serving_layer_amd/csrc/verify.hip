@@ -411,8 +411,12 @@ __device__ Decision decide(const Verify& a, int seq, DrawLds& lds) {
           need = (double)u * (double)qx;
           const double sum = need * (double)s.z;
           // the sum's error, relative: its terms' and their sums' (a.error), and what
-          // the rounding of m c does to every exponent
-          const double error = (double)a.error + fmin(fabs((double)s.m * c), 0x1p80) * 0x1p-23;
+          // the rounding of m c does to every exponent; none is known where c was cut
+          // to 2^100, or is so small that l - m may overflow and still have weight
+          const double error =
+              c < 0x1p100 && c > 0x1p-120
+                  ? (double)a.error + fmin(fabs((double)s.m * c), 0x1p80) * 0x1p-23
+                  : INFINITY;
           state = fabs(sum - ex) <= error * fabs(sum) ? 2 : sum < ex;
         }
       }

@@ -36,3 +36,17 @@ def test_a_temperature_without_end(dtype, vocab, probs, monkeypatch):
     check(lens, logits, tokens, numbers, q, temps=[0.5, math.inf, 0.0, MOST])
     check(lens, logits, tokens, numbers, q, temps=MOST)
     check(lens, logits, tokens, numbers, q, temps=1e39)
+
+
+@pytest.mark.parametrize("probs", [None, F32])
+def test_temperatures_next_to_the_floats_ends(probs):
+    """Logits so close together, or so far apart, that log2(e) / temperature, or the
+    difference itself, leaves 32 bits."""
+    lens = [2] * 24
+    logits, tokens, numbers, q = inputs(lens, 700, F32, seed=3, probs=probs)
+    g = torch.Generator().manual_seed(9)
+    for scale, temp in ((2.0 ** -102, 1e-38), (2.0 ** -120, 2.0 ** -120), (1.4e38, 1e38),
+                        (8e37, 2.0 ** 126)):
+        near = (torch.randn((48, 700), generator=g).clamp(-2.3, 2.3) * scale).float()
+        assert torch.isfinite(near).all()
+        check(lens, near, tokens, numbers, q, temp)

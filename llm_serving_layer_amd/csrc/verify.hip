@@ -403,7 +403,7 @@ __device__ Decision decide(const Verify& a, int seq, DrawLds& lds) {
     if (tid < m) {
       const RowStats s = lds.rows[tid];
       int state = 0;                 // 0: falls, 1: stands, 2: too close to tell
-      if (x >= 0 && s.z == s.z) {
+      if (x >= 0 && s.z == s.z && s.m != -INFINITY) {   // (else: no distribution)
         if (greedy) {
           state = s.arg == x;
         } else {

@@ -50,3 +50,16 @@ def test_temperatures_next_to_the_floats_ends(probs):
         near = (torch.randn((48, 700), generator=g).clamp(-2.3, 2.3) * scale).float()
         assert torch.isfinite(near).all()
         check(lens, near, tokens, numbers, q, temp)
+
+
+def test_a_row_of_nothing_but_minus_infinity_at_temperature_zero():
+    """It has no distribution: no draft stands, not that of its greedy id either."""
+    lens = [3, 2]
+    logits, tokens, numbers, q = inputs(lens, 600, F32, seed=4)
+    logits[0] = -math.inf
+    logits[3] = -math.inf
+    tokens[1] = tokens[4] = 0
+    for probs in (q, None):
+        count = check(lens, logits, tokens, numbers, probs, [0.0, 0.0])
+        assert count.tolist() == [0, 0]
+        check(lens, logits, tokens, numbers, probs, [1.0, 0.0])

@@ -946,7 +946,7 @@ int pkv_attend_4bit(const void* batch, const void* q, void* out, const void* k_p
     // (of each XCD: its pieces' heads, four to a workgroup where a wave takes one)
     const int64_t per_xcd = (int64_t)((n + 7) / 8) * b.n_kv_heads;
     const int64_t grid = (waves == 1 ? (per_xcd + 3) / 4 : per_xcd) * 8;
-    if (grid > 0x7fffffffLL) return fail(PKV_ERR_INVALID, "too many pieces");
+    if (!launchable(grid, 256)) return fail(PKV_ERR_INVALID, "too many pieces");
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(waves == 1 ? 256 : 64 * waves), 0, s, a);
     PKV_LAUNCH_CHECK();
     return PKV_OK;

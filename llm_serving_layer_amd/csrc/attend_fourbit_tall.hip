@@ -382,7 +382,7 @@ int run_4bit_tall(const Attend4& args, int32_t head_dim, int32_t dtype, const in
   a.items = items;
   a.n_items = n_items;
   const int64_t grid = (int64_t)((n_items + 7) / 8) * a.n_kv * 8;
-  if (grid > 0x7fffffffLL) return fail(PKV_ERR_INVALID, "too many row tiles");
+  if (!launchable(grid, 256)) return fail(PKV_ERR_INVALID, "too many row tiles");
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, s, a);
   };

@@ -391,7 +391,9 @@ int pkv_append_4bit(void* k_pool, void* v_pool, int64_t num_blocks, const void* 
   const bool wide = f.tiled && ((uintptr_t)k | (uintptr_t)v | (uint64_t)(k_stride * eb) |
                                 (uint64_t)(v_stride * eb)) % 16 == 0;
   const int64_t work = n_tokens > 0x7fffffffLL ? n_tokens : n_tokens * 2 * f.n_kv * f.groups;
-  if (work > 0x7fffffffLL) return fail(PKV_ERR_INVALID, "too many rows in one append");
+  if (work > 0x7fffffffLL || !(wide ? launchable((work + 31) / 32, 256)
+                                    : launchable(n_tokens * 2 * f.n_kv, 64)))
+    return fail(PKV_ERR_INVALID, "too many rows in one append");
   auto go = [&](auto type) {
     typedef decltype(type) T;
     if (wide)
@@ -460,7 +462,7 @@ int run_4bit_any(const pkv_4bit& b, const void* q, void* out, const void* k_pool
                  const void* v_pool, float scale, hipStream_t s) {
   const FourBit f = four_bit(b.n_kv_heads, b.head_dim, b.page_size);
   const int64_t work = (int64_t)b.n_tokens * b.n_heads;
-  if (work > 0x7fffffffLL) return fail(PKV_ERR_INVALID, "too many query rows");
+  if (!launchable(work, 64)) return fail(PKV_ERR_INVALID, "too many query rows");
   auto go = [&](auto type) {
     typedef decltype(type) T;
     hipLaunchKernelGGL(attend_4bit_any_kernel<T>, dim3((unsigned)work), dim3(64), 0, s,

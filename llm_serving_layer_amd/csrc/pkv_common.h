@@ -27,6 +27,9 @@ int fail(int code, const char* fmt, ...);
                          hipGetErrorString(e_));                               \
   } while (0)
 
+// A launch of one dimension has fewer than 2^32 threads.
+inline bool launchable(int64_t groups, int32_t threads) { return groups <= 0xffffffffLL / threads; }
+
 // Report a launch error (bad configuration, missing code object) right away.
 #define PKV_LAUNCH_CHECK()                                                     \
   do {                                                                         \

@@ -752,7 +752,11 @@ int pkv_verify_drafts(const void* logits, int64_t n_rows, int64_t vocab, int64_t
   // 2^-24 of itself, the exponential by 2^-22; sums: one rounding a term
   a.error = 0x1p-16f + (float)(vocab / ((int64_t)a.splits * kVT) + 64) * 0x1p-24f;
   hipStream_t s = (hipStream_t)stream;
-  const unsigned rows = (unsigned)(n_rows * a.splits), seqs = (unsigned)(n_seqs * a.parts);
+  const int64_t row_groups = n_rows * a.splits, seq_groups = n_seqs * a.parts;
+  if (!launchable(row_groups, kVT) || !launchable(seq_groups, kDT))
+    return fail(PKV_ERR_INVALID, "%lld rows of %lld sequences are too many for one call",
+                (long long)n_rows, (long long)n_seqs);
+  const unsigned rows = (unsigned)row_groups, seqs = (unsigned)seq_groups;
   auto run = [&](auto type, auto probs) -> int {
     typedef decltype(type) T;
     typedef decltype(probs) Q;

@@ -755,6 +755,9 @@ static int plan_4bit(const int32_t* cu_query_lens, const int32_t* kv_indptr,
   };
   for (int32_t i = 0; i < n_seqs; ++i) {
     const int32_t kv = kv_lens[i], ql = cu_query_lens[i + 1] - cu_query_lens[i];
+    // (keys are counted in whole tiles, here and in the kernels)
+    if (kv > 0x7fffffff - 2 * kTile)
+      return fail(PKV_ERR_INVALID, "seq %d: kv_len=%d is above 2^31 - 129", i, kv);
     const int rc = check_seq_pages(i, kv_indptr[i + 1] - kv_indptr[i], kv, kv_last_page_len[i],
                                    page_size);
     if (rc) return rc;

@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes as C
 
+import numpy as np
 import pytest
 
 from llm_serving_layer_amd import _native
@@ -45,3 +46,19 @@ def test_verify(rows, seqs, vocab):
                                None, 1.0, 256, 1, 256, 256, size, None)
     with pytest.raises(ValueError, match="too many"):
         _native.check(rc, "verify")
+
+
+@pytest.mark.parametrize("kv", [2**31 - 1, 2**31 - 16, 2**31 - 100])
+@pytest.mark.parametrize("d", [64, 80])
+def test_a_plan_of_lengths_next_to_the_largest(kv, d):
+    """Tiles are counted past a sequence's end, in 32 bits."""
+    ps, i32 = 16, lambda *a: np.array(a, dtype=np.int32)
+    cu, pages, lens = i32(0, 1), -(-kv // ps), i32(kv)
+    indptr, ids, last = i32(0, pages), np.zeros(pages, np.int32), i32(kv - (pages - 1) * ps)
+    needed, args = C.c_int64(), _native.FourBit()
+    items = np.empty(28 * 1024, np.int32)
+    rc = _native.load().pkv_plan_4bit(
+        cu.ctypes.data, indptr.ctypes.data, ids.ctypes.data, lens.ctypes.data, last.ctypes.data, 1,
+        1, 1, d, ps, 0, 4, items.ctypes.data, items.size, C.byref(needed), C.addressof(args))
+    with pytest.raises(ValueError, match="kv_len"):
+        _native.check(rc, "plan")

@@ -245,6 +245,10 @@ class FourBitBackend(PagedPool):
         n = int(ql.shape[0])
         if n == 0:
             raise ValueError("attend needs at least one sequence")
+        for name, field, want in (("cu_query_lens", cu, n + 1), ("kv_lens", kvl, n),
+                                  ("kv_indptr", indptr, n + 1), ("kv_last_page_len", last, n)):
+            if field.shape[0] != want:
+                raise ValueError(f"{name} has {field.shape[0]} entries for {n} sequences")
         if bool(meta.is_prefill) != bool((ql > 1).any()):
             raise ValueError(
                 f"BatchMeta.is_prefill={meta.is_prefill} disagrees with query_lens "

@@ -286,7 +286,8 @@ __global__ __launch_bounds__(64) void attend_4bit_any_kernel(
   const int seq = batch_idx[tok];
   if (seq < 0 || seq >= n_seqs) return;
   const int q0 = cu_q[seq], q_len = cu_q[seq + 1] - q0;
-  const int limit = kv_lens[seq] - q_len + (tok - q0) + 1;   // keys this token sees
+  // keys this token sees (no more than there are, for a token of another sequence)
+  const int limit = min(kv_lens[seq] - q_len + (tok - q0) + 1, kv_lens[seq]);
   const int first_page = indptr[seq];
   const T* qr = q + ((int64_t)tok * n_heads + hq) * f.d;
   for (int i = lane; i < f.d; i += 64) qs[i] = Elem<T>::to_f(qr[i]);

@@ -120,3 +120,18 @@ def test_pieces_whose_scores_are_all_nan(d, hq, units):
         fill(c, spoilt, v)
         _, out = attend_last(c, 1, d ** -0.5)
         assert out.isnan().all(), (first, tiles)
+
+
+def test_owners_that_the_lengths_contradict():
+    """A token said to be a sequence's, but behind its end: it sees the keys that the
+    sequence has."""
+    c = Cache([40, 9], F16, 2, 4, 80)
+    counts = [2, 5]
+    meta = c.append(counts)
+    q = c.q(counts)
+    meta.batch_indices[:] = 0
+    out = c.bk.attend(q.to(DEV), 0, 0.1, meta).cpu()
+    for t in range(7):
+        n = min(41 + t, 42)
+        want, bound = attend64(q[t:t + 1], c.k[0][:n], c.v[0][:n], 0.1, F16)
+        assert_within(out[t:t + 1], want, bound, f"token {t}")

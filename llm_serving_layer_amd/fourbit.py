@@ -124,6 +124,13 @@ class FourBitBackend(PagedPool):
 
     # -- write path ---------------------------------------------------------------
 
+    def _slots(self, slots: torch.Tensor) -> torch.Tensor:
+        """Slots in 32 bits on the device; one that does not fit them is none of the
+        pool's, and stays so."""
+        if slots.dtype is torch.int64:
+            slots = slots.clamp(-1, 2**31 - 1)
+        return self._dev_i32(slots)
+
     def append_kv(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor,
                   meta: BatchMeta) -> None:
         """
@@ -148,7 +155,7 @@ class FourBitBackend(PagedPool):
                              "were supplied")
         if not tokens:
             return
-        k, v, slots = self._token_rows(k), self._token_rows(v), self._dev_i32(slots)
+        k, v, slots = self._token_rows(k), self._token_rows(v), self._slots(slots)
         if k.data_ptr() % 16:
             k = k.clone(memory_format=torch.contiguous_format)
         if v.data_ptr() % 16:
@@ -183,9 +190,7 @@ class FourBitBackend(PagedPool):
                              f"shape {tuple(slots.shape)}")
         if _capturing():
             self._keep(slots)
-        if slots.dtype is torch.int64:   # (beyond 32 bits: no pool has such a slot)
-            slots = slots.clamp(-1, 2**31 - 1)
-        slots = self._dev_i32(slots)
+        slots = self._slots(slots)
         n = slots.shape[0]
         k = torch.empty((n, self.n_kv_heads, self.head_dim), dtype=self.dtype, device=self.device)
         v = torch.empty_like(k)

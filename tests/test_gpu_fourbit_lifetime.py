@@ -1,4 +1,5 @@
-"""Graphs of the 4-bit cache's calls: what they read stays."""
+"""Slots of the 4-bit cache's calls: those that a graph reads stay, and those past 32
+bits are none of the pool's."""
 
 from __future__ import annotations
 
@@ -43,3 +44,19 @@ def test_a_captured_append_keeps_its_slots(dtype):
             same_bits(got, held64(want), F16)
     assert len(over) == 400
     c.bk.check_device_errors()
+
+
+def test_slots_past_32_bits_are_flagged():
+    c = Cache([20], F16, 2, 8, 64)
+    meta = c.append([2])
+    before = c.bk._pool.clone()
+    wide = torch.tensor([2**32 + 3, -2**32 + 4], device=DEV)
+    x = rows((2, 2, 64), F16, 9).to(DEV)
+    c.bk.append_kv(0, x, x, dataclasses.replace(meta, slot_mapping=wide, host=None))
+    assert torch.equal(c.bk._pool, before)
+    with pytest.raises(IndexError, match="slot_mapping"):
+        c.bk.check_device_errors()
+    k, v = c.bk.read_kv(0, wide)
+    assert not k.any() and not v.any()
+    with pytest.raises(IndexError):
+        c.bk.check_device_errors()

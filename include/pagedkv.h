@@ -548,7 +548,8 @@ int pkv_read_4bit(const void* k_pool, const void* v_pool, int64_t num_blocks,
  * [n_tokens, n_heads, head_dim] in dtype; a batch's arguments are set once and
  * serve every layer.
  *
- * pkv_plan_4bit (host, synchronous) checks the metadata as pkv_plan_decode does
+ * pkv_plan_4bit (host, synchronous) checks the metadata as pkv_plan_decode does (a
+ * kv_len is at most 2^31 - 129)
  * and fills items (capacity ints; *needed of them, PKV_ERR_CAPACITY if there are
  * fewer) with pieces of 28 ints {first token's row in q, tokens, its position,
  * kv_len, first page in kv_indices, pages, first tile of 64 keys, tiles, partial

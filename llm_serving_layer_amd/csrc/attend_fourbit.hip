@@ -60,14 +60,15 @@ constexpr int kFewRows = 16, kWideRows = 32, kTallFrom = 64;
 // Pieces of a cut row at most, four waves and one: what the last of them joins.
 constexpr int kMostPieces = 128, kMostPieces1 = 32;
 // Workgroups a compute unit that pieces are cut for. Few rows, four waves: 2 (one
-// sequence of 32750 tokens, head_dim 64: 13.0 us; 1 took 12.4, 4 16.6; 16 of 20000 to
-// 60000, head_dim 128: 115, 163 and 116). Wide rows: 2 (48 sequences of 2000 to 8000 with
-// 2 to 6 new tokens, head_dim 128: 79; 1 took 88, 4 81).
+// sequence of 32750 tokens, head_dim 64: 12.4 us; 1 took 11.9, 4 15.9; 16 of 20000 to
+// 60000, head_dim 128: 113, 145 and 115). Wide rows: 2 (48 sequences of 2000 to 8000 with
+// 2 to 6 new tokens, head_dim 128: 76.8; 1 took 89.8, 4 78.9).
 constexpr int kFewResident = 2, kWideResident = 2;
 // From kOneWaveRows rows (x KV heads) a compute unit on, a piece of few rows is one
 // wave's, of kOneLeast tiles at least, 16 a compute unit: 256 sequences of 1 to 2048
-// tokens (258 on average) take 14.4 us, as four waves' 18.0; pieces from 3 tiles 15.3,
-// from 6 14.0, from 10 18.9.
+// tokens (258 on average) take 13.5 us, as four waves' 15.1; pieces from 3 tiles 14.7,
+// from 5 and 6 13.7, from 8 15.4. (100 and 500 sequences, and 300 of 100 to 1000: 4, 5, 6
+// and 8 within 2%.)
 constexpr int kOneResident = 16, kOneLeast = 4, kOneWaveRows = 8;
 // Few rows beside wide ones run as wide ones up to kJoin times their tiles: one launch
 // with one ramp and tail, for a row of them at least half idle in the matrix cores.
@@ -75,9 +76,9 @@ constexpr int kJoin = 4;
 // A sequence is tall where kTallAlong tiles x compute units <= work (tiles of all wide
 // pieces): a tile takes a tall piece by itself 1.7 us at head_dim 64, a wide one 1.3 us
 // / 4 of a compute unit (2.9 and 1.9 / 4 at 128). Measured, 4 query heads each of 8, tall
-// and wide: 8 chunks of 512 over 1536 153 and 177 us (head_dim 128: 267 and 318), 16 of
-// 512 over 100 67 and 117, 64 of 20 over 300 30 and 43 (128); one of 2000 tokens 57 and
-// 46, 8 of 128 over 1000 35 and 30.
+// and wide: 8 chunks of 512 over 1536 148 and 185 us (head_dim 128: 266 and 320), 16 of
+// 512 over 100 72 and 114, 64 of 20 over 300 32 and 42 (128); one of 2000 tokens 58 and
+// 47, 8 of 128 over 1000 35 and 31.
 constexpr int64_t kTallAlong = 5;
 
 // Floats per wave for a tile's steps, zeros of K, steps and middles of V

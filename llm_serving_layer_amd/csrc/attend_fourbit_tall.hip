@@ -14,7 +14,7 @@
 //    bits p zero + 7.5 p step. With 2^E at least the largest step that the row has seen,
 //    p counts 2^-E more, so that p step stays within float16.
 // 8 x 512 tokens over 1536, head_dim 64, 8 KV heads of 4: 122 us, 490 TFLOP/s (as wide
-// pieces 155). With keys and values rounded to float16 in LDS and p beside them it took
+// pieces 150). With keys and values rounded to float16 in LDS and p beside them it took
 // 95, but three roundings of 2^-11 added 1.4 times the output's own error; this one adds
 // as much as it.
 // Rows of 144 bytes (272 for K at head_dim 128) put the 16 lanes of a 16-byte read on

@@ -11,11 +11,11 @@ namespace pkv {
 
 // A tiled row group (64 elements) by 8 lanes of 8 elements: 16-byte loads, a minimum
 // and maximum over the 8 lanes, then each lane's codes: K one word, V four bytes.
-// HBM-bound by its inputs (4 of 5 bytes) if the vector work is short: a group's
+// Its inputs are 4 of 5 bytes that it moves; what bounds it is the vector work: a group's
 // elements next to a border between codes are looked for together and all decided in
 // 64 bits where there is one (a wave in 16), codes are packed as sums in float.
-// 5 to 6 thousand tokens of 8 heads of 128 (32 MB) take 14.6 us, 2.2 TB/s: some 300
-// vector instructions a wave and the ramps of a short launch (one token: 2.3).
+// 5 to 6 thousand tokens of 8 heads of 128 (32 MB) take 14.4 us, 2.2 TB/s: 284 vector
+// instructions a wave are 11 of them, the ramps of a short launch (one token: 2.3) the rest.
 template <typename T>
 __global__ __launch_bounds__(256) void append_4bit_kernel(
     unsigned char* __restrict__ kpool, unsigned char* __restrict__ vpool, int64_t num_slots,

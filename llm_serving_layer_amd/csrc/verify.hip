@@ -23,8 +23,10 @@
 //  * verify_rest_kernel, with draft probabilities: the same over max(p - q, 0).
 //    In 32 bits the sum's error would move the border of every token behind it.
 // 64 sequences of 2 to 6 rows of 128256 bf16 logits, fp32 draft probabilities: 17.4 (64
-// MB, 3.7 TB/s) + 18.2 + 18.0 us; 24 of 9 rows in fp32 21.5 (5.1 TB/s) + 14.1 + 14.4; one
-// sequence of 5 rows 4.5 + 5.7 + 9.0, a chain of waits.
+// MB, 3.7 TB/s) + 18.1 + 18.3 us; 24 of 9 rows in fp32 21.2 (5.2 TB/s) + 14.4 + 14.4; one
+// sequence of 5 rows 4.5 + 5.8 + 8.8, a chain of waits. Of the second and third kernel's 18
+// us, vector instructions are 6 and 4: the rest is each workgroup's table and decision
+// before its first useful load, the arrival, and the last one's search, not timed apart.
 #include <algorithm>
 
 #include "mfma.h"
@@ -34,7 +36,7 @@ namespace pkv {
 constexpr int kVT = 256;            // threads of a workgroup
 constexpr int kMaxSplits = 64;      // of a row: a lane each
 constexpr int kChunks = 8;          // of 16 bytes a thread and round, in the first kernel
-                                    // (249 rows of 128256 in bf16: 17.4 us; 4 take 18.7)
+                                    // (249 rows of 128256 in bf16: 17.4 us; 4 take 1.2 more)
 
 struct RowStats { float m, z; int32_t arg, pad; };
 
@@ -663,7 +665,8 @@ static int32_t row_units(int64_t vocab) {
   return (int32_t)((vocab + unit - 1) / unit);
 }
 // Parts of a drawn row: about 512 workgroups (two a compute unit; each repeats the
-// decision): 64 sequences take 53.5 us, with 256 56, with 1024 60; a unit each at least.
+// decision): 64 sequences take 51.4 us, with 256 53.7, with 1024 54.6; a unit each at
+// least.
 static int32_t seq_parts(int64_t n_seqs, int64_t vocab) {
   return (int32_t)std::min<int64_t>((512 + n_seqs - 1) / n_seqs, row_units(vocab));
 }

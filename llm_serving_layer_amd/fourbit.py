@@ -212,7 +212,13 @@ class FourBitBackend(PagedPool):
         """
         Causal GQA attention over each sequence's full paged history, any number
         of new tokens a sequence. The result depends, in its last bits, on what
-        shares the batch (long sequences are cut to fill the device).
+        shares the batch (long sequences are cut to fill the device), and on the
+        keys that a token sees alone: NaN where one of them is.
+
+        Weights times steps of V are rounded to float16, the matrix cores' input:
+        by 2^-11 of a product at most, or, of products below some 2^-13 of the
+        largest weight times the largest step among the token's keys, by 2^-24 of
+        that.
 
         To capture a graph, call it with the meta before, with no other meta's
         call between. Graphs captured with one meta share its buffers: neither

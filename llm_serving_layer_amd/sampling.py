@@ -128,8 +128,9 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, meta: BatchMeta,
     row without a distribution (a NaN, +inf, nothing but -inf) lets no draft
     stand and gives its ``greedy`` id; a draft outside [0, vocab) falls.
     Asynchronous on torch's current stream; every call has a workspace of its
-    own, so calls may overlap and be captured. A meta without host arrays is read
-    back from the device (not in a capture).
+    own, so calls may overlap and be captured; a captured call reads ``meta``'s
+    ``cu_query_lens`` and ``batch_indices``, which have to stay as long as the graph
+    does. A meta without host arrays is read back from the device (not in a capture).
     """
     if logits.dim() != 2:
         raise ValueError(f"logits must be (n_tokens, vocab), got shape {tuple(logits.shape)}")

@@ -234,7 +234,8 @@ class FourBitBackend(PagedPool):
             raise ValueError(f"meta describes {meta.n_tokens} tokens but q has {tokens}")
         p = self._planned
         if p is None or p.meta is not meta:
-            p = self._plan(meta)
+            with self._on_device():
+                p = self._plan(meta)
         stream = self._enter(p)
         q = self._as_pool(q)
         if q.data_ptr() % 16:

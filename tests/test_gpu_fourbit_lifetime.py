@@ -1,8 +1,9 @@
 """Slots of the 4-bit cache's calls: those that a graph reads stay, and those past 32
-bits are none of the pool's."""
+bits are none of the pool's. Every launch is the backend's device's."""
 
 from __future__ import annotations
 
+import contextlib
 import dataclasses
 import gc
 
@@ -60,3 +61,38 @@ def test_slots_past_32_bits_are_flagged():
     assert not k.any() and not v.any()
     with pytest.raises(IndexError):
         c.bk.check_device_errors()
+
+
+def test_every_launch_is_made_on_the_backends_device():
+    """The plan's upload too. (With one device: inside what makes it the current one.)"""
+    c = Cache([40], F16, 2, 8, 64)
+    meta = c.append([2])
+    q = c.q([2])
+    bk, inside, seen = c.bk, [0], []
+
+    @contextlib.contextmanager
+    def here():
+        inside[0] += 1
+        yield
+        inside[0] -= 1
+
+    def watched(name, call):
+        def f(*args):
+            seen.append((name, inside[0] > 0))
+            return call(*args)
+        return f
+
+    class Library:
+        def __init__(self, lib):
+            self._lib = lib
+
+        def __getattr__(self, name):
+            return watched(name, getattr(self._lib, name))
+
+    bk._on_device, bk._lib = here, Library(bk._lib)
+    bk._upload = watched("upload", bk._upload)
+    out = bk.attend(q.to(DEV), 0, 0.125, meta)
+    bk.read_kv(0, meta.slot_mapping)
+    c.check(out, q, [2], 0.125)
+    assert {n for n, _ in seen} >= {"upload", "pkv_attend_4bit", "pkv_read_4bit"}
+    assert all(ok for _, ok in seen), seen

@@ -112,13 +112,14 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, meta: BatchMeta,
     ``logits`` (``(T, vocab)`` f16, bf16 or f32) the target's for what follows
     each. Draft x behind row r stands if ``uniforms[r] * q(x) < p(x)``: p the
     softmax of the row over ``temperature`` (a number, or a float32 tensor of one
-    a sequence; as a float32, at most the largest finite one), q the drafting distribution (``draft_probs``, ``(T - n_seqs,
-    vocab)``, a row a draft in order; None: 1 at the draft). The first that does
-    not stand ends a sequence's run and is replaced by a token drawn from
-    ``max(p - q, 0)`` (p where that is nothing); behind a run that stands whole
-    one is drawn from the last row's p. Drawn is the first token whose running
-    sum of weights exceeds the sequence's last number times their sum, so the
-    ``(T,)`` float32 ``uniforms`` in [0, 1) serve all decisions once each.
+    a sequence; as a float32, at most the largest finite one), q the drafting
+    distribution (``draft_probs``, ``(T - n_seqs, vocab)``, a row a draft in order;
+    None: 1 at the draft). The first that does not stand ends a sequence's run and
+    is replaced by a token drawn from ``max(p - q, 0)`` (p where that is nothing);
+    behind a run that stands whole one is drawn from the last row's p. Drawn is the
+    first token whose running sum of weights exceeds the sequence's last number
+    times their sum, so the ``(T,)`` float32 ``uniforms`` in [0, 1) serve all
+    decisions once each.
 
     Returns ``(ids, accepted)``, int64: per sequence the drafts that stand, one
     more token, -1 behind it (``(n_seqs, max(query_lens))``), and how many stand.

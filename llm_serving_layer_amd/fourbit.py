@@ -218,7 +218,9 @@ class FourBitBackend(PagedPool):
         Weights times steps of V are rounded to float16, the matrix cores' input:
         by 2^-11 of a product at most, or, of products below some 2^-13 of the
         largest weight times the largest step among the token's keys, by 2^-24 of
-        that.
+        that. Scores (times scale) have to stay below some 2^26: from there on a
+        reference in 32 bits lies a unit and more off the largest one, and with the
+        matrix-core kernels an output may be NaN.
 
         To capture a graph, call it with the meta before, with no other meta's
         call between. Graphs captured with one meta share its buffers: neither

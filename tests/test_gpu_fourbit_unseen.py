@@ -135,3 +135,23 @@ def test_owners_that_the_lengths_contradict():
         n = min(41 + t, 42)
         want, bound = attend64(q[t:t + 1], c.k[0][:n], c.v[0][:n], 0.1, F16)
         assert_within(out[t:t + 1], want, bound, f"token {t}")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,new,units", FORMS)
+@pytest.mark.parametrize("power", [16, 20, 23])
+def test_scores_next_to_the_largest(d, hq, new, units, power):
+    """Scores to 2^25.7, so far apart that the largest takes all the weight: that key's V
+    comes out."""
+    n = 70 + new
+    c = Cache([0], BF16, 2, hq, d, room=400, compute_units=units)
+    k, v = rows((n, 2, d), BF16, 1), rows((n, 2, d), BF16, 2)
+    k *= 0.25
+    k[33] = 8.0                      # (a constant row is held exactly)
+    fill(c, k, v)
+    q = torch.full((new, hq, d), 2.0 ** (power - 4), dtype=BF16)
+    q[..., 0] = 2.0 ** power
+    _, out = attend_last(c, new, d ** -0.5, q)
+    want, _ = attend64(q, k, v, d ** -0.5, BF16)
+    _, bound = attend64(q * 0, k[33:34].expand(new, 2, d), v[33:34].expand(new, 2, d), 1.0, BF16)
+    assert_within(out, want, bound)
